@@ -1,0 +1,557 @@
+"""Sequence mixers beside causal attention, as cases that can be timed and compared.
+
+Three operators of a decoder whose own state does not grow and that reads an
+encoder: the short causal convolution over time, the selective state space
+scan, and attention to an encoder's states of another length. Each comes as a
+whole sequence without gradients ("prompt"), as a forward and backward pass
+("train") and for one new token per sequence ("step").
+
+With `own` false, `run` is the plain form: elementary torch operations, a loop
+over time for the scan, materialised scores for the attention. With `own` true
+it makes the calls a program makes of `dtmi.autograd`. `exact` is the operators'
+definition in float64 by other means (a doubling scan, torch's own gradients).
+"""
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+
+# ------------------------------------------------------------------- cases
+def listed():
+    return [
+        # one token each for a few sequences of a small character model: the
+        # smallest call, latency only
+        dict(name="conv_step_small", op="conv", form="step", dtype="float32", batch=4, dim=256, taps=4),
+        # padded prompts of an odd width, their states kept for generation
+        dict(name="conv_prompt_ragged", op="conv", form="prompt", dtype="float32", batch=5, ctx=777, dim=1001, taps=3,
+             ragged=True),
+        # the convolution of a training step: twice GPT-2-small's width at its
+        # context, input and gate out of one projection
+        dict(name="conv_train", op="conv", form="train", dtype="float32", batch=8, ctx=1024, dim=1536, taps=4,
+             fused=True),
+        # one token each for a full serving batch
+        dict(name="scan_step", op="scan", form="step", dtype="float32", batch=64, dim=1536, states=16, groups=1),
+        # one long prompt: few channels for the card, many steps
+        dict(name="scan_prompt_long", op="scan", form="prompt", dtype="float32", batch=1, ctx=2047, dim=768, states=16,
+             groups=1, fused=True),
+        # padded prompts, a number of states that fills no vector, shared
+        # input and output maps per group of channels
+        dict(name="scan_prompt_ragged", op="scan", form="prompt", dtype="float32", batch=6, ctx=501, dim=600, states=13,
+             groups=2, ragged=True),
+        # the scan of a training step
+        dict(name="scan_train", op="scan", form="train", dtype="float32", batch=4, ctx=1024, dim=1536, states=16,
+             groups=1, fused=True),
+        # the same in float64, as gradients are checked with
+        dict(name="scan_train_f64", op="scan", form="train", dtype="float64", batch=3, ctx=257, dim=384, states=8,
+             groups=1),
+        # one new token per sequence against a long memory with shared heads
+        dict(name="cross_step_shared", op="cross", form="step", dtype="float32", batch=8, heads=16, kvheads=4, ctx=1,
+             mem=4999, hdim=128, ragged=True),
+        # GPT-2-small's heads at its context over an encoder half as long
+        dict(name="cross_train", op="cross", form="train", dtype="float32", batch=8, heads=12, kvheads=12, ctx=1024,
+             mem=512, hdim=64, fused=True),
+        # padded memories, shared heads, an odd head dimension
+        dict(name="cross_train_ragged", op="cross", form="train", dtype="float32", batch=4, heads=8, kvheads=2, ctx=333,
+             mem=1501, hdim=72, ragged=True),
+        # float64, a decoder prompt
+        dict(name="cross_prompt_f64", op="cross", form="prompt", dtype="float64", batch=2, heads=6, kvheads=6, ctx=300,
+             mem=700, hdim=64),
+    ]
+
+
+def _between(rng, lo, hi):
+    """A whole number, spread evenly over the logarithm."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1)))))))
+
+
+def draw(rng):
+    op = rng.choice(["conv", "scan", "scan", "cross", "cross"])
+    form = rng.choice(["step", "prompt", "train", "train"])
+    f64 = rng.random() < 0.25
+    c = dict(op=op, form=form, dtype="float64" if f64 else "float32")
+    if form != "step" or op == "cross":
+        c["ragged"] = rng.random() < 0.4
+    if op == "conv":
+        c.update(dim=_between(rng, 48, 2048), taps=rng.choice([2, 3, 4, 4, 5, 8]))
+        if form == "step":
+            c["batch"] = _between(rng, 1, 512)
+        else:
+            c.update(ctx=_between(rng, 1, 4096), fused=rng.random() < 0.3)
+            c["batch"] = _between(rng, 1, max(1, min(32, 6_000_000 // (c["ctx"] * c["dim"]))))
+    elif op == "scan":
+        g = rng.choice([1, 1, 1, 2, 4])
+        c.update(dim=g * _between(rng, 16, 1536 // g), groups=g, states=rng.choice([4, 8, 13, 16, 16, 16, 32, 64]))
+        if form == "step":
+            c["batch"] = _between(rng, 1, min(256, 25_000_000 // (c["dim"] * c["states"])))
+        else:
+            c.update(ctx=_between(rng, 1, 1024 if form == "train" else 2047), fused=rng.random() < 0.3)
+            most = (20_000_000 if f64 else 90_000_000) // (c["ctx"] * c["dim"] * c["states"])
+            c["batch"] = _between(rng, 1, max(1, min(16, most)))
+            c["ctx"] = max(1, min(c["ctx"], c["ctx"] * most if most else c["ctx"] // 4))
+    else:
+        k = rng.choice([1, 2, 4, 6, 8])
+        c.update(kvheads=k, heads=k * rng.choice([1, 1, 2, 4]), hdim=rng.choice([32, 40, 64, 64, 72, 80, 96, 128]))
+        c["ctx"] = 1 if form == "step" else _between(rng, 1, 1024)
+        c["mem"] = _between(rng, 1, 8192 if form == "step" else 2048)
+        most = (300_000_000 if f64 else 2_500_000_000) // (c["heads"] * c["ctx"] * c["mem"] * c["hdim"])
+        c["batch"] = _between(rng, 1, max(1, min(16, most)))
+        if form != "step":
+            c["fused"] = rng.random() < 0.4
+    return c
+
+
+# ------------------------------------------------------------------ inputs
+def _lengths(case, seed, n):
+    """How far each sequence of a padded batch reaches: the longest first, an
+    empty one last where there are three or more."""
+    if not case.get("ragged"):
+        return None
+    r = random.Random(seed * 7919 + 17)
+    out = [n] + [r.randint(1, n) for _ in range(case["batch"] - 1)]
+    if len(out) >= 3:
+        out[-1] = 0
+    return out
+
+
+def _inputs(case, seed):
+    """The case's inputs as torch tensors on the GPU, from the seed alone. Where
+    `fused`, arrays that one projection makes are views of one buffer."""
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    dt = torch.float64 if case["dtype"] == "float64" else torch.float32
+
+    def normal(*shape, std=1.0, mean=0.0):
+        return torch.randn(shape, generator=g, device="cuda", dtype=dt) * std + mean
+
+    def uniform(*shape):
+        return torch.rand(shape, generator=g, device="cuda", dtype=dt)
+
+    B, form = case["batch"], case["form"]
+    t = {}
+    if case["op"] == "conv":
+        C, K = case["dim"], case["taps"]
+        t["w"], t["b"] = normal(K, C, std=K ** -0.5), normal(C, std=0.1)
+        if form == "step":
+            t["x"] = normal(B, C)
+            t["state"] = normal(B, K - 1, C)
+            return t
+        T = case["ctx"]
+        t["x"] = normal(B, T, 2, C)[:, :, 0] if case.get("fused") else normal(B, T, C)
+        t["lengths"] = _lengths(case, seed, T)
+        if form == "train":
+            t["g"] = normal(B, T, C)
+        return t
+    if case["op"] == "scan":
+        C, N, G = case["dim"], case["states"], case["groups"]
+        # decay rates -1 .. -N as such layers start with, step sizes of 1e-3 to 1e-1
+        t["A"] = -torch.arange(1, N + 1, device="cuda", dtype=dt) * torch.exp(normal(C, N, std=0.1))
+        step = torch.exp(uniform(C) * math.log(100.0) + math.log(1e-3))
+        t["bias"] = step + torch.log(-torch.expm1(-step))
+        t["D"] = normal(C, std=0.1, mean=1.0)
+        lead = (B,) if form == "step" else (B, case["ctx"])
+        t["u"], t["dt"] = normal(*lead, C), normal(*lead, C, std=0.5)
+        if case.get("fused"):
+            t["z"] = normal(*lead, 2, C)[..., 1, :]
+            bc = normal(*lead, 2, G, N)
+            t["B"], t["C"] = bc[..., 0, :, :], bc[..., 1, :, :]
+        else:
+            t["z"], t["B"], t["C"] = normal(*lead, C), normal(*lead, G, N), normal(*lead, G, N)
+        if form == "step":
+            t["state"] = normal(B, C, N, std=0.1)
+        else:
+            t["lengths"] = _lengths(case, seed, case["ctx"])
+            if form == "train":
+                t["g"] = normal(*lead, C)
+        return t
+    H, Hk, T, M, D = (case[x] for x in ("heads", "kvheads", "ctx", "mem", "hdim"))
+    t["q"] = normal(B, T, H, D).permute(0, 2, 1, 3)
+    if case.get("fused"):
+        kv = normal(B, M, 2, Hk, D)
+        t["k"], t["v"] = kv[:, :, 0].permute(0, 2, 1, 3), kv[:, :, 1].permute(0, 2, 1, 3)
+    else:
+        t["k"], t["v"] = normal(B, Hk, M, D), normal(B, Hk, M, D)
+    t["lengths"] = _lengths(case, seed, M)
+    if form == "train":
+        t["g"] = normal(B, H, T, D)
+    return t
+
+
+# ----------------------------------------------------------- the framework's
+def _dtmi():
+    pkg = str(Path(__file__).resolve().parents[1] / "distributed-training_amd")
+    if pkg not in sys.path:
+        sys.path.insert(1, pkg)
+    from dtmi import _lib, autograd, device
+    _lib.lib()
+    return autograd, device
+
+
+class _Memory:
+    """A DeviceArray's memory as torch takes it (no copy; keeps the array alive)."""
+
+    def __init__(self, a):
+        self.array = a
+        self.__cuda_array_interface__ = {"shape": a.shape, "typestr": a.dtype.str, "data": (a.ptr, False),
+                                         "strides": tuple(s * a.itemsize for s in a.strides), "version": 2}
+
+
+def _tensor(a):
+    return torch.as_tensor(_Memory(a), device="cuda")
+
+
+def _array(t, dev):
+    """A DeviceArray with a torch tensor's values and strides."""
+    extent = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    a = dev.empty((extent,), str(t.dtype).split(".")[1])
+    a = dev.DeviceArray(a.block, tuple(t.shape), a.dtype, 0, t.stride())
+    _tensor(a).copy_(t)
+    return a
+
+
+def prepare(case, seed):
+    torch.cuda.synchronize()
+    t = _inputs(case, seed)
+    s = {"op": case["op"], "form": case["form"], "own": own}
+    if own:
+        A, dev = _dtmi()
+        for k, v in t.items():
+            if k == "lengths":
+                s[k] = None if v is None else A.Indices(v)
+            else:
+                s[k] = _array(v, dev)
+        torch.cuda.synchronize()
+        return s
+    s.update(t)
+    if t.get("lengths") is not None:
+        s["lengths"] = torch.tensor(t["lengths"], device="cuda")
+    torch.cuda.synchronize()
+    return s
+
+
+def _own(s):
+    A, _ = _dtmi()
+    op, form = s["op"], s["form"]
+    if form == "train":
+        def leaf(name):
+            return A.Tensor(s[name], requires_grad=True)
+    else:
+        def leaf(name):
+            return A.Tensor(s[name])
+    if op == "conv":
+        if form == "step":
+            y = A.causal_conv_step(leaf("x"), leaf("w"), leaf("b"), s["state"])
+            return [_tensor(y.data), _tensor(s["state"])]
+        x, w, b = leaf("x"), leaf("w"), leaf("b")
+        if form == "prompt":
+            y, state = A.causal_conv(x, w, b, lengths=s["lengths"], return_state=True)
+            return [_tensor(y.data), _tensor(state)]
+        y = A.causal_conv(x, w, b, lengths=s["lengths"])
+        y.backward(s["g"])
+        return [_tensor(a) for a in (y.data, x.grad, w.grad, b.grad)]
+    if op == "scan":
+        names = ("u", "dt", "A", "B", "C", "D", "z", "bias")
+        L = [leaf(n) for n in names]
+        if form == "step":
+            y = A.ssm_scan_step(*L, state=s["state"])
+            return [_tensor(y.data), _tensor(s["state"])]
+        if form == "prompt":
+            y, state = A.ssm_scan(*L, lengths=s["lengths"], return_state=True)
+            return [_tensor(y.data), _tensor(state)]
+        y = A.ssm_scan(*L, lengths=s["lengths"])
+        y.backward(s["g"])
+        return [_tensor(y.data)] + [_tensor(x.grad) for x in L]
+    q, k, v = leaf("q"), leaf("k"), leaf("v")
+    o = A.cross_attention(q, k, v, lengths=s["lengths"])
+    if form != "train":
+        return _tensor(o.data)
+    o.backward(s["g"])
+    return [_tensor(a) for a in (o.data, q.grad, k.grad, v.grad)]
+
+
+# -------------------------------------------------------------- plain forms
+def _valid(lengths, T, like):
+    """[B, T, 1] of 0 and 1, or None."""
+    if lengths is None:
+        return None
+    return (torch.arange(T, device="cuda")[None, :] < lengths[:, None])[:, :, None]
+
+
+def _conv(s):
+    x, w, b = s["x"], s["w"], s["b"]
+    K = w.shape[0]
+    if s["form"] == "step":
+        full = torch.cat([s["state"], x[:, None]], 1)
+        pre = (full * w).sum(1) + b
+        s["state"].copy_(full[:, 1:])
+        return [pre * torch.sigmoid(pre), s["state"]]
+    B, T, C = x.shape
+    ok = _valid(s["lengths"], T, x)
+    if ok is not None:
+        x = torch.where(ok, x, 0.0)
+    xp = torch.cat([x.new_zeros(B, K - 1, C), x], 1)
+    pre = b.expand(B, T, C).clone()
+    for k in range(K):
+        pre += w[k] * xp[:, k:k + T]
+    sg = torch.sigmoid(pre)
+    y = pre * sg
+    if ok is not None:
+        y = torch.where(ok, y, 0.0)
+    if s["form"] == "prompt":
+        if ok is None:
+            return [y, xp[:, T:].clone()]
+        at = s["lengths"][:, None] + torch.arange(K - 1, device="cuda")[None]
+        return [y, torch.gather(xp, 1, at[:, :, None].expand(B, K - 1, C))]
+    g = s["g"] * (sg * (1 + pre * (1 - sg)))
+    if ok is not None:
+        g = torch.where(ok, g, 0.0)
+    gp = torch.cat([g, g.new_zeros(B, K - 1, C)], 1)
+    dx = torch.zeros_like(g)
+    for k in range(K):
+        dx += w[k] * gp[:, K - 1 - k:K - 1 - k + T]
+    dw = torch.stack([(g * xp[:, k:k + T]).sum((0, 1)) for k in range(K)])
+    return [y, dx, dw, g.sum((0, 1))]
+
+
+def _softplus(x):
+    return torch.clamp(x, min=0) + torch.log1p(torch.exp(-torch.abs(x)))
+
+
+def _spread(m, C):
+    """A group's row for each of its channels: [B, G, N] -> [B, C, N]."""
+    G = m.shape[1]
+    return m[:, :, None].expand(-1, -1, C // G, -1).reshape(m.shape[0], C, -1)
+
+
+def _scan(s):
+    u, A, D, z = s["u"], s["A"], s["D"], s["z"]
+    raw = s["dt"] + s["bias"]
+    d = _softplus(raw)
+    C = u.shape[-1]
+    sz = torch.sigmoid(z)
+    if s["form"] == "step":
+        h = s["state"]
+        h.mul_(torch.exp(d[:, :, None] * A)).add_((d * u)[:, :, None] * _spread(s["B"], C))
+        y = (h * _spread(s["C"], C)).sum(-1) + D * u
+        return [y * (z * sz), h]
+    B, T, _ = u.shape
+    ok = _valid(s["lengths"], T, u)
+    Bm, Cm, g = s["B"], s["C"], s.get("g")
+    if ok is not None:
+        zero = torch.zeros((), device="cuda", dtype=u.dtype)
+        u, d, z, sz, raw = (torch.where(ok, v, zero) for v in (u, d, z, sz, raw))
+        Bm, Cm = torch.where(ok[..., None], Bm, zero), torch.where(ok[..., None], Cm, zero)
+        g = torch.where(ok, g, zero) if g is not None else None
+    train = s["form"] == "train"
+    h = u.new_zeros(B, C, A.shape[1])
+    hs, ys = [h], []
+    for t in range(T):
+        h = h * torch.exp(d[:, t, :, None] * A) + (d[:, t] * u[:, t])[:, :, None] * _spread(Bm[:, t], C)
+        ys.append((h * _spread(Cm[:, t], C)).sum(-1))
+        if train:
+            hs.append(h)
+    y = torch.stack(ys, 1) + D * u
+    out = y * (z * sz)
+    if not train:
+        return [out, h]
+    G, N = Bm.shape[2], A.shape[1]
+    dz = g * y * (sz * (1 + z * (1 - sz)))
+    dy = g * (z * sz)
+    dD = (dy * u).sum((0, 1))
+    dA, dh = torch.zeros_like(A), torch.zeros_like(h)
+    dB, dC = torch.empty_like(Bm, memory_format=torch.contiguous_format), torch.empty(Cm.shape, device="cuda",
+                                                                                      dtype=u.dtype)
+    du, dd = torch.empty(u.shape, device="cuda", dtype=u.dtype), torch.empty(u.shape, device="cuda", dtype=u.dtype)
+    for t in range(T - 1, -1, -1):
+        Bt = _spread(Bm[:, t], C)
+        dyt, dt_, ut = dy[:, t, :, None], d[:, t, :, None], u[:, t, :, None]
+        dh = dh + dyt * _spread(Cm[:, t], C)
+        dC[:, t] = (dyt * hs[t + 1]).reshape(B, G, C // G, N).sum(2)
+        dB[:, t] = (dh * (dt_ * ut)).reshape(B, G, C // G, N).sum(2)
+        a = torch.exp(dt_ * A)
+        q = dh * hs[t] * a
+        dx = (dh * Bt).sum(-1)
+        du[:, t] = dx * d[:, t]
+        dd[:, t] = (q * A).sum(-1) + dx * u[:, t]
+        dA += (q * dt_).sum(0)
+        dh = dh * a
+    du += dy * D
+    ddt = dd * torch.sigmoid(raw)
+    if ok is not None:
+        ddt = torch.where(ok, ddt, 0.0)
+    return [out, du, ddt, dA, dB, dC, dD, dz, ddt.sum((0, 1))]
+
+
+def _cross(s):
+    q, k, v = s["q"], s["k"], s["v"]
+    B, H, T, D = q.shape
+    Hk, M = k.shape[1], k.shape[2]
+    R = H // Hk
+    scale = D ** -0.5
+    qg, k, v = q.reshape(B, Hk, R * T, D), k.contiguous(), v.contiguous()
+    p = torch.matmul(qg, k.transpose(-1, -2).contiguous()) * scale
+    if s["lengths"] is not None:
+        ok = (torch.arange(M, device="cuda")[None] < s["lengths"][:, None])[:, None, None, :]
+        p = torch.where(ok, p, float("-inf"))
+    m = p.amax(-1, keepdim=True)
+    p = torch.exp(p - torch.where(torch.isinf(m), 0.0, m))
+    l = p.sum(-1, keepdim=True)
+    p = p / torch.where(l > 0, l, 1.0)
+    o = torch.matmul(p, v)
+    if s["form"] != "train":
+        return o.reshape(B, H, T, D)
+    g = s["g"].reshape(B, Hk, R * T, D)
+    dv = torch.matmul(p.transpose(-1, -2).contiguous(), g)
+    dp = torch.matmul(g, v.transpose(-1, -2).contiguous())
+    ds = p * (dp - (g * o).sum(-1, keepdim=True)) * scale
+    dq = torch.matmul(ds, k)
+    dk = torch.matmul(ds.transpose(-1, -2).contiguous(), qg)
+    return [o.reshape(B, H, T, D), dq.reshape(B, H, T, D), dk, dv]
+
+
+def run(state):
+    if state["own"]:
+        return _own(state)
+    return {"conv": _conv, "scan": _scan, "cross": _cross}[state["op"]](state)
+
+
+# ------------------------------------------------------------------- work
+def work(case):
+    """One pass: inputs read once, outputs written once. A scan's arithmetic per
+    state and step: decay, input and output products forward (7), and about
+    twice that backward."""
+    es = 8 if case["dtype"] == "float64" else 4
+    B, form = case["batch"], case["form"]
+    train = form == "train"
+    if case["op"] == "conv":
+        C, K = case["dim"], case["taps"]
+        if form == "step":
+            return {"bytes": es * (2 * B * C + 2 * B * (K - 1) * C + (K + 1) * C), "flops": B * C * (2 * K + 4)}
+        n = B * case["ctx"] * C
+        return {"bytes": es * (n * (4 if train else 2) + (K + 1) * C * (2 if train else 1)),
+                "flops": n * ((2 * K + 4) * (4 if train else 1))}
+    if case["op"] == "scan":
+        C, N, G = case["dim"], case["states"], case["groups"]
+        if form == "step":
+            return {"bytes": es * (4 * B * C + 2 * B * G * N + 2 * B * C * N + C * (N + 2)), "flops": 7 * B * C * N}
+        n = B * case["ctx"]
+        arrays = (4 + 4) if train else 4
+        return {"bytes": es * (n * C * arrays + n * G * N * (4 if train else 2) + C * (N + 2) * (2 if train else 1)),
+                "flops": n * C * N * (21 if train else 7)}
+    H, Hk, T, M, D = (case[x] for x in ("heads", "kvheads", "ctx", "mem", "hdim"))
+    return {"bytes": es * B * D * ((5 if train else 2) * H * T + (4 if train else 2) * Hk * M),
+            "flops": B * H * T * M * D * (14 if train else 4)}
+
+
+# ------------------------------------------------------------------ exact
+def _exact_conv(t, case):
+    x, w, b = t["x"], t["w"], t["b"]
+    K = w.shape[0]
+    silu = torch.nn.functional.silu
+    if case["form"] == "step":
+        full = torch.cat([t["state"], x[:, None]], 1)
+        return [silu(torch.einsum("bkc,kc->bc", full, w) + b), full[:, 1:].clone()]
+    leaves = [v.clone().requires_grad_(True) for v in (x, w, b)]
+    outs, states = [], []
+    for i in range(case["batch"]):
+        n = case["ctx"] if t["lengths"] is None else t["lengths"][i]
+        xi = torch.nn.functional.pad(leaves[0][i, :n], (0, 0, K - 1, 0))
+        win = xi.unfold(0, K, 1) if n else xi.new_zeros(0, case["dim"], K)
+        y = silu((win * leaves[1].T).sum(-1) + leaves[2])
+        outs.append(torch.nn.functional.pad(y, (0, 0, 0, case["ctx"] - n)))
+        states.append(xi[n:].detach())
+    y = torch.stack(outs)
+    if case["form"] == "prompt":
+        return [y.detach(), torch.stack(states)]
+    return [y.detach(), *torch.autograd.grad(y, leaves, t["g"])]
+
+
+def _doubling(a, x):
+    """h[t] = a[t] h[t-1] + x[t] along the first axis, by doubling the span."""
+    a, x, s = a.clone(), x.clone(), 1
+    while s < x.shape[0]:
+        x[s:] += a[s:] * x[:-s].clone()
+        a[s:] *= a[:-s].clone()
+        s *= 2
+    return x
+
+
+def _exact_scan(t, case):
+    C, N, G = case["dim"], case["states"], case["groups"]
+    A, D, bias = t["A"], t["D"], t["bias"]
+    each = C // G
+    if case["form"] == "step":
+        d = torch.nn.functional.softplus(t["dt"] + bias, threshold=200)
+        rep = lambda m: m.repeat_interleave(each, 1)  # noqa: E731
+        h = torch.exp(torch.einsum("bc,cn->bcn", d, A)) * t["state"] + torch.einsum("bc,bcn->bcn", d * t["u"], rep(t["B"]))
+        y = torch.einsum("bcn,bcn->bc", h, rep(t["C"])) + D * t["u"]
+        return [y * torch.nn.functional.silu(t["z"]), h]
+    T, train = case["ctx"], case["form"] == "train"
+    if case["batch"] * T * C * N > 400_000_000:
+        return None
+    names = ("u", "dt", "B", "C", "z")
+    out = torch.zeros_like(t["u"], memory_format=torch.contiguous_format)
+    state = out.new_zeros(case["batch"], C, N)
+    gr = {n: torch.zeros(t[n].shape, device="cuda", dtype=torch.float64) for n in names}
+    gA, gD, gbias = torch.zeros_like(A), torch.zeros_like(D), torch.zeros_like(bias)
+    for i in range(case["batch"]):
+        n = T if t["lengths"] is None else t["lengths"][i]
+        if n == 0:
+            continue
+        u, raw, z = t["u"][i, :n], t["dt"][i, :n] + bias, t["z"][i, :n]
+        Bm, Cm = (t[k][i, :n].repeat_interleave(each, 1) for k in "BC")
+        d = torch.nn.functional.softplus(raw, threshold=200)
+        a = torch.exp(d[..., None] * A)
+        h = _doubling(a, (d * u)[..., None] * Bm)
+        y = (h * Cm).sum(-1) + D * u
+        out[i, :n] = y * torch.nn.functional.silu(z)
+        state[i] = h[-1]
+        if not train:
+            continue
+        g, sg = t["g"][i, :n], torch.sigmoid(z)
+        gr["z"][i, :n] = g * y * sg * (1 + z * (1 - sg))
+        dy = g * z * sg
+        back = torch.cat([a[1:], a.new_zeros(1, C, N)]).flip(0)
+        dh = _doubling(back, (dy[..., None] * Cm).flip(0)).flip(0)
+        gr["C"][i, :n] = (dy[..., None] * h).reshape(n, G, each, N).sum(2)
+        gr["B"][i, :n] = (dh * (d * u)[..., None]).reshape(n, G, each, N).sum(2)
+        into = (dh * Bm).sum(-1)
+        q = dh * a * torch.cat([h.new_zeros(1, C, N), h[:-1]])
+        gr["u"][i, :n] = into * d + dy * D
+        dd = ((q * A).sum(-1) + into * u) * torch.sigmoid(raw)
+        gr["dt"][i, :n] = dd
+        gA += (q * d[..., None]).sum(0)
+        gD += (dy * u).sum(0)
+        gbias += dd.sum(0)
+    if not train:
+        return [out, state]
+    return [out, gr["u"], gr["dt"], gA, gr["B"], gr["C"], gD, gr["z"], gbias]
+
+
+def _exact_cross(t, case):
+    R = case["heads"] // case["kvheads"]
+    train = case["form"] == "train"
+    outs, grads = [], [[], [], []]
+    for i in range(case["batch"]):
+        n = case["mem"] if t["lengths"] is None else t["lengths"][i]
+        q, k, v = (t[x][i].contiguous().requires_grad_(train) for x in "qkv")
+        kr, vr = (x[:, :n].repeat_interleave(R, 0).contiguous() for x in (k, v))
+        sc = torch.matmul(q, kr.transpose(1, 2).contiguous()) / math.sqrt(case["hdim"])
+        o = torch.matmul(torch.softmax(sc, -1), vr)
+        outs.append(o.detach())
+        if train:
+            for acc, x in zip(grads, torch.autograd.grad(o, (q, k, v), t["g"][i])):
+                acc.append(x)
+    if not train:
+        return torch.stack(outs)
+    return [torch.stack(outs)] + [torch.stack(x) for x in grads]
+
+
+def exact(case, seed):
+    t = {k: v.double() if torch.is_tensor(v) else v for k, v in _inputs(case, seed).items()}
+    return {"conv": _exact_conv, "scan": _exact_scan, "cross": _exact_cross}[case["op"]](t, case)
