@@ -220,6 +220,7 @@ def prepare(case, seed):
     s = {"op": case["op"], "form": case["form"], "own": own}
     if own:
         A, dev = _dtmi()
+        s["dtmi"] = A
         for k, v in t.items():
             if k == "lengths":
                 s[k] = None if v is None else A.Indices(v)
@@ -235,7 +236,7 @@ def prepare(case, seed):
 
 
 def _own(s):
-    A, _ = _dtmi()
+    A = s["dtmi"]
     op, form = s["op"], s["form"]
     if form == "train":
         def leaf(name):
