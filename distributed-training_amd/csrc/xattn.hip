@@ -1,0 +1,799 @@
+// Attention to another sequence's states: o = softmax(q k^T scale) v over the
+// first lengths[b] of Tk keys, with H query heads sharing Hk key/value heads
+// (head h reads h / (H / Hk)). A row whose memory is empty is 0 and passes
+// no gradient; keys past the length are never read.
+//
+// The queries of all heads that share a key/value head form one matrix of
+// R = (H / Hk) Tq rows (row r: head r / Tq of the group, query r % Tq), so one
+// query token with shared heads fills the columns of a matrix tile, and dK and
+// dV sum over the heads that share them in the loop over rows, without atomics.
+//
+// Tiles of 16 x 16 x 4 MFMAs in the transposed formulation of the causal
+// kernels: the operand a wave owns (queries in the forward and the dQ pass,
+// keys in the dK/dV pass) is the tile's columns and stays in registers; the
+// other operand passes through LDS, shared by the block's four waves. A
+// result register i of lane group g then is what that lane feeds to the next
+// product as its slot g of step i, with the other operand read from LDS at row
+// row(i, g).
+//
+// Forward: scores in base 2, a reference maximum per query that moves only
+// when a score exceeds it by 2^8, sum and output rescaled then. Backward: the
+// probabilities from the forward's reference and sum (the same products in the
+// same order, so the same scores), dV += P^T dO, dP = dO V^T, dS = P (dP -
+// rowsum(dO O)), dK += dS^T Q in the pass over keys; S, dP and dQ = dS K in
+// the pass over queries.
+//
+// Few rows or few keys give few blocks: the loop (over keys in the forward and
+// the dQ pass, over rows in the dK/dV pass) is then split over blocks, whose
+// partial results a small kernel joins in a fixed order.
+#include <cmath>
+
+#include "common.h"
+
+namespace dtmi {
+
+template <typename T>
+struct XM;
+template <>
+struct XM<float> {
+  static constexpr int VEC = 4, PAD = 4;
+  typedef float acc_t __attribute__((ext_vector_type(4)));
+  typedef float vec_t __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ acc_t mma(float a, float b, acc_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int i, int g) { return 4 * g + i; }
+  static __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+  static constexpr float lowest = -3.40282347e38f;
+};
+template <>
+struct XM<double> {
+  static constexpr int VEC = 2, PAD = 2;
+  typedef double acc_t __attribute__((ext_vector_type(4)));
+  typedef double vec_t __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ acc_t mma(double a, double b, acc_t c) {
+    return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ int row(int i, int g) { return g + 4 * i; }
+  static __device__ __forceinline__ double ex2(double x) { return exp2(x); }
+  static constexpr double lowest = -1.7976931348623157e308;
+};
+
+struct HT {
+  int64_t b, h, t;
+};
+
+struct XArgs {
+  const void *q, *k, *v, *o, *dO;
+  void *out, *dq, *dk, *dv;
+  void *rowmax, *rowsum;  // [B, H, Tq]: the reference maximum (base 2) and the sum against it
+  void* drow;             // [B, H, Tq]: rowsum(dO O)
+  void *po, *pm, *pl;     // partial results of a split loop
+  const int64_t* lengths;
+  HT sq, sk, sv, so, sdo, sdq, sdk, sdv;
+  int64_t B, H, Hk, Tq, Tk, D, R;
+  double scale;
+  int nsplit;   // parts of the loop
+  int ntile;    // blocks along the owned axis
+  int64_t per;  // loop positions per part, a multiple of the tile
+  int vec;      // 16-byte loads and stores allowed for every operand
+};
+
+__device__ __forceinline__ int64_t key_count(const XArgs& a, int64_t b) {
+  if (!a.lengths) return a.Tk;
+  const int64_t n = a.lengths[b];
+  return n < 0 ? 0 : n > a.Tk ? a.Tk : n;
+}
+
+// Element offset of row r of the group's rows (head and query) in an array with strides s
+__device__ __forceinline__ int64_t row_at(const XArgs& a, const HT& s, int64_t b, int64_t kh, int64_t r) {
+  const int64_t h = kh * (a.H / a.Hk) + r / a.Tq;
+  return b * s.b + h * s.h + (r % a.Tq) * s.t;
+}
+__device__ __forceinline__ int64_t stat_at(const XArgs& a, int64_t b, int64_t kh, int64_t r) {
+  return (b * a.H + kh * (a.H / a.Hk)) * a.Tq + r;
+}
+
+// A lane's slice of one row as MFMA operand: element e of vector f is
+// d = 4 VEC f + VEC g + e, so the lane groups' reads of a row are contiguous.
+template <typename T, int DP>
+__device__ __forceinline__ void load_slice(typename XM<T>::vec_t (&f)[DP / (4 * XM<T>::VEC)], const T* __restrict__ row,
+                                           bool in, int D, int g, bool vec) {
+  constexpr int VEC = XM<T>::VEC;
+  typedef typename XM<T>::vec_t VT;
+#pragma unroll
+  for (int i = 0; i < DP / (4 * VEC); ++i) {
+    const int d = 4 * VEC * i + VEC * g;
+    VT x = VT(0);
+    if (vec) {
+      if (in && d < D) x = *reinterpret_cast<const VT*>(row + d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (in && d + e < D) x[e] = row[d + e];
+    }
+    f[i] = x;
+  }
+}
+
+// NR rows of a tile on their way from global memory to LDS [NR][DP + PAD];
+// rows that do not exist and columns at and past D are zero.
+template <typename T, int NR, int DP>
+struct Rows {
+  typedef typename XM<T>::vec_t VT;
+  static constexpr int VEC = XM<T>::VEC, LD = DP + XM<T>::PAD, NV = NR * DP / VEC / 256;
+  static_assert(NR * DP % (VEC * 256) == 0, "whole vectors per thread");
+  VT x[NV];
+  // base(r): element pointer of row r of the tile, or NULL
+  template <typename F>
+  __device__ __forceinline__ void fetch(const F& base, int D, bool vec) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int f = threadIdx.x + 256 * i, r = f / (DP / VEC), d = f % (DP / VEC) * VEC;
+      const T* p = base(r);
+      VT v = VT(0);
+      if (vec) {
+        if (p && d < D) v = *reinterpret_cast<const VT*>(p + d);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (p && d + e < D) v[e] = p[d + e];
+      }
+      x[i] = v;
+    }
+  }
+  __device__ __forceinline__ void put(T* __restrict__ lds) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int f = threadIdx.x + 256 * i, r = f / (DP / VEC), d = f % (DP / VEC) * VEC;
+      *reinterpret_cast<VT*>(lds + r * LD + d) = x[i];
+    }
+  }
+};
+
+// 16 x 16 tile += rows r0 .. r0 + 15 of LDS times the lane's slice
+template <typename T, int DP>
+__device__ __forceinline__ typename XM<T>::acc_t mul_rows(const T* __restrict__ lds, int r0,
+                                                          const typename XM<T>::vec_t (&f)[DP / (4 * XM<T>::VEC)], int g,
+                                                          int c) {
+  constexpr int VEC = XM<T>::VEC, LD = DP + XM<T>::PAD;
+  typename XM<T>::acc_t acc = typename XM<T>::acc_t(0);
+#pragma unroll
+  for (int i = 0; i < DP / (4 * VEC); ++i) {
+    const typename XM<T>::vec_t x =
+        *reinterpret_cast<const typename XM<T>::vec_t*>(lds + (r0 + c) * LD + 4 * VEC * i + VEC * g);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc = XM<T>::mma(x[e], f[i][e], acc);
+  }
+  return acc;
+}
+
+// out^T (d = N m + t by column) += sum over a tile's 16 rows of LDS[row][d] p(row, column)
+template <typename T, int DP, int CT>
+__device__ __forceinline__ void mul_cols(typename XM<T>::acc_t (&out)[CT][DP / 16], const T* __restrict__ lds, int r0,
+                                         const typename XM<T>::acc_t (&p)[CT], int g, int c) {
+  constexpr int N = DP / 16, VEC = XM<T>::VEC, LD = DP + XM<T>::PAD;
+  typedef typename XM<T>::vec_t VT;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    T x[N];
+    const T* row = lds + (r0 + XM<T>::row(i, g)) * LD + N * c;
+    if constexpr (N % VEC == 0) {
+#pragma unroll
+      for (int v = 0; v < N / VEC; ++v) {
+        const VT y = *reinterpret_cast<const VT*>(row + VEC * v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[VEC * v + e] = y[e];
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < N; ++t) x[t] = row[t];
+    }
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int u = 0; u < CT; ++u) out[u][t] = XM<T>::mma(x[t], p[u][i], out[u][t]);
+  }
+}
+
+// The lane's part of a result row: registers (t, i) are d = N row(i, g) + t
+template <typename T, int DP>
+__device__ __forceinline__ void put_row(T* __restrict__ row, const typename XM<T>::acc_t (&x)[DP / 16], T mul, int D,
+                                        int g, bool vec) {
+  constexpr int N = DP / 16, VEC = XM<T>::VEC;
+  typedef typename XM<T>::vec_t VT;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = N * XM<T>::row(i, g);
+    if constexpr (N % VEC == 0) {
+      if (vec) {
+#pragma unroll
+        for (int v = 0; v < N / VEC; ++v) {
+          VT y;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) y[e] = x[VEC * v + e][i] * mul;
+          if (d + VEC * v < D) *reinterpret_cast<VT*>(row + d + VEC * v) = y;
+        }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+      if (d + t < D) row[d + t] = x[t][i] * mul;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T over_groups_max(T x) {
+  x = fmax(x, __shfl_xor(x, 16, 64));
+  return fmax(x, __shfl_xor(x, 32, 64));
+}
+template <typename T>
+__device__ __forceinline__ T over_groups_sum(T x) {
+  x = x + __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+struct XBlock {
+  int64_t b, kh;
+  int tile, split;
+};
+__device__ __forceinline__ XBlock x_block(const XArgs& a) {
+  const int64_t id = blockIdx.x;
+  XBlock k;
+  k.tile = (int)(id % a.ntile);
+  const int64_t r = id / a.ntile;
+  k.split = (int)(r % a.nsplit);
+  const int64_t bh = r / a.nsplit;
+  k.b = bh / a.Hk;
+  k.kh = bh % a.Hk;
+  return k;
+}
+
+constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
+
+template <typename T, int DP, int CT>
+__global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
+  using M = XM<T>;
+  typedef typename M::acc_t AT;
+  typedef typename M::vec_t VT;
+  constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys;
+  __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const XBlock k = x_block(a);
+  const int64_t len = key_count(a, k.b);
+  const int64_t lo = k.split * a.per, hi = lo + a.per < len ? lo + a.per : len;
+  const int64_t r0 = ((int64_t)k.tile * 4 + w) * 16 * CT;
+  const bool vec = a.vec != 0;
+  VT qf[CT][DP / (4 * M::VEC)];
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const int64_t r = r0 + 16 * u + c;
+    load_slice<T, DP>(qf[u], (const T*)a.q + (r < a.R ? row_at(a, a.sq, k.b, k.kh, r) : 0), r < a.R, D, g, vec);
+  }
+  const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
+  const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
+  Rows<T, KT, DP> fk, fv;
+  auto fetch = [&](int64_t j0) {
+    fk.fetch([&](int r) { return j0 + r < hi ? Kb + (j0 + r) * a.sk.t : nullptr; }, D, vec);
+    fv.fetch([&](int r) { return j0 + r < hi ? Vb + (j0 + r) * a.sv.t : nullptr; }, D, vec);
+  };
+  const T sl2 = (T)(a.scale * 1.4426950408889634);
+  AT o[CT][N];
+  T mref[CT], l[CT];
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    mref[u] = M::lowest;
+    l[u] = T(0);
+#pragma unroll
+    for (int t = 0; t < N; ++t) o[u][t] = AT(0);
+  }
+  const bool busy = r0 < a.R;
+  if (lo < hi) fetch(lo);
+  for (int64_t j0 = lo; j0 < hi; j0 += KT) {
+    __syncthreads();
+    fk.put(Ks);
+    fv.put(Vs);
+    __syncthreads();
+    if (j0 + KT < hi) fetch(j0 + KT);
+    if (!busy) continue;
+#pragma unroll
+    for (int kt = 0; kt < KT / 16; ++kt) {
+      AT p[CT];
+#pragma unroll
+      for (int u = 0; u < CT; ++u) {
+        AT s = mul_rows<T, DP>(Ks, 16 * kt, qf[u], g, c) * sl2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = j0 + 16 * kt + M::row(i, g) < hi ? s[i] : -INFINITY;
+        const T top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
+        if (__any(top > mref[u] + T(8))) {
+          const T next = fmax(mref[u], over_groups_max(top));
+          const T alpha = M::ex2(mref[u] - next);
+          l[u] = l[u] * alpha;
+#pragma unroll
+          for (int t = 0; t < N; ++t) o[u][t] *= alpha;
+          mref[u] = next;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[i] = M::ex2(s[i] - mref[u]);
+          l[u] = l[u] + s[i];
+        }
+        p[u] = s;
+      }
+      mul_cols<T, DP, CT>(o, Vs, 16 * kt, p, g, c);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const int64_t r = r0 + 16 * u + c;
+    const T sum = over_groups_sum(l[u]);
+    if (r >= a.R) continue;
+    if (a.nsplit > 1) {
+      const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
+      put_row<T, DP>((T*)a.po + at * DP, o[u], T(1), DP, g, true);
+      if (g == 0) {
+        ((T*)a.pm)[at] = mref[u];
+        ((T*)a.pl)[at] = sum;
+      }
+      continue;
+    }
+    put_row<T, DP>((T*)a.out + row_at(a, a.so, k.b, k.kh, r), o[u], sum == T(0) ? T(0) : T(1) / sum, D, g, vec);
+    if (g == 0 && a.rowmax) {
+      const int64_t at = stat_at(a, k.b, k.kh, r);
+      ((T*)a.rowmax)[at] = mref[u];
+      ((T*)a.rowsum)[at] = sum;
+    }
+  }
+}
+
+// Joins the forward's parts: a wave per row, lanes over d.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), r = id % a.R, bh = id / a.R;
+  if (bh >= a.B * a.Hk) return;
+  const int lane = threadIdx.x & 63;
+  const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * a.nsplit * a.R + r;
+  const T* pm = (const T*)a.pm + at;
+  const T* pl = (const T*)a.pl + at;
+  const T* po = (const T*)a.po + at * DP;
+  T top = XM<T>::lowest, sum = T(0);
+  for (int s = 0; s < a.nsplit; ++s) top = fmax(top, pm[s * a.R]);
+  constexpr int PER = (DP + 63) / 64;
+  T o[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = T(0);
+  for (int s = 0; s < a.nsplit; ++s) {
+    const T wt = pm[s * a.R] == top ? T(1) : XM<T>::ex2(pm[s * a.R] - top);
+    sum = fma(pl[s * a.R], wt, sum);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int d = lane + 64 * e;
+      if (d < DP) o[e] = fma(po[s * a.R * DP + d], wt, o[e]);
+    }
+  }
+  const T inv = sum == T(0) ? T(0) : T(1) / sum;
+  T* out = (T*)a.out + row_at(a, a.so, b, kh, r);
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int d = lane + 64 * e;
+    if (d < a.D) out[d] = o[e] * inv;
+  }
+  if (lane == 0 && a.rowmax) {
+    ((T*)a.rowmax)[stat_at(a, b, kh, r)] = top;
+    ((T*)a.rowsum)[stat_at(a, b, kh, r)] = sum;
+  }
+}
+
+// rowsum(dO O): 16 lanes per row
+template <typename T>
+__global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
+  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), r = id % a.R, bh = id / a.R;
+  const bool on = bh < a.B * a.Hk;
+  T s = T(0);
+  if (on) {
+    const int64_t b = bh / a.Hk, kh = bh % a.Hk;
+    const T* o = (const T*)a.o + row_at(a, a.so, b, kh, r);
+    const T* g = (const T*)a.dO + row_at(a, a.sdo, b, kh, r);
+    for (int d = threadIdx.x & 15; d < a.D; d += 16) s = fma(o[d], g[d], s);
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) s = s + __shfl_xor(s, m, 64);
+  if (on && (threadIdx.x & 15) == 0) ((T*)a.drow)[stat_at(a, bh / a.Hk, bh % a.Hk, r)] = s;
+}
+
+// dQ: a wave owns 16 CT rows and loops over the keys of its part.
+template <typename T, int DP, int CT>
+__global__ void __launch_bounds__(256) xattn_bwd_q_kernel(XArgs a) {
+  using M = XM<T>;
+  typedef typename M::acc_t AT;
+  typedef typename M::vec_t VT;
+  constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys, NF = DP / (4 * M::VEC);
+  __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const XBlock k = x_block(a);
+  const int64_t len = key_count(a, k.b);
+  const int64_t lo = k.split * a.per, hi = lo + a.per < len ? lo + a.per : len;
+  const int64_t r0 = ((int64_t)k.tile * 4 + w) * 16 * CT;
+  const bool vec = a.vec != 0;
+  VT qf[CT][NF], gf[CT][NF];
+  T m[CT], inv[CT], dr[CT];
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const int64_t r = r0 + 16 * u + c;
+    const bool in = r < a.R;
+    load_slice<T, DP>(qf[u], (const T*)a.q + (in ? row_at(a, a.sq, k.b, k.kh, r) : 0), in, D, g, vec);
+    load_slice<T, DP>(gf[u], (const T*)a.dO + (in ? row_at(a, a.sdo, k.b, k.kh, r) : 0), in, D, g, vec);
+    const int64_t at = stat_at(a, k.b, k.kh, in ? r : 0);
+    const T sum = ((const T*)a.rowsum)[at];
+    m[u] = ((const T*)a.rowmax)[at];
+    inv[u] = !in || sum == T(0) ? T(0) : T(1) / sum;
+    dr[u] = ((const T*)a.drow)[at];
+  }
+  const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
+  const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
+  Rows<T, KT, DP> fk, fv;
+  auto fetch = [&](int64_t j0) {
+    fk.fetch([&](int r) { return j0 + r < hi ? Kb + (j0 + r) * a.sk.t : nullptr; }, D, vec);
+    fv.fetch([&](int r) { return j0 + r < hi ? Vb + (j0 + r) * a.sv.t : nullptr; }, D, vec);
+  };
+  const T sl2 = (T)(a.scale * 1.4426950408889634);
+  AT dq[CT][N];
+#pragma unroll
+  for (int u = 0; u < CT; ++u)
+#pragma unroll
+    for (int t = 0; t < N; ++t) dq[u][t] = AT(0);
+  const bool busy = r0 < a.R;
+  if (lo < hi) fetch(lo);
+  for (int64_t j0 = lo; j0 < hi; j0 += KT) {
+    __syncthreads();
+    fk.put(Ks);
+    fv.put(Vs);
+    __syncthreads();
+    if (j0 + KT < hi) fetch(j0 + KT);
+    if (!busy) continue;
+#pragma unroll
+    for (int kt = 0; kt < KT / 16; ++kt) {
+      AT ds[CT];
+#pragma unroll
+      for (int u = 0; u < CT; ++u) {
+        const AT s = mul_rows<T, DP>(Ks, 16 * kt, qf[u], g, c) * sl2;
+        const AT dp = mul_rows<T, DP>(Vs, 16 * kt, gf[u], g, c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = j0 + 16 * kt + M::row(i, g) < hi;
+          ds[u][i] = in && inv[u] != T(0) ? M::ex2(s[i] - m[u]) * inv[u] * (dp[i] - dr[u]) : T(0);
+        }
+      }
+      mul_cols<T, DP, CT>(dq, Ks, 16 * kt, ds, g, c);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const int64_t r = r0 + 16 * u + c;
+    if (r >= a.R) continue;
+    if (a.nsplit > 1) {
+      const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
+      put_row<T, DP>((T*)a.po + at * DP, dq[u], (T)a.scale, DP, g, true);
+    } else {
+      put_row<T, DP>((T*)a.dq + row_at(a, a.sdq, k.b, k.kh, r), dq[u], (T)a.scale, D, g, vec);
+    }
+  }
+}
+
+// dK and dV: a wave owns 16 CT keys and loops over the rows of its part.
+template <typename T, int DP, int CT>
+__global__ void __launch_bounds__(256) xattn_bwd_kv_kernel(XArgs a) {
+  using M = XM<T>;
+  typedef typename M::acc_t AT;
+  typedef typename M::vec_t VT;
+  constexpr int N = DP / 16, LD = DP + M::PAD, QT = kKeys, NF = DP / (4 * M::VEC);
+  __shared__ __attribute__((aligned(16))) T Qs[QT * LD], Gs[QT * LD];
+  __shared__ T sm[QT], si[QT], sr[QT];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const XBlock k = x_block(a);
+  const int64_t len = key_count(a, k.b);
+  const int64_t lo = k.split * a.per, hi = lo + a.per < a.R ? lo + a.per : a.R;
+  const int64_t j0 = ((int64_t)k.tile * 4 + w) * 16 * CT;
+  const bool vec = a.vec != 0;
+  const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
+  const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
+  VT kf[CT][NF], vf[CT][NF];
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const int64_t j = j0 + 16 * u + c;
+    load_slice<T, DP>(kf[u], Kb + (j < len ? j : 0) * a.sk.t, j < len, D, g, vec);
+    load_slice<T, DP>(vf[u], Vb + (j < len ? j : 0) * a.sv.t, j < len, D, g, vec);
+  }
+  Rows<T, QT, DP> fq, fg;
+  T nm = T(0), ni = T(0), nr = T(0);
+  auto fetch = [&](int64_t r0) {
+    fq.fetch([&](int r) { return r0 + r < hi ? (const T*)a.q + row_at(a, a.sq, k.b, k.kh, r0 + r) : nullptr; }, D, vec);
+    fg.fetch([&](int r) { return r0 + r < hi ? (const T*)a.dO + row_at(a, a.sdo, k.b, k.kh, r0 + r) : nullptr; }, D,
+             vec);
+    if (threadIdx.x < QT) {
+      const bool in = r0 + threadIdx.x < hi;
+      const int64_t at = stat_at(a, k.b, k.kh, in ? r0 + threadIdx.x : 0);
+      const T sum = in ? ((const T*)a.rowsum)[at] : T(0);
+      nm = ((const T*)a.rowmax)[at];
+      ni = sum == T(0) ? T(0) : T(1) / sum;
+      nr = ((const T*)a.drow)[at];
+    }
+  };
+  const T sl2 = (T)(a.scale * 1.4426950408889634);
+  AT dk[CT][N], dv[CT][N];
+#pragma unroll
+  for (int u = 0; u < CT; ++u)
+#pragma unroll
+    for (int t = 0; t < N; ++t) dk[u][t] = dv[u][t] = AT(0);
+  // a block past the sequence's keys has only zeros to write
+  const bool any = (int64_t)k.tile * 64 * CT < len, busy = j0 < len;
+  if (any && lo < hi) fetch(lo);
+  for (int64_t r0 = lo; any && r0 < hi; r0 += QT) {
+    __syncthreads();
+    fq.put(Qs);
+    fg.put(Gs);
+    if (threadIdx.x < QT) {
+      sm[threadIdx.x] = nm;
+      si[threadIdx.x] = ni;
+      sr[threadIdx.x] = nr;
+    }
+    __syncthreads();
+    if (r0 + QT < hi) fetch(r0 + QT);
+    if (!busy) continue;
+#pragma unroll
+    for (int qt = 0; qt < QT / 16; ++qt) {
+      AT p[CT], ds[CT];
+#pragma unroll
+      for (int u = 0; u < CT; ++u) {
+        const AT s = mul_rows<T, DP>(Qs, 16 * qt, kf[u], g, c) * sl2;
+        const AT dp = mul_rows<T, DP>(Gs, 16 * qt, vf[u], g, c);
+        const bool in = j0 + 16 * u + c < len;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * qt + M::row(i, g);
+          const bool on = in && si[r] != T(0);
+          p[u][i] = on ? M::ex2(s[i] - sm[r]) * si[r] : T(0);
+          ds[u][i] = on ? p[u][i] * (dp[i] - sr[r]) : T(0);
+        }
+      }
+      mul_cols<T, DP, CT>(dv, Gs, 16 * qt, p, g, c);
+      mul_cols<T, DP, CT>(dk, Qs, 16 * qt, ds, g, c);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < CT; ++u) {
+    const int64_t j = j0 + 16 * u + c;
+    if (j >= a.Tk) continue;
+    if (a.nsplit > 1) {
+      const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.Tk + j;
+      put_row<T, DP>((T*)a.po + at * DP, dk[u], (T)a.scale, DP, g, true);
+      put_row<T, DP>((T*)a.pm + at * DP, dv[u], T(1), DP, g, true);
+    } else {
+      put_row<T, DP>((T*)a.dk + k.b * a.sdk.b + k.kh * a.sdk.h + j * a.sdk.t, dk[u], (T)a.scale, D, g, vec);
+      put_row<T, DP>((T*)a.dv + k.b * a.sdv.b + k.kh * a.sdv.h + j * a.sdv.t, dv[u], T(1), D, g, vec);
+    }
+  }
+}
+
+// Sums the parts of dQ (rows: the group's) or of dK and dV (blockIdx.y 0, 1; rows: keys).
+template <typename T, int DP, bool KV>
+__global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
+  const int64_t rows = KV ? a.Tk : a.R, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t d = id % DP, r = id / DP % rows, bh = id / DP / rows;
+  if (bh >= a.B * a.Hk || d >= a.D) return;
+  const int64_t b = bh / a.Hk, kh = bh % a.Hk;
+  const T* p = (const T*)(KV && blockIdx.y ? a.pm : a.po) + (bh * a.nsplit * rows + r) * DP + d;
+  T s = T(0);
+  for (int i = 0; i < a.nsplit; ++i) s = s + p[(int64_t)i * rows * DP];
+  if constexpr (KV) {
+    if (blockIdx.y)
+      ((T*)a.dv)[b * a.sdv.b + kh * a.sdv.h + r * a.sdv.t + d] = s;
+    else
+      ((T*)a.dk)[b * a.sdk.b + kh * a.sdk.h + r * a.sdk.t + d] = s;
+  } else {
+    ((T*)a.dq)[row_at(a, a.sdq, b, kh, r) + d] = s;
+  }
+}
+
+// Blocks along the owned axis, and the parts of the loop over `loop` positions:
+// more than one where the card would have fewer than two blocks per CU, of at
+// least two tiles each.
+static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop) {
+  const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = 2 * (int64_t)num_cus();
+  const int64_t steps = cdiv(loop, kKeys);
+  int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
+  if (s > steps / 2) s = steps / 2;
+  if (s < 1) s = 1;
+  a.per = cdiv(steps > 0 ? steps : 1, s) * kKeys;
+  a.nsplit = loop > 0 ? (int)cdiv(loop, a.per) : 1;
+  DTMI_CHECK(tiles <= 0x7fffffff && blocks * a.nsplit <= 0x7fffffff, "cross attention: too many elements");
+  a.ntile = (int)tiles;
+  return DTMI_OK;
+}
+
+#define X_LAUNCH(KERNEL, CTV)                                                     \
+  {                                                                               \
+    const unsigned grid = (unsigned)(a.B * a.Hk * a.nsplit * a.ntile);            \
+    KERNEL<T, DP, CTV><<<grid, 256, 0, stream()>>>(a);                            \
+  }
+
+template <typename T, int DP>
+static int x_fwd(XArgs& a) {
+  constexpr int WIDE = sizeof(T) == 4 ? 2 : 1;
+  const bool wide = WIDE > 1 && a.R > 64;
+  if (int rc = plan(a, a.R, wide ? 64 * WIDE : 64, a.Tk)) return rc;
+  void* ws = nullptr;
+  if (a.nsplit > 1) {
+    const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.R;
+    if (int rc = pool_alloc(&ws, n * (DP + 2) * sizeof(T))) return rc;
+    a.po = ws;
+    a.pm = (T*)ws + n * DP;
+    a.pl = (T*)a.pm + n;
+  }
+  if (wide)
+    X_LAUNCH(xattn_fwd_kernel, WIDE)
+  else
+    X_LAUNCH(xattn_fwd_kernel, 1)
+  if (a.nsplit > 1) xattn_join_kernel<T, DP><<<(unsigned)cdiv(a.B * a.Hk * a.R, 4), 256, 0, stream()>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (ws) pool_free(ws);
+  return e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_fwd", __FILE__, __LINE__);
+}
+
+template <typename T, int DP>
+static int x_bwd_kv(XArgs& a) {
+  constexpr int CT = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
+  if (int rc = plan(a, a.Tk, 64 * CT, a.R)) return rc;
+  void* ws = nullptr;
+  if (a.nsplit > 1) {
+    const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.Tk * DP;
+    if (int rc = pool_alloc(&ws, 2 * n * sizeof(T))) return rc;
+    a.po = ws;
+    a.pm = (T*)ws + n;
+  }
+  X_LAUNCH(xattn_bwd_kv_kernel, CT)
+  if (a.nsplit > 1)
+    xattn_sum_kernel<T, DP, true>
+        <<<dim3((unsigned)cdiv(a.B * a.Hk * a.Tk * DP, 256), 2), 256, 0, stream()>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (ws) pool_free(ws);
+  return e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_bwd: dK, dV", __FILE__, __LINE__);
+}
+
+template <typename T, int DP>
+static int x_bwd_q(XArgs& a) {
+  constexpr int CT = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
+  if (int rc = plan(a, a.R, 64 * CT, a.Tk)) return rc;
+  void* ws = nullptr;
+  if (a.nsplit > 1) {
+    if (int rc = pool_alloc(&ws, (size_t)a.B * a.Hk * a.nsplit * a.R * DP * sizeof(T))) return rc;
+    a.po = ws;
+  }
+  X_LAUNCH(xattn_bwd_q_kernel, CT)
+  if (a.nsplit > 1)
+    xattn_sum_kernel<T, DP, false><<<(unsigned)cdiv(a.B * a.Hk * a.R * DP, 256), 256, 0, stream()>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (ws) pool_free(ws);
+  return e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_bwd: dQ", __FILE__, __LINE__);
+}
+#undef X_LAUNCH
+
+template <typename T, int DP>
+static int x_bwd(XArgs& a) {
+  void* dr = nullptr;
+  if (int rc = pool_alloc(&dr, (size_t)a.B * a.H * a.Tq * sizeof(T))) return rc;
+  a.drow = dr;
+  xattn_drow_kernel<T><<<(unsigned)cdiv(a.B * a.Hk * a.R, 16), 256, 0, stream()>>>(a);
+  const hipError_t e = hipGetLastError();
+  int rc = e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_bwd: row dots", __FILE__, __LINE__);
+  if (rc == DTMI_OK) rc = x_bwd_kv<T, DP>(a);
+  if (rc == DTMI_OK) rc = x_bwd_q<T, DP>(a);
+  pool_free(dr);
+  return rc;
+}
+
+template <typename T>
+static int x_dispatch(XArgs& a, bool bwd) {
+  if (a.D <= 32) return bwd ? x_bwd<T, 32>(a) : x_fwd<T, 32>(a);
+  if (a.D <= 64) return bwd ? x_bwd<T, 64>(a) : x_fwd<T, 64>(a);
+  if (a.D <= 96) return bwd ? x_bwd<T, 96>(a) : x_fwd<T, 96>(a);
+  return bwd ? x_bwd<T, 128>(a) : x_fwd<T, 128>(a);
+}
+
+static int x_shape(const char* what, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D) {
+  DTMI_CHECK(dtype == DTMI_F32 || dtype == DTMI_F64, "%s: dtype must be DTMI_F32 or DTMI_F64 (got %d)", what, dtype);
+  DTMI_CHECK(B >= 0 && H >= 0 && Tq >= 0 && Tk >= 0, "%s: negative size", what);
+  DTMI_CHECK(Hk >= 1 && H % Hk == 0, "%s: %lld heads do not share %lld key/value heads", what, (long long)H,
+             (long long)Hk);
+  DTMI_CHECK(D >= 1 && D <= 128, "%s: head dimension 1 to 128 (got %lld)", what, (long long)D);
+  DTMI_CHECK(B * H * Tq < ((int64_t)1 << 31) && B * Hk * Tk * 128 < ((int64_t)1 << 38), "%s: too many elements", what);
+  return DTMI_OK;
+}
+
+static HT ht(const int64_t* s) { return s ? HT{s[0], s[1], s[2]} : HT{0, 0, 0}; }
+template <typename T>
+static bool x_vec(const void* p, const HT& s) {
+  constexpr int V = 16 / sizeof(T);
+  return aligned(p, 16) && s.b % V == 0 && s.h % V == 0 && s.t % V == 0;
+}
+
+template <typename T>
+static int x_zero_rows(void* p, const HT& s, int64_t B, int64_t H, int64_t T_, int64_t D) {
+  const int64_t shape[4] = {B, H, T_, D}, to[4] = {s.b, s.h, s.t, 1}, from[4] = {0, 0, 0, 0};
+  void* zero = nullptr;
+  if (int rc = pool_alloc(&zero, sizeof(T))) return rc;
+  const int dt = sizeof(T) == 4 ? DTMI_F32 : DTMI_F64;
+  int rc = dtmi_fill(dt, zero, 0.0, 1);
+  if (rc == DTMI_OK) rc = dtmi_copy_strided(dt, p, to, zero, from, 4, shape);
+  pool_free(zero);
+  return rc;
+}
+
+template <typename T>
+static int xattn_fwd(XArgs& a) {
+  a.vec = a.D % (16 / sizeof(T)) == 0 && x_vec<T>(a.q, a.sq) && x_vec<T>(a.k, a.sk) && x_vec<T>(a.v, a.sv) &&
+          x_vec<T>(a.out, a.so);
+  return x_dispatch<T>(a, false);
+}
+template <typename T>
+static int xattn_bwd(XArgs& a) {
+  if (a.R == 0 || a.Tk == 0) {
+    int rc = DTMI_OK;
+    if (a.R > 0) rc = x_zero_rows<T>(a.dq, a.sdq, a.B, a.H, a.Tq, a.D);
+    if (rc == DTMI_OK && a.Tk > 0) rc = x_zero_rows<T>(a.dk, a.sdk, a.B, a.Hk, a.Tk, a.D);
+    if (rc == DTMI_OK && a.Tk > 0) rc = x_zero_rows<T>(a.dv, a.sdv, a.B, a.Hk, a.Tk, a.D);
+    return rc;
+  }
+  a.vec = a.D % (16 / sizeof(T)) == 0 && x_vec<T>(a.q, a.sq) && x_vec<T>(a.k, a.sk) && x_vec<T>(a.v, a.sv) &&
+          x_vec<T>(a.dO, a.sdo) && x_vec<T>(a.dq, a.sdq) && x_vec<T>(a.dk, a.sdk) && x_vec<T>(a.dv, a.sdv);
+  return x_dispatch<T>(a, true);
+}
+
+}  // namespace dtmi
+
+using namespace dtmi;
+
+DTMI_EXPORT int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D,
+                               double scale, const void* q, const int64_t* q_strides, const void* k,
+                               const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                               const int64_t* lengths, void* o, const int64_t* o_strides, void* rowmax, void* rowsum) {
+  DTMI_BODY_BEGIN
+  DTMI_REQUIRE_INIT();
+  if (int rc = x_shape("dtmi_xattn_fwd", dtype, B, H, Hk, Tq, Tk, D)) return rc;
+  if (B == 0 || H == 0 || Tq == 0) return DTMI_OK;
+  DTMI_CHECK(q && o && q_strides && o_strides && (Tk == 0 || (k && v && k_strides && v_strides)) && !rowmax == !rowsum,
+             "dtmi_xattn_fwd: NULL operand");
+  XArgs a{};
+  a.q = q, a.k = k, a.v = v, a.out = o, a.lengths = lengths, a.rowmax = rowmax, a.rowsum = rowsum;
+  a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides);
+  a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.R = H / Hk * Tq, a.scale = scale;
+  TimedLaunch tl(DTMI_FAM_OTHER, 4.0 * B * H * Tq * Tk * D);
+  return dtype == DTMI_F32 ? xattn_fwd<float>(a) : xattn_fwd<double>(a);
+  DTMI_BODY_END
+}
+
+DTMI_EXPORT int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D,
+                               double scale, const void* q, const int64_t* q_strides, const void* k,
+                               const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                               const int64_t* lengths, const void* o, const int64_t* o_strides, const void* dO,
+                               const int64_t* dO_strides, const void* rowmax, const void* rowsum, void* dq,
+                               const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                               const int64_t* dv_strides) {
+  DTMI_BODY_BEGIN
+  DTMI_REQUIRE_INIT();
+  if (int rc = x_shape("dtmi_xattn_bwd", dtype, B, H, Hk, Tq, Tk, D)) return rc;
+  if (B == 0 || H == 0) return DTMI_OK;
+  DTMI_CHECK((Tq == 0 || (q && o && dO && dq && rowmax && rowsum && q_strides && o_strides && dO_strides && dq_strides)) &&
+                 (Tk == 0 || (k && v && dk && dv && k_strides && v_strides && dk_strides && dv_strides)),
+             "dtmi_xattn_bwd: NULL operand");
+  XArgs a{};
+  a.q = q, a.k = k, a.v = v, a.o = o, a.dO = dO, a.dq = dq, a.dk = dk, a.dv = dv, a.lengths = lengths;
+  a.rowmax = const_cast<void*>(rowmax), a.rowsum = const_cast<void*>(rowsum);
+  a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides), a.sdo = ht(dO_strides);
+  a.sdq = ht(dq_strides), a.sdk = ht(dk_strides), a.sdv = ht(dv_strides);
+  a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.R = H / Hk * Tq, a.scale = scale;
+  TimedLaunch tl(DTMI_FAM_OTHER, 14.0 * B * H * Tq * Tk * D);
+  return dtype == DTMI_F32 ? xattn_bwd<float>(a) : xattn_bwd<double>(a);
+  DTMI_BODY_END
+}

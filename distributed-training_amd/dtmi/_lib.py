@@ -91,6 +91,19 @@ SIGNATURES: dict[str, list] = {
     "dtmi_attn_bwd_rowsum": [i32, i64, i64, i64, i64, f64, vp, pi64, vp, pi64, vp, pi64, vp, pi64, vp, pi64, vp, vp,
                              vp, vp, pi64, vp, pi64, vp, pi64],
     "dtmi_attn_set_ds_limit": [i64, pi64],
+    "dtmi_conv_fwd": [i32, i64, i64, i64, i64, vp, pi64, vp, vp, vp, vp, i32, vp, pi64, vp],
+    "dtmi_conv_bwd": [i32, i64, i64, i64, i64, vp, pi64, vp, vp, vp, vp, i32, vp, pi64, vp, pi64, vp, vp, vp],
+    "dtmi_conv_step": [i32, i64, i64, i64, vp, i64, vp, vp, vp, i32, vp, i64],
+    "dtmi_scan_kept": [i32, i64, i64, i64, i64, pi64],
+    "dtmi_scan_fwd": [i32, i64, i64, i64, i64, i64, vp, pi64, vp, pi64, vp, vp, pi64, vp, pi64, vp, vp, pi64, vp, vp,
+                      vp, i32, vp, pi64, vp, vp],
+    "dtmi_scan_bwd": [i32, i64, i64, i64, i64, i64, vp, pi64, vp, pi64, vp, vp, pi64, vp, pi64, vp, vp, pi64, vp, vp,
+                      i32, vp, vp, pi64, vp, pi64, vp, pi64, vp, vp, pi64, vp, pi64, vp, vp, pi64, vp, vp],
+    "dtmi_scan_step": [i32, i64, i64, i64, i64, vp, i64, vp, i64, vp, vp, pi64, vp, pi64, vp, vp, i64, vp, vp, i32,
+                       vp, i64],
+    "dtmi_xattn_fwd": [i32, i64, i64, i64, i64, i64, i64, f64, vp, pi64, vp, pi64, vp, pi64, vp, vp, pi64, vp, vp],
+    "dtmi_xattn_bwd": [i32, i64, i64, i64, i64, i64, i64, f64, vp, pi64, vp, pi64, vp, pi64, vp, vp, pi64, vp, pi64,
+                       vp, vp, vp, pi64, vp, pi64, vp, pi64],
 }
 
 _lib = None

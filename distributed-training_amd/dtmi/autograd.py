@@ -442,3 +442,138 @@ def cross_entropy(logits: Tensor, targets) -> Tensor:
             return (K.xent_grad_scale(pending.pop(), g1),)
         return (K.xent_bwd(z, t.dev, rmax, rsum, g=g1),)
     return Tensor._make(loss, (logits,), bw)
+
+
+# --------------------------------------------------------- sequence mixers
+# Beside causal_attention, for decoders whose own state does not grow and that
+# read an encoder. dtrain has no counterpart.
+def _rows(x: DeviceArray) -> DeviceArray:
+    """x itself where its last axis is contiguous, else a copy."""
+    return x if x.ndim == 0 or x.shape[-1] <= 1 or x.strides[-1] == 1 else x.contiguous()
+
+
+def _lengths_of(lengths, B: int, T: int):
+    """The lengths of a padded batch on the device, checked on the host: one
+    whole number of 0..T per sequence (a host array or an Indices)."""
+    if lengths is None:
+        return None
+    if not isinstance(lengths, Indices) and np.size(lengths) == 0:
+        lengths = np.zeros(np.shape(lengths), np.int64)
+    ix = as_indices(lengths)
+    if ix.shape != (B,):
+        raise ValueError(f"lengths must have one entry for each of the {B} sequences, not shape {ix.shape}")
+    ix.check(T + 1, "length", allow_negative=False)
+    return ix.dev
+
+
+def _state_of(state):
+    return state if state is None or isinstance(state, Tensor) else Tensor(state)
+
+
+def causal_conv(x: Tensor, w: Tensor, b: Tensor | None = None, silu: bool = True, state=None, lengths=None,
+                return_state: bool = False):
+    """Short causal convolution over time of x [B, T, C], each channel by itself:
+    y[t] = act(b + sum_k w[k] x[t - K + 1 + k]) with w [K, C], K of 1 to 8, and act
+    SiLU (silu=False: none).
+
+    `state` [B, K - 1, C] (a Tensor or DeviceArray) holds the inputs before the
+    first position, zeros without one. `lengths` (one per sequence, a host array
+    or an Indices) marks a padded batch: y and the gradients are zero from a
+    sequence's length on, and what lies there is not read. With `return_state`,
+    returns (y, state): the last K - 1 inputs of every sequence as a DeviceArray,
+    which carries no gradient."""
+    X = _rows(x.data)
+    if X.ndim != 3:
+        raise ValueError(f"causal_conv: x must be [B, T, C], not {x.shape}")
+    ln = _lengths_of(lengths, X.shape[0], X.shape[1])
+    st = _state_of(state)
+    W, bd, S = _contig(w.data), _contig(b.data) if b is not None else None, _contig(st.data) if st is not None else None
+    y, new = K.conv_fwd(X, W, bd, S, ln, silu, return_state)
+
+    def bw(g):
+        dx, dw, db, ds = K.conv_bwd(X, W, bd, _rows(g), S, ln, silu, need_dstate=st is not None and st.requires_grad,
+                                    dw_out=grad_out(w), db_out=grad_out(b) if b is not None else None)
+        return tuple([dx, dw] + ([db] if b is not None else []) + ([ds] if st is not None else []))
+    t = Tensor._make(y, tuple([x, w] + ([b] if b is not None else []) + ([st] if st is not None else [])), bw)
+    return (t, new) if return_state else t
+
+
+def causal_conv_step(x: Tensor, w: Tensor, b: Tensor | None, state: DeviceArray, silu: bool = True) -> Tensor:
+    """causal_conv for one new position per sequence: x [B, C]. `state`
+    [B, K - 1, C], contiguous, moves on in place. No gradient."""
+    y = K.conv_step(_rows(x.data), _contig(w.data), _contig(b.data) if b is not None else None, state, silu)
+    return Tensor(y)
+
+
+def _maps(m: Tensor, lead: int) -> DeviceArray:
+    """B or C of a scan as [..., G, N]: one group where the axis is left out."""
+    d = _rows(m.data)
+    if d.ndim == lead + 1:
+        d = DeviceArray(d.block, d.shape[:-1] + (1,) + d.shape[-1:], d.dtype, d.offset,
+                        tuple(d.strides[:-1]) + (0,) + tuple(d.strides[-1:]))
+    return d
+
+
+def ssm_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None = None, z: Tensor | None = None,
+             dt_bias: Tensor | None = None, state=None, lengths=None, return_state: bool = False,
+             softplus: bool = True):
+    """Selective state space scan of u [B, T, C]: with d = softplus(dt + dt_bias)
+    (softplus=False: dt + dt_bias),
+        h[c, n] = exp(d A[c, n]) h[c, n] + d u B[t, n],   y = sum_n C[t, n] h[c, n] + D u
+    and the result y silu(z), or y without z. dt and z are [B, T, C], A is [C, N]
+    (N up to 64), B and C are [B, T, N], or [B, T, G, N] for G groups of channels.
+
+    `state` [B, C, N] (a Tensor or DeviceArray) is h before the first position,
+    zeros without one. `lengths` and `return_state` as in causal_conv; the state
+    returned is h at each sequence's length."""
+    U = _rows(u.data)
+    if U.ndim != 3:
+        raise ValueError(f"ssm_scan: u must be [B, T, C], not {u.shape}")
+    ln = _lengths_of(lengths, U.shape[0], U.shape[1])
+    st = _state_of(state)
+    opt = [D, z, dt_bias, st]
+    args = [_rows(dt.data), _contig(A.data), _maps(B, 2), _maps(C, 2), _contig(D.data) if D is not None else None,
+            _rows(z.data) if z is not None else None, _contig(dt_bias.data) if dt_bias is not None else None]
+    train = _grad_enabled and any(p is not None and p.requires_grad for p in [u, dt, A, B, C] + opt)
+    out, new, kept = K.scan_fwd(U, *args, state=_contig(st.data) if st is not None else None, lengths=ln,
+                                softplus=softplus, return_state=return_state, keep=train)
+
+    def bw(g):
+        du, ddt, dA, dB, dC, dD, dz, dbias, ds = K.scan_bwd(
+            U, *args, kept, _rows(g), ln, softplus, need_dstate=st is not None and st.requires_grad,
+            dA_out=grad_out(A), dD_out=grad_out(D) if D is not None else None,
+            dbias_out=grad_out(dt_bias) if dt_bias is not None else None)
+        grads = [du, ddt, dA, dB.reshape(B.shape), dC.reshape(C.shape)]
+        return tuple(grads + [x for p, x in zip(opt, (dD, dz, dbias, ds)) if p is not None])
+    t = Tensor._make(out, tuple([u, dt, A, B, C] + [p for p in opt if p is not None]), bw)
+    return (t, new) if return_state else t
+
+
+def ssm_scan_step(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor | None, z: Tensor | None,
+                  dt_bias: Tensor | None, state: DeviceArray, softplus: bool = True) -> Tensor:
+    """ssm_scan for one new position per sequence: u, dt and z [B, C], the maps
+    [B, N] or [B, G, N]. `state` [B, C, N], contiguous, is updated in place. No
+    gradient."""
+    y = K.scan_step(_rows(u.data), _rows(dt.data), _contig(A.data), _maps(B, 1), _maps(C, 1),
+                    _contig(D.data) if D is not None else None, _rows(z.data) if z is not None else None,
+                    _contig(dt_bias.data) if dt_bias is not None else None, state, softplus)
+    return Tensor(y)
+
+
+def cross_attention(q: Tensor, k: Tensor, v: Tensor, lengths=None, scale: float | None = None) -> Tensor:
+    """Attention of q [B, H, Tq, D] to another sequence's k, v [B, Hk, Tk, D]: no
+    causal mask, any two lengths (one query token included), D up to 128, any
+    strides with a contiguous last axis. H is a multiple of Hk; head h reads
+    key/value head h // (H // Hk). `lengths` (one per sequence, a host array or an
+    Indices) masks the keys from there on, which are not read; a query without
+    keys gives 0. `scale` defaults to 1 / sqrt(D)."""
+    Q, Kd, V = _rows(q.data), _rows(k.data), _rows(v.data)
+    if Q.ndim != 4 or Kd.ndim != 4:
+        raise ValueError(f"cross_attention: q and k must be (B, heads, T, D), not {q.shape} and {k.shape}")
+    ln = _lengths_of(lengths, Q.shape[0], Kd.shape[2])
+    train = _grad_enabled and (q.requires_grad or k.requires_grad or v.requires_grad)
+    o, rmax, rsum = K.xattn_fwd(Q, Kd, V, ln, scale, stats=train)
+
+    def bw(g):
+        return K.xattn_bwd(Q, Kd, V, o, _rows(g), rmax, rsum, ln, scale)
+    return Tensor._make(o, (q, k, v), bw)

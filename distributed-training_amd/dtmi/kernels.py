@@ -670,3 +670,226 @@ def attn_set_ds_limit(nbytes: int) -> int:
     prev = C.c_int64()
     _c("dtmi_attn_set_ds_limit", int(nbytes), C.byref(prev))
     return prev.value
+
+
+# --------------------------------------------------------- sequence mixers
+def _rows_strides(x: DeviceArray, what: str, lead: int = 2):
+    """The element strides of all but the last axis, which must be contiguous."""
+    if x.ndim != lead + 1 or (x.shape[-1] > 1 and x.strides[-1] != 1):
+        raise ValueError(f"{what} must have {lead + 1} axes, the last contiguous")
+    return _lib.i64_array(x.strides[:lead])
+
+
+def _opt_ptr(x: DeviceArray | None):
+    return x.ptr if x is not None else None
+
+
+def _lengths_ptr(lengths: DeviceArray | None, B: int):
+    if lengths is None:
+        return None
+    _contig(lengths)
+    if lengths.dtype != np.int64 or lengths.size != B:
+        raise ValueError("lengths must be int64 with one entry per sequence")
+    return lengths.ptr
+
+
+def _same(x: DeviceArray, shape, dtype, what: str, contiguous: bool = True):
+    if tuple(x.shape) != tuple(shape) or x.dtype != dtype:
+        raise ValueError(f"{what} must be {np.dtype(dtype).name} of shape {tuple(shape)}, not {x.dtype} {x.shape}")
+    if contiguous:
+        _contig(x)
+
+
+def _conv_check(x, w, b, state, what):
+    C_ = x.shape[-1]
+    if w.ndim != 2 or w.shape[1] != C_ or not 1 <= w.shape[0] <= 8:
+        raise ValueError(f"{what}: w must be [taps, {C_}] with 1 to 8 taps, not {w.shape}")
+    K = w.shape[0]
+    _same(w, (K, C_), x.dtype, f"{what}: w")
+    if b is not None:
+        _same(b, (C_,), x.dtype, f"{what}: b")
+    if state is not None:
+        _same(state, (x.shape[0], K - 1, C_), x.dtype, f"{what}: state")
+    return K
+
+
+def conv_fwd(x: DeviceArray, w: DeviceArray, b: DeviceArray | None = None, state: DeviceArray | None = None,
+             lengths: DeviceArray | None = None, silu: bool = True, return_state: bool = False):
+    """Causal depthwise convolution of x [B, T, C] with w [K, C]. Returns
+    (y, new state [B, K - 1, C] or None)."""
+    sx = _rows_strides(x, "conv_fwd: x")
+    K = _conv_check(x, w, b, state, "conv_fwd")
+    B, T, C_ = x.shape
+    d = _dt(x, w)
+    y = empty(x.shape, x.dtype)
+    out = empty((B, K - 1, C_), x.dtype) if return_state else None
+    _c("dtmi_conv_fwd", d, B, T, C_, K, x.ptr, sx, w.ptr, _opt_ptr(b), _opt_ptr(state),
+       _lengths_ptr(lengths, B), 1 if silu else 0, y.ptr, _rows_strides(y, "y"), _opt_ptr(out))
+    return y, out
+
+
+def conv_bwd(x: DeviceArray, w: DeviceArray, b: DeviceArray | None, g: DeviceArray,
+             state: DeviceArray | None = None, lengths: DeviceArray | None = None, silu: bool = True,
+             need_dstate: bool = False, dw_out: DeviceArray | None = None, db_out: DeviceArray | None = None):
+    """Returns (dx, dw, db or None, dstate or None)."""
+    sx, sg = _rows_strides(x, "conv_bwd: x"), _rows_strides(g, "conv_bwd: g")
+    K = _conv_check(x, w, b, state, "conv_bwd")
+    _same(g, x.shape, x.dtype, "conv_bwd: g", contiguous=False)
+    B, T, C_ = x.shape
+    d = _dt(x, w, g)
+    dx = empty(x.shape, x.dtype)
+    dw = _out_or_new(dw_out, (K, C_), x.dtype, "conv_bwd")
+    db = _out_or_new(db_out, (C_,), x.dtype, "conv_bwd") if b is not None else None
+    ds = empty((B, K - 1, C_), x.dtype) if need_dstate else None
+    _c("dtmi_conv_bwd", d, B, T, C_, K, x.ptr, sx, w.ptr, _opt_ptr(b), _opt_ptr(state),
+       _lengths_ptr(lengths, B), 1 if silu else 0, g.ptr, sg, dx.ptr, _rows_strides(dx, "dx"), dw.ptr, _opt_ptr(db),
+       _opt_ptr(ds))
+    return dx, dw, db, ds
+
+
+def conv_step(x: DeviceArray, w: DeviceArray, b: DeviceArray | None, state: DeviceArray,
+              silu: bool = True) -> DeviceArray:
+    """One position per sequence: x [B, C]; state [B, K - 1, C] moves on in place."""
+    sx = _rows_strides(x, "conv_step: x", 1)
+    K = _conv_check(x, w, b, state, "conv_step")
+    B, C_ = x.shape
+    d = _dt(x, w, state)
+    y = empty(x.shape, x.dtype)
+    _c("dtmi_conv_step", d, B, C_, K, x.ptr, sx[0], w.ptr, _opt_ptr(b), state.ptr, 1 if silu else 0,
+       y.ptr, C_)
+    return y
+
+
+def _scan_check(what, lead, C_, u, dt, A, Bm, Cm, D, z, dt_bias, state):
+    """Shapes of a scan's operands; lead is (B, T), or (B,) for a step. Returns (N, G)."""
+    if A.ndim != 2 or A.shape[0] != C_ or not 1 <= A.shape[1] <= 64:
+        raise ValueError(f"{what}: A must be [{C_}, states] with 1 to 64 states, not {A.shape}")
+    N = A.shape[1]
+    if Bm.ndim != len(lead) + 2 or Bm.shape[-2] < 1 or C_ % Bm.shape[-2]:
+        raise ValueError(f"{what}: the maps must be {lead + ('groups', N)} with groups dividing {C_}, not {Bm.shape}")
+    G = Bm.shape[-2]
+    _same(A, (C_, N), u.dtype, f"{what}: A")
+    for name, x, shape in (("dt", dt, u.shape), ("B", Bm, lead + (G, N)), ("C", Cm, lead + (G, N)), ("z", z, u.shape)):
+        if x is not None:
+            _same(x, shape, u.dtype, f"{what}: {name}", contiguous=False)
+    for name, x, shape in (("D", D, (C_,)), ("dt_bias", dt_bias, (C_,)), ("state", state, (lead[0], C_, N))):
+        if x is not None:
+            _same(x, shape, u.dtype, f"{what}: {name}")
+    return N, G
+
+
+def scan_fwd(u, dt, A, Bm, Cm, D=None, z=None, dt_bias=None, state=None, lengths=None, softplus: bool = True,
+             return_state: bool = False, keep: bool = False):
+    """Selective scan of u [B, T, C] with A [C, N] and maps [B, T, G, N]. Returns
+    (out, final state [B, C, N] or None, kept states for scan_bwd or None)."""
+    su = _rows_strides(u, "scan_fwd: u")
+    B, T, C_ = u.shape
+    N, G = _scan_check("scan_fwd", (B, T), C_, u, dt, A, Bm, Cm, D, z, dt_bias, state)
+    d = _dt(u)
+    out = empty(u.shape, u.dtype)
+    hT = empty((B, C_, N), u.dtype) if return_state else None
+    kept = None
+    if keep:
+        n = C.c_int64()
+        _c("dtmi_scan_kept", d, B, T, C_, N, C.byref(n))
+        kept = empty((n.value,), u.dtype)
+    _c("dtmi_scan_fwd", d, B, T, C_, N, G, u.ptr, su, dt.ptr, _rows_strides(dt, "scan_fwd: dt"), A.ptr, Bm.ptr,
+       _rows_strides(Bm, "scan_fwd: B", 3), Cm.ptr, _rows_strides(Cm, "scan_fwd: C", 3), _opt_ptr(D), _opt_ptr(z),
+       _rows_strides(z, "scan_fwd: z") if z is not None else None, _opt_ptr(dt_bias), _opt_ptr(state),
+       _lengths_ptr(lengths, B), 1 if softplus else 0, out.ptr, _rows_strides(out, "out"), _opt_ptr(hT),
+       _opt_ptr(kept))
+    return out, hT, kept
+
+
+def scan_bwd(u, dt, A, Bm, Cm, D, z, dt_bias, kept, g, lengths=None, softplus: bool = True, need_dstate: bool = False,
+             dA_out=None, dD_out=None, dbias_out=None):
+    """Gradients of scan_fwd: (du, ddt, dA, dB, dC, dD, dz, ddt_bias, dstate), None
+    for operands that are None (dstate: not asked for)."""
+    su = _rows_strides(u, "scan_bwd: u")
+    B, T, C_ = u.shape
+    N, G = _scan_check("scan_bwd", (B, T), C_, u, dt, A, Bm, Cm, D, z, dt_bias, None)
+    _same(g, u.shape, u.dtype, "scan_bwd: g", contiguous=False)
+    d = _dt(u)
+    n = C.c_int64()
+    _c("dtmi_scan_kept", d, B, T, C_, N, C.byref(n))
+    _same(kept, (n.value,), u.dtype, "scan_bwd: kept")
+    du, ddt = empty(u.shape, u.dtype), empty(u.shape, u.dtype)
+    dB, dC = empty(Bm.shape, u.dtype), empty(Bm.shape, u.dtype)
+    dA = _out_or_new(dA_out, (C_, N), u.dtype, "scan_bwd")
+    dD = _out_or_new(dD_out, (C_,), u.dtype, "scan_bwd") if D is not None else None
+    dbias = _out_or_new(dbias_out, (C_,), u.dtype, "scan_bwd") if dt_bias is not None else None
+    dz = empty(u.shape, u.dtype) if z is not None else None
+    ds = empty((B, C_, N), u.dtype) if need_dstate else None
+    st, sm = _rows_strides(du, "du"), _rows_strides(dB, "dB", 3)
+    _c("dtmi_scan_bwd", d, B, T, C_, N, G, u.ptr, su, dt.ptr, _rows_strides(dt, "scan_bwd: dt"), A.ptr, Bm.ptr,
+       _rows_strides(Bm, "scan_bwd: B", 3), Cm.ptr, _rows_strides(Cm, "scan_bwd: C", 3), _opt_ptr(D), _opt_ptr(z),
+       _rows_strides(z, "scan_bwd: z") if z is not None else None, _opt_ptr(dt_bias), _lengths_ptr(lengths, B),
+       1 if softplus else 0, kept.ptr, g.ptr, _rows_strides(g, "scan_bwd: g"), du.ptr, st, ddt.ptr, st, dA.ptr,
+       dB.ptr, sm, dC.ptr, sm, _opt_ptr(dD), _opt_ptr(dz), st, _opt_ptr(dbias), _opt_ptr(ds))
+    return du, ddt, dA, dB, dC, dD, dz, dbias, ds
+
+
+def scan_step(u, dt, A, Bm, Cm, D, z, dt_bias, state: DeviceArray, softplus: bool = True) -> DeviceArray:
+    """One position per sequence: u, dt, z [B, C], maps [B, G, N]; state [B, C, N] in place."""
+    su = _rows_strides(u, "scan_step: u", 1)
+    B, C_ = u.shape
+    N, G = _scan_check("scan_step", (B,), C_, u, dt, A, Bm, Cm, D, z, dt_bias, state)
+    d = _dt(u)
+    out = empty(u.shape, u.dtype)
+    _c("dtmi_scan_step", d, B, C_, N, G, u.ptr, su[0], dt.ptr, _rows_strides(dt, "scan_step: dt", 1)[0], A.ptr,
+       Bm.ptr, _rows_strides(Bm, "scan_step: B", 2), Cm.ptr, _rows_strides(Cm, "scan_step: C", 2), _opt_ptr(D),
+       _opt_ptr(z), _rows_strides(z, "scan_step: z", 1)[0] if z is not None else 0, _opt_ptr(dt_bias), state.ptr,
+       1 if softplus else 0, out.ptr, C_)
+    return out
+
+
+def _xattn_check(what, q, k, v):
+    B, H, T, D = q.shape
+    if k.ndim != 4 or k.shape != v.shape:
+        raise ValueError(f"{what}: k and v must be (B, heads, T, D) of one shape, not {k.shape} and {v.shape}")
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"{what}: k and v {k.shape} do not match q {q.shape} in batch and head dimension")
+    Hk = k.shape[1]
+    if Hk < 1 or H % Hk:
+        raise ValueError(f"{what}: {H} heads cannot share {Hk} key/value heads")
+    if not 1 <= D <= 128:
+        raise ValueError(f"{what}: head dimension 1 to 128, not {D}")
+    return B, H, Hk, T, k.shape[2], D
+
+
+def xattn_fwd(q: DeviceArray, k: DeviceArray, v: DeviceArray, lengths: DeviceArray | None = None, scale=None,
+              out: DeviceArray | None = None, stats: bool = True):
+    """Attention of q [B, H, Tq, D] to the first `lengths` of k, v [B, Hk, Tk, D].
+    Returns (o, rowmax, rowsum), the statistics None without `stats`."""
+    sq, sk, sv = _bht_strides(q), _bht_strides(k), _bht_strides(v)
+    B, H, Hk, Tq, Tk, D = _xattn_check("xattn_fwd", q, k, v)
+    d = _dt(q, k, v)
+    if out is None:
+        out = empty(q.shape, q.dtype)
+    _same(out, q.shape, q.dtype, "xattn_fwd: out", contiguous=False)
+    rmax = empty((B, H, Tq), q.dtype) if stats else None
+    rsum = empty((B, H, Tq), q.dtype) if stats else None
+    s = float(1.0 / np.sqrt(D)) if scale is None else float(scale)
+    _c("dtmi_xattn_fwd", d, B, H, Hk, Tq, Tk, D, s, q.ptr, sq, k.ptr, sk, v.ptr, sv, _lengths_ptr(lengths, B), out.ptr,
+       _bht_strides(out), _opt_ptr(rmax), _opt_ptr(rsum))
+    return out, rmax, rsum
+
+
+def xattn_bwd(q, k, v, o, dO, rowmax, rowsum, lengths=None, scale=None, dq=None, dk=None, dv=None):
+    """Returns (dq, dk, dv); each may be passed as a view to fill."""
+    B, H, Hk, Tq, Tk, D = _xattn_check("xattn_bwd", q, k, v)
+    d = _dt(q, k, v, o, dO, rowmax, rowsum)
+    for name, x in (("o", o), ("dO", dO)):
+        _same(x, q.shape, q.dtype, f"xattn_bwd: {name}", contiguous=False)
+    for name, x in (("rowmax", rowmax), ("rowsum", rowsum)):
+        _same(x, (B, H, Tq), q.dtype, f"xattn_bwd: {name}")
+    dq = dq if dq is not None else empty(q.shape, q.dtype)
+    dk = dk if dk is not None else empty(k.shape, q.dtype)
+    dv = dv if dv is not None else empty(k.shape, q.dtype)
+    for name, x, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, k)):
+        _same(x, like.shape, q.dtype, f"xattn_bwd: {name}", contiguous=False)
+    s = float(1.0 / np.sqrt(D)) if scale is None else float(scale)
+    _c("dtmi_xattn_bwd", d, B, H, Hk, Tq, Tk, D, s, q.ptr, _bht_strides(q), k.ptr, _bht_strides(k), v.ptr,
+       _bht_strides(v), _lengths_ptr(lengths, B), o.ptr, _bht_strides(o), dO.ptr, _bht_strides(dO), rowmax.ptr,
+       rowsum.ptr, dq.ptr, _bht_strides(dq), dk.ptr, _bht_strides(dk), dv.ptr, _bht_strides(dv))
+    return dq, dk, dv

@@ -416,6 +416,79 @@ int dtmi_attn_bwd_rowsum(int dtype, int64_t B, int64_t H, int64_t T, int64_t D, 
  * NULL). */
 int dtmi_attn_set_ds_limit(int64_t bytes, int64_t* previous);
 
+/* --------------------------------------------------- sequence mixers
+ * Beside causal attention; dtrain has no counterpart. [B, T, C] arrays have C
+ * contiguous, and *_strides point at their (b, t) element strides (the maps of
+ * the scan: (b, t, g)), so operands and results may be views into fused
+ * projections. `lengths` (device int64 [B], or NULL: all T) marks padded batches:
+ * positions at and past lengths[b] are not read, their outputs and gradients are
+ * zero, and states are those at the sequence's end. Lengths outside 0..T count as
+ * the nearer end. Results must not overlap operands. Deterministic; scratch
+ * memory comes from the pool.
+ *
+ * Short causal convolution, each channel by itself, K = 1 to 8 taps:
+ *   pre[t, c] = b[c] + sum_k w[k, c] x[t - K + 1 + k, c], y = silu(pre) (silu != 0) or pre
+ * w [K, C]; b [C] or NULL; state [B, K-1, C]: the inputs before position 0, oldest
+ * first (NULL: zeros); state_out [B, K-1, C] (or NULL): the last K-1 inputs.
+ * The backward forms pre again; db and dstate may be NULL. The step takes one
+ * position per sequence (x, y [B, C], b strides) and moves the state on in place. */
+int dtmi_conv_fwd(int dtype, int64_t B, int64_t T, int64_t C, int64_t K, const void* x, const int64_t* x_strides,
+                  const void* w, const void* b, const void* state, const int64_t* lengths, int silu, void* y,
+                  const int64_t* y_strides, void* state_out);
+int dtmi_conv_bwd(int dtype, int64_t B, int64_t T, int64_t C, int64_t K, const void* x, const int64_t* x_strides,
+                  const void* w, const void* b, const void* state, const int64_t* lengths, int silu, const void* g,
+                  const int64_t* g_strides, void* dx, const int64_t* dx_strides, void* dw, void* db, void* dstate);
+int dtmi_conv_step(int dtype, int64_t B, int64_t C, int64_t K, const void* x, int64_t x_stride, const void* w,
+                   const void* b, void* state, int silu, void* y, int64_t y_stride);
+
+/* Selective state space scan, N = 1 to 64 states per channel, G groups of C / G
+ * channels that share the maps Bm and Cm [B, T, G, N] (N contiguous):
+ *   d = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias
+ *   h[c, n] = exp(d A[c, n]) h[c, n] + d u Bm[t, g, n];  y = sum_n Cm[t, g, n] h[c, n] + D[c] u
+ *   out = y silu(z), or y without z
+ * A [C, N]; D, dt_bias [C], z [B, T, C], state [B, C, N] may be NULL (0; no gate);
+ * state_out [B, C, N] or NULL. `kept`, for the backward: dtmi_scan_kept() elements
+ * that the forward fills with the states before each tile of positions (NULL: not
+ * kept). The backward writes every gradient it is given room for; dD, ddt_bias and
+ * dstate may be NULL. The step takes one position per sequence (u, dt, z, out
+ * [B, C], b strides; maps [B, G, N], (b, g) strides) and updates the state in place. */
+int dtmi_scan_kept(int dtype, int64_t B, int64_t T, int64_t C, int64_t N, int64_t* count);
+int dtmi_scan_fwd(int dtype, int64_t B, int64_t T, int64_t C, int64_t N, int64_t G, const void* u,
+                  const int64_t* u_strides, const void* dt, const int64_t* dt_strides, const void* A, const void* Bm,
+                  const int64_t* B_strides, const void* Cm, const int64_t* C_strides, const void* D, const void* z,
+                  const int64_t* z_strides, const void* dt_bias, const void* state, const int64_t* lengths,
+                  int softplus, void* out, const int64_t* out_strides, void* state_out, void* kept);
+int dtmi_scan_bwd(int dtype, int64_t B, int64_t T, int64_t C, int64_t N, int64_t G, const void* u,
+                  const int64_t* u_strides, const void* dt, const int64_t* dt_strides, const void* A, const void* Bm,
+                  const int64_t* B_strides, const void* Cm, const int64_t* C_strides, const void* D, const void* z,
+                  const int64_t* z_strides, const void* dt_bias, const int64_t* lengths, int softplus,
+                  const void* kept, const void* g, const int64_t* g_strides, void* du, const int64_t* du_strides,
+                  void* ddt, const int64_t* ddt_strides, void* dA, void* dB, const int64_t* dB_strides, void* dC,
+                  const int64_t* dC_strides, void* dD, void* dz, const int64_t* dz_strides, void* ddt_bias,
+                  void* dstate);
+int dtmi_scan_step(int dtype, int64_t B, int64_t C, int64_t N, int64_t G, const void* u, int64_t u_stride,
+                   const void* dt, int64_t dt_stride, const void* A, const void* Bm, const int64_t* B_strides,
+                   const void* Cm, const int64_t* C_strides, const void* D, const void* z, int64_t z_stride,
+                   const void* dt_bias, void* state, int softplus, void* out, int64_t out_stride);
+
+/* Attention to another sequence: o = softmax(q k^T scale) v for q [B, H, Tq, D] over
+ * the first lengths[b] of k, v [B, Hk, Tk, D], H a multiple of Hk (head h reads
+ * h / (H / Hk)), D = 1 to 128 contiguous, (b, h, t) strides as dtmi_attn_fwd takes
+ * them. A row without keys, or whose scores are all -inf, is 0 and passes no
+ * gradient. The forward writes the row statistics the backward reads (contiguous
+ * [B, H, Tq], both or neither NULL): rowmax, a reference within 2^8 of the maximum
+ * in base-2 units, and rowsum = sum_j 2^(log2(e) q . k_j scale - rowmax). */
+int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D, double scale,
+                   const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                   const int64_t* v_strides, const int64_t* lengths, void* o, const int64_t* o_strides, void* rowmax,
+                   void* rowsum);
+int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D, double scale,
+                   const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                   const int64_t* v_strides, const int64_t* lengths, const void* o, const int64_t* o_strides,
+                   const void* dO, const int64_t* dO_strides, const void* rowmax, const void* rowsum, void* dq,
+                   const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                   const int64_t* dv_strides);
+
 #ifdef __cplusplus
 }
 #endif
