@@ -31,18 +31,24 @@ namespace dtmi {
 constexpr int kStates = 4;  // states per lane
 constexpr double kLog2e = 1.4426950408889634;
 
-// Positions per tile, by waves W per block: the backward holds a tile's
-// states and decays in registers (2 * TT * 4 values of a lane), and W = 16
-// waves leave a wave 128 registers.
+// Positions per tile; the state before each tile is kept for the backward.
 template <typename T>
-__host__ __device__ constexpr int tile_len(int W) {
-  return sizeof(T) == 4 ? (W <= 8 ? 16 : 8) : (W <= 8 ? 8 : 4);
+__host__ __device__ constexpr int tile_len() {
+  return sizeof(T) == 4 ? 16 : 8;
 }
-// Positions whose per-wave sums pass through LDS together (three of them in the backward).
+// Positions whose per-wave sums pass through LDS together in the forward.
 template <typename T>
 __host__ __device__ constexpr int sum_len(int W) {
-  const int n = (sizeof(T) == 4 ? 64 : 32) / W, t = tile_len<T>(W);
+  const int n = (sizeof(T) == 4 ? 64 : 32) / W, t = tile_len<T>();
   return n < t ? n : t;
+}
+// Positions whose states and decays a backward wave holds in registers at a
+// time (8 per position and lane): a whole tile's would leave room for one wave
+// per SIMD, so a tile is gone over in parts, the states before each part
+// rebuilt once. Sixteen waves share the registers of a block of twice the size.
+template <typename T>
+__host__ __device__ constexpr int held_len(int W) {
+  return (sizeof(T) == 4 ? 8 : 4) / (W <= 8 ? 1 : 2);
 }
 static int waves_for(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
@@ -57,33 +63,32 @@ struct ScanArgs {
   BT su, sdt, sz, sout, sg, sdu, sddt, sdz, sB, sC;
   int64_t gB, gC;       // group strides of B and C
   int64_t B, T, C, N, G;
-  int64_t seglen;       // positions per segment, a multiple of the tile
+  int seglen;           // positions per segment, a multiple of the tile
   int nseg, ct, tpg;    // segments; channel tiles in all and per group
   int softplus;
 };
 
 struct ScanBlock {
-  int64_t b, c, cc, len, lo, hi;  // cc: c, or the group's last channel for an idle lane
-  int seg, grp, tile;             // segment, group, channel tile within the group
+  int64_t b, c, cc;    // cc: c, or the group's last channel for an idle lane
+  int len, lo, hi;     // the sequence's length, the segment's positions
+  int seg, grp, tile;  // segment, group, channel tile within the group
   bool on;
 };
 
 __device__ __forceinline__ ScanBlock scan_block(const ScanArgs& a) {
   ScanBlock k;
-  const int64_t id = blockIdx.x;
-  const int ct = (int)(id % a.ct);
-  const int64_t bs = id / a.ct;
-  k.seg = (int)(bs % a.nseg);
-  k.b = bs / a.nseg;
-  k.grp = ct / a.tpg;
-  k.tile = ct % a.tpg;
+  const unsigned id = blockIdx.x, bs = id / (unsigned)a.ct, ct = id - bs * (unsigned)a.ct;
+  k.b = bs / (unsigned)a.nseg;
+  k.seg = (int)(bs % (unsigned)a.nseg);
+  k.grp = (int)(ct / (unsigned)a.tpg);
+  k.tile = (int)(ct % (unsigned)a.tpg);
   const int64_t each = a.C / a.G, off = (int64_t)k.tile * 64 + (threadIdx.x & 63);
   k.on = off < each;
   k.c = k.grp * each + off;
   k.cc = k.on ? k.c : k.grp * each + each - 1;
-  k.len = seq_len(a.lengths, k.b, a.T);
+  k.len = (int)seq_len(a.lengths, k.b, a.T);
   k.lo = k.seg * a.seglen;
-  k.hi = k.lo + a.seglen < a.T ? k.lo + a.seglen : a.T;
+  k.hi = (int)(a.T - k.lo > a.seglen ? k.lo + a.seglen : a.T);
   return k;
 }
 
@@ -92,22 +97,52 @@ __device__ __forceinline__ T step_size(T raw, int softp) {
   return softp ? softplus(raw) : raw;
 }
 
-// B or C rows of a tile into LDS [TT][4 W], zero where there is no position or state
+// A wave's rows of a tile (r = w, w + W, ...) and the block's share of the
+// tile's maps, on their way from global memory. Positions at and past the
+// length read the last one that holds data and are masked when the tile is
+// staged, so no load waits for a branch.
 template <typename T, int W, int TT>
-__device__ __forceinline__ void stage_map(T* __restrict__ s, const T* __restrict__ src, int64_t st, int64_t t0,
-                                          int64_t len, int N) {
-  for (int f = threadIdx.x; f < TT * W * kStates; f += 64 * W) {
-    const int r = f / (W * kStates), n = f % (W * kStates);
-    s[f] = t0 + r < len && n < N ? src[(t0 + r) * st + n] : T(0);
+struct Tile {
+  static constexpr int RPW = (TT + W - 1) / W, NP = W * kStates, MAPS = (TT * NP + 64 * W - 1) / (64 * W);
+  T u[RPW], d[RPW], z[RPW], g[RPW], b[MAPS], c[MAPS];
+  __device__ __forceinline__ void rows(T (&x)[RPW], const T* __restrict__ p, int64_t st, int t0, int len, int w) {
+    if (t0 + (TT > W ? TT : W) <= len) {
+      const T* q = p + (t0 + w) * st;
+#pragma unroll
+      for (int i = 0; i < RPW; ++i, q += W * st) x[i] = *q;
+    } else {
+#pragma unroll
+      for (int i = 0; i < RPW; ++i) {
+        const int t = t0 + w + W * i;
+        x[i] = p[(t < len ? t : len - 1) * st];
+      }
+    }
   }
-}
+  __device__ __forceinline__ void map(T (&x)[MAPS], const T* __restrict__ p, int64_t st, int t0, int len, int N) {
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+      const int f = threadIdx.x + 64 * W * i, n = f % NP, t = t0 + f / NP;
+      x[i] = p[(t < len ? t : len - 1) * st + (n < N ? n : N - 1)];
+    }
+  }
+  static __device__ __forceinline__ void put_map(T* __restrict__ s, const T (&x)[MAPS], int t0, int len, int N) {
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) {
+      const int f = threadIdx.x + 64 * W * i;
+      if (TT * NP % (64 * W) != 0 && f >= TT * NP) continue;
+      s[f] = t0 + f / NP < len && f % NP < N ? x[i] : T(0);
+    }
+  }
+};
 
 // CARRY: only the segment's end state from a zero start, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(W), YT = sum_len<T>(W), RPW = (TT + W - 1) / W;
+  constexpr int NS = kStates, TT = tile_len<T>(), YT = sum_len<T>(W);
+  using In = Tile<T, W, TT>;
+  constexpr int RPW = In::RPW, NP = In::NP;
   __shared__ T sd[TT][64], sx[TT][64], yp[CARRY ? 1 : W][CARRY ? 1 : YT][64];
-  __shared__ __attribute__((aligned(16))) T sB[TT * W * NS], sC[TT * W * NS];
+  __shared__ __attribute__((aligned(16))) T sB[TT * NP], sC[CARRY ? 1 : TT * NP];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ScanBlock k = scan_block(a);
   const int N = (int)a.N, n0 = w * NS;
@@ -132,37 +167,43 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
     }
   }
   const int64_t ntiles = (a.T + TT - 1) / TT;
-  for (int64_t t0 = k.lo; t0 < k.hi; t0 += TT) {
-    if (t0 >= k.len) {  // nothing left of this sequence: its outputs are zero
-      if (!CARRY && k.on)
-        for (int64_t t = t0 + w; t < k.hi; t += W) op[t * a.sout.t] = T(0);
-      break;
+  const int stop = k.hi < k.len ? k.hi : k.len;  // positions at and past it do nothing
+  In in;
+  auto fetch = [&](int t0) {
+    in.rows(in.u, up, a.su.t, t0, k.len, w);
+    in.rows(in.d, dp, a.sdt.t, t0, k.len, w);
+    in.map(in.b, Bp, a.sB.t, t0, k.len, N);
+    if constexpr (!CARRY) {
+      if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w);
+      in.map(in.c, Cp, a.sC.t, t0, k.len, N);
     }
+  };
+  if (k.lo < stop) fetch(k.lo);
+  for (int t0 = k.lo; t0 < stop; t0 += TT) {
     T ur[RPW], zr[RPW];
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       const int r = w + W * i;
       if (W * RPW != TT && r >= TT) break;
-      const bool in = t0 + r < k.len;
-      T d = T(0);
-      ur[i] = zr[i] = T(0);
-      if (in) {
-        ur[i] = up[(t0 + r) * a.su.t];
-        d = step_size(dp[(t0 + r) * a.sdt.t] + bias, a.softplus);
-        if (!CARRY && zp) zr[i] = zp[(t0 + r) * a.sz.t];
-      }
+      const bool on = t0 + r < k.len;
+      const T d = on ? step_size(in.d[i] + bias, a.softplus) : T(0);
+      ur[i] = on ? in.u[i] : T(0);
+      if (!CARRY) zr[i] = in.z[i];
       sd[r][lane] = d;
       sx[r][lane] = d * ur[i];
     }
-    stage_map<T, W, TT>(sB, Bp, a.sB.t, t0, k.len, N);
-    if (!CARRY) stage_map<T, W, TT>(sC, Cp, a.sC.t, t0, k.len, N);
-    if (!CARRY && a.kept && k.on) {
-      T* kp = (T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c;
+    In::put_map(sB, in.b, t0, k.len, N);
+    if constexpr (!CARRY) {
+      In::put_map(sC, in.c, t0, k.len, N);
+      if (a.kept && k.on) {
+        T* kp = (T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c;
 #pragma unroll
-      for (int j = 0; j < NS; ++j)
-        if (n0 + j < N) kp[j * a.C] = h[j];
+        for (int j = 0; j < NS; ++j)
+          if (n0 + j < N) kp[j * a.C] = h[j];
+      }
     }
     __syncthreads();
+    if (t0 + TT < stop) fetch(t0 + TT);
 #pragma unroll
     for (int s = 0; s < TT / YT; ++s) {
 #pragma unroll
@@ -172,18 +213,19 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
         T y = T(0);
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-          h[j] = fma(exp2_of(d * A2[j]), h[j], x * sB[r * W * NS + n0 + j]);
-          if (!CARRY) y = fma(sC[r * W * NS + n0 + j], h[j], y);
+          h[j] = fma(exp2_of(d * A2[j]), h[j], x * sB[r * NP + n0 + j]);
+          if constexpr (!CARRY) y = fma(sC[r * NP + n0 + j], h[j], y);
         }
-        if (CARRY)
+        if constexpr (CARRY)
           total = total + d;
         else
           yp[w][q][lane] = y;
       }
       __syncthreads();
       if constexpr (!CARRY) {
+        T* q = op + (t0 + w) * a.sout.t;
 #pragma unroll
-        for (int i = 0; i < RPW; ++i) {
+        for (int i = 0; i < RPW; ++i, q += W * a.sout.t) {
           const int r = w + W * i;
           if (r / YT != s || r >= TT) continue;
           T y = T(0);
@@ -191,7 +233,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
           for (int v = 0; v < W; ++v) y = y + yp[v][r % YT][lane];
           y = fma(Dc, ur[i], y);
           if (zp) y = y * (zr[i] * sigmoid(zr[i]));
-          if (k.on && t0 + r < k.hi) op[(t0 + r) * a.sout.t] = t0 + r < k.len ? y : T(0);
+          if (k.on && t0 + r < stop) *q = y;
         }
         if (TT != YT) __syncthreads();
       }
@@ -204,10 +246,13 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
     for (int j = 0; j < NS; ++j)
       if (n0 + j < N) ((T*)a.carry)[(at * N + n0 + j) * a.C + k.c] = h[j];
     if (w == 0) ((T*)a.dsum)[at * a.C + k.c] = total;
-  } else if (a.hT && k.seg == a.nseg - 1) {
+  } else {
+    for (int t = (stop > k.lo ? stop : k.lo) + w; t < k.hi; t += W) op[t * a.sout.t] = T(0);
+    if (a.hT && k.seg == a.nseg - 1) {
 #pragma unroll
-    for (int j = 0; j < NS; ++j)
-      if (n0 + j < N) ((T*)a.hT)[(k.b * a.C + k.c) * N + n0 + j] = h[j];
+      for (int j = 0; j < NS; ++j)
+        if (n0 + j < N) ((T*)a.hT)[(k.b * a.C + k.c) * N + n0 + j] = h[j];
+    }
   }
 }
 
@@ -230,19 +275,58 @@ __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backwar
   }
 }
 
-// Sum over the wave of each of 8 values: lane l ends with that of value l / 8.
+// x of the lane that DPP control CTRL names
+template <int CTRL>
+__device__ __forceinline__ float lane_of(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double lane_of(double x) {
+  typedef int i2 __attribute__((ext_vector_type(2)));
+  i2 v = __builtin_bit_cast(i2, x);
+  v.x = __builtin_amdgcn_update_dpp(0, v.x, CTRL, 0xf, 0xf, true);
+  v.y = __builtin_amdgcn_update_dpp(0, v.y, CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, v);
+}
+// p's sums of lane halves (ROW = 32: lanes l and l + 32; 16: l and l + 16) in the
+// lower half of each pair, q's in the upper: one exchange, one addition
+template <int ROW>
+__device__ __forceinline__ void swap_rows(unsigned& p, unsigned& q) {
+  if constexpr (ROW == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(p, q, false, false);
+    p = r[0], q = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane16_swap(p, q, false, false);
+    p = r[0], q = r[1];
+  }
+}
+template <int ROW>
+__device__ __forceinline__ float fold(float p, float q) {
+  unsigned a = __builtin_bit_cast(unsigned, p), b = __builtin_bit_cast(unsigned, q);
+  swap_rows<ROW>(a, b);
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+template <int ROW>
+__device__ __forceinline__ double fold(double p, double q) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  u2 a = __builtin_bit_cast(u2, p), b = __builtin_bit_cast(u2, q);
+  unsigned ax = a.x, ay = a.y, bx = b.x, by = b.y;
+  swap_rows<ROW>(ax, bx);
+  swap_rows<ROW>(ay, by);
+  a = u2{ax, ay}, b = u2{bx, by};
+  return __builtin_bit_cast(double, a) + __builtin_bit_cast(double, b);
+}
+// Sums over the wave of 8 values, 18 instructions: lane l ends with that of
+// value l / 8. Each step halves the values a lane holds; the last three add
+// within the eight lanes that hold the same one.
 template <typename T>
-__device__ __forceinline__ T sum8(const T (&v)[8], int lane) {
-  T x[4], y[2];
-  const bool b5 = lane & 32, b4 = lane & 16, b3 = lane & 8;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = (b5 ? v[i + 4] : v[i]) + __shfl_xor(b5 ? v[i] : v[i + 4], 32, 64);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) y[i] = (b4 ? x[i + 2] : x[i]) + __shfl_xor(b4 ? x[i] : x[i + 2], 16, 64);
-  T r = (b3 ? y[1] : y[0]) + __shfl_xor(b3 ? y[0] : y[1], 8, 64);
-  r = r + __shfl_xor(r, 4, 64);
-  r = r + __shfl_xor(r, 2, 64);
-  return r + __shfl_xor(r, 1, 64);
+__device__ __forceinline__ T sum8(const T (&v)[8], bool upper8) {
+  const T x0 = fold<32>(v[0], v[4]), x1 = fold<32>(v[1], v[5]), x2 = fold<32>(v[2], v[6]), x3 = fold<32>(v[3], v[7]);
+  const T y0 = fold<16>(x0, x2), y1 = fold<16>(x1, x3);
+  T r = (upper8 ? y1 : y0) + lane_of<0x128>(upper8 ? y0 : y1);  // row_ror:8
+  r = r + lane_of<0x141>(r);                                    // row_half_mirror
+  r = r + lane_of<0xB1>(r);                                     // quad_perm 1,0,3,2
+  return r + lane_of<0x4E>(r);                                  // quad_perm 2,3,0,1
 }
 
 // The backward over a segment, last tile first. dh carries the gradient of the
@@ -252,11 +336,14 @@ __device__ __forceinline__ T sum8(const T (&v)[8], int lane) {
 //   dB[t] = sum_c dh d u,  dC[t] = sum_c dy h[t]
 // A tile's states are rebuilt in registers from the state kept before it. The
 // sums over a wave's channels (dB, dC) are taken as sum8, eight values of a
-// step together. CARRY: only dh over the segment, and its sum of d.
+// step together, and eight steps' results leave a wave as one LDS write.
+// CARRY: only dh over the segment, and its sum of d.
 template <typename T, int W, bool CARRY>
-__global__ void __launch_bounds__(64 * W) scan_bwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(W), YT = sum_len<T>(W), RPW = (TT + W - 1) / W, NP = W * NS;
-  __shared__ T sd[TT][64], sx[CARRY ? 1 : TT][64], sy[TT][64], yp[CARRY ? 1 : 3][CARRY ? 1 : W][CARRY ? 1 : YT][64];
+__global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanArgs a) {
+  constexpr int NS = kStates, TT = tile_len<T>(), HT = held_len<T>(W);
+  using In = Tile<T, W, TT>;
+  constexpr int RPW = In::RPW, NP = In::NP, RB = HT < 8 ? HT : 8;
+  __shared__ T sd[TT][64], sx[CARRY ? 1 : TT][64], sy[TT][64], yp[CARRY ? 1 : 3][CARRY ? 1 : W][CARRY ? 1 : HT][64];
   __shared__ __attribute__((aligned(16))) T sB[CARRY ? 1 : TT * NP], sC[TT * NP];
   __shared__ T sg[CARRY ? 1 : TT][CARRY ? 1 : 2 * NP];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -280,52 +367,70 @@ __global__ void __launch_bounds__(64 * W) scan_bwd_kernel(ScanArgs a) {
       dh[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.cc];
   }
   const int64_t ntiles = (a.T + TT - 1) / TT;
+  const int stop = k.hi < k.len ? k.hi : k.len;
   // this block's dB and dC terms: row t of part k.tile
   const int64_t prow = ((k.tile * a.B + k.b) * a.T) * a.G + k.grp;
-  for (int64_t t0 = k.lo + (k.hi - 1 - k.lo) / TT * TT; t0 >= k.lo; t0 -= TT) {
-    if (t0 >= k.len) {
-      if constexpr (!CARRY) {
-        const int rows = (int)(k.hi - t0 < TT ? k.hi - t0 : TT);
-        if (k.on)
-          for (int r = w; r < rows; r += W) {
-            ((T*)a.du)[k.b * a.sdu.b + (t0 + r) * a.sdu.t + k.c] = T(0);
-            ((T*)a.ddt)[k.b * a.sddt.b + (t0 + r) * a.sddt.t + k.c] = T(0);
-            if (zp) ((T*)a.dz)[k.b * a.sdz.b + (t0 + r) * a.sdz.t + k.c] = T(0);
-          }
-        for (int f = threadIdx.x; f < rows * N; f += 64 * W) {
-          const int64_t at = (prow + (t0 + f / N) * a.G) * N + f % N;
-          ((T*)a.dBp)[at] = T(0);
-          ((T*)a.dCp)[at] = T(0);
-        }
+  if constexpr (!CARRY) {  // positions past the sequence: zeros
+    const int from = stop > k.lo ? stop : k.lo;
+    if (k.on)
+      for (int t = from + w; t < k.hi; t += W) {
+        ((T*)a.du)[k.b * a.sdu.b + t * a.sdu.t + k.c] = T(0);
+        ((T*)a.ddt)[k.b * a.sddt.b + t * a.sddt.t + k.c] = T(0);
+        if (zp) ((T*)a.dz)[k.b * a.sdz.b + t * a.sdz.t + k.c] = T(0);
       }
-      continue;
+    for (int64_t f = threadIdx.x; f < (int64_t)(k.hi - from) * N; f += 64 * W) {
+      const int64_t at = (prow + (from + f / N) * a.G) * N + f % N;
+      ((T*)a.dBp)[at] = T(0);
+      ((T*)a.dCp)[at] = T(0);
     }
+  }
+  In in;
+  T kept[NS];
+  auto fetch = [&](int t0) {
+    in.rows(in.d, dp, a.sdt.t, t0, k.len, w);
+    in.rows(in.g, gp, a.sg.t, t0, k.len, w);
+    if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w);
+    in.map(in.c, Cp, a.sC.t, t0, k.len, N);
+    if constexpr (!CARRY) {
+      in.rows(in.u, up, a.su.t, t0, k.len, w);
+      in.map(in.b, Bp, a.sB.t, t0, k.len, N);
+      const T* kp = (const T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.cc;
+#pragma unroll
+      for (int j = 0; j < NS; ++j) kept[j] = n0 + j < N ? kp[j * a.C] : T(0);
+    }
+  };
+  const int first = k.lo + (stop - 1 - k.lo) / TT * TT;
+  T *dup = nullptr, *ddp = nullptr, *dzp = nullptr;
+  if constexpr (!CARRY) {
+    dup = (T*)a.du + k.b * a.sdu.b + k.c;
+    ddp = (T*)a.ddt + k.b * a.sddt.b + k.c;
+    if (zp) dzp = (T*)a.dz + k.b * a.sdz.b + k.c;
+  }
+  if (k.lo < stop) fetch(first);
+  for (int t0 = first; k.lo < stop && t0 >= k.lo; t0 -= TT) {
     T ur[RPW], zr[RPW], gr[RPW], dr[RPW], rr[RPW];
     __syncthreads();  // the previous tile's LDS has been read
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       const int r = w + W * i;
       if (W * RPW != TT && r >= TT) break;
-      ur[i] = zr[i] = gr[i] = dr[i] = rr[i] = T(0);
-      T dy = T(0);
-      if (t0 + r < k.len) {
-        ur[i] = up[(t0 + r) * a.su.t];
-        rr[i] = dp[(t0 + r) * a.sdt.t] + bias;
-        gr[i] = gp[(t0 + r) * a.sg.t];
-        dr[i] = step_size(rr[i], a.softplus);
-        dy = gr[i];
-        if (zp) {
-          zr[i] = zp[(t0 + r) * a.sz.t];
-          dy = dy * (zr[i] * sigmoid(zr[i]));
-        }
-      }
+      const bool on = t0 + r < k.len && k.on;  // an idle lane's terms are zero
+      rr[i] = in.d[i] + bias;
+      gr[i] = on ? in.g[i] : T(0);
+      dr[i] = on ? step_size(rr[i], a.softplus) : T(0);
+      zr[i] = zp && on ? in.z[i] : T(0);
+      const T dy = zp ? gr[i] * (zr[i] * sigmoid(zr[i])) : gr[i];
       sd[r][lane] = dr[i];
       sy[r][lane] = dy;
-      if (!CARRY) sx[r][lane] = dr[i] * ur[i];
+      if constexpr (!CARRY) {
+        ur[i] = on ? in.u[i] : T(0);
+        sx[r][lane] = dr[i] * ur[i];
+      }
     }
-    stage_map<T, W, TT>(sC, Cp, a.sC.t, t0, k.len, N);
+    In::put_map(sC, in.c, t0, k.len, N);
     if constexpr (CARRY) {
       __syncthreads();
+      if (t0 > k.lo) fetch(t0 - TT);
 #pragma unroll
       for (int r = TT - 1; r >= 0; --r) {
         const T d = sd[r][lane], dy = sy[r][lane];
@@ -333,94 +438,113 @@ __global__ void __launch_bounds__(64 * W) scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
         for (int j = 0; j < NS; ++j) dh[j] = exp2_of(d * A2[j]) * fma(dy, sC[r * NP + n0 + j], dh[j]);
       }
-      continue;
     } else {
-      stage_map<T, W, TT>(sB, Bp, a.sB.t, t0, k.len, N);
-      T hs[NS], dec[TT][NS], h[TT][NS];
-      const T* kp = (const T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.cc;
+      In::put_map(sB, in.b, t0, k.len, N);
+      // the states before each part of the tile
+      T start[TT / HT][NS];
 #pragma unroll
-      for (int j = 0; j < NS; ++j) hs[j] = n0 + j < N ? kp[j * a.C] : T(0);
+      for (int j = 0; j < NS; ++j) start[0][j] = kept[j];
       __syncthreads();
+      if (t0 > k.lo) fetch(t0 - TT);
 #pragma unroll
-      for (int r = 0; r < TT; ++r) {
-        const T d = sd[r][lane], x = sx[r][lane];
+      for (int s = 1; s < TT / HT; ++s) {
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          dec[r][j] = exp2_of(d * A2[j]);
-          h[r][j] = fma(dec[r][j], r ? h[r ? r - 1 : 0][j] : hs[j], x * sB[r * NP + n0 + j]);
+        for (int j = 0; j < NS; ++j) start[s][j] = start[s - 1][j];
+#pragma unroll
+        for (int q = 0; q < HT; ++q) {
+          const int r = (s - 1) * HT + q;
+          const T d = sd[r][lane], x = sx[r][lane];
+#pragma unroll
+          for (int j = 0; j < NS; ++j)
+            start[s][j] = fma(exp2_of(d * A2[j]), start[s][j], x * sB[r * NP + n0 + j]);
+          if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
       }
+      T sums = T(0);
 #pragma unroll
-      for (int s = TT / YT - 1; s >= 0; --s) {
+      for (int s = TT / HT - 1; s >= 0; --s) {
+        T dec[HT][NS], h[HT + 1][NS];  // h[q]: the states before position q of the part
 #pragma unroll
-        for (int q = YT - 1; q >= 0; --q) {
-          const int r = s * YT + q;
+        for (int j = 0; j < NS; ++j) h[0][j] = start[s][j];
+#pragma unroll
+        for (int q = 0; q < HT; ++q) {
+          const int r = s * HT + q;
+          const T d = sd[r][lane], x = sx[r][lane];
+#pragma unroll
+          for (int j = 0; j < NS; ++j) {
+            dec[q][j] = exp2_of(d * A2[j]);
+            h[q + 1][j] = fma(dec[q][j], h[q][j], x * sB[r * NP + n0 + j]);
+          }
+          if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int q = HT - 1; q >= 0; --q) {
+          const int r = s * HT + q;
           const T d = sd[r][lane], x = sx[r][lane], dy = sy[r][lane];
           T dx = T(0), e = T(0), y = T(0), v[8];
 #pragma unroll
           for (int j = 0; j < NS; ++j) {
             const T Cn = sC[r * NP + n0 + j], Bn = sB[r * NP + n0 + j];
-            y = fma(Cn, h[r][j], y);
-            v[4 + j] = dy * h[r][j];
+            y = fma(Cn, h[q + 1][j], y);
+            v[4 + j] = dy * h[q + 1][j];
             dh[j] = fma(dy, Cn, dh[j]);
             dx = fma(dh[j], Bn, dx);
             v[j] = dh[j] * x;
-            dh[j] = dh[j] * dec[r][j];
-            const T p = dh[j] * (r ? h[r ? r - 1 : 0][j] : hs[j]);
+            dh[j] = dh[j] * dec[q][j];
+            const T p = dh[j] * h[q][j];
             e = fma(An[j], p, e);
             dA[j] = fma(d, p, dA[j]);
           }
           yp[0][w][q][lane] = y;
           yp[1][w][q][lane] = dx;
           yp[2][w][q][lane] = e;
-          // an idle lane repeats another channel: its terms do not count
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = k.on ? v[j] : T(0);
-          const T sum = sum8<T>(v, lane);
-          if ((lane & 7) == 0) sg[r][(lane >> 5) * NP + n0 + ((lane >> 3) & 3)] = sum;
+          // lane l keeps value l / 8 of step r with r % 8 = l % 8
+          const T sum = sum8<T>(v, lane & 8);
+          sums = (lane & (RB - 1)) == r % RB ? sum : sums;
+          __builtin_amdgcn_sched_barrier(0);
+          if (r % RB == 0 && (lane & 7) < RB)
+            sg[r + (lane & 7)][(lane >> 5) * NP + n0 + ((lane >> 3) & 3)] = sums;
         }
         __syncthreads();
+        T *qu = dup + (t0 + w) * a.sdu.t, *qd = ddp + (t0 + w) * a.sddt.t, *qz = dzp + (t0 + w) * a.sdz.t;
 #pragma unroll
-        for (int i = 0; i < RPW; ++i) {
+        for (int i = 0; i < RPW; ++i, qu += W * a.sdu.t, qd += W * a.sddt.t, qz += W * a.sdz.t) {
           const int r = w + W * i;
-          if (r / YT != s || r >= TT) continue;
+          if (r / HT != s || r >= TT) continue;
           T y = T(0), dx = T(0), e = T(0);
 #pragma unroll
           for (int v = 0; v < W; ++v) {
-            y = y + yp[0][v][r % YT][lane];
-            dx = dx + yp[1][v][r % YT][lane];
-            e = e + yp[2][v][r % YT][lane];
+            y = y + yp[0][v][r % HT][lane];
+            dx = dx + yp[1][v][r % HT][lane];
+            e = e + yp[2][v][r % HT][lane];
           }
+          const bool put = k.on && t0 + r < stop;
           T dy = gr[i];
           if (zp) {
             const T sz = sigmoid(zr[i]);
             y = fma(Dc, ur[i], y);
             const T dz = gr[i] * y * (sz * fma(zr[i], T(1) - sz, T(1)));
             dy = gr[i] * (zr[i] * sz);
-            if (k.on && t0 + r < k.hi)
-              ((T*)a.dz)[k.b * a.sdz.b + (t0 + r) * a.sdz.t + k.c] = t0 + r < k.len ? dz : T(0);
+            if (put) *qz = dz;
           }
           T dd = fma(dx, ur[i], e);
           if (a.softplus) dd = dd * sigmoid(rr[i]);
-          if (t0 + r < k.len) {
+          if (put) {
             dD = fma(dy, ur[i], dD);
             dbias = dbias + dd;
-          }
-          if (k.on && t0 + r < k.hi) {
-            const bool in = t0 + r < k.len;
-            ((T*)a.du)[k.b * a.sdu.b + (t0 + r) * a.sdu.t + k.c] = in ? fma(dx, dr[i], Dc * dy) : T(0);
-            ((T*)a.ddt)[k.b * a.sddt.b + (t0 + r) * a.sddt.t + k.c] = in ? dd : T(0);
+            *qu = fma(dx, dr[i], Dc * dy);
+            *qd = dd;
           }
         }
         if (s > 0) __syncthreads();
       }
-      const int rows = (int)(k.hi - t0 < TT ? k.hi - t0 : TT);
-      for (int f = threadIdx.x; f < rows * N; f += 64 * W) {
-        const int r = f / N, n = f % N;
+      const int rows = (int)(stop - t0 < TT ? stop - t0 : TT);
+      for (int f = threadIdx.x; f < rows * NP; f += 64 * W) {
+        const int r = f / NP, n = f % NP;
+        if (n >= N) continue;
         const int64_t at = (prow + (t0 + r) * a.G) * N + n;
-        const bool in = t0 + r < k.len;
-        ((T*)a.dBp)[at] = in ? sg[r][n] : T(0);
-        ((T*)a.dCp)[at] = in ? sg[r][NP + n] : T(0);
+        ((T*)a.dBp)[at] = sg[r][n];
+        ((T*)a.dCp)[at] = sg[r][NP + n];
       }
     }
   }
@@ -561,27 +685,27 @@ static void scan_launch(const ScanArgs& a, int W) {
 #undef SCAN_W
 }
 
-static int scan_tile(int dtype, int64_t N) {
-  const int W = waves_for(N);
-  return dtype == DTMI_F32 ? tile_len<float>(W) : tile_len<double>(W);
+static int scan_tile(int dtype) {
+  return dtype == DTMI_F32 ? tile_len<float>() : tile_len<double>();
 }
 
 // Segments of T: one where B * C / 64 blocks already occupy the card. A split
 // costs the exponentials a second time, so it has to more than double the
 // blocks that run at once; then enough segments for two blocks per CU, of at
 // least two tiles each.
-static void scan_segments(ScanArgs& a, int TT) {
-  const int64_t blocks = a.B * a.ct, want = 2 * (int64_t)num_cus(), tiles = cdiv(a.T, TT);
-  int64_t s = blocks * 4 > want ? 1 : want / blocks;
+static void scan_segments(ScanArgs& a, int TT, int per_cu) {
+  const int64_t blocks = a.B * a.ct, want = per_cu * (int64_t)num_cus(), tiles = cdiv(a.T, TT);
+  int64_t s = blocks >= num_cus() ? 1 : want / blocks;
   if (s > tiles / 2) s = tiles / 2;
   if (s < 1) s = 1;
-  a.seglen = cdiv(tiles, s) * TT;
+  a.seglen = (int)(cdiv(tiles, s) * TT);
   a.nseg = (int)cdiv(a.T, a.seglen);
 }
 
 static int scan_shape(const char* what, int dtype, int64_t B, int64_t T, int64_t C, int64_t N, int64_t G) {
   DTMI_CHECK(dtype == DTMI_F32 || dtype == DTMI_F64, "%s: dtype must be DTMI_F32 or DTMI_F64 (got %d)", what, dtype);
   DTMI_CHECK(B >= 0 && T >= 0 && C >= 0, "%s: negative size", what);
+  DTMI_CHECK(T <= 0x7fffff00, "%s: too many positions", what);
   DTMI_CHECK(N >= 1 && N <= 64, "%s: 1 to 64 states (got %lld)", what, (long long)N);
   DTMI_CHECK(G >= 1 && C % G == 0, "%s: %lld channels do not form %lld groups", what, (long long)C, (long long)G);
   return DTMI_OK;
@@ -602,7 +726,7 @@ static int scan_chain(ScanArgs& a, int W, bool backward) {
 template <typename T>
 static int scan_fwd(ScanArgs& a) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(W));
+  scan_segments(a, tile_len<T>(), 4);
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256,
              "dtmi_scan_fwd: too many elements");
   void* ws = nullptr;
@@ -628,7 +752,7 @@ template <typename T>
 static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* dC, BT sdC, int64_t gdC, void* dD,
                     void* dbias) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(W));
+  scan_segments(a, tile_len<T>(), 2);
   const int64_t maps = a.B * a.T * a.G * a.N;
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256 &&
                  maps <= (int64_t)0x7fffffff * 256,
@@ -675,7 +799,7 @@ DTMI_EXPORT int dtmi_scan_kept(int dtype, int64_t B, int64_t T, int64_t C, int64
   DTMI_BODY_BEGIN
   if (int rc = scan_shape("dtmi_scan_kept", dtype, B, T, C, N, 1)) return rc;
   DTMI_CHECK(count, "dtmi_scan_kept: NULL result");
-  *count = B * cdiv(T, scan_tile(dtype, N)) * N * C;
+  *count = B * cdiv(T, scan_tile(dtype)) * N * C;
   return DTMI_OK;
   DTMI_BODY_END
 }
