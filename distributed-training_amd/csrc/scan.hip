@@ -52,6 +52,12 @@ __host__ __device__ constexpr int held_len(int W) {
 }
 static int waves_for(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
+// Element strides of the batch axis and of positions (below 2^31, checked on the host).
+struct Rows {
+  int64_t b;
+  int t;
+};
+
 struct ScanArgs {
   const void *u, *dt, *A, *Bm, *Cm, *D, *z, *bias, *h0, *g;
   const int64_t* lengths;
@@ -60,7 +66,7 @@ struct ScanArgs {
   void *dBp, *dCp;      // [channel tiles of a group][B][T][G][N], contiguous
   void *prm;            // [B * segments][N + 2][C]: dA, dD, dbias terms
   void *carry, *dsum;   // [B][segments][N][C], [B][segments][C]
-  BT su, sdt, sz, sout, sg, sdu, sddt, sdz, sB, sC;
+  Rows su, sdt, sz, sout, sg, sdu, sddt, sdz, sB, sC;
   int64_t gB, gC;       // group strides of B and C
   int64_t B, T, C, N, G;
   int seglen;           // positions per segment, a multiple of the tile
@@ -69,7 +75,8 @@ struct ScanArgs {
 };
 
 struct ScanBlock {
-  int64_t b, c, cc;    // cc: c, or the group's last channel for an idle lane
+  int64_t b, c, c0;    // c0: the wave's first channel
+  unsigned at;         // the lane's channel from c0 on (an idle lane: the group's last)
   int len, lo, hi;     // the sequence's length, the segment's positions
   int seg, grp, tile;  // segment, group, channel tile within the group
   bool on;
@@ -85,7 +92,8 @@ __device__ __forceinline__ ScanBlock scan_block(const ScanArgs& a) {
   const int64_t each = a.C / a.G, off = (int64_t)k.tile * 64 + (threadIdx.x & 63);
   k.on = off < each;
   k.c = k.grp * each + off;
-  k.cc = k.on ? k.c : k.grp * each + each - 1;
+  k.c0 = k.grp * each + (int64_t)k.tile * 64;
+  k.at = (unsigned)(k.on ? off : each - 1) - (unsigned)k.tile * 64u;
   k.len = (int)seq_len(a.lengths, k.b, a.T);
   k.lo = k.seg * a.seglen;
   k.hi = (int)(a.T - k.lo > a.seglen ? k.lo + a.seglen : a.T);
@@ -105,24 +113,25 @@ template <typename T, int W, int TT>
 struct Tile {
   static constexpr int RPW = (TT + W - 1) / W, NP = W * kStates, MAPS = (TT * NP + 64 * W - 1) / (64 * W);
   T u[RPW], d[RPW], z[RPW], g[RPW], b[MAPS], c[MAPS];
-  __device__ __forceinline__ void rows(T (&x)[RPW], const T* __restrict__ p, int64_t st, int t0, int len, int w) {
+  // p: the wave's first channel, so row addresses are scalars and a lane adds 32 bits
+  __device__ __forceinline__ void rows(T (&x)[RPW], const T* __restrict__ p, int st, int t0, int len, int w, unsigned at) {
     if (t0 + (TT > W ? TT : W) <= len) {
-      const T* q = p + (t0 + w) * st;
+      const T* q = p + (int64_t)(t0 + w) * st;
 #pragma unroll
-      for (int i = 0; i < RPW; ++i, q += W * st) x[i] = *q;
+      for (int i = 0; i < RPW; ++i, q += (int64_t)W * st) x[i] = q[at];
     } else {
 #pragma unroll
       for (int i = 0; i < RPW; ++i) {
         const int t = t0 + w + W * i;
-        x[i] = p[(t < len ? t : len - 1) * st];
+        x[i] = (p + (int64_t)(t < len ? t : len - 1) * st)[at];
       }
     }
   }
-  __device__ __forceinline__ void map(T (&x)[MAPS], const T* __restrict__ p, int64_t st, int t0, int len, int N) {
+  __device__ __forceinline__ void map(T (&x)[MAPS], const T* __restrict__ p, int st, int t0, int len, int N) {
 #pragma unroll
     for (int i = 0; i < MAPS; ++i) {
       const int f = threadIdx.x + 64 * W * i, n = f % NP, t = t0 + f / NP;
-      x[i] = p[(t < len ? t : len - 1) * st + (n < N ? n : N - 1)];
+      x[i] = p[(int64_t)(t < len ? t : len - 1) * st + (n < N ? n : N - 1)];
     }
   }
   static __device__ __forceinline__ void put_map(T* __restrict__ s, const T (&x)[MAPS], int t0, int len, int N) {
@@ -141,41 +150,41 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
   constexpr int NS = kStates, TT = tile_len<T>(), YT = sum_len<T>(W);
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP;
-  __shared__ T sd[TT][64], sx[TT][64], yp[CARRY ? 1 : W][CARRY ? 1 : YT][64];
   __shared__ __attribute__((aligned(16))) T sB[TT * NP], sC[CARRY ? 1 : TT * NP];
+  __shared__ T sd[TT][64], sx[TT][64], yp[CARRY ? 1 : W][CARRY ? 1 : YT][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ScanBlock k = scan_block(a);
   const int N = (int)a.N, n0 = w * NS;
-  const T* up = (const T*)a.u + k.b * a.su.b + k.cc;
-  const T* dp = (const T*)a.dt + k.b * a.sdt.b + k.cc;
-  const T* zp = a.z ? (const T*)a.z + k.b * a.sz.b + k.cc : nullptr;
+  const T* up = (const T*)a.u + k.b * a.su.b + k.c0;
+  const T* dp = (const T*)a.dt + k.b * a.sdt.b + k.c0;
+  const T* zp = a.z ? (const T*)a.z + k.b * a.sz.b + k.c0 : nullptr;
   const T* Bp = (const T*)a.Bm + k.b * a.sB.b + k.grp * a.gB;
   const T* Cp = (const T*)a.Cm + k.b * a.sC.b + k.grp * a.gC;
-  T* op = CARRY ? nullptr : (T*)a.out + k.b * a.sout.b + k.cc;
-  const T bias = a.bias ? ((const T*)a.bias)[k.cc] : T(0);
-  const T Dc = !CARRY && a.D ? ((const T*)a.D)[k.cc] : T(0);
+  T* op = CARRY ? nullptr : (T*)a.out + k.b * a.sout.b + k.c0;
+  const T bias = a.bias ? ((const T*)a.bias + k.c0)[k.at] : T(0);
+  const T Dc = !CARRY && a.D ? ((const T*)a.D + k.c0)[k.at] : T(0);
   T A2[NS], h[NS], total = T(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    A2[j] = n0 + j < N ? ((const T*)a.A)[k.cc * N + n0 + j] * T(kLog2e) : T(0);
+    A2[j] = n0 + j < N ? ((const T*)a.A)[(k.c0 + k.at) * N + n0 + j] * T(kLog2e) : T(0);
     h[j] = T(0);
     if (!CARRY && n0 + j < N) {
       if (a.nseg > 1)
-        h[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.cc];
+        h[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c0 + k.at];
       else if (a.h0)
-        h[j] = ((const T*)a.h0)[(k.b * a.C + k.cc) * N + n0 + j];
+        h[j] = ((const T*)a.h0)[(k.b * a.C + k.c0 + k.at) * N + n0 + j];
     }
   }
   const int64_t ntiles = (a.T + TT - 1) / TT;
   const int stop = k.hi < k.len ? k.hi : k.len;  // positions at and past it do nothing
   In in;
   auto fetch = [&](int t0) {
-    in.rows(in.u, up, a.su.t, t0, k.len, w);
-    in.rows(in.d, dp, a.sdt.t, t0, k.len, w);
+    in.rows(in.u, up, a.su.t, t0, k.len, w, k.at);
+    in.rows(in.d, dp, a.sdt.t, t0, k.len, w, k.at);
     in.map(in.b, Bp, a.sB.t, t0, k.len, N);
+    if constexpr (!CARRY) in.map(in.c, Cp, a.sC.t, t0, k.len, N);
     if constexpr (!CARRY) {
-      if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w);
-      in.map(in.c, Cp, a.sC.t, t0, k.len, N);
+      if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w, k.at);
     }
   };
   if (k.lo < stop) fetch(k.lo);
@@ -193,13 +202,13 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
       sx[r][lane] = d * ur[i];
     }
     In::put_map(sB, in.b, t0, k.len, N);
+    if constexpr (!CARRY) In::put_map(sC, in.c, t0, k.len, N);
     if constexpr (!CARRY) {
-      In::put_map(sC, in.c, t0, k.len, N);
       if (a.kept && k.on) {
-        T* kp = (T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c;
+        T* kp = (T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c0;
 #pragma unroll
         for (int j = 0; j < NS; ++j)
-          if (n0 + j < N) kp[j * a.C] = h[j];
+          if (n0 + j < N) (kp + j * a.C)[k.at] = h[j];
       }
     }
     __syncthreads();
@@ -223,9 +232,9 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
       }
       __syncthreads();
       if constexpr (!CARRY) {
-        T* q = op + (t0 + w) * a.sout.t;
+        T* q = op + (int64_t)(t0 + w) * a.sout.t;
 #pragma unroll
-        for (int i = 0; i < RPW; ++i, q += W * a.sout.t) {
+        for (int i = 0; i < RPW; ++i, q += (int64_t)W * a.sout.t) {
           const int r = w + W * i;
           if (r / YT != s || r >= TT) continue;
           T y = T(0);
@@ -233,7 +242,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
           for (int v = 0; v < W; ++v) y = y + yp[v][r % YT][lane];
           y = fma(Dc, ur[i], y);
           if (zp) y = y * (zr[i] * sigmoid(zr[i]));
-          if (k.on && t0 + r < stop) *q = y;
+          if (k.on && t0 + r < stop) q[k.at] = y;
         }
         if (TT != YT) __syncthreads();
       }
@@ -247,7 +256,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
       if (n0 + j < N) ((T*)a.carry)[(at * N + n0 + j) * a.C + k.c] = h[j];
     if (w == 0) ((T*)a.dsum)[at * a.C + k.c] = total;
   } else {
-    for (int t = (stop > k.lo ? stop : k.lo) + w; t < k.hi; t += W) op[t * a.sout.t] = T(0);
+    for (int t = (stop > k.lo ? stop : k.lo) + w; t < k.hi; t += W) (op + (int64_t)t * a.sout.t)[k.at] = T(0);
     if (a.hT && k.seg == a.nseg - 1) {
 #pragma unroll
       for (int j = 0; j < NS; ++j)
@@ -266,12 +275,25 @@ __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backwar
   if (b >= a.B) return;
   const T A2 = ((const T*)a.A)[c * a.N + n] * T(kLog2e);
   T in = !backward && a.h0 ? ((const T*)a.h0)[(b * a.C + c) * a.N + n] : T(0);
-  for (int i = 0; i < a.nseg; ++i) {
-    const int64_t at = b * a.nseg + (backward ? a.nseg - 1 - i : i);
-    T* p = (T*)a.carry + (at * a.N + n) * a.C + c;
-    const T local = *p, decay = exp2_of(A2 * ((const T*)a.dsum)[at * a.C + c]);
-    *p = in;
-    in = fma(decay, in, local);
+  // the loads do not wait for the chain: eight segments' at a time
+  constexpr int U = 8;
+  const int64_t step = backward ? -1 : 1, from = b * a.nseg + (backward ? a.nseg - 1 : 0);
+  T* p = (T*)a.carry + (from * a.N + n) * a.C + c;
+  const T* d = (const T*)a.dsum + from * a.C + c;
+  for (int i = 0; i < a.nseg; i += U) {
+    T local[U], sum[U];
+#pragma unroll
+    for (int v = 0; v < U; ++v) {
+      const int64_t at = step * (i + v < a.nseg ? i + v : a.nseg - 1);
+      local[v] = p[at * a.N * a.C];
+      sum[v] = d[at * a.C];
+    }
+#pragma unroll
+    for (int v = 0; v < U; ++v) {
+      if (i + v >= a.nseg) break;
+      p[step * (i + v) * a.N * a.C] = in;
+      in = fma(exp2_of(A2 * sum[v]), in, local[v]);
+    }
   }
 }
 
@@ -349,22 +371,22 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const ScanBlock k = scan_block(a);
   const int N = (int)a.N, n0 = w * NS;
-  const T* up = (const T*)a.u + k.b * a.su.b + k.cc;
-  const T* dp = (const T*)a.dt + k.b * a.sdt.b + k.cc;
-  const T* zp = a.z ? (const T*)a.z + k.b * a.sz.b + k.cc : nullptr;
-  const T* gp = (const T*)a.g + k.b * a.sg.b + k.cc;
+  const T* up = (const T*)a.u + k.b * a.su.b + k.c0;
+  const T* dp = (const T*)a.dt + k.b * a.sdt.b + k.c0;
+  const T* zp = a.z ? (const T*)a.z + k.b * a.sz.b + k.c0 : nullptr;
+  const T* gp = (const T*)a.g + k.b * a.sg.b + k.c0;
   const T* Bp = (const T*)a.Bm + k.b * a.sB.b + k.grp * a.gB;
   const T* Cp = (const T*)a.Cm + k.b * a.sC.b + k.grp * a.gC;
-  const T bias = a.bias ? ((const T*)a.bias)[k.cc] : T(0);
-  const T Dc = a.D ? ((const T*)a.D)[k.cc] : T(0);
+  const T bias = a.bias ? ((const T*)a.bias + k.c0)[k.at] : T(0);
+  const T Dc = a.D ? ((const T*)a.D + k.c0)[k.at] : T(0);
   T An[NS], A2[NS], dh[NS], dA[NS], total = T(0), dD = T(0), dbias = T(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    An[j] = n0 + j < N ? ((const T*)a.A)[k.cc * N + n0 + j] : T(0);
+    An[j] = n0 + j < N ? ((const T*)a.A)[(k.c0 + k.at) * N + n0 + j] : T(0);
     A2[j] = An[j] * T(kLog2e);
     dA[j] = dh[j] = T(0);
     if (!CARRY && a.nseg > 1 && n0 + j < N)
-      dh[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.cc];
+      dh[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c0 + k.at];
   }
   const int64_t ntiles = (a.T + TT - 1) / TT;
   const int stop = k.hi < k.len ? k.hi : k.len;
@@ -374,9 +396,9 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
     const int from = stop > k.lo ? stop : k.lo;
     if (k.on)
       for (int t = from + w; t < k.hi; t += W) {
-        ((T*)a.du)[k.b * a.sdu.b + t * a.sdu.t + k.c] = T(0);
-        ((T*)a.ddt)[k.b * a.sddt.b + t * a.sddt.t + k.c] = T(0);
-        if (zp) ((T*)a.dz)[k.b * a.sdz.b + t * a.sdz.t + k.c] = T(0);
+        ((T*)a.du)[k.b * a.sdu.b + (int64_t)t * a.sdu.t + k.c] = T(0);
+        ((T*)a.ddt)[k.b * a.sddt.b + (int64_t)t * a.sddt.t + k.c] = T(0);
+        if (zp) ((T*)a.dz)[k.b * a.sdz.b + (int64_t)t * a.sdz.t + k.c] = T(0);
       }
     for (int64_t f = threadIdx.x; f < (int64_t)(k.hi - from) * N; f += 64 * W) {
       const int64_t at = (prow + (from + f / N) * a.G) * N + f % N;
@@ -387,24 +409,24 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
   In in;
   T kept[NS];
   auto fetch = [&](int t0) {
-    in.rows(in.d, dp, a.sdt.t, t0, k.len, w);
-    in.rows(in.g, gp, a.sg.t, t0, k.len, w);
-    if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w);
+    in.rows(in.d, dp, a.sdt.t, t0, k.len, w, k.at);
+    in.rows(in.g, gp, a.sg.t, t0, k.len, w, k.at);
+    if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w, k.at);
     in.map(in.c, Cp, a.sC.t, t0, k.len, N);
     if constexpr (!CARRY) {
-      in.rows(in.u, up, a.su.t, t0, k.len, w);
+      in.rows(in.u, up, a.su.t, t0, k.len, w, k.at);
       in.map(in.b, Bp, a.sB.t, t0, k.len, N);
-      const T* kp = (const T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.cc;
+      const T* kp = (const T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c0;
 #pragma unroll
-      for (int j = 0; j < NS; ++j) kept[j] = n0 + j < N ? kp[j * a.C] : T(0);
+      for (int j = 0; j < NS; ++j) kept[j] = n0 + j < N ? (kp + j * a.C)[k.at] : T(0);
     }
   };
   const int first = k.lo + (stop - 1 - k.lo) / TT * TT;
   T *dup = nullptr, *ddp = nullptr, *dzp = nullptr;
   if constexpr (!CARRY) {
-    dup = (T*)a.du + k.b * a.sdu.b + k.c;
-    ddp = (T*)a.ddt + k.b * a.sddt.b + k.c;
-    if (zp) dzp = (T*)a.dz + k.b * a.sdz.b + k.c;
+    dup = (T*)a.du + k.b * a.sdu.b + k.c0;
+    ddp = (T*)a.ddt + k.b * a.sddt.b + k.c0;
+    if (zp) dzp = (T*)a.dz + k.b * a.sdz.b + k.c0;
   }
   if (k.lo < stop) fetch(first);
   for (int t0 = first; k.lo < stop && t0 >= k.lo; t0 -= TT) {
@@ -506,9 +528,10 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
             sg[r + (lane & 7)][(lane >> 5) * NP + n0 + ((lane >> 3) & 3)] = sums;
         }
         __syncthreads();
-        T *qu = dup + (t0 + w) * a.sdu.t, *qd = ddp + (t0 + w) * a.sddt.t, *qz = dzp + (t0 + w) * a.sdz.t;
+        T *qu = dup + (int64_t)(t0 + w) * a.sdu.t, *qd = ddp + (int64_t)(t0 + w) * a.sddt.t;
+        T* qz = dzp + (int64_t)(t0 + w) * a.sdz.t;
 #pragma unroll
-        for (int i = 0; i < RPW; ++i, qu += W * a.sdu.t, qd += W * a.sddt.t, qz += W * a.sdz.t) {
+        for (int i = 0; i < RPW; ++i, qu += (int64_t)W * a.sdu.t, qd += (int64_t)W * a.sddt.t, qz += (int64_t)W * a.sdz.t) {
           const int r = w + W * i;
           if (r / HT != s || r >= TT) continue;
           T y = T(0), dx = T(0), e = T(0);
@@ -525,15 +548,15 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
             y = fma(Dc, ur[i], y);
             const T dz = gr[i] * y * (sz * fma(zr[i], T(1) - sz, T(1)));
             dy = gr[i] * (zr[i] * sz);
-            if (put) *qz = dz;
+            if (put) qz[k.at] = dz;
           }
           T dd = fma(dx, ur[i], e);
           if (a.softplus) dd = dd * sigmoid(rr[i]);
           if (put) {
             dD = fma(dy, ur[i], dD);
             dbias = dbias + dd;
-            *qu = fma(dx, dr[i], Dc * dy);
-            *qd = dd;
+            qu[k.at] = fma(dx, dr[i], Dc * dy);
+            qd[k.at] = dd;
           }
         }
         if (s > 0) __syncthreads();
@@ -785,6 +808,12 @@ static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* 
 }
 
 static BT bt(const int64_t* s) { return s ? BT{s[0], s[1]} : BT{0, 0}; }
+// False for a distance between positions that 32 bits do not hold.
+static bool rows_of(Rows& r, const int64_t* s) {
+  if (!s) return true;
+  r = {s[0], (int)s[1]};
+  return s[1] == r.t;
+}
 
 static void scan_tiles(ScanArgs& a) {
   a.tpg = (int)cdiv(a.C / a.G, 64);
@@ -825,8 +854,10 @@ DTMI_EXPORT int dtmi_scan_fwd(int dtype, int64_t B, int64_t T, int64_t C, int64_
   ScanArgs a{};
   a.u = u, a.dt = dt, a.A = A, a.Bm = Bm, a.Cm = Cm, a.D = D, a.z = z, a.bias = dt_bias, a.h0 = state;
   a.lengths = lengths, a.out = out, a.hT = state_out, a.kept = kept, a.softplus = softplus;
-  a.su = bt(u_strides), a.sdt = bt(dt_strides), a.sz = bt(z_strides), a.sout = bt(out_strides);
-  a.sB = bt(B_strides), a.gB = B_strides[2], a.sC = bt(C_strides), a.gC = C_strides[2];
+  DTMI_CHECK(rows_of(a.su, u_strides) && rows_of(a.sdt, dt_strides) && rows_of(a.sz, z_strides) &&
+                 rows_of(a.sout, out_strides) && rows_of(a.sB, B_strides) && rows_of(a.sC, C_strides),
+             "dtmi_scan_fwd: positions more than 2^31 elements apart");
+  a.gB = B_strides[2], a.gC = C_strides[2];
   a.B = B, a.T = T, a.C = C, a.N = N, a.G = G;
   scan_tiles(a);
   TimedLaunch tl(DTMI_FAM_OTHER, 7.0 * B * T * C * N);
@@ -864,9 +895,11 @@ DTMI_EXPORT int dtmi_scan_bwd(int dtype, int64_t B, int64_t T, int64_t C, int64_
   a.u = u, a.dt = dt, a.A = A, a.Bm = Bm, a.Cm = Cm, a.D = D, a.z = z, a.bias = dt_bias, a.g = g;
   a.lengths = lengths, a.kept = const_cast<void*>(kept), a.softplus = softplus;
   a.du = du, a.ddt = ddt, a.dz = dz, a.dh0 = dstate;
-  a.su = bt(u_strides), a.sdt = bt(dt_strides), a.sz = bt(z_strides), a.sg = bt(g_strides);
-  a.sdu = bt(du_strides), a.sddt = bt(ddt_strides), a.sdz = bt(dz_strides);
-  a.sB = bt(B_strides), a.gB = B_strides[2], a.sC = bt(C_strides), a.gC = C_strides[2];
+  DTMI_CHECK(rows_of(a.su, u_strides) && rows_of(a.sdt, dt_strides) && rows_of(a.sz, z_strides) &&
+                 rows_of(a.sg, g_strides) && rows_of(a.sB, B_strides) && rows_of(a.sC, C_strides) &&
+                 rows_of(a.sdu, du_strides) && rows_of(a.sddt, ddt_strides) && rows_of(a.sdz, dz_strides),
+             "dtmi_scan_bwd: positions more than 2^31 elements apart");
+  a.gB = B_strides[2], a.gC = C_strides[2];
   a.B = B, a.T = T, a.C = C, a.N = N, a.G = G;
   scan_tiles(a);
   TimedLaunch tl(DTMI_FAM_OTHER, 14.0 * B * T * C * N);
