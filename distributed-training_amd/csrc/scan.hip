@@ -24,14 +24,15 @@
 // exp(A sum d): no products of decays are kept), and the full pass starts
 // each segment from its true state. Results do not depend on timing; the
 // number of segments follows from the shape alone.
+#include "bufrsrc.h"
 #include "seqmath.h"
 
 namespace dtmi {
 
 constexpr int kStates = 4;  // states per lane
-constexpr double kLog2e = 1.4426950408889634;
+constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
-// Positions per tile; the state before each tile is kept for the backward.
+// Positions per tile.
 template <typename T>
 __host__ __device__ constexpr int tile_len() {
   return sizeof(T) == 4 ? 16 : 8;
@@ -43,12 +44,23 @@ __host__ __device__ constexpr int sum_len(int W) {
   return n < t ? n : t;
 }
 // Positions whose states and decays a backward wave holds in registers at a
-// time (8 per position and lane): a whole tile's would leave room for one wave
-// per SIMD, so a tile is gone over in parts, the states before each part
-// rebuilt once. Sixteen waves share the registers of a block of twice the size.
+// time (8 values per position and lane): a whole tile's would leave room for
+// one wave per SIMD, so a tile is gone over in parts. Sixteen waves share the
+// registers of a block of twice the size.
 template <typename T>
 __host__ __device__ constexpr int held_len(int W) {
   return (sizeof(T) == 4 ? 8 : 4) / (W <= 8 ? 1 : 2);
+}
+// Waves per SIMD the backward's registers are cut to: two of 219 (float32, 9 to
+// 16 states). Three of 168 spill, and a spill's store counts as one to wait for.
+__host__ __device__ constexpr int bwd_waves(int W) { return W == 16 ? 4 : 2; }
+// Positions per state kept for the backward, which rebuilds the states in
+// between. float32 keeps one per part (16 states: two activations' memory,
+// 5 us more traffic against 10 us of exponentials at 4 x 1024 x 1536 x 16);
+// from 33 states on, and in float64, memory counts for more: one per tile.
+template <typename T>
+__host__ __device__ constexpr int keep_len(int W) {
+  return sizeof(T) == 4 && W <= 8 ? held_len<T>(W) : tile_len<T>();
 }
 static int waves_for(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
@@ -75,10 +87,10 @@ struct ScanArgs {
 };
 
 struct ScanBlock {
-  int64_t b, c, c0;    // c0: the wave's first channel
-  unsigned at;         // the lane's channel from c0 on (an idle lane: the group's last)
+  int64_t b, c, c0;    // the lane's channel, the first of the block's
   int len, lo, hi;     // the sequence's length, the segment's positions
   int seg, grp, tile;  // segment, group, channel tile within the group
+  int cnt;             // channels of the block: lanes from there on are idle
   bool on;
 };
 
@@ -93,45 +105,85 @@ __device__ __forceinline__ ScanBlock scan_block(const ScanArgs& a) {
   k.on = off < each;
   k.c = k.grp * each + off;
   k.c0 = k.grp * each + (int64_t)k.tile * 64;
-  k.at = (unsigned)(k.on ? off : each - 1) - (unsigned)k.tile * 64u;
+  k.cnt = (int)(each - (int64_t)k.tile * 64 < 64 ? each - (int64_t)k.tile * 64 : 64);
   k.len = (int)seq_len(a.lengths, k.b, a.T);
   k.lo = k.seg * a.seglen;
   k.hi = (int)(a.T - k.lo > a.seglen ? k.lo + a.seglen : a.T);
   return k;
 }
 
+// d of one position, 0 where there is none. Both branches are the same for all
+// lanes; the sum is formed ahead of them, so that they hold no wait for a load
+// (the count of stores since would be lost, see Row).
 template <typename T>
-__device__ __forceinline__ T step_size(T raw, int softp) {
-  return softp ? softplus(raw) : raw;
+__device__ __forceinline__ T step_size(T raw, int softp, bool there) {
+  asm volatile("" : "+v"(raw));
+  const T d = softp ? softplus(raw) : raw;
+  return there ? d : T(0);
 }
 
+template <typename T>
+__device__ __forceinline__ void store_at(Rsrc r, int off, T x) {
+  typedef int i2 __attribute__((ext_vector_type(2)));
+  if constexpr (sizeof(T) == 4)
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, x), r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i2, x), r, off, 0, 0);
+}
+
+// A row of a block's channels (p: its first, the same for all lanes): a buffer
+// that ends with the block's channels, or is empty for a row that is not there.
+// Lanes and rows outside read 0 and write nothing. The addresses take no vector
+// registers (64-bit lane addresses of a tile's rows in seven arrays took 56),
+// and the tile loop's loads and stores no branches: where a store may or may
+// not have been issued, the wait for the next tile's loads becomes a wait for
+// every store as well, 1.7 us per tile for a wave alone on its SIMD.
+template <typename T>
+struct Row {
+  Rsrc r;
+  __device__ __forceinline__ Row(const T* p, bool there, int cnt) : r(make_rsrc(p, there ? cnt * (int)sizeof(T) : 0)) {}
+  __device__ __forceinline__ T get() const {
+    const int off = (threadIdx.x & 63) * (int)sizeof(T);
+    if constexpr (sizeof(T) == 4)
+      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    else
+      return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+  }
+  __device__ __forceinline__ void put(T x) const { store_at(r, (threadIdx.x & 63) * (int)sizeof(T), x); }
+};
+
+// A value the compiler takes as new: row addresses formed from it are computed
+// where they are used, not carried as a scalar per row and array through the
+// loop (more than the scalar registers hold).
+__device__ __forceinline__ int renewed(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
+// s_waitcnt vmcnt(0) ahead of the tile loop: with loads in flight at its entry
+// the first wait inside would cover both ways into the loop, which is every
+// store of the tile before.
+__device__ __forceinline__ void drain_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // A wave's rows of a tile (r = w, w + W, ...) and the block's share of the
-// tile's maps, on their way from global memory. Positions at and past the
-// length read the last one that holds data and are masked when the tile is
-// staged, so no load waits for a branch.
+// tile's maps, on their way from global memory.
 template <typename T, int W, int TT>
 struct Tile {
   static constexpr int RPW = (TT + W - 1) / W, NP = W * kStates, MAPS = (TT * NP + 64 * W - 1) / (64 * W);
   T u[RPW], d[RPW], z[RPW], g[RPW], b[MAPS], c[MAPS];
-  // p: the wave's first channel, so row addresses are scalars and a lane adds 32 bits
-  __device__ __forceinline__ void rows(T (&x)[RPW], const T* __restrict__ p, int st, int t0, int len, int w, unsigned at) {
-    if (t0 + (TT > W ? TT : W) <= len) {
-      const T* q = p + (int64_t)(t0 + w) * st;
+  __device__ __forceinline__ void rows(T (&x)[RPW], const T* __restrict__ p, int st, int t0, const ScanBlock& k, int w,
+                                       bool there = true) {
+    const T* q = p + (int64_t)(t0 + w) * st;
 #pragma unroll
-      for (int i = 0; i < RPW; ++i, q += (int64_t)W * st) x[i] = q[at];
-    } else {
-#pragma unroll
-      for (int i = 0; i < RPW; ++i) {
-        const int t = t0 + w + W * i;
-        x[i] = (p + (int64_t)(t < len ? t : len - 1) * st)[at];
-      }
-    }
+    for (int i = 0; i < RPW; ++i, q += (int64_t)W * st)
+      x[i] = Row<T>(q, there && (unsigned)(t0 + w + W * i) < (unsigned)k.len, k.cnt).get();
   }
+  // (a map's position outside the sequence reads one inside and is masked when staged)
   __device__ __forceinline__ void map(T (&x)[MAPS], const T* __restrict__ p, int st, int t0, int len, int N) {
 #pragma unroll
     for (int i = 0; i < MAPS; ++i) {
-      const int f = threadIdx.x + 64 * W * i, n = f % NP, t = t0 + f / NP;
-      x[i] = p[(int64_t)(t < len ? t : len - 1) * st + (n < N ? n : N - 1)];
+      const int f = threadIdx.x + 64 * W * i, n = f % NP, t = t0 + f / NP < len ? t0 + f / NP : len - 1;
+      x[i] = p[(int64_t)(t > 0 ? t : 0) * st + (n < N ? n : N - 1)];
     }
   }
   static __device__ __forceinline__ void put_map(T* __restrict__ s, const T (&x)[MAPS], int t0, int len, int N) {
@@ -144,10 +196,19 @@ struct Tile {
   }
 };
 
+// What a wave reads from LDS for one position. The next positions' are asked
+// for before the current ones' arithmetic, and kept there by scheduling
+// barriers: left to itself the compiler reads them right before their use, and
+// a wave alone on its SIMD then waits out the LDS latency at every position.
+template <typename T>
+struct Step {
+  T d, x, g, b[kStates], c[kStates];
+};
+
 // CARRY: only the segment's end state from a zero start, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(), YT = sum_len<T>(W);
+  constexpr int NS = kStates, TT = tile_len<T>(), YT = sum_len<T>(W), KT = keep_len<T>(W);
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP;
   __shared__ __attribute__((aligned(16))) T sB[TT * NP], sC[CARRY ? 1 : TT * NP];
@@ -157,92 +218,116 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
   const int N = (int)a.N, n0 = w * NS;
   const T* up = (const T*)a.u + k.b * a.su.b + k.c0;
   const T* dp = (const T*)a.dt + k.b * a.sdt.b + k.c0;
-  const T* zp = a.z ? (const T*)a.z + k.b * a.sz.b + k.c0 : nullptr;
+  const T* zp = (const T*)a.z + k.b * a.sz.b + k.c0;
+  const bool gate = a.z != nullptr, keep = a.kept != nullptr;
   const T* Bp = (const T*)a.Bm + k.b * a.sB.b + k.grp * a.gB;
   const T* Cp = (const T*)a.Cm + k.b * a.sC.b + k.grp * a.gC;
   T* op = CARRY ? nullptr : (T*)a.out + k.b * a.sout.b + k.c0;
-  const T bias = a.bias ? ((const T*)a.bias + k.c0)[k.at] : T(0);
-  const T Dc = !CARRY && a.D ? ((const T*)a.D + k.c0)[k.at] : T(0);
+  const T bias = a.bias ? Row<T>((const T*)a.bias + k.c0, true, k.cnt).get() : T(0);
+  const T Dc = !CARRY && a.D ? Row<T>((const T*)a.D + k.c0, true, k.cnt).get() : T(0);
   T A2[NS], h[NS], total = T(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    A2[j] = n0 + j < N ? ((const T*)a.A)[(k.c0 + k.at) * N + n0 + j] * T(kLog2e) : T(0);
+    A2[j] = k.on && n0 + j < N ? ((const T*)a.A)[k.c * N + n0 + j] * T(kLog2e) : T(0);
     h[j] = T(0);
-    if (!CARRY && n0 + j < N) {
+    if (!CARRY && k.on && n0 + j < N) {
       if (a.nseg > 1)
-        h[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c0 + k.at];
+        h[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c];
       else if (a.h0)
-        h[j] = ((const T*)a.h0)[(k.b * a.C + k.c0 + k.at) * N + n0 + j];
+        h[j] = ((const T*)a.h0)[(k.b * a.C + k.c) * N + n0 + j];
     }
   }
-  const int64_t ntiles = (a.T + TT - 1) / TT;
+  const int64_t nkept = (a.T + KT - 1) / KT;
   const int stop = k.hi < k.len ? k.hi : k.len;  // positions at and past it do nothing
   In in;
-  auto fetch = [&](int t0) {
-    in.rows(in.u, up, a.su.t, t0, k.len, w, k.at);
-    in.rows(in.d, dp, a.sdt.t, t0, k.len, w, k.at);
+  auto fetch = [&](int from) {
+    const int t0 = renewed(from);
+    in.rows(in.u, up, a.su.t, t0, k, w);
+    in.rows(in.d, dp, a.sdt.t, t0, k, w);
     in.map(in.b, Bp, a.sB.t, t0, k.len, N);
     if constexpr (!CARRY) in.map(in.c, Cp, a.sC.t, t0, k.len, N);
     if constexpr (!CARRY) {
-      if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w, k.at);
+      in.rows(in.z, zp, a.sz.t, t0, k, w, gate);
     }
   };
   if (k.lo < stop) fetch(k.lo);
+  drain_loads();
   for (int t0 = k.lo; t0 < stop; t0 += TT) {
     T ur[RPW], zr[RPW];
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       const int r = w + W * i;
       if (W * RPW != TT && r >= TT) break;
-      const bool on = t0 + r < k.len;
-      const T d = on ? step_size(in.d[i] + bias, a.softplus) : T(0);
-      ur[i] = on ? in.u[i] : T(0);
+      const T d = step_size(in.d[i] + bias, a.softplus, t0 + r < k.len);
+      ur[i] = in.u[i];
       if (!CARRY) zr[i] = in.z[i];
       sd[r][lane] = d;
       sx[r][lane] = d * ur[i];
     }
     In::put_map(sB, in.b, t0, k.len, N);
     if constexpr (!CARRY) In::put_map(sC, in.c, t0, k.len, N);
-    if constexpr (!CARRY) {
-      if (a.kept && k.on) {
-        T* kp = (T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c0;
-#pragma unroll
-        for (int j = 0; j < NS; ++j)
-          if (n0 + j < N) (kp + j * a.C)[k.at] = h[j];
-      }
-    }
     __syncthreads();
-    if (t0 + TT < stop) fetch(t0 + TT);
+    fetch(t0 + TT);
+    constexpr int PF = 2;  // positions read ahead
+    Step<T> at[PF], next[PF];
+    auto read = [&](Step<T>(&x)[PF], int r) {
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        x[i].d = sd[r + i][lane];
+        x[i].x = sx[r + i][lane];
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          x[i].b[j] = sB[(r + i) * NP + n0 + j];
+          if constexpr (!CARRY) x[i].c[j] = sC[(r + i) * NP + n0 + j];
+        }
+      }
+    };
+    read(at, 0);
 #pragma unroll
     for (int s = 0; s < TT / YT; ++s) {
 #pragma unroll
-      for (int q = 0; q < YT; ++q) {
-        const int r = s * YT + q;
-        const T d = sd[r][lane], x = sx[r][lane];
-        T y = T(0);
+      for (int q = 0; q < YT; q += PF) {
+        if (s * YT + q + PF < TT) read(next, s * YT + q + PF);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < NS; ++j) {
-          h[j] = fma(exp2_of(d * A2[j]), h[j], x * sB[r * NP + n0 + j]);
-          if constexpr (!CARRY) y = fma(sC[r * NP + n0 + j], h[j], y);
+        for (int i = 0; i < PF; ++i) {
+          const int r = s * YT + q + i;
+          if constexpr (!CARRY) {
+            if (r % KT == 0) {
+              const int t = renewed(t0) + r;
+              const T* kp = (const T*)a.kept + ((k.b * nkept + t / KT) * N + n0) * a.C + k.c0;
+#pragma unroll
+              for (int j = 0; j < NS; ++j) Row<T>(kp + j * a.C, keep && t < stop && n0 + j < N, k.cnt).put(h[j]);
+            }
+          }
+          T y = T(0);
+#pragma unroll
+          for (int j = 0; j < NS; ++j) {
+            h[j] = fma(exp2_of(at[i].d * A2[j]), h[j], at[i].x * at[i].b[j]);
+            if constexpr (!CARRY) y = fma(at[i].c[j], h[j], y);
+          }
+          if constexpr (CARRY)
+            total = total + at[i].d;
+          else
+            yp[w][q + i][lane] = y;
         }
-        if constexpr (CARRY)
-          total = total + d;
-        else
-          yp[w][q][lane] = y;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PF; ++i) at[i] = next[i];
       }
       __syncthreads();
       if constexpr (!CARRY) {
-        T* q = op + (int64_t)(t0 + w) * a.sout.t;
+        const int tn = renewed(t0);
 #pragma unroll
-        for (int i = 0; i < RPW; ++i, q += (int64_t)W * a.sout.t) {
+        for (int i = 0; i < RPW; ++i) {
           const int r = w + W * i;
-          if (r / YT != s || r >= TT) continue;
+          if ((W <= YT ? W * i / YT : r / YT) != s || r >= TT) continue;
           T y = T(0);
 #pragma unroll
           for (int v = 0; v < W; ++v) y = y + yp[v][r % YT][lane];
           y = fma(Dc, ur[i], y);
-          if (zp) y = y * (zr[i] * sigmoid(zr[i]));
-          if (k.on && t0 + r < stop) q[k.at] = y;
+          y = gate ? y * (zr[i] * sigmoid(zr[i])) : y;
+          Row<T>(op + (int64_t)(tn + r) * a.sout.t, tn + r < stop, k.cnt).put(y);
         }
         if (TT != YT) __syncthreads();
       }
@@ -256,7 +341,8 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
       if (n0 + j < N) ((T*)a.carry)[(at * N + n0 + j) * a.C + k.c] = h[j];
     if (w == 0) ((T*)a.dsum)[at * a.C + k.c] = total;
   } else {
-    for (int t = (stop > k.lo ? stop : k.lo) + w; t < k.hi; t += W) (op + (int64_t)t * a.sout.t)[k.at] = T(0);
+    for (int t = (stop > k.lo ? stop : k.lo) + w; t < k.hi; t += W)
+      Row<T>(op + (int64_t)t * a.sout.t, true, k.cnt).put(T(0));
     if (a.hT && k.seg == a.nseg - 1) {
 #pragma unroll
       for (int j = 0; j < NS; ++j)
@@ -361,8 +447,8 @@ __device__ __forceinline__ T sum8(const T (&v)[8], bool upper8) {
 // step together, and eight steps' results leave a wave as one LDS write.
 // CARRY: only dh over the segment, and its sum of d.
 template <typename T, int W, bool CARRY>
-__global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(), HT = held_len<T>(W);
+__global__ void __launch_bounds__(64 * W, bwd_waves(W)) scan_bwd_kernel(ScanArgs a) {
+  constexpr int NS = kStates, TT = tile_len<T>(), HT = held_len<T>(W), KT = keep_len<T>(W);
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP, RB = HT < 8 ? HT : 8;
   __shared__ T sd[TT][64], sx[CARRY ? 1 : TT][64], sy[TT][64], yp[CARRY ? 1 : 3][CARRY ? 1 : W][CARRY ? 1 : HT][64];
@@ -373,22 +459,22 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
   const int N = (int)a.N, n0 = w * NS;
   const T* up = (const T*)a.u + k.b * a.su.b + k.c0;
   const T* dp = (const T*)a.dt + k.b * a.sdt.b + k.c0;
-  const T* zp = a.z ? (const T*)a.z + k.b * a.sz.b + k.c0 : nullptr;
+  const T* zp = (const T*)a.z + k.b * a.sz.b + k.c0;
+  const bool gate = a.z != nullptr;
   const T* gp = (const T*)a.g + k.b * a.sg.b + k.c0;
   const T* Bp = (const T*)a.Bm + k.b * a.sB.b + k.grp * a.gB;
   const T* Cp = (const T*)a.Cm + k.b * a.sC.b + k.grp * a.gC;
-  const T bias = a.bias ? ((const T*)a.bias + k.c0)[k.at] : T(0);
-  const T Dc = a.D ? ((const T*)a.D + k.c0)[k.at] : T(0);
-  T An[NS], A2[NS], dh[NS], dA[NS], total = T(0), dD = T(0), dbias = T(0);
+  const T bias = a.bias ? Row<T>((const T*)a.bias + k.c0, true, k.cnt).get() : T(0);
+  const T Dc = a.D ? Row<T>((const T*)a.D + k.c0, true, k.cnt).get() : T(0);
+  T A2[NS], dh[NS], dA[NS], total = T(0), dD = T(0), dbias = T(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    An[j] = n0 + j < N ? ((const T*)a.A)[(k.c0 + k.at) * N + n0 + j] : T(0);
-    A2[j] = An[j] * T(kLog2e);
+    A2[j] = k.on && n0 + j < N ? ((const T*)a.A)[k.c * N + n0 + j] * T(kLog2e) : T(0);
     dA[j] = dh[j] = T(0);
-    if (!CARRY && a.nseg > 1 && n0 + j < N)
-      dh[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c0 + k.at];
+    if (!CARRY && a.nseg > 1 && k.on && n0 + j < N)
+      dh[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c];
   }
-  const int64_t ntiles = (a.T + TT - 1) / TT;
+  const int64_t nkept = (a.T + KT - 1) / KT;
   const int stop = k.hi < k.len ? k.hi : k.len;
   // this block's dB and dC terms: row t of part k.tile
   const int64_t prow = ((k.tile * a.B + k.b) * a.T) * a.G + k.grp;
@@ -398,7 +484,7 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
       for (int t = from + w; t < k.hi; t += W) {
         ((T*)a.du)[k.b * a.sdu.b + (int64_t)t * a.sdu.t + k.c] = T(0);
         ((T*)a.ddt)[k.b * a.sddt.b + (int64_t)t * a.sddt.t + k.c] = T(0);
-        if (zp) ((T*)a.dz)[k.b * a.sdz.b + (int64_t)t * a.sdz.t + k.c] = T(0);
+        if (gate) ((T*)a.dz)[k.b * a.sdz.b + (int64_t)t * a.sdz.t + k.c] = T(0);
       }
     for (int64_t f = threadIdx.x; f < (int64_t)(k.hi - from) * N; f += 64 * W) {
       const int64_t at = (prow + (from + f / N) * a.G) * N + f % N;
@@ -407,18 +493,23 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
     }
   }
   In in;
-  T kept[NS];
-  auto fetch = [&](int t0) {
-    in.rows(in.d, dp, a.sdt.t, t0, k.len, w, k.at);
-    in.rows(in.g, gp, a.sg.t, t0, k.len, w, k.at);
-    if (zp) in.rows(in.z, zp, a.sz.t, t0, k.len, w, k.at);
+  T kept[TT / KT][NS];
+  auto fetch = [&](int from) {
+    const int t0 = renewed(from);
+    in.rows(in.d, dp, a.sdt.t, t0, k, w);
+    in.rows(in.g, gp, a.sg.t, t0, k, w);
+    in.rows(in.z, zp, a.sz.t, t0, k, w, gate);
     in.map(in.c, Cp, a.sC.t, t0, k.len, N);
     if constexpr (!CARRY) {
-      in.rows(in.u, up, a.su.t, t0, k.len, w, k.at);
+      in.rows(in.u, up, a.su.t, t0, k, w);
       in.map(in.b, Bp, a.sB.t, t0, k.len, N);
-      const T* kp = (const T*)a.kept + ((k.b * ntiles + t0 / TT) * N + n0) * a.C + k.c0;
 #pragma unroll
-      for (int j = 0; j < NS; ++j) kept[j] = n0 + j < N ? (kp + j * a.C)[k.at] : T(0);
+      for (int s = 0; s < TT / KT; ++s) {
+        const int t = t0 + s * KT;
+        const T* kp = (const T*)a.kept + ((k.b * nkept + t / KT) * N + n0) * a.C + k.c0;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) kept[s][j] = Row<T>(kp + j * a.C, (unsigned)t < (unsigned)stop && n0 + j < N, k.cnt).get();
+      }
     }
   };
   const int first = k.lo + (stop - 1 - k.lo) / TT * TT;
@@ -426,50 +517,74 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
   if constexpr (!CARRY) {
     dup = (T*)a.du + k.b * a.sdu.b + k.c0;
     ddp = (T*)a.ddt + k.b * a.sddt.b + k.c0;
-    if (zp) dzp = (T*)a.dz + k.b * a.sdz.b + k.c0;
+    dzp = (T*)a.dz + k.b * a.sdz.b + k.c0;
   }
   if (k.lo < stop) fetch(first);
+  drain_loads();
   for (int t0 = first; k.lo < stop && t0 >= k.lo; t0 -= TT) {
-    T ur[RPW], zr[RPW], gr[RPW], dr[RPW], rr[RPW];
+    T ur[RPW], gz[RPW], ds[RPW];  // u; the factors of dz and ddt
     __syncthreads();  // the previous tile's LDS has been read
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       const int r = w + W * i;
       if (W * RPW != TT && r >= TT) break;
-      const bool on = t0 + r < k.len && k.on;  // an idle lane's terms are zero
-      rr[i] = in.d[i] + bias;
-      gr[i] = on ? in.g[i] : T(0);
-      dr[i] = on ? step_size(rr[i], a.softplus) : T(0);
-      zr[i] = zp && on ? in.z[i] : T(0);
-      const T dy = zp ? gr[i] * (zr[i] * sigmoid(zr[i])) : gr[i];
-      sd[r][lane] = dr[i];
+      // (of an idle lane or a position past the end u, g and z are zero, and so are all terms)
+      const T raw = in.d[i] + bias, g = in.g[i];
+      const T d = step_size(raw, a.softplus, t0 + r < k.len);
+      const T z = in.z[i], sz = sigmoid(z), dy = gate ? g * (z * sz) : g;
+      if constexpr (!CARRY) gz[i] = g * (sz * fma(z, T(1) - sz, T(1)));
+      if constexpr (!CARRY) ds[i] = a.softplus ? sigmoid(raw) : T(1);
+      sd[r][lane] = d;
       sy[r][lane] = dy;
       if constexpr (!CARRY) {
-        ur[i] = on ? in.u[i] : T(0);
-        sx[r][lane] = dr[i] * ur[i];
+        ur[i] = in.u[i];
+        sx[r][lane] = d * ur[i];
       }
     }
     In::put_map(sC, in.c, t0, k.len, N);
     if constexpr (CARRY) {
       __syncthreads();
-      if (t0 > k.lo) fetch(t0 - TT);
+      fetch(t0 - TT);
+      constexpr int PF = 2;  // positions read ahead
+      Step<T> at[PF], next[PF];
+      auto read = [&](Step<T>(&x)[PF], int r) {
 #pragma unroll
-      for (int r = TT - 1; r >= 0; --r) {
-        const T d = sd[r][lane], dy = sy[r][lane];
-        total = total + d;
+        for (int i = 0; i < PF; ++i) {
+          x[i].d = sd[r + i][lane];
+          x[i].g = sy[r + i][lane];
 #pragma unroll
-        for (int j = 0; j < NS; ++j) dh[j] = exp2_of(d * A2[j]) * fma(dy, sC[r * NP + n0 + j], dh[j]);
+          for (int j = 0; j < NS; ++j) x[i].c[j] = sC[(r + i) * NP + n0 + j];
+        }
+      };
+      read(at, TT - PF);
+#pragma unroll
+      for (int r = TT - PF; r >= 0; r -= PF) {
+        if (r > 0) read(next, r - PF);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = PF - 1; i >= 0; --i) {
+          total = total + at[i].d;
+#pragma unroll
+          for (int j = 0; j < NS; ++j) dh[j] = exp2_of(at[i].d * A2[j]) * fma(at[i].g, at[i].c[j], dh[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PF; ++i) at[i] = next[i];
       }
     } else {
       In::put_map(sB, in.b, t0, k.len, N);
       // the states before each part of the tile
       T start[TT / HT][NS];
 #pragma unroll
-      for (int j = 0; j < NS; ++j) start[0][j] = kept[j];
+      for (int s = 0; s < TT / KT; ++s)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) start[s * (KT / HT)][j] = kept[s][j];
       __syncthreads();
-      if (t0 > k.lo) fetch(t0 - TT);
+      fetch(t0 - TT);
+      // those that were not kept
 #pragma unroll
       for (int s = 1; s < TT / HT; ++s) {
+        if (s % (KT / HT) == 0) continue;
 #pragma unroll
         for (int j = 0; j < NS; ++j) start[s][j] = start[s - 1][j];
 #pragma unroll
@@ -488,35 +603,50 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
         T dec[HT][NS], h[HT + 1][NS];  // h[q]: the states before position q of the part
 #pragma unroll
         for (int j = 0; j < NS; ++j) h[0][j] = start[s][j];
-#pragma unroll
-        for (int q = 0; q < HT; ++q) {
-          const int r = s * HT + q;
-          const T d = sd[r][lane], x = sx[r][lane];
+        auto read = [&](int r, bool back) {
+          Step<T> x;
+          x.d = sd[r][lane];
+          x.x = sx[r][lane];
+          if (back) x.g = sy[r][lane];
 #pragma unroll
           for (int j = 0; j < NS; ++j) {
-            dec[q][j] = exp2_of(d * A2[j]);
-            h[q + 1][j] = fma(dec[q][j], h[q][j], x * sB[r * NP + n0 + j]);
+            x.b[j] = sB[r * NP + n0 + j];
+            if (back) x.c[j] = sC[r * NP + n0 + j];
           }
-          if (q % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+          return x;
+        };
+        Step<T> at = read(s * HT, false);
+#pragma unroll
+        for (int q = 0; q < HT; ++q) {
+          const Step<T> next = q + 1 < HT ? read(s * HT + q + 1, false) : read(s * HT + q, true);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < NS; ++j) {
+            dec[q][j] = exp2_of(at.d * A2[j]);
+            h[q + 1][j] = fma(dec[q][j], h[q][j], at.x * at.b[j]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          at = next;
         }
 #pragma unroll
         for (int q = HT - 1; q >= 0; --q) {
           const int r = s * HT + q;
-          const T d = sd[r][lane], x = sx[r][lane], dy = sy[r][lane];
+          const Step<T> next = q > 0 ? read(r - 1, true) : at;
+          __builtin_amdgcn_sched_barrier(0);
           T dx = T(0), e = T(0), y = T(0), v[8];
 #pragma unroll
           for (int j = 0; j < NS; ++j) {
-            const T Cn = sC[r * NP + n0 + j], Bn = sB[r * NP + n0 + j];
-            y = fma(Cn, h[q + 1][j], y);
-            v[4 + j] = dy * h[q + 1][j];
-            dh[j] = fma(dy, Cn, dh[j]);
-            dx = fma(dh[j], Bn, dx);
-            v[j] = dh[j] * x;
+            y = fma(at.c[j], h[q + 1][j], y);
+            v[4 + j] = at.g * h[q + 1][j];
+            dh[j] = fma(at.g, at.c[j], dh[j]);
+            dx = fma(dh[j], at.b[j], dx);
+            v[j] = dh[j] * at.x;
             dh[j] = dh[j] * dec[q][j];
             const T p = dh[j] * h[q][j];
-            e = fma(An[j], p, e);
-            dA[j] = fma(d, p, dA[j]);
+            e = fma(A2[j], p, e);
+            dA[j] = fma(at.d, p, dA[j]);
           }
+          at = next;
           yp[0][w][q][lane] = y;
           yp[1][w][q][lane] = dx;
           yp[2][w][q][lane] = e;
@@ -528,12 +658,11 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
             sg[r + (lane & 7)][(lane >> 5) * NP + n0 + ((lane >> 3) & 3)] = sums;
         }
         __syncthreads();
-        T *qu = dup + (int64_t)(t0 + w) * a.sdu.t, *qd = ddp + (int64_t)(t0 + w) * a.sddt.t;
-        T* qz = dzp + (int64_t)(t0 + w) * a.sdz.t;
+        const int tn = renewed(t0);
 #pragma unroll
-        for (int i = 0; i < RPW; ++i, qu += (int64_t)W * a.sdu.t, qd += (int64_t)W * a.sddt.t, qz += (int64_t)W * a.sdz.t) {
+        for (int i = 0; i < RPW; ++i) {
           const int r = w + W * i;
-          if (r / HT != s || r >= TT) continue;
+          if ((W <= HT ? W * i / HT : r / HT) != s || r >= TT) continue;
           T y = T(0), dx = T(0), e = T(0);
 #pragma unroll
           for (int v = 0; v < W; ++v) {
@@ -541,33 +670,27 @@ __global__ void __launch_bounds__(64 * W, W <= 8 ? 2 : 4) scan_bwd_kernel(ScanAr
             dx = dx + yp[1][v][r % HT][lane];
             e = e + yp[2][v][r % HT][lane];
           }
-          const bool put = k.on && t0 + r < stop;
-          T dy = gr[i];
-          if (zp) {
-            const T sz = sigmoid(zr[i]);
-            y = fma(Dc, ur[i], y);
-            const T dz = gr[i] * y * (sz * fma(zr[i], T(1) - sz, T(1)));
-            dy = gr[i] * (zr[i] * sz);
-            if (put) qz[k.at] = dz;
-          }
-          T dd = fma(dx, ur[i], e);
-          if (a.softplus) dd = dd * sigmoid(rr[i]);
-          if (put) {
-            dD = fma(dy, ur[i], dD);
-            dbias = dbias + dd;
-            qu[k.at] = fma(dx, dr[i], Dc * dy);
-            qd[k.at] = dd;
-          }
+          const int t = tn + r;
+          const bool there = t < stop;
+          Row<T>(dzp + (int64_t)t * a.sdz.t, there && gate, k.cnt).put(gz[i] * fma(Dc, ur[i], y));
+          const T dy = sy[r][lane], dd = fma(dx, ur[i], e * T(kLn2)) * ds[i];
+          dD = fma(dy, ur[i], dD);
+          dbias = dbias + dd;
+          Row<T>(dup + (int64_t)t * a.sdu.t, there, k.cnt).put(fma(dx, sd[r][lane], Dc * dy));
+          Row<T>(ddp + (int64_t)t * a.sddt.t, there, k.cnt).put(dd);
         }
         if (s > 0) __syncthreads();
       }
-      const int rows = (int)(stop - t0 < TT ? stop - t0 : TT);
-      for (int f = threadIdx.x; f < rows * NP; f += 64 * W) {
-        const int r = f / NP, n = f % NP;
-        if (n >= N) continue;
-        const int64_t at = (prow + (t0 + r) * a.G) * N + n;
-        ((T*)a.dBp)[at] = sg[r][n];
-        ((T*)a.dCp)[at] = sg[r][NP + n];
+      const int rows = stop - t0 < TT ? stop - t0 : TT, gn = (int)(a.G * N) * (int)sizeof(T);
+      const int64_t at = (prow + (int64_t)t0 * a.G) * N;
+      const Rsrc rb = make_rsrc((const T*)a.dBp + at, rows * gn), rc = make_rsrc((const T*)a.dCp + at, rows * gn);
+#pragma unroll
+      for (int i = 0; i < In::MAPS; ++i) {
+        const int f = threadIdx.x + 64 * W * i, r = f / NP, n = f % NP;
+        const int off = n < N && r < TT ? r * gn + n * (int)sizeof(T) : -1;
+        const int rr = TT * NP % (64 * W) != 0 && r >= TT ? 0 : r;
+        store_at(rb, off, sg[rr][n]);
+        store_at(rc, off, sg[rr][NP + n]);
       }
     }
   }
@@ -654,7 +777,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs a) {
     u = ((const T*)a.u)[b * a.su.b + c];
     T raw = ((const T*)a.dt)[b * a.sdt.b + c];
     if (a.bias) raw = raw + ((const T*)a.bias)[c];
-    const T d = step_size(raw, a.softplus), x = d * u;
+    const T d = step_size(raw, a.softplus, true), x = d * u;
     const int64_t g = c / (a.C / a.G);
     const T* Bp = (const T*)a.Bm + b * a.sB.b + g * a.gB + n0;
     const T* Cp = (const T*)a.Cm + b * a.sC.b + g * a.gC + n0;
@@ -708,16 +831,19 @@ static void scan_launch(const ScanArgs& a, int W) {
 #undef SCAN_W
 }
 
-static int scan_tile(int dtype) {
-  return dtype == DTMI_F32 ? tile_len<float>() : tile_len<double>();
+static int scan_keep(int dtype, int64_t N) {
+  const int W = waves_for(N);
+  return dtype == DTMI_F32 ? keep_len<float>(W) : keep_len<double>(W);
 }
 
 // Segments of T: one where B * C / 64 blocks already occupy the card. A split
-// costs the exponentials a second time, so it has to more than double the
-// blocks that run at once; then enough segments for two blocks per CU, of at
-// least two tiles each.
-static void scan_segments(ScanArgs& a, int TT, int per_cu) {
-  const int64_t blocks = a.B * a.ct, want = per_cu * (int64_t)num_cus(), tiles = cdiv(a.T, TT);
+// costs the exponentials a second time, so it pays while less than a block per
+// CU would run (float32, 1536 channels x 16 states x 1024 positions, forward
+// and backward without and with: 96 blocks 498 / 208 us, 192 blocks 516 / 410,
+// at 256 blocks equal); then enough segments for 12 waves per SIMD group of a
+// CU (three blocks at 16 states), of at least two tiles each.
+static void scan_segments(ScanArgs& a, int TT, int W) {
+  const int64_t blocks = a.B * a.ct, want = (W <= 4 ? 12 / W : 2) * (int64_t)num_cus(), tiles = cdiv(a.T, TT);
   int64_t s = blocks >= num_cus() ? 1 : want / blocks;
   if (s > tiles / 2) s = tiles / 2;
   if (s < 1) s = 1;
@@ -731,6 +857,7 @@ static int scan_shape(const char* what, int dtype, int64_t B, int64_t T, int64_t
   DTMI_CHECK(T <= 0x7fffff00, "%s: too many positions", what);
   DTMI_CHECK(N >= 1 && N <= 64, "%s: 1 to 64 states (got %lld)", what, (long long)N);
   DTMI_CHECK(G >= 1 && C % G == 0, "%s: %lld channels do not form %lld groups", what, (long long)C, (long long)G);
+  DTMI_CHECK(G * N < (1 << 23), "%s: %lld groups of %lld states", what, (long long)G, (long long)N);
   return DTMI_OK;
 }
 
@@ -749,7 +876,7 @@ static int scan_chain(ScanArgs& a, int W, bool backward) {
 template <typename T>
 static int scan_fwd(ScanArgs& a) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(), 4);
+  scan_segments(a, tile_len<T>(), W);
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256,
              "dtmi_scan_fwd: too many elements");
   void* ws = nullptr;
@@ -775,7 +902,7 @@ template <typename T>
 static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* dC, BT sdC, int64_t gdC, void* dD,
                     void* dbias) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(), 2);
+  scan_segments(a, tile_len<T>(), W);
   const int64_t maps = a.B * a.T * a.G * a.N;
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256 &&
                  maps <= (int64_t)0x7fffffff * 256,
@@ -828,7 +955,7 @@ DTMI_EXPORT int dtmi_scan_kept(int dtype, int64_t B, int64_t T, int64_t C, int64
   DTMI_BODY_BEGIN
   if (int rc = scan_shape("dtmi_scan_kept", dtype, B, T, C, N, 1)) return rc;
   DTMI_CHECK(count, "dtmi_scan_kept: NULL result");
-  *count = B * cdiv(T, scan_tile(dtype)) * N * C;
+  *count = B * cdiv(T, scan_keep(dtype, N)) * N * C;
   return DTMI_OK;
   DTMI_BODY_END
 }
