@@ -8,13 +8,12 @@
 // owns VW neighbouring channels (16 bytes) over SEG positions and keeps the K
 // rows of its window in registers, so a row is loaded once per segment (and
 // K - 1 rows twice, from L2).
-#include "colreduce.h"
 #include "seqmath.h"
 
 namespace dtmi {
 
 struct ConvArgs {
-  void *y, *state_out, *dx, *dstate, *dwp, *dbp;
+  void *y, *state_out, *dx, *dstate, *parts;
   const void *x, *w, *b, *state, *g;
   const int64_t* lengths;
   BT sx, sy, sg, sdx;
@@ -188,8 +187,41 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
       }
   }
 #pragma unroll
-  for (int k = 0; k < K; ++k) vstore<T, VW>((T*)a.dwp + (bs * K + k) * a.C + c, dw[k]);
-  vstore<T, VW>((T*)a.dbp + bs * a.C + c, db);
+  for (int k = 0; k < K; ++k) vstore<T, VW>((T*)a.parts + (bs * (K + 1) + k) * a.C + c, dw[k]);
+  vstore<T, VW>((T*)a.parts + (bs * (K + 1) + K) * a.C + c, db);
+}
+
+// dw [K, C] and db [C] (NULL: not wanted): the segments' terms [parts][K + 1][C].
+// A block sums 64 columns, each of its 16 waves every 16th part with eight
+// loads in flight, then the waves' sums in order.
+template <typename T>
+__global__ void __launch_bounds__(1024) conv_sum_kernel(const T* __restrict__ parts, int64_t n, int64_t KC, int64_t C,
+                                                        T* __restrict__ dw, T* __restrict__ db) {
+  __shared__ T sh[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t cols = KC + C, c = (int64_t)blockIdx.x * 64 + lane;
+  T s = T(0);
+  if (c < cols) {
+    int64_t p = w;
+    for (; p + 16 * 7 < n; p += 128) {
+      T v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = parts[(p + 16 * u) * cols + c];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s = s + v[u];
+    }
+    for (; p < n; p += 16) s = s + parts[p * cols + c];
+  }
+  sh[w][lane] = s;
+  __syncthreads();
+  if (w != 0 || c >= cols) return;
+  s = T(0);
+#pragma unroll
+  for (int v = 0; v < 16; ++v) s = s + sh[v][lane];
+  if (c < KC)
+    dw[c] = s;
+  else if (db)
+    db[c - KC] = s;
 }
 
 // One position per sequence: the state's K - 1 rows and the new input give y,
@@ -247,10 +279,10 @@ static void conv_taps(ConvOp op, const ConvArgs& a, int K, unsigned grid) {
   }
 }
 
-// Fills in the vector width and the grid and launches. rows: threads per
-// vector of channels. Whole 16-byte vectors where every row allows them.
+// Vectors of channels per row: whole 16-byte ones where every row allows them,
+// else single elements.
 template <typename T>
-static int conv_run(ConvOp op, ConvArgs& a, int K, int64_t rows, const char* what) {
+static void conv_vectors(ConvArgs& a) {
   constexpr int VW = 16 / sizeof(T);
   const void* ptrs[] = {a.y, a.state_out, a.dx, a.dstate, a.x, a.w, a.b, a.state, a.g};
   const int64_t steps[] = {a.C, a.sx.b, a.sx.t, a.sy.b, a.sy.t, a.sg.b, a.sg.t, a.sdx.b, a.sdx.t};
@@ -258,22 +290,41 @@ static int conv_run(ConvOp op, ConvArgs& a, int K, int64_t rows, const char* wha
   for (const void* p : ptrs) vec = vec && aligned(p, 16);
   for (int64_t s : steps) vec = vec && s % VW == 0;
   a.cv = vec ? a.C / VW : a.C;
+}
+
+// Positions per thread: the longest segments that leave 600 threads per CU.
+// 8 x 1024 x 1536 float32, forward / backward in us: 8 positions (1536 threads
+// per CU) 20.2 / 40.4, 16: 18.7 / 32.1, 32: 22.8 / 35.0, 64: 36.8 / 52.6; short
+// segments load more rows twice and leave more terms of dw to sum.
+static void conv_segments(ConvArgs& a) {
+  a.seg = 64;
+  while (a.seg > 8 && a.B * cdiv(a.T, a.seg) * a.cv < (int64_t)num_cus() * 600) a.seg /= 2;
+  a.nseg = cdiv(a.T, a.seg);
+}
+
+// rows: threads per vector of channels.
+template <typename T>
+static int conv_run(ConvOp op, const ConvArgs& a, int K, int64_t rows, const char* what) {
   const int64_t blocks = cdiv(a.cv * rows, 256);
   DTMI_CHECK(blocks <= 0x7fffffff, "%s: too many elements", what);
-  if (vec)
-    conv_taps<T, VW>(op, a, K, (unsigned)blocks);
+  if (a.cv != a.C)
+    conv_taps<T, 16 / sizeof(T)>(op, a, K, (unsigned)blocks);
   else
     conv_taps<T, 1>(op, a, K, (unsigned)blocks);
   LAUNCH_CHECK(what);
   return DTMI_OK;
 }
 
-// Positions per thread: long segments load few rows twice, short ones make
-// enough threads for the card.
-static int conv_segment(int64_t B, int64_t T, int64_t C) {
-  int seg = 64;
-  while (seg > 8 && B * cdiv(T, seg) * C < (int64_t)num_cus() * 4096) seg /= 2;
-  return seg;
+template <typename T>
+static int conv_fwd(ConvArgs& a, int K) {
+  conv_vectors<T>(a);
+  conv_segments(a);
+  return conv_run<T>(CONV_FWD, a, K, a.B * a.nseg, "dtmi_conv_fwd");
+}
+template <typename T>
+static int conv_step(ConvArgs& a, int K) {
+  conv_vectors<T>(a);
+  return conv_run<T>(CONV_STEP, a, K, a.B, "dtmi_conv_step");
 }
 
 static int conv_shape(const char* what, int dtype, int64_t B, int64_t T, int64_t C, int64_t K) {
@@ -304,26 +355,24 @@ DTMI_EXPORT int dtmi_conv_fwd(int dtype, int64_t B, int64_t T, int64_t C, int64_
   a.y = y, a.state_out = state_out, a.x = x, a.w = w, a.b = b, a.state = state, a.lengths = lengths;
   a.sx = {x_strides[0], x_strides[1]}, a.sy = {y_strides[0], y_strides[1]};
   a.B = B, a.T = T, a.C = C, a.silu = silu;
-  a.seg = conv_segment(B, T, C);
-  a.nseg = cdiv(T, a.seg);
   TimedLaunch tl(DTMI_FAM_OTHER, 2.0 * B * T * C * (dtype == DTMI_F32 ? 4 : 8));
-  return dtype == DTMI_F32 ? conv_run<float>(CONV_FWD, a, (int)K, B * a.nseg, "dtmi_conv_fwd")
-                           : conv_run<double>(CONV_FWD, a, (int)K, B * a.nseg, "dtmi_conv_fwd");
+  return dtype == DTMI_F32 ? conv_fwd<float>(a, (int)K) : conv_fwd<double>(a, (int)K);
   DTMI_BODY_END
 }
 
 template <typename T>
 static int conv_bwd(ConvArgs& a, int K, void* dw, void* db) {
+  conv_vectors<T>(a);
+  conv_segments(a);
   const int64_t parts = a.B * a.nseg;
   DTMI_CHECK(parts <= 0x7fffffff, "dtmi_conv_bwd: too many elements");
   void* p = nullptr;
   if (int rc = pool_alloc(&p, (size_t)parts * (K + 1) * a.C * sizeof(T))) return rc;
-  a.dwp = p;
-  a.dbp = (T*)p + parts * K * a.C;
+  a.parts = p;
   int rc = conv_run<T>(CONV_BWD, a, K, parts, "dtmi_conv_bwd");
   if (rc == DTMI_OK) {
-    launch_colreduce<T>((T*)dw, (const T*)a.dwp, (int)parts, K * a.C, 0);
-    if (db) launch_colreduce<T>((T*)db, (const T*)a.dbp, (int)parts, a.C, 0);
+    conv_sum_kernel<T><<<(unsigned)cdiv((K + 1) * a.C, 64), 1024, 0, stream()>>>((const T*)p, parts, K * a.C, a.C, (T*)dw,
+                                                                               (T*)db);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) rc = fail_hip(e, "dtmi_conv_bwd", __FILE__, __LINE__);
   }
@@ -352,8 +401,6 @@ DTMI_EXPORT int dtmi_conv_bwd(int dtype, int64_t B, int64_t T, int64_t C, int64_
   a.x = x, a.w = w, a.b = b, a.state = state, a.g = g, a.lengths = lengths, a.dx = dx, a.dstate = dstate;
   a.sx = {x_strides[0], x_strides[1]}, a.sg = {g_strides[0], g_strides[1]}, a.sdx = {dx_strides[0], dx_strides[1]};
   a.B = B, a.T = T, a.C = C, a.silu = silu;
-  a.seg = conv_segment(B, T, C);
-  a.nseg = cdiv(T, a.seg);
   TimedLaunch tl(DTMI_FAM_OTHER, 3.0 * B * T * C * es);
   return dtype == DTMI_F32 ? conv_bwd<float>(a, (int)K, dw, db) : conv_bwd<double>(a, (int)K, dw, db);
   DTMI_BODY_END
@@ -371,7 +418,6 @@ DTMI_EXPORT int dtmi_conv_step(int dtype, int64_t B, int64_t C, int64_t K, const
   a.sx.b = x_stride, a.sy.b = y_stride;
   a.B = B, a.C = C, a.silu = silu;
   TimedLaunch tl(DTMI_FAM_OTHER, 2.0 * B * C * K * (dtype == DTMI_F32 ? 4 : 8));
-  return dtype == DTMI_F32 ? conv_run<float>(CONV_STEP, a, (int)K, B, "dtmi_conv_step")
-                           : conv_run<double>(CONV_STEP, a, (int)K, B, "dtmi_conv_step");
+  return dtype == DTMI_F32 ? conv_step<float>(a, (int)K) : conv_step<double>(a, (int)K);
   DTMI_BODY_END
 }
