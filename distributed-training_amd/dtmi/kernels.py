@@ -7,6 +7,7 @@ allocated here unless passed in.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import numpy as np
 
@@ -673,11 +674,18 @@ def attn_set_ds_limit(nbytes: int) -> int:
 
 
 # --------------------------------------------------------- sequence mixers
+@lru_cache(maxsize=4096)
+def _i64s(vals: tuple):
+    """int64_t[] of `vals` (read only, so one per set of values)."""
+    return _lib.i64_array(vals)
+
+
 def _rows_strides(x: DeviceArray, what: str, lead: int = 2):
     """The element strides of all but the last axis, which must be contiguous."""
-    if x.ndim != lead + 1 or (x.shape[-1] > 1 and x.strides[-1] != 1):
+    st = x.strides
+    if len(st) != lead + 1 or (st[lead] != 1 and x.shape[lead] > 1):
         raise ValueError(f"{what} must have {lead + 1} axes, the last contiguous")
-    return _lib.i64_array(x.strides[:lead])
+    return _i64s(st[:lead])
 
 
 def _opt_ptr(x: DeviceArray | None):
@@ -693,9 +701,9 @@ def _lengths_ptr(lengths: DeviceArray | None, B: int):
     return lengths.ptr
 
 
-def _same(x: DeviceArray, shape, dtype, what: str, contiguous: bool = True):
-    if tuple(x.shape) != tuple(shape) or x.dtype != dtype:
-        raise ValueError(f"{what} must be {np.dtype(dtype).name} of shape {tuple(shape)}, not {x.dtype} {x.shape}")
+def _same(x: DeviceArray, shape: tuple, dtype, what: str, contiguous: bool = True):
+    if x.shape != shape or x.dtype != dtype:
+        raise ValueError(f"{what} must be {np.dtype(dtype).name} of shape {shape}, not {x.dtype} {x.shape}")
     if contiguous:
         _contig(x)
 
