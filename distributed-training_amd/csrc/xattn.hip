@@ -28,6 +28,7 @@
 // partial results a small kernel joins in a fixed order.
 #include <cmath>
 
+#include "bufrsrc.h"
 #include "common.h"
 
 namespace dtmi {
@@ -63,6 +64,19 @@ struct HT {
   int64_t b, h, t;
 };
 
+// Division by a fixed d >= 1 of numbers below 2^31 as a multiplication
+// (Granlund and Montgomery, 1994): n / d = (mulhi(n, m) + n) >> l.
+struct FastDiv {
+  uint32_t m, l, d;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t d_) : d(d_) {
+    l = 0;
+    while ((1ull << l) < d) ++l;
+    m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, m) + n) >> l; }
+};
+
 struct XArgs {
   const void *q, *k, *v, *o, *dO;
   void *out, *dq, *dk, *dv;
@@ -73,10 +87,11 @@ struct XArgs {
   HT sq, sk, sv, so, sdo, sdq, sdk, sdv;
   int64_t B, H, Hk, Tq, Tk, D, R;
   double scale;
+  FastDiv by_tq;  // rows to heads
   int nsplit;   // parts of the loop
   int ntile;    // blocks along the owned axis
-  int64_t per;  // loop positions per part, a multiple of the tile
-  int vec;      // 16-byte loads and stores allowed for every operand
+  int per;      // loop positions per part, a multiple of the tile
+  int vec;      // 16-byte loads and stores allowed for every operand, positions less than 2^23 elements apart
 };
 
 __device__ __forceinline__ int64_t key_count(const XArgs& a, int64_t b) {
@@ -86,11 +101,11 @@ __device__ __forceinline__ int64_t key_count(const XArgs& a, int64_t b) {
 }
 
 // Element offset of row r of the group's rows (head and query) in an array with strides s
-__device__ __forceinline__ int64_t row_at(const XArgs& a, const HT& s, int64_t b, int64_t kh, int64_t r) {
-  const int64_t h = kh * (a.H / a.Hk) + r / a.Tq;
-  return b * s.b + h * s.h + (r % a.Tq) * s.t;
+__device__ __forceinline__ int64_t row_at(const XArgs& a, const HT& s, int64_t b, int64_t kh, int r) {
+  const uint32_t h = a.by_tq.div((uint32_t)r), t = (uint32_t)r - h * a.by_tq.d;
+  return b * s.b + kh * (a.H / a.Hk) * s.h + (int64_t)h * s.h + (int64_t)t * s.t;
 }
-__device__ __forceinline__ int64_t stat_at(const XArgs& a, int64_t b, int64_t kh, int64_t r) {
+__device__ __forceinline__ int64_t stat_at(const XArgs& a, int64_t b, int64_t kh, int r) {
   return (b * a.H + kh * (a.H / a.Hk)) * a.Tq + r;
 }
 
@@ -118,25 +133,46 @@ __device__ __forceinline__ void load_slice(typename XM<T>::vec_t (&f)[DP / (4 * 
 
 // NR rows of a tile on their way from global memory to LDS [NR][DP + PAD];
 // rows that do not exist and columns at and past D are zero.
-template <typename T, int NR, int DP>
+// VEC: 16-byte loads, and rows that 32 bits reach from a tile's first.
+template <typename T, int NR, int DP, bool VEC>
 struct Rows {
   typedef typename XM<T>::vec_t VT;
-  static constexpr int VEC = XM<T>::VEC, LD = DP + XM<T>::PAD, NV = NR * DP / VEC / 256;
-  static_assert(NR * DP % (VEC * 256) == 0, "whole vectors per thread");
+  static constexpr int V = XM<T>::VEC, LD = DP + XM<T>::PAD, NV = NR * DP / V / 256;
+  static_assert(NR * DP % (V * 256) == 0, "whole vectors per thread");
   VT x[NV];
-  // base(r): element pointer of row r of the tile, or NULL
+  uint32_t off[NV];  // bytes from the tile's first row; past every buffer's end in columns from D on
+  static __device__ __forceinline__ int row(int i) { return (threadIdx.x + 256 * i) / (DP / V); }
+  static __device__ __forceinline__ int col(int i) { return (threadIdx.x + 256 * i) % (DP / V) * V; }
+  __device__ __forceinline__ void start(int64_t st, int D) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) off[i] = col(i) < D ? (uint32_t)((row(i) * st + col(i)) * sizeof(T)) : 0x80000000u;
+  }
+  // `n` rows from p on, `st` elements apart (start()): the buffer ends with the
+  // last of them, so the address work of a tile is scalar
+  __device__ __forceinline__ void fetch(const T* p, int64_t st, int n, int D) {
+    if constexpr (VEC) {
+      n = n < NR ? n : NR;
+      const Rsrc r = make_rsrc(p, n > 0 ? (uint64_t)(((n - 1) * st + D) * sizeof(T)) : 0);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        x[i] = __builtin_bit_cast(VT, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off[i], 0, 0));
+    } else {
+      gather([&](int i) { return i < n ? p + i * st : nullptr; }, D);
+    }
+  }
+  // rows at base(r), NULL for none
   template <typename F>
-  __device__ __forceinline__ void fetch(const F& base, int D, bool vec) {
+  __device__ __forceinline__ void gather(const F& base, int D) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int f = threadIdx.x + 256 * i, r = f / (DP / VEC), d = f % (DP / VEC) * VEC;
-      const T* p = base(r);
+      const T* p = base(row(i));
+      const int d = col(i);
       VT v = VT(0);
-      if (vec) {
+      if (VEC) {
         if (p && d < D) v = *reinterpret_cast<const VT*>(p + d);
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
+        for (int e = 0; e < V; ++e)
           if (p && d + e < D) v[e] = p[d + e];
       }
       x[i] = v;
@@ -144,10 +180,7 @@ struct Rows {
   }
   __device__ __forceinline__ void put(T* __restrict__ lds) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int f = threadIdx.x + 256 * i, r = f / (DP / VEC), d = f % (DP / VEC) * VEC;
-      *reinterpret_cast<VT*>(lds + r * LD + d) = x[i];
-    }
+    for (int i = 0; i < NV; ++i) *reinterpret_cast<VT*>(lds + row(i) * LD + col(i)) = x[i];
   }
 };
 
@@ -239,21 +272,24 @@ struct XBlock {
   int tile, split;
 };
 __device__ __forceinline__ XBlock x_block(const XArgs& a) {
-  const int64_t id = blockIdx.x;
+  // blocks are dealt to the eight XCDs in turn: XCD x takes the x-th eighth of
+  // the blocks, so that those sharing a head's keys share an L2; not with
+  // lengths, where an eighth may hold the long sequences
+  const unsigned n = gridDim.x, xcd = blockIdx.x & 7, more = n & 7;
+  const unsigned id = a.lengths ? blockIdx.x : xcd * (n >> 3) + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
   XBlock k;
-  k.tile = (int)(id % a.ntile);
-  const int64_t r = id / a.ntile;
-  k.split = (int)(r % a.nsplit);
-  const int64_t bh = r / a.nsplit;
-  k.b = bh / a.Hk;
-  k.kh = bh % a.Hk;
+  const unsigned r = id / (unsigned)a.ntile, bh = r / (unsigned)a.nsplit;
+  k.tile = (int)(id - r * (unsigned)a.ntile);
+  k.split = (int)(r - bh * (unsigned)a.nsplit);
+  k.b = bh / (unsigned)a.Hk;
+  k.kh = bh % (unsigned)a.Hk;
   return k;
 }
 
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 
-template <typename T, int DP, int CT>
-__global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
+template <typename T, int DP, int CT, bool VEC>
+__global__ void __launch_bounds__(256, 2) xattn_fwd_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
@@ -261,22 +297,24 @@ __global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
   __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
-  const int64_t len = key_count(a, k.b);
-  const int64_t lo = k.split * a.per, hi = lo + a.per < len ? lo + a.per : len;
-  const int64_t r0 = ((int64_t)k.tile * 4 + w) * 16 * CT;
-  const bool vec = a.vec != 0;
+  const int len = (int)key_count(a, k.b), lo = k.split * a.per, hi = len - lo > a.per ? lo + a.per : len;
+  const int r0 = (k.tile * 4 + w) * 16 * CT, R = (int)a.R;
   VT qf[CT][DP / (4 * M::VEC)];
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int64_t r = r0 + 16 * u + c;
-    load_slice<T, DP>(qf[u], (const T*)a.q + (r < a.R ? row_at(a, a.sq, k.b, k.kh, r) : 0), r < a.R, D, g, vec);
+    const int r = r0 + 16 * u + c;
+    load_slice<T, DP>(qf[u], (const T*)a.q + (r < R ? row_at(a, a.sq, k.b, k.kh, r) : 0), r < R, D, g, VEC);
   }
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
-  Rows<T, KT, DP> fk, fv;
-  auto fetch = [&](int64_t j0) {
-    fk.fetch([&](int r) { return j0 + r < hi ? Kb + (j0 + r) * a.sk.t : nullptr; }, D, vec);
-    fv.fetch([&](int r) { return j0 + r < hi ? Vb + (j0 + r) * a.sv.t : nullptr; }, D, vec);
+  Rows<T, KT, DP, VEC> fk, fv;
+  if constexpr (VEC) {
+    fk.start(a.sk.t, D);
+    fv.start(a.sv.t, D);
+  }
+  auto fetch = [&](int j0) {
+    fk.fetch(Kb + j0 * a.sk.t, a.sk.t, hi - j0, D);
+    fv.fetch(Vb + j0 * a.sv.t, a.sv.t, hi - j0, D);
   };
   const T sl2 = (T)(a.scale * 1.4426950408889634);
   AT o[CT][N];
@@ -288,9 +326,9 @@ __global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
 #pragma unroll
     for (int t = 0; t < N; ++t) o[u][t] = AT(0);
   }
-  const bool busy = r0 < a.R;
+  const bool busy = r0 < R;
   if (lo < hi) fetch(lo);
-  for (int64_t j0 = lo; j0 < hi; j0 += KT) {
+  for (int j0 = lo; j0 < hi; j0 += KT) {
     __syncthreads();
     fk.put(Ks);
     fv.put(Vs);
@@ -326,9 +364,9 @@ __global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int64_t r = r0 + 16 * u + c;
+    const int r = r0 + 16 * u + c;
     const T sum = over_groups_sum(l[u]);
-    if (r >= a.R) continue;
+    if (r >= R) continue;
     if (a.nsplit > 1) {
       const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
       put_row<T, DP>((T*)a.po + at * DP, o[u], T(1), DP, g, true);
@@ -338,7 +376,7 @@ __global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
       }
       continue;
     }
-    put_row<T, DP>((T*)a.out + row_at(a, a.so, k.b, k.kh, r), o[u], sum == T(0) ? T(0) : T(1) / sum, D, g, vec);
+    put_row<T, DP>((T*)a.out + row_at(a, a.so, k.b, k.kh, r), o[u], sum == T(0) ? T(0) : T(1) / sum, D, g, VEC);
     if (g == 0 && a.rowmax) {
       const int64_t at = stat_at(a, k.b, k.kh, r);
       ((T*)a.rowmax)[at] = mref[u];
@@ -350,7 +388,8 @@ __global__ void __launch_bounds__(256) xattn_fwd_kernel(XArgs a) {
 // Joins the forward's parts: a wave per row, lanes over d.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), r = id % a.R, bh = id / a.R;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), bh = id / a.R;
+  const int r = (int)(id % a.R);
   if (bh >= a.B * a.Hk) return;
   const int lane = threadIdx.x & 63;
   const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * a.nsplit * a.R + r;
@@ -388,7 +427,8 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
 // rowsum(dO O): 16 lanes per row
 template <typename T>
 __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), r = id % a.R, bh = id / a.R;
+  const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), bh = id / a.R;
+  const int r = (int)(id % a.R);
   const bool on = bh < a.B * a.Hk;
   T s = T(0);
   if (on) {
@@ -403,8 +443,8 @@ __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
 }
 
 // dQ: a wave owns 16 CT rows and loops over the keys of its part.
-template <typename T, int DP, int CT>
-__global__ void __launch_bounds__(256) xattn_bwd_q_kernel(XArgs a) {
+template <typename T, int DP, int CT, bool VEC>
+__global__ void __launch_bounds__(256, 2) xattn_bwd_q_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
@@ -412,18 +452,16 @@ __global__ void __launch_bounds__(256) xattn_bwd_q_kernel(XArgs a) {
   __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
-  const int64_t len = key_count(a, k.b);
-  const int64_t lo = k.split * a.per, hi = lo + a.per < len ? lo + a.per : len;
-  const int64_t r0 = ((int64_t)k.tile * 4 + w) * 16 * CT;
-  const bool vec = a.vec != 0;
+  const int len = (int)key_count(a, k.b), lo = k.split * a.per, hi = len - lo > a.per ? lo + a.per : len;
+  const int r0 = (k.tile * 4 + w) * 16 * CT, R = (int)a.R;
   VT qf[CT][NF], gf[CT][NF];
   T m[CT], inv[CT], dr[CT];
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int64_t r = r0 + 16 * u + c;
-    const bool in = r < a.R;
-    load_slice<T, DP>(qf[u], (const T*)a.q + (in ? row_at(a, a.sq, k.b, k.kh, r) : 0), in, D, g, vec);
-    load_slice<T, DP>(gf[u], (const T*)a.dO + (in ? row_at(a, a.sdo, k.b, k.kh, r) : 0), in, D, g, vec);
+    const int r = r0 + 16 * u + c;
+    const bool in = r < R;
+    load_slice<T, DP>(qf[u], (const T*)a.q + (in ? row_at(a, a.sq, k.b, k.kh, r) : 0), in, D, g, VEC);
+    load_slice<T, DP>(gf[u], (const T*)a.dO + (in ? row_at(a, a.sdo, k.b, k.kh, r) : 0), in, D, g, VEC);
     const int64_t at = stat_at(a, k.b, k.kh, in ? r : 0);
     const T sum = ((const T*)a.rowsum)[at];
     m[u] = ((const T*)a.rowmax)[at];
@@ -432,10 +470,14 @@ __global__ void __launch_bounds__(256) xattn_bwd_q_kernel(XArgs a) {
   }
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
-  Rows<T, KT, DP> fk, fv;
-  auto fetch = [&](int64_t j0) {
-    fk.fetch([&](int r) { return j0 + r < hi ? Kb + (j0 + r) * a.sk.t : nullptr; }, D, vec);
-    fv.fetch([&](int r) { return j0 + r < hi ? Vb + (j0 + r) * a.sv.t : nullptr; }, D, vec);
+  Rows<T, KT, DP, VEC> fk, fv;
+  if constexpr (VEC) {
+    fk.start(a.sk.t, D);
+    fv.start(a.sv.t, D);
+  }
+  auto fetch = [&](int j0) {
+    fk.fetch(Kb + j0 * a.sk.t, a.sk.t, hi - j0, D);
+    fv.fetch(Vb + j0 * a.sv.t, a.sv.t, hi - j0, D);
   };
   const T sl2 = (T)(a.scale * 1.4426950408889634);
   AT dq[CT][N];
@@ -443,9 +485,9 @@ __global__ void __launch_bounds__(256) xattn_bwd_q_kernel(XArgs a) {
   for (int u = 0; u < CT; ++u)
 #pragma unroll
     for (int t = 0; t < N; ++t) dq[u][t] = AT(0);
-  const bool busy = r0 < a.R;
+  const bool busy = r0 < R;
   if (lo < hi) fetch(lo);
-  for (int64_t j0 = lo; j0 < hi; j0 += KT) {
+  for (int j0 = lo; j0 < hi; j0 += KT) {
     __syncthreads();
     fk.put(Ks);
     fv.put(Vs);
@@ -470,20 +512,20 @@ __global__ void __launch_bounds__(256) xattn_bwd_q_kernel(XArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int64_t r = r0 + 16 * u + c;
-    if (r >= a.R) continue;
+    const int r = r0 + 16 * u + c;
+    if (r >= R) continue;
     if (a.nsplit > 1) {
       const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
       put_row<T, DP>((T*)a.po + at * DP, dq[u], (T)a.scale, DP, g, true);
     } else {
-      put_row<T, DP>((T*)a.dq + row_at(a, a.sdq, k.b, k.kh, r), dq[u], (T)a.scale, D, g, vec);
+      put_row<T, DP>((T*)a.dq + row_at(a, a.sdq, k.b, k.kh, r), dq[u], (T)a.scale, D, g, VEC);
     }
   }
 }
 
 // dK and dV: a wave owns 16 CT keys and loops over the rows of its part.
-template <typename T, int DP, int CT>
-__global__ void __launch_bounds__(256) xattn_bwd_kv_kernel(XArgs a) {
+template <typename T, int DP, int CT, bool VEC>
+__global__ void __launch_bounds__(256, 2) xattn_bwd_kv_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
@@ -492,28 +534,25 @@ __global__ void __launch_bounds__(256) xattn_bwd_kv_kernel(XArgs a) {
   __shared__ T sm[QT], si[QT], sr[QT];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
-  const int64_t len = key_count(a, k.b);
-  const int64_t lo = k.split * a.per, hi = lo + a.per < a.R ? lo + a.per : a.R;
-  const int64_t j0 = ((int64_t)k.tile * 4 + w) * 16 * CT;
-  const bool vec = a.vec != 0;
+  const int len = (int)key_count(a, k.b), R = (int)a.R, lo = k.split * a.per, hi = R - lo > a.per ? lo + a.per : R;
+  const int j0 = (k.tile * 4 + w) * 16 * CT;
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
   VT kf[CT][NF], vf[CT][NF];
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int64_t j = j0 + 16 * u + c;
-    load_slice<T, DP>(kf[u], Kb + (j < len ? j : 0) * a.sk.t, j < len, D, g, vec);
-    load_slice<T, DP>(vf[u], Vb + (j < len ? j : 0) * a.sv.t, j < len, D, g, vec);
+    const int j = j0 + 16 * u + c;
+    load_slice<T, DP>(kf[u], Kb + (int64_t)(j < len ? j : 0) * a.sk.t, j < len, D, g, VEC);
+    load_slice<T, DP>(vf[u], Vb + (int64_t)(j < len ? j : 0) * a.sv.t, j < len, D, g, VEC);
   }
-  Rows<T, QT, DP> fq, fg;
+  Rows<T, QT, DP, VEC> fq, fg;
   T nm = T(0), ni = T(0), nr = T(0);
-  auto fetch = [&](int64_t r0) {
-    fq.fetch([&](int r) { return r0 + r < hi ? (const T*)a.q + row_at(a, a.sq, k.b, k.kh, r0 + r) : nullptr; }, D, vec);
-    fg.fetch([&](int r) { return r0 + r < hi ? (const T*)a.dO + row_at(a, a.sdo, k.b, k.kh, r0 + r) : nullptr; }, D,
-             vec);
+  auto fetch = [&](int r0) {
+    fq.gather([&](int r) { return r0 + r < hi ? (const T*)a.q + row_at(a, a.sq, k.b, k.kh, r0 + r) : nullptr; }, D);
+    fg.gather([&](int r) { return r0 + r < hi ? (const T*)a.dO + row_at(a, a.sdo, k.b, k.kh, r0 + r) : nullptr; }, D);
     if (threadIdx.x < QT) {
-      const bool in = r0 + threadIdx.x < hi;
-      const int64_t at = stat_at(a, k.b, k.kh, in ? r0 + threadIdx.x : 0);
+      const bool in = r0 + (int)threadIdx.x < hi;
+      const int64_t at = stat_at(a, k.b, k.kh, in ? r0 + (int)threadIdx.x : 0);
       const T sum = in ? ((const T*)a.rowsum)[at] : T(0);
       nm = ((const T*)a.rowmax)[at];
       ni = sum == T(0) ? T(0) : T(1) / sum;
@@ -527,9 +566,9 @@ __global__ void __launch_bounds__(256) xattn_bwd_kv_kernel(XArgs a) {
 #pragma unroll
     for (int t = 0; t < N; ++t) dk[u][t] = dv[u][t] = AT(0);
   // a block past the sequence's keys has only zeros to write
-  const bool any = (int64_t)k.tile * 64 * CT < len, busy = j0 < len;
+  const bool any = k.tile * 64 * CT < len, busy = j0 < len;
   if (any && lo < hi) fetch(lo);
-  for (int64_t r0 = lo; any && r0 < hi; r0 += QT) {
+  for (int r0 = lo; any && r0 < hi; r0 += QT) {
     __syncthreads();
     fq.put(Qs);
     fg.put(Gs);
@@ -563,15 +602,15 @@ __global__ void __launch_bounds__(256) xattn_bwd_kv_kernel(XArgs a) {
   }
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
-    const int64_t j = j0 + 16 * u + c;
+    const int j = j0 + 16 * u + c;
     if (j >= a.Tk) continue;
     if (a.nsplit > 1) {
       const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.Tk + j;
       put_row<T, DP>((T*)a.po + at * DP, dk[u], (T)a.scale, DP, g, true);
       put_row<T, DP>((T*)a.pm + at * DP, dv[u], T(1), DP, g, true);
     } else {
-      put_row<T, DP>((T*)a.dk + k.b * a.sdk.b + k.kh * a.sdk.h + j * a.sdk.t, dk[u], (T)a.scale, D, g, vec);
-      put_row<T, DP>((T*)a.dv + k.b * a.sdv.b + k.kh * a.sdv.h + j * a.sdv.t, dv[u], T(1), D, g, vec);
+      put_row<T, DP>((T*)a.dk + k.b * a.sdk.b + k.kh * a.sdk.h + (int64_t)j * a.sdk.t, dk[u], (T)a.scale, D, g, VEC);
+      put_row<T, DP>((T*)a.dv + k.b * a.sdv.b + k.kh * a.sdv.h + (int64_t)j * a.sdv.t, dv[u], T(1), D, g, VEC);
     }
   }
 }
@@ -592,7 +631,7 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
     else
       ((T*)a.dk)[b * a.sdk.b + kh * a.sdk.h + r * a.sdk.t + d] = s;
   } else {
-    ((T*)a.dq)[row_at(a, a.sdq, b, kh, r) + d] = s;
+    ((T*)a.dq)[row_at(a, a.sdq, b, kh, (int)r) + d] = s;
   }
 }
 
@@ -605,7 +644,7 @@ static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop) {
   int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
   if (s > steps / 2) s = steps / 2;
   if (s < 1) s = 1;
-  a.per = cdiv(steps > 0 ? steps : 1, s) * kKeys;
+  a.per = (int)(cdiv(steps > 0 ? steps : 1, s) * kKeys);
   a.nsplit = loop > 0 ? (int)cdiv(loop, a.per) : 1;
   DTMI_CHECK(tiles <= 0x7fffffff && blocks * a.nsplit <= 0x7fffffff, "cross attention: too many elements");
   a.ntile = (int)tiles;
@@ -615,7 +654,10 @@ static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop) {
 #define X_LAUNCH(KERNEL, CTV)                                                     \
   {                                                                               \
     const unsigned grid = (unsigned)(a.B * a.Hk * a.nsplit * a.ntile);            \
-    KERNEL<T, DP, CTV><<<grid, 256, 0, stream()>>>(a);                            \
+    if (a.vec)                                                                     \
+      KERNEL<T, DP, CTV, true><<<grid, 256, 0, stream()>>>(a);                     \
+    else                                                                           \
+      KERNEL<T, DP, CTV, false><<<grid, 256, 0, stream()>>>(a);                    \
   }
 
 template <typename T, int DP>
@@ -707,6 +749,7 @@ static int x_shape(const char* what, int dtype, int64_t B, int64_t H, int64_t Hk
   DTMI_CHECK(Hk >= 1 && H % Hk == 0, "%s: %lld heads do not share %lld key/value heads", what, (long long)H,
              (long long)Hk);
   DTMI_CHECK(D >= 1 && D <= 128, "%s: head dimension 1 to 128 (got %lld)", what, (long long)D);
+  DTMI_CHECK(Tk < ((int64_t)1 << 31) - 4096, "%s: too many keys", what);
   DTMI_CHECK(B * H * Tq < ((int64_t)1 << 31) && B * Hk * Tk * 128 < ((int64_t)1 << 38), "%s: too many elements", what);
   return DTMI_OK;
 }
@@ -715,7 +758,7 @@ static HT ht(const int64_t* s) { return s ? HT{s[0], s[1], s[2]} : HT{0, 0, 0}; 
 template <typename T>
 static bool x_vec(const void* p, const HT& s) {
   constexpr int V = 16 / sizeof(T);
-  return aligned(p, 16) && s.b % V == 0 && s.h % V == 0 && s.t % V == 0;
+  return aligned(p, 16) && s.b % V == 0 && s.h % V == 0 && s.t % V == 0 && s.t >= 0 && s.t < (1 << 23);
 }
 
 template <typename T>
@@ -768,6 +811,7 @@ DTMI_EXPORT int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   a.q = q, a.k = k, a.v = v, a.out = o, a.lengths = lengths, a.rowmax = rowmax, a.rowsum = rowsum;
   a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides);
   a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.R = H / Hk * Tq, a.scale = scale;
+  a.by_tq = FastDiv((uint32_t)(Tq > 0 ? Tq : 1));
   TimedLaunch tl(DTMI_FAM_OTHER, 4.0 * B * H * Tq * Tk * D);
   return dtype == DTMI_F32 ? xattn_fwd<float>(a) : xattn_fwd<double>(a);
   DTMI_BODY_END
@@ -793,6 +837,7 @@ DTMI_EXPORT int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides), a.sdo = ht(dO_strides);
   a.sdq = ht(dq_strides), a.sdk = ht(dk_strides), a.sdv = ht(dv_strides);
   a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.R = H / Hk * Tq, a.scale = scale;
+  a.by_tq = FastDiv((uint32_t)(Tq > 0 ? Tq : 1));
   TimedLaunch tl(DTMI_FAM_OTHER, 14.0 * B * H * Tq * Tk * D);
   return dtype == DTMI_F32 ? xattn_bwd<float>(a) : xattn_bwd<double>(a);
   DTMI_BODY_END
