@@ -85,7 +85,7 @@ struct XArgs {
   void *po, *pm, *pl;     // partial results of a split loop
   const int64_t* lengths;
   HT sq, sk, sv, so, sdo, sdq, sdk, sdv;
-  int64_t B, H, Hk, Tq, Tk, D, R;
+  int64_t B, H, Hk, G, Tq, Tk, D, R;  // G: heads per group, H / Hk; R: rows, G Tq
   double scale;
   FastDiv by_tq;  // rows to heads
   int nsplit;   // parts of the loop
@@ -100,13 +100,17 @@ __device__ __forceinline__ int64_t key_count(const XArgs& a, int64_t b) {
   return n < 0 ? 0 : n > a.Tk ? a.Tk : n;
 }
 
-// Element offset of row r of the group's rows (head and query) in an array with strides s
-__device__ __forceinline__ int64_t row_at(const XArgs& a, const HT& s, int64_t b, int64_t kh, int r) {
+// First element of a group's rows in an array with strides s, and row r's offset from there
+template <typename T>
+__device__ __forceinline__ T* group_of(const XArgs& a, const void* p, const HT& s, int64_t b, int64_t kh) {
+  return (T*)p + b * s.b + kh * a.G * s.h;
+}
+__device__ __forceinline__ int64_t row_at(const XArgs& a, const HT& s, int r) {
   const uint32_t h = a.by_tq.div((uint32_t)r), t = (uint32_t)r - h * a.by_tq.d;
-  return b * s.b + kh * (a.H / a.Hk) * s.h + (int64_t)h * s.h + (int64_t)t * s.t;
+  return (int64_t)h * s.h + (int64_t)t * s.t;
 }
 __device__ __forceinline__ int64_t stat_at(const XArgs& a, int64_t b, int64_t kh, int r) {
-  return (b * a.H + kh * (a.H / a.Hk)) * a.Tq + r;
+  return (b * a.H + kh * a.G) * a.Tq + r;
 }
 
 // A lane's slice of one row as MFMA operand: element e of vector f is
@@ -286,10 +290,18 @@ __device__ __forceinline__ XBlock x_block(const XArgs& a) {
   return k;
 }
 
+// Waves per SIMD the registers are cut to: more than two would spill, and the
+// wide float64 tiles do at two. (With no bound the accumulators go to the
+// accumulation registers and every use of a score is a move more.)
+template <typename T>
+constexpr int x_waves(int DP) {
+  return sizeof(T) == 8 && DP >= 96 ? 1 : 2;
+}
+
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 
 template <typename T, int DP, int CT, bool VEC>
-__global__ void __launch_bounds__(256, 2) xattn_fwd_kernel(XArgs a) {
+__global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
@@ -299,11 +311,12 @@ __global__ void __launch_bounds__(256, 2) xattn_fwd_kernel(XArgs a) {
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b), lo = k.split * a.per, hi = len - lo > a.per ? lo + a.per : len;
   const int r0 = (k.tile * 4 + w) * 16 * CT, R = (int)a.R;
+  const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
   VT qf[CT][DP / (4 * M::VEC)];
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
     const int r = r0 + 16 * u + c;
-    load_slice<T, DP>(qf[u], (const T*)a.q + (r < R ? row_at(a, a.sq, k.b, k.kh, r) : 0), r < R, D, g, VEC);
+    load_slice<T, DP>(qf[u], Qb + (r < R ? row_at(a, a.sq, r) : 0), r < R, D, g, VEC);
   }
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
@@ -376,7 +389,7 @@ __global__ void __launch_bounds__(256, 2) xattn_fwd_kernel(XArgs a) {
       }
       continue;
     }
-    put_row<T, DP>((T*)a.out + row_at(a, a.so, k.b, k.kh, r), o[u], sum == T(0) ? T(0) : T(1) / sum, D, g, VEC);
+    put_row<T, DP>(group_of<T>(a, a.out, a.so, k.b, k.kh) + row_at(a, a.so, r), o[u], sum == T(0) ? T(0) : T(1) / sum, D, g, VEC);
     if (g == 0 && a.rowmax) {
       const int64_t at = stat_at(a, k.b, k.kh, r);
       ((T*)a.rowmax)[at] = mref[u];
@@ -412,7 +425,7 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
     }
   }
   const T inv = sum == T(0) ? T(0) : T(1) / sum;
-  T* out = (T*)a.out + row_at(a, a.so, b, kh, r);
+  T* out = group_of<T>(a, a.out, a.so, b, kh) + row_at(a, a.so, r);
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
     const int d = lane + 64 * e;
@@ -433,8 +446,8 @@ __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
   T s = T(0);
   if (on) {
     const int64_t b = bh / a.Hk, kh = bh % a.Hk;
-    const T* o = (const T*)a.o + row_at(a, a.so, b, kh, r);
-    const T* g = (const T*)a.dO + row_at(a, a.sdo, b, kh, r);
+    const T* o = group_of<const T>(a, a.o, a.so, b, kh) + row_at(a, a.so, r);
+    const T* g = group_of<const T>(a, a.dO, a.sdo, b, kh) + row_at(a, a.sdo, r);
     for (int d = threadIdx.x & 15; d < a.D; d += 16) s = fma(o[d], g[d], s);
   }
 #pragma unroll
@@ -444,7 +457,7 @@ __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
 
 // dQ: a wave owns 16 CT rows and loops over the keys of its part.
 template <typename T, int DP, int CT, bool VEC>
-__global__ void __launch_bounds__(256, 2) xattn_bwd_q_kernel(XArgs a) {
+__global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
@@ -454,14 +467,16 @@ __global__ void __launch_bounds__(256, 2) xattn_bwd_q_kernel(XArgs a) {
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b), lo = k.split * a.per, hi = len - lo > a.per ? lo + a.per : len;
   const int r0 = (k.tile * 4 + w) * 16 * CT, R = (int)a.R;
+  const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
+  const T* Gb = group_of<const T>(a, a.dO, a.sdo, k.b, k.kh);
   VT qf[CT][NF], gf[CT][NF];
   T m[CT], inv[CT], dr[CT];
 #pragma unroll
   for (int u = 0; u < CT; ++u) {
     const int r = r0 + 16 * u + c;
     const bool in = r < R;
-    load_slice<T, DP>(qf[u], (const T*)a.q + (in ? row_at(a, a.sq, k.b, k.kh, r) : 0), in, D, g, VEC);
-    load_slice<T, DP>(gf[u], (const T*)a.dO + (in ? row_at(a, a.sdo, k.b, k.kh, r) : 0), in, D, g, VEC);
+    load_slice<T, DP>(qf[u], Qb + (in ? row_at(a, a.sq, r) : 0), in, D, g, VEC);
+    load_slice<T, DP>(gf[u], Gb + (in ? row_at(a, a.sdo, r) : 0), in, D, g, VEC);
     const int64_t at = stat_at(a, k.b, k.kh, in ? r : 0);
     const T sum = ((const T*)a.rowsum)[at];
     m[u] = ((const T*)a.rowmax)[at];
@@ -518,14 +533,14 @@ __global__ void __launch_bounds__(256, 2) xattn_bwd_q_kernel(XArgs a) {
       const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
       put_row<T, DP>((T*)a.po + at * DP, dq[u], (T)a.scale, DP, g, true);
     } else {
-      put_row<T, DP>((T*)a.dq + row_at(a, a.sdq, k.b, k.kh, r), dq[u], (T)a.scale, D, g, VEC);
+      put_row<T, DP>(group_of<T>(a, a.dq, a.sdq, k.b, k.kh) + row_at(a, a.sdq, r), dq[u], (T)a.scale, D, g, VEC);
     }
   }
 }
 
 // dK and dV: a wave owns 16 CT keys and loops over the rows of its part.
 template <typename T, int DP, int CT, bool VEC>
-__global__ void __launch_bounds__(256, 2) xattn_bwd_kv_kernel(XArgs a) {
+__global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
@@ -545,14 +560,17 @@ __global__ void __launch_bounds__(256, 2) xattn_bwd_kv_kernel(XArgs a) {
     load_slice<T, DP>(kf[u], Kb + (int64_t)(j < len ? j : 0) * a.sk.t, j < len, D, g, VEC);
     load_slice<T, DP>(vf[u], Vb + (int64_t)(j < len ? j : 0) * a.sv.t, j < len, D, g, VEC);
   }
+  const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
+  const T* Gb = group_of<const T>(a, a.dO, a.sdo, k.b, k.kh);
+  const int64_t stats = stat_at(a, k.b, k.kh, 0);
   Rows<T, QT, DP, VEC> fq, fg;
   T nm = T(0), ni = T(0), nr = T(0);
   auto fetch = [&](int r0) {
-    fq.gather([&](int r) { return r0 + r < hi ? (const T*)a.q + row_at(a, a.sq, k.b, k.kh, r0 + r) : nullptr; }, D);
-    fg.gather([&](int r) { return r0 + r < hi ? (const T*)a.dO + row_at(a, a.sdo, k.b, k.kh, r0 + r) : nullptr; }, D);
+    fq.gather([&](int r) { return r0 + r < hi ? Qb + row_at(a, a.sq, r0 + r) : nullptr; }, D);
+    fg.gather([&](int r) { return r0 + r < hi ? Gb + row_at(a, a.sdo, r0 + r) : nullptr; }, D);
     if (threadIdx.x < QT) {
       const bool in = r0 + (int)threadIdx.x < hi;
-      const int64_t at = stat_at(a, k.b, k.kh, in ? r0 + (int)threadIdx.x : 0);
+      const int64_t at = stats + (in ? r0 + (int)threadIdx.x : 0);
       const T sum = in ? ((const T*)a.rowsum)[at] : T(0);
       nm = ((const T*)a.rowmax)[at];
       ni = sum == T(0) ? T(0) : T(1) / sum;
@@ -631,7 +649,7 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
     else
       ((T*)a.dk)[b * a.sdk.b + kh * a.sdk.h + r * a.sdk.t + d] = s;
   } else {
-    ((T*)a.dq)[row_at(a, a.sdq, b, kh, (int)r) + d] = s;
+    group_of<T>(a, a.dq, a.sdq, b, kh)[row_at(a, a.sdq, (int)r) + d] = s;
   }
 }
 
@@ -810,7 +828,7 @@ DTMI_EXPORT int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   XArgs a{};
   a.q = q, a.k = k, a.v = v, a.out = o, a.lengths = lengths, a.rowmax = rowmax, a.rowsum = rowsum;
   a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides);
-  a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.R = H / Hk * Tq, a.scale = scale;
+  a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.G = H / Hk, a.R = a.G * Tq, a.scale = scale;
   a.by_tq = FastDiv((uint32_t)(Tq > 0 ? Tq : 1));
   TimedLaunch tl(DTMI_FAM_OTHER, 4.0 * B * H * Tq * Tk * D);
   return dtype == DTMI_F32 ? xattn_fwd<float>(a) : xattn_fwd<double>(a);
@@ -836,7 +854,7 @@ DTMI_EXPORT int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   a.rowmax = const_cast<void*>(rowmax), a.rowsum = const_cast<void*>(rowsum);
   a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides), a.sdo = ht(dO_strides);
   a.sdq = ht(dq_strides), a.sdk = ht(dk_strides), a.sdv = ht(dv_strides);
-  a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.R = H / Hk * Tq, a.scale = scale;
+  a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.G = H / Hk, a.R = a.G * Tq, a.scale = scale;
   a.by_tq = FastDiv((uint32_t)(Tq > 0 ? Tq : 1));
   TimedLaunch tl(DTMI_FAM_OTHER, 14.0 * B * H * Tq * Tk * D);
   return dtype == DTMI_F32 ? xattn_bwd<float>(a) : xattn_bwd<double>(a);
