@@ -90,7 +90,6 @@ struct XArgs {
   FastDiv by_tq;  // rows to heads
   int nsplit;   // parts of the loop
   int ntile;    // blocks along the owned axis
-  int per;      // loop positions per part, a multiple of the tile
   int vec;      // 16-byte loads and stores allowed for every operand, positions less than 2^23 elements apart
 };
 
@@ -188,51 +187,59 @@ struct Rows {
   }
 };
 
-// 16 x 16 tile += rows r0 .. r0 + 15 of LDS times the lane's slice
+// A lane's slice of row r0 + c of an LDS tile, and its N columns N c .. of the
+// rows row(i, g): the two ways a tile's rows enter a product.
 template <typename T, int DP>
-__device__ __forceinline__ typename XM<T>::acc_t mul_rows(const T* __restrict__ lds, int r0,
-                                                          const typename XM<T>::vec_t (&f)[DP / (4 * XM<T>::VEC)], int g,
-                                                          int c) {
+__device__ __forceinline__ void lds_slice(typename XM<T>::vec_t (&x)[DP / (4 * XM<T>::VEC)], const T* __restrict__ lds, int r0,
+                                          int g, int c) {
   constexpr int VEC = XM<T>::VEC, LD = DP + XM<T>::PAD;
-  typename XM<T>::acc_t acc = typename XM<T>::acc_t(0);
 #pragma unroll
-  for (int i = 0; i < DP / (4 * VEC); ++i) {
-    const typename XM<T>::vec_t x =
-        *reinterpret_cast<const typename XM<T>::vec_t*>(lds + (r0 + c) * LD + 4 * VEC * i + VEC * g);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) acc = XM<T>::mma(x[e], f[i][e], acc);
-  }
-  return acc;
+  for (int i = 0; i < DP / (4 * VEC); ++i)
+    x[i] = *reinterpret_cast<const typename XM<T>::vec_t*>(lds + (r0 + c) * LD + 4 * VEC * i + VEC * g);
 }
-
-// out^T (d = N m + t by column) += sum over a tile's 16 rows of LDS[row][d] p(row, column)
-template <typename T, int DP, int CT>
-__device__ __forceinline__ void mul_cols(typename XM<T>::acc_t (&out)[CT][DP / 16], const T* __restrict__ lds, int r0,
-                                         const typename XM<T>::acc_t (&p)[CT], int g, int c) {
-  constexpr int N = DP / 16, VEC = XM<T>::VEC, LD = DP + XM<T>::PAD;
-  typedef typename XM<T>::vec_t VT;
+template <typename T, int DP>
+__device__ __forceinline__ void lds_cols(T (&x)[4][DP / 16], const T* __restrict__ lds, int r0, int g, int c) {
+  constexpr int N = DP / 16, LD = DP + XM<T>::PAD, VW = N % XM<T>::VEC == 0 ? XM<T>::VEC : N % 2 == 0 ? 2 : 1;
+  typedef T vt __attribute__((ext_vector_type(VW == 1 ? 2 : VW)));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    T x[N];
     const T* row = lds + (r0 + XM<T>::row(i, g)) * LD + N * c;
-    if constexpr (N % VEC == 0) {
+    if constexpr (VW > 1) {
 #pragma unroll
-      for (int v = 0; v < N / VEC; ++v) {
-        const VT y = *reinterpret_cast<const VT*>(row + VEC * v);
+      for (int v = 0; v < N / VW; ++v) {
+        const vt y = *reinterpret_cast<const vt*>(row + VW * v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[VEC * v + e] = y[e];
+        for (int e = 0; e < VW; ++e) x[i][VW * v + e] = y[e];
       }
     } else {
 #pragma unroll
-      for (int t = 0; t < N; ++t) x[t] = row[t];
+      for (int t = 0; t < N; ++t) x[i][t] = row[t];
     }
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-      for (int u = 0; u < CT; ++u) out[u][t] = XM<T>::mma(x[t], p[u][i], out[u][t]);
   }
 }
-
+// Two 16 x 16 tiles of products of slices, their chains of dependent MFMAs interleaved
+template <typename T, int NF>
+__device__ __forceinline__ void mul_slices(typename XM<T>::acc_t& p, const typename XM<T>::vec_t (&xp)[NF],
+                                           const typename XM<T>::vec_t (&fp)[NF], typename XM<T>::acc_t& q,
+                                           const typename XM<T>::vec_t (&xq)[NF], const typename XM<T>::vec_t (&fq)[NF]) {
+  p = q = typename XM<T>::acc_t(0);
+#pragma unroll
+  for (int i = 0; i < NF; ++i)
+#pragma unroll
+    for (int e = 0; e < XM<T>::VEC; ++e) {
+      p = XM<T>::mma(xp[i][e], fp[i][e], p);
+      q = XM<T>::mma(xq[i][e], fq[i][e], q);
+    }
+}
+// out^T (d = N m + t by column) += sum over a tile's 16 rows of x(row, d) p(row, column)
+template <typename T, int N>
+__device__ __forceinline__ void mul_cols(typename XM<T>::acc_t (&out)[N], const T (&x)[4][N],
+                                         const typename XM<T>::acc_t& p) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < N; ++t) out[t] = XM<T>::mma(x[i][t], p[i], out[t]);
+}
 // The lane's part of a result row: registers (t, i) are d = N row(i, g) + t
 template <typename T, int DP>
 __device__ __forceinline__ void put_row(T* __restrict__ row, const typename XM<T>::acc_t (&x)[DP / 16], T mul, int D,
@@ -274,6 +281,13 @@ __device__ __forceinline__ T over_groups_sum(T x) {
 struct XBlock {
   int64_t b, kh;
   int tile, split;
+  // this block's part of a loop over n positions, whole tiles of `tile`
+  __device__ __forceinline__ void part(const XArgs& a, int n, int step, int& lo, int& hi) const {
+    const int per = ((n + a.nsplit - 1) / a.nsplit + step - 1) / step * step;
+    const int64_t from = (int64_t)split * per;
+    lo = from < n ? (int)from : n;
+    hi = n - lo > per ? lo + per : n;
+  }
 };
 __device__ __forceinline__ XBlock x_block(const XArgs& a) {
   // blocks are dealt to the eight XCDs in turn: XCD x takes the x-th eighth of
@@ -300,24 +314,21 @@ constexpr int x_waves(int DP) {
 
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 
-template <typename T, int DP, int CT, bool VEC>
+template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
-  typedef typename M::vec_t VT;
   constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys;
   __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
-  const int len = (int)key_count(a, k.b), lo = k.split * a.per, hi = len - lo > a.per ? lo + a.per : len;
-  const int r0 = (k.tile * 4 + w) * 16 * CT, R = (int)a.R;
+  const int len = (int)key_count(a, k.b);
+  int lo, hi;
+  k.part(a, len, KT, lo, hi);
+  const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
-  VT qf[CT][DP / (4 * M::VEC)];
-#pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const int r = r0 + 16 * u + c;
-    load_slice<T, DP>(qf[u], Qb + (r < R ? row_at(a, a.sq, r) : 0), r < R, D, g, VEC);
-  }
+  typename M::vec_t qf[DP / (4 * M::VEC)];
+  load_slice<T, DP>(qf, Qb + (r < R ? row_at(a, a.sq, r) : 0), r < R, D, g, VEC);
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
   Rows<T, KT, DP, VEC> fk, fv;
@@ -330,106 +341,242 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
     fv.fetch(Vb + j0 * a.sv.t, a.sv.t, hi - j0, D);
   };
   const T sl2 = (T)(a.scale * 1.4426950408889634);
-  AT o[CT][N];
-  T mref[CT], l[CT];
+  AT o[N];
+  T mref = M::lowest, l = T(0);
 #pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    mref[u] = M::lowest;
-    l[u] = T(0);
-#pragma unroll
-    for (int t = 0; t < N; ++t) o[u][t] = AT(0);
-  }
+  for (int t = 0; t < N; ++t) o[t] = AT(0);
   const bool busy = r0 < R;
-  if (lo < hi) fetch(lo);
-  for (int j0 = lo; j0 < hi; j0 += KT) {
-    __syncthreads();
+  if (lo < hi) {
+    fetch(lo);
     fk.put(Ks);
     fv.put(Vs);
-    __syncthreads();
-    if (j0 + KT < hi) fetch(j0 + KT);
-    if (!busy) continue;
-#pragma unroll
-    for (int kt = 0; kt < KT / 16; ++kt) {
-      AT p[CT];
-#pragma unroll
-      for (int u = 0; u < CT; ++u) {
-        AT s = mul_rows<T, DP>(Ks, 16 * kt, qf[u], g, c) * sl2;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = j0 + 16 * kt + M::row(i, g) < hi ? s[i] : -INFINITY;
-        const T top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
-        if (__any(top > mref[u] + T(8))) {
-          const T next = fmax(mref[u], over_groups_max(top));
-          const T alpha = M::ex2(mref[u] - next);
-          l[u] = l[u] * alpha;
-#pragma unroll
-          for (int t = 0; t < N; ++t) o[u][t] *= alpha;
-          mref[u] = next;
-        }
+  }
+  __syncthreads();
+  for (int j0 = lo; j0 < hi; j0 += KT) {
+    const bool more = j0 + KT < hi;
+    if (more) fetch(j0 + KT);
+    if (busy) {
+      constexpr int NF = DP / (4 * M::VEC);
+      typename M::vec_t x0[NF], x1[NF];
+      T v0[4][N], v1[4][N];
+      AT p0, p1;
+      lds_slice<T, DP>(x0, Ks, 0, g, c);
+      lds_slice<T, DP>(x1, Ks, 16, g, c);
+      lds_cols<T, DP>(v0, Vs, 0, g, c);
+      lds_cols<T, DP>(v1, Vs, 16, g, c);
+      mul_slices<T, NF>(p0, x0, qf, p1, x1, qf);
+      p0 *= sl2;
+      p1 *= sl2;
+      if (!more)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[i] = M::ex2(s[i] - mref[u]);
-          l[u] = l[u] + s[i];
+          p0[i] = j0 + M::row(i, g) < hi ? p0[i] : -INFINITY;
+          p1[i] = j0 + 16 + M::row(i, g) < hi ? p1[i] : -INFINITY;
         }
-        p[u] = s;
-      }
-      mul_cols<T, DP, CT>(o, Vs, 16 * kt, p, g, c);
-    }
-  }
+      T top = fmax(p0[0], p1[0]);
 #pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const int r = r0 + 16 * u + c;
-    const T sum = over_groups_sum(l[u]);
-    if (r >= R) continue;
+      for (int i = 1; i < 4; ++i) top = fmax(top, fmax(p0[i], p1[i]));
+      if (__any(top > mref + T(8))) {
+        const T next = fmax(mref, over_groups_max(top));
+        const T alpha = M::ex2(mref - next);
+        l = l * alpha;
+#pragma unroll
+        for (int t = 0; t < N; ++t) o[t] *= alpha;
+        mref = next;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p0[i] = M::ex2(p0[i] - mref);
+        p1[i] = M::ex2(p1[i] - mref);
+        l = l + (p0[i] + p1[i]);
+      }
+      mul_cols<T, N>(o, v0, p0);
+      mul_cols<T, N>(o, v1, p1);
+    }
+    __syncthreads();
+    if (more) {
+      fk.put(Ks);
+      fv.put(Vs);
+    }
+    __syncthreads();
+  }
+  const T sum = over_groups_sum(l);
+  if (r >= R) return;
+  if (a.nsplit > 1) {
+    const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
+    put_row<T, DP>((T*)a.po + at * DP, o, T(1), DP, g, true);
+    if (g == 0) {
+      ((T*)a.pm)[at] = mref;
+      ((T*)a.pl)[at] = sum;
+    }
+    return;
+  }
+  put_row<T, DP>(group_of<T>(a, a.out, a.so, k.b, k.kh) + row_at(a, a.so, r), o, sum == T(0) ? T(0) : T(1) / sum, D, g, VEC);
+  if (g == 0 && a.rowmax) {
+    const int64_t at = stat_at(a, k.b, k.kh, r);
+    ((T*)a.rowmax)[at] = mref;
+    ((T*)a.rowsum)[at] = sum;
+  }
+}
+
+// Up to 16 rows per key/value head (one query token with shared heads): bound
+// by reading k and v once. Each wave takes every fourth 16 keys of the block's
+// part and loads them straight into the products' operand registers, the next
+// 16 while it works; the waves' results are joined through LDS.
+template <typename T, int DP, bool VEC>
+__global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a) {
+  using M = XM<T>;
+  typedef typename M::acc_t AT;
+  typedef typename M::vec_t VT;
+  constexpr int N = DP / 16, NF = DP / (4 * M::VEC), VW = N % M::VEC == 0 ? M::VEC : 2;
+  typedef T vw __attribute__((ext_vector_type(VW)));
+  __shared__ T so[4][16][DP + 1], sm[4][16], sl[4][16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D, R = (int)a.R;
+  const XBlock k = x_block(a);
+  const int len = (int)key_count(a, k.b);
+  int lo, hi;
+  k.part(a, len, 64, lo, hi);
+  const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
+  VT qf[NF];
+  load_slice<T, DP>(qf, Qb + (c < R ? row_at(a, a.sq, c) : 0), c < R, D, g, VEC);
+  const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
+  const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
+  auto fetch = [&](VT(&x)[NF], T(&v)[4][N], int j) {
+    load_slice<T, DP>(x, Kb + (int64_t)(j + c < hi ? j + c : 0) * a.sk.t, j + c < hi, D, g, VEC);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = j + M::row(i, g);
+      const T* row = Vb + (int64_t)(r < hi ? r : 0) * a.sv.t + N * c;
+#pragma unroll
+      for (int u = 0; u < N / VW; ++u) {
+        vw y = vw(0);
+        if (VEC) {
+          if (r < hi && N * c + VW * u < D) y = *reinterpret_cast<const vw*>(row + VW * u);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VW; ++e)
+            if (r < hi && N * c + VW * u + e < D) y[e] = row[VW * u + e];
+        }
+#pragma unroll
+        for (int e = 0; e < VW; ++e) v[i][VW * u + e] = y[e];
+      }
+    }
+  };
+  const T sl2 = (T)(a.scale * 1.4426950408889634);
+  AT o[N];
+  T mref = M::lowest, l = T(0);
+#pragma unroll
+  for (int t = 0; t < N; ++t) o[t] = AT(0);
+  VT x[NF], nx[NF];
+  T v[4][N], nv[4][N];
+  if (lo + 16 * w < hi) fetch(x, v, lo + 16 * w);
+  for (int j = lo + 16 * w; j < hi; j += 64) {
+    if (j + 64 < hi) fetch(nx, nv, j + 64);
+    AT s = AT(0);
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+      for (int e = 0; e < M::VEC; ++e) s = M::mma(x[i][e], qf[i][e], s);
+    s *= sl2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = j + M::row(i, g) < hi ? s[i] : -INFINITY;
+    const T top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
+    if (__any(top > mref + T(8))) {
+      const T next = fmax(mref, over_groups_max(top));
+      const T alpha = M::ex2(mref - next);
+      l = l * alpha;
+#pragma unroll
+      for (int t = 0; t < N; ++t) o[t] *= alpha;
+      mref = next;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = M::ex2(s[i] - mref);
+      l = l + s[i];
+    }
+    mul_cols<T, N>(o, v, s);
+#pragma unroll
+    for (int i = 0; i < NF; ++i) x[i] = nx[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < N; ++t) v[i][t] = nv[i][t];
+  }
+  const T sum = over_groups_sum(l);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < N; ++t) so[w][c][N * M::row(i, g) + t] = o[t][i];
+  if (g == 0) {
+    sm[w][c] = mref;
+    sl[w][c] = sum;
+  }
+  __syncthreads();
+  for (int f = threadIdx.x; f < R * DP; f += 256) {
+    const int r = f / DP, d = f % DP;
+    T top = sm[0][r];
+#pragma unroll
+    for (int u = 1; u < 4; ++u) top = fmax(top, sm[u][r]);
+    T y = T(0), tot = T(0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const T wt = sm[u][r] == top ? T(1) : M::ex2(sm[u][r] - top);
+      y = fma(so[u][r][d], wt, y);
+      tot = fma(sl[u][r], wt, tot);
+    }
     if (a.nsplit > 1) {
       const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
-      put_row<T, DP>((T*)a.po + at * DP, o[u], T(1), DP, g, true);
-      if (g == 0) {
-        ((T*)a.pm)[at] = mref[u];
-        ((T*)a.pl)[at] = sum;
+      ((T*)a.po)[at * DP + d] = y;
+      if (d == 0) {
+        ((T*)a.pm)[at] = top;
+        ((T*)a.pl)[at] = tot;
       }
-      continue;
-    }
-    put_row<T, DP>(group_of<T>(a, a.out, a.so, k.b, k.kh) + row_at(a, a.so, r), o[u], sum == T(0) ? T(0) : T(1) / sum, D, g, VEC);
-    if (g == 0 && a.rowmax) {
-      const int64_t at = stat_at(a, k.b, k.kh, r);
-      ((T*)a.rowmax)[at] = mref[u];
-      ((T*)a.rowsum)[at] = sum;
+    } else {
+      if (d < D) (group_of<T>(a, a.out, a.so, k.b, k.kh) + row_at(a, a.so, r))[d] = tot == T(0) ? T(0) : y / tot;
+      if (d == 0 && a.rowmax) {
+        ((T*)a.rowmax)[stat_at(a, k.b, k.kh, r)] = top;
+        ((T*)a.rowsum)[stat_at(a, k.b, k.kh, r)] = tot;
+      }
     }
   }
 }
 
-// Joins the forward's parts: a wave per row, lanes over d.
+// Joins the forward's parts (at most 64): a wave per row. Lane s weighs part s;
+// then the lanes go over d, eight parts' loads in flight.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), bh = id / a.R;
   const int r = (int)(id % a.R);
   if (bh >= a.B * a.Hk) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * a.nsplit * a.R + r;
-  const T* pm = (const T*)a.pm + at;
-  const T* pl = (const T*)a.pl + at;
-  const T* po = (const T*)a.po + at * DP;
-  T top = XM<T>::lowest, sum = T(0);
-  for (int s = 0; s < a.nsplit; ++s) top = fmax(top, pm[s * a.R]);
-  constexpr int PER = (DP + 63) / 64;
-  T o[PER];
+  const int lane = threadIdx.x & 63, n = a.nsplit;
+  const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * n * a.R + r;
+  const bool mine = lane < n;
+  const T m = mine ? ((const T*)a.pm)[at + lane * a.R] : XM<T>::lowest;
+  T top = m;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) o[e] = T(0);
-  for (int s = 0; s < a.nsplit; ++s) {
-    const T wt = pm[s * a.R] == top ? T(1) : XM<T>::ex2(pm[s * a.R] - top);
-    sum = fma(pl[s * a.R], wt, sum);
+  for (int x = 1; x < 64; x <<= 1) top = fmax(top, __shfl_xor(top, x, 64));
+  const T wt = m == top ? T(1) : XM<T>::ex2(m - top);
+  T sum = mine ? ((const T*)a.pl)[at + lane * a.R] * wt : T(0);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int d = lane + 64 * e;
-      if (d < DP) o[e] = fma(po[s * a.R * DP + d], wt, o[e]);
-    }
-  }
+  for (int x = 1; x < 64; x <<= 1) sum = sum + __shfl_xor(sum, x, 64);
   const T inv = sum == T(0) ? T(0) : T(1) / sum;
   T* out = group_of<T>(a, a.out, a.so, b, kh) + row_at(a, a.so, r);
 #pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int d = lane + 64 * e;
-    if (d < a.D) out[d] = o[e] * inv;
+  for (int e = 0; e < (DP + 63) / 64; ++e) {
+    const int d = lane + 64 * e < DP ? lane + 64 * e : DP - 1;
+    const T* p = (const T*)a.po + at * DP + d;
+    T y = T(0);
+    for (int s = 0; s < n; s += 8) {
+      T x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = p[(int64_t)(s + u < n ? s + u : n - 1) * a.R * DP];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const T f = __shfl(wt, s + u < n ? s + u : 0, 64);
+        if (s + u < n) y = fma(x[u], f, y);
+      }
+    }
+    if (lane + 64 * e < a.D) out[lane + 64 * e] = y * inv;
   }
   if (lane == 0 && a.rowmax) {
     ((T*)a.rowmax)[stat_at(a, b, kh, r)] = top;
@@ -455,34 +602,28 @@ __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
   if (on && (threadIdx.x & 15) == 0) ((T*)a.drow)[stat_at(a, bh / a.Hk, bh % a.Hk, r)] = s;
 }
 
-// dQ: a wave owns 16 CT rows and loops over the keys of its part.
-template <typename T, int DP, int CT, bool VEC>
+// dQ: a wave owns 16 rows and loops over the keys of its part.
+template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
-  typedef typename M::vec_t VT;
   constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys, NF = DP / (4 * M::VEC);
   __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
-  const int len = (int)key_count(a, k.b), lo = k.split * a.per, hi = len - lo > a.per ? lo + a.per : len;
-  const int r0 = (k.tile * 4 + w) * 16 * CT, R = (int)a.R;
+  const int len = (int)key_count(a, k.b);
+  int lo, hi;
+  k.part(a, len, KT, lo, hi);
+  const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
+  const bool in = r < R;
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
   const T* Gb = group_of<const T>(a, a.dO, a.sdo, k.b, k.kh);
-  VT qf[CT][NF], gf[CT][NF];
-  T m[CT], inv[CT], dr[CT];
-#pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const int r = r0 + 16 * u + c;
-    const bool in = r < R;
-    load_slice<T, DP>(qf[u], Qb + (in ? row_at(a, a.sq, r) : 0), in, D, g, VEC);
-    load_slice<T, DP>(gf[u], Gb + (in ? row_at(a, a.sdo, r) : 0), in, D, g, VEC);
-    const int64_t at = stat_at(a, k.b, k.kh, in ? r : 0);
-    const T sum = ((const T*)a.rowsum)[at];
-    m[u] = ((const T*)a.rowmax)[at];
-    inv[u] = !in || sum == T(0) ? T(0) : T(1) / sum;
-    dr[u] = ((const T*)a.drow)[at];
-  }
+  typename M::vec_t qf[NF], gf[NF];
+  load_slice<T, DP>(qf, Qb + (in ? row_at(a, a.sq, r) : 0), in, D, g, VEC);
+  load_slice<T, DP>(gf, Gb + (in ? row_at(a, a.sdo, r) : 0), in, D, g, VEC);
+  const int64_t st = stat_at(a, k.b, k.kh, in ? r : 0);
+  const T sum = ((const T*)a.rowsum)[st], m = ((const T*)a.rowmax)[st], dr = ((const T*)a.drow)[st];
+  const T inv = !in || sum == T(0) ? T(0) : T(1) / sum;
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
   Rows<T, KT, DP, VEC> fk, fv;
@@ -495,71 +636,79 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
     fv.fetch(Vb + j0 * a.sv.t, a.sv.t, hi - j0, D);
   };
   const T sl2 = (T)(a.scale * 1.4426950408889634);
-  AT dq[CT][N];
+  AT dq[N];
 #pragma unroll
-  for (int u = 0; u < CT; ++u)
-#pragma unroll
-    for (int t = 0; t < N; ++t) dq[u][t] = AT(0);
+  for (int t = 0; t < N; ++t) dq[t] = AT(0);
   const bool busy = r0 < R;
-  if (lo < hi) fetch(lo);
-  for (int j0 = lo; j0 < hi; j0 += KT) {
-    __syncthreads();
+  if (lo < hi) {
+    fetch(lo);
     fk.put(Ks);
     fv.put(Vs);
-    __syncthreads();
-    if (j0 + KT < hi) fetch(j0 + KT);
-    if (!busy) continue;
+  }
+  __syncthreads();
+  for (int j0 = lo; j0 < hi; j0 += KT) {
+    const bool more = j0 + KT < hi;
+    if (more) fetch(j0 + KT);
+    if (busy) {
+      typename M::vec_t xk[NF], xv[NF];
+      T kc[4][N];
+      lds_slice<T, DP>(xk, Ks, 0, g, c);
+      lds_slice<T, DP>(xv, Vs, 0, g, c);
 #pragma unroll
-    for (int kt = 0; kt < KT / 16; ++kt) {
-      AT ds[CT];
-#pragma unroll
-      for (int u = 0; u < CT; ++u) {
-        const AT s = mul_rows<T, DP>(Ks, 16 * kt, qf[u], g, c) * sl2;
-        const AT dp = mul_rows<T, DP>(Vs, 16 * kt, gf[u], g, c);
+      for (int kt = 0; kt < KT / 16; ++kt) {
+        lds_cols<T, DP>(kc, Ks, 16 * kt, g, c);
+        AT s, dp, ds;
+        mul_slices<T, NF>(s, xk, qf, dp, xv, gf);
+        if (kt + 1 < KT / 16) {
+          lds_slice<T, DP>(xk, Ks, 16 * (kt + 1), g, c);
+          lds_slice<T, DP>(xv, Vs, 16 * (kt + 1), g, c);
+        }
+        s *= sl2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool in = j0 + 16 * kt + M::row(i, g) < hi;
-          ds[u][i] = in && inv[u] != T(0) ? M::ex2(s[i] - m[u]) * inv[u] * (dp[i] - dr[u]) : T(0);
+          const bool on = inv != T(0) && (more || j0 + 16 * kt + M::row(i, g) < hi);
+          const T d = M::ex2(s[i] - m) * inv * (dp[i] - dr);
+          ds[i] = on ? d : T(0);
         }
+        mul_cols<T, N>(dq, kc, ds);
       }
-      mul_cols<T, DP, CT>(dq, Ks, 16 * kt, ds, g, c);
     }
+    __syncthreads();
+    if (more) {
+      fk.put(Ks);
+      fv.put(Vs);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const int r = r0 + 16 * u + c;
-    if (r >= R) continue;
-    if (a.nsplit > 1) {
-      const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
-      put_row<T, DP>((T*)a.po + at * DP, dq[u], (T)a.scale, DP, g, true);
-    } else {
-      put_row<T, DP>(group_of<T>(a, a.dq, a.sdq, k.b, k.kh) + row_at(a, a.sdq, r), dq[u], (T)a.scale, D, g, VEC);
-    }
+  if (!in) return;
+  if (a.nsplit > 1) {
+    const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
+    put_row<T, DP>((T*)a.po + at * DP, dq, (T)a.scale, DP, g, true);
+  } else {
+    put_row<T, DP>(group_of<T>(a, a.dq, a.sdq, k.b, k.kh) + row_at(a, a.sdq, r), dq, (T)a.scale, D, g, VEC);
   }
 }
 
-// dK and dV: a wave owns 16 CT keys and loops over the rows of its part.
-template <typename T, int DP, int CT, bool VEC>
+// dK and dV: a wave owns 16 keys and loops over the rows of its part.
+template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
-  typedef typename M::vec_t VT;
   constexpr int N = DP / 16, LD = DP + M::PAD, QT = kKeys, NF = DP / (4 * M::VEC);
   __shared__ __attribute__((aligned(16))) T Qs[QT * LD], Gs[QT * LD];
-  __shared__ T sm[QT], si[QT], sr[QT];
+  __shared__ __attribute__((aligned(16))) T sm[QT], si[QT], sr[QT];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
-  const int len = (int)key_count(a, k.b), R = (int)a.R, lo = k.split * a.per, hi = R - lo > a.per ? lo + a.per : R;
-  const int j0 = (k.tile * 4 + w) * 16 * CT;
+  const int len = (int)key_count(a, k.b), R = (int)a.R;
+  int lo, hi;
+  k.part(a, R, QT, lo, hi);
+  const int j0 = (k.tile * 4 + w) * 16, j = j0 + c;
+  const bool in = j < len;
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   const T* Vb = (const T*)a.v + k.b * a.sv.b + k.kh * a.sv.h;
-  VT kf[CT][NF], vf[CT][NF];
-#pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const int j = j0 + 16 * u + c;
-    load_slice<T, DP>(kf[u], Kb + (int64_t)(j < len ? j : 0) * a.sk.t, j < len, D, g, VEC);
-    load_slice<T, DP>(vf[u], Vb + (int64_t)(j < len ? j : 0) * a.sv.t, j < len, D, g, VEC);
-  }
+  typename M::vec_t kf[NF], vf[NF];
+  load_slice<T, DP>(kf, Kb + (int64_t)(in ? j : 0) * a.sk.t, in, D, g, VEC);
+  load_slice<T, DP>(vf, Vb + (int64_t)(in ? j : 0) * a.sv.t, in, D, g, VEC);
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
   const T* Gb = group_of<const T>(a, a.dO, a.sdo, k.b, k.kh);
   const int64_t stats = stat_at(a, k.b, k.kh, 0);
@@ -569,25 +718,15 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
     fq.gather([&](int r) { return r0 + r < hi ? Qb + row_at(a, a.sq, r0 + r) : nullptr; }, D);
     fg.gather([&](int r) { return r0 + r < hi ? Gb + row_at(a, a.sdo, r0 + r) : nullptr; }, D);
     if (threadIdx.x < QT) {
-      const bool in = r0 + (int)threadIdx.x < hi;
-      const int64_t at = stats + (in ? r0 + (int)threadIdx.x : 0);
-      const T sum = in ? ((const T*)a.rowsum)[at] : T(0);
+      const bool there = r0 + (int)threadIdx.x < hi;
+      const int64_t at = stats + (there ? r0 + (int)threadIdx.x : 0);
+      const T sum = there ? ((const T*)a.rowsum)[at] : T(0);
       nm = ((const T*)a.rowmax)[at];
       ni = sum == T(0) ? T(0) : T(1) / sum;
       nr = ((const T*)a.drow)[at];
     }
   };
-  const T sl2 = (T)(a.scale * 1.4426950408889634);
-  AT dk[CT][N], dv[CT][N];
-#pragma unroll
-  for (int u = 0; u < CT; ++u)
-#pragma unroll
-    for (int t = 0; t < N; ++t) dk[u][t] = dv[u][t] = AT(0);
-  // a block past the sequence's keys has only zeros to write
-  const bool any = k.tile * 64 * CT < len, busy = j0 < len;
-  if (any && lo < hi) fetch(lo);
-  for (int r0 = lo; any && r0 < hi; r0 += QT) {
-    __syncthreads();
+  auto put = [&] {
     fq.put(Qs);
     fg.put(Gs);
     if (threadIdx.x < QT) {
@@ -595,41 +734,68 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
       si[threadIdx.x] = ni;
       sr[threadIdx.x] = nr;
     }
-    __syncthreads();
-    if (r0 + QT < hi) fetch(r0 + QT);
-    if (!busy) continue;
+  };
+  const T sl2 = (T)(a.scale * 1.4426950408889634);
+  AT dk[N], dv[N];
 #pragma unroll
-    for (int qt = 0; qt < QT / 16; ++qt) {
-      AT p[CT], ds[CT];
+  for (int t = 0; t < N; ++t) dk[t] = dv[t] = AT(0);
+  // a block past the sequence's keys has only zeros to write
+  const bool any = k.tile * 64 < len, busy = j0 < len;
+  if (any && lo < hi) {
+    fetch(lo);
+    put();
+  }
+  __syncthreads();
+  for (int r0 = lo; any && r0 < hi; r0 += QT) {
+    const bool more = r0 + QT < hi;
+    if (more) fetch(r0 + QT);
+    if (busy) {
+      typename M::vec_t xq[NF], xg[NF];
+      T qc[4][N], gc[4][N];
+      lds_slice<T, DP>(xq, Qs, 0, g, c);
+      lds_slice<T, DP>(xg, Gs, 0, g, c);
 #pragma unroll
-      for (int u = 0; u < CT; ++u) {
-        const AT s = mul_rows<T, DP>(Qs, 16 * qt, kf[u], g, c) * sl2;
-        const AT dp = mul_rows<T, DP>(Gs, 16 * qt, vf[u], g, c);
-        const bool in = j0 + 16 * u + c < len;
+      for (int qt = 0; qt < QT / 16; ++qt) {
+        T m[4], inv[4], dr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 16 * qt + M::row(i, g);
-          const bool on = in && si[r] != T(0);
-          p[u][i] = on ? M::ex2(s[i] - sm[r]) * si[r] : T(0);
-          ds[u][i] = on ? p[u][i] * (dp[i] - sr[r]) : T(0);
+          m[i] = sm[r];
+          inv[i] = si[r];
+          dr[i] = sr[r];
         }
-      }
-      mul_cols<T, DP, CT>(dv, Gs, 16 * qt, p, g, c);
-      mul_cols<T, DP, CT>(dk, Qs, 16 * qt, ds, g, c);
-    }
-  }
+        lds_cols<T, DP>(gc, Gs, 16 * qt, g, c);
+        AT s, dp, p, ds;
+        mul_slices<T, NF>(s, xq, kf, dp, xg, vf);
+        lds_cols<T, DP>(qc, Qs, 16 * qt, g, c);
+        if (qt + 1 < QT / 16) {
+          lds_slice<T, DP>(xq, Qs, 16 * (qt + 1), g, c);
+          lds_slice<T, DP>(xg, Gs, 16 * (qt + 1), g, c);
+        }
+        s *= sl2;
 #pragma unroll
-  for (int u = 0; u < CT; ++u) {
-    const int j = j0 + 16 * u + c;
-    if (j >= a.Tk) continue;
-    if (a.nsplit > 1) {
-      const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.Tk + j;
-      put_row<T, DP>((T*)a.po + at * DP, dk[u], (T)a.scale, DP, g, true);
-      put_row<T, DP>((T*)a.pm + at * DP, dv[u], T(1), DP, g, true);
-    } else {
-      put_row<T, DP>((T*)a.dk + k.b * a.sdk.b + k.kh * a.sdk.h + (int64_t)j * a.sdk.t, dk[u], (T)a.scale, D, g, VEC);
-      put_row<T, DP>((T*)a.dv + k.b * a.sdv.b + k.kh * a.sdv.h + (int64_t)j * a.sdv.t, dv[u], T(1), D, g, VEC);
+        for (int i = 0; i < 4; ++i) {
+          const bool on = in && inv[i] != T(0);
+          const T e = M::ex2(s[i] - m[i]) * inv[i], d = e * (dp[i] - dr[i]);
+          p[i] = on ? e : T(0);
+          ds[i] = on ? d : T(0);
+        }
+        mul_cols<T, N>(dv, gc, p);
+        mul_cols<T, N>(dk, qc, ds);
+      }
     }
+    __syncthreads();
+    if (more) put();
+    __syncthreads();
+  }
+  if (j >= a.Tk) return;
+  if (a.nsplit > 1) {
+    const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.Tk + j;
+    put_row<T, DP>((T*)a.po + at * DP, dk, (T)a.scale, DP, g, true);
+    put_row<T, DP>((T*)a.pm + at * DP, dv, T(1), DP, g, true);
+  } else {
+    put_row<T, DP>((T*)a.dk + k.b * a.sdk.b + k.kh * a.sdk.h + (int64_t)j * a.sdk.t, dk, (T)a.scale, D, g, VEC);
+    put_row<T, DP>((T*)a.dv + k.b * a.sdv.b + k.kh * a.sdv.h + (int64_t)j * a.sdv.t, dv, T(1), D, g, VEC);
   }
 }
 
@@ -653,36 +819,32 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
   }
 }
 
-// Blocks along the owned axis, and the parts of the loop over `loop` positions:
-// more than one where the card would have fewer than two blocks per CU, of at
-// least two tiles each.
-static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop) {
-  const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = 2 * (int64_t)num_cus();
-  const int64_t steps = cdiv(loop, kKeys);
+// Blocks along the owned axis, `per_block` of it each, and the parts of the loop
+// over `loop` positions: more than one where the card would have fewer than
+// `per_cu` blocks per CU, of at least `least` positions each, at most 64.
+static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int least) {
+  const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = per_cu * (int64_t)num_cus();
   int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
-  if (s > steps / 2) s = steps / 2;
-  if (s < 1) s = 1;
-  a.per = (int)(cdiv(steps > 0 ? steps : 1, s) * kKeys);
-  a.nsplit = loop > 0 ? (int)cdiv(loop, a.per) : 1;
+  if (s > loop / least) s = loop / least;
+  a.nsplit = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   DTMI_CHECK(tiles <= 0x7fffffff && blocks * a.nsplit <= 0x7fffffff, "cross attention: too many elements");
   a.ntile = (int)tiles;
   return DTMI_OK;
 }
 
-#define X_LAUNCH(KERNEL, CTV)                                                     \
-  {                                                                               \
-    const unsigned grid = (unsigned)(a.B * a.Hk * a.nsplit * a.ntile);            \
-    if (a.vec)                                                                     \
-      KERNEL<T, DP, CTV, true><<<grid, 256, 0, stream()>>>(a);                     \
-    else                                                                           \
-      KERNEL<T, DP, CTV, false><<<grid, 256, 0, stream()>>>(a);                    \
+#define X_LAUNCH(KERNEL)                                                        \
+  {                                                                             \
+    const unsigned grid = (unsigned)(a.B * a.Hk * a.nsplit * a.ntile);          \
+    if (a.vec)                                                                  \
+      KERNEL<T, DP, true><<<grid, 256, 0, stream()>>>(a);                       \
+    else                                                                        \
+      KERNEL<T, DP, false><<<grid, 256, 0, stream()>>>(a);                      \
   }
 
 template <typename T, int DP>
 static int x_fwd(XArgs& a) {
-  constexpr int WIDE = sizeof(T) == 4 ? 2 : 1;
-  const bool wide = WIDE > 1 && a.R > 64;
-  if (int rc = plan(a, a.R, wide ? 64 * WIDE : 64, a.Tk)) return rc;
+  const bool few = a.R <= 16;
+  if (int rc = few ? plan(a, a.R, 16, a.Tk, 4, 64) : plan(a, a.R, 64, a.Tk, 2, 2 * kKeys)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.R;
@@ -691,10 +853,10 @@ static int x_fwd(XArgs& a) {
     a.pm = (T*)ws + n * DP;
     a.pl = (T*)a.pm + n;
   }
-  if (wide)
-    X_LAUNCH(xattn_fwd_kernel, WIDE)
+  if (few)
+    X_LAUNCH(xattn_rows_kernel)
   else
-    X_LAUNCH(xattn_fwd_kernel, 1)
+    X_LAUNCH(xattn_fwd_kernel)
   if (a.nsplit > 1) xattn_join_kernel<T, DP><<<(unsigned)cdiv(a.B * a.Hk * a.R, 4), 256, 0, stream()>>>(a);
   const hipError_t e = hipGetLastError();
   if (ws) pool_free(ws);
@@ -703,8 +865,7 @@ static int x_fwd(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_kv(XArgs& a) {
-  constexpr int CT = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
-  if (int rc = plan(a, a.Tk, 64 * CT, a.R)) return rc;
+  if (int rc = plan(a, a.Tk, 64, a.R, 2, 2 * kKeys)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.Tk * DP;
@@ -712,7 +873,7 @@ static int x_bwd_kv(XArgs& a) {
     a.po = ws;
     a.pm = (T*)ws + n;
   }
-  X_LAUNCH(xattn_bwd_kv_kernel, CT)
+  X_LAUNCH(xattn_bwd_kv_kernel)
   if (a.nsplit > 1)
     xattn_sum_kernel<T, DP, true>
         <<<dim3((unsigned)cdiv(a.B * a.Hk * a.Tk * DP, 256), 2), 256, 0, stream()>>>(a);
@@ -723,14 +884,13 @@ static int x_bwd_kv(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_q(XArgs& a) {
-  constexpr int CT = sizeof(T) == 4 && DP <= 64 ? 2 : 1;
-  if (int rc = plan(a, a.R, 64 * CT, a.Tk)) return rc;
+  if (int rc = plan(a, a.R, 64, a.Tk, 2, 2 * kKeys)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     if (int rc = pool_alloc(&ws, (size_t)a.B * a.Hk * a.nsplit * a.R * DP * sizeof(T))) return rc;
     a.po = ws;
   }
-  X_LAUNCH(xattn_bwd_q_kernel, CT)
+  X_LAUNCH(xattn_bwd_q_kernel)
   if (a.nsplit > 1)
     xattn_sum_kernel<T, DP, false><<<(unsigned)cdiv(a.B * a.Hk * a.R * DP, 256), 256, 0, stream()>>>(a);
   const hipError_t e = hipGetLastError();
