@@ -2156,6 +2156,7 @@ static int attn_fwd_impl(AttnArgs& a) {
 // dQ pass recomputes S, P and dP itself. 4 GiB by default; settable so that
 // the recompute path can be exercised at any size.
 static int64_t g_max_ds_bytes = (int64_t)4 << 30;
+int64_t ds_limit() { return g_max_ds_bytes; }
 
 // The ragged paired-range backward in parts whose dS fits a.ds: `bhs` (batch,
 // head)s at a time, whole batch elements where they fit.

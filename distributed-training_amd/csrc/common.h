@@ -26,6 +26,9 @@ bool initialized();
 int num_cus();
 int device_id();  // the device dtmi_init selected (-1 before)
 
+// The bound on an attention backward's dS workspace (dtmi_attn_set_ds_limit).
+int64_t ds_limit();
+
 // Set-up of the allocation-free LayerNorm backward's device scratch array on
 // `device` (which must be current); called once per device by dtmi_init.
 int ln_scratch_setup(int device);

@@ -83,12 +83,15 @@ struct XArgs {
   void *rowmax, *rowsum;  // [B, H, Tq]: the reference maximum (base 2) and the sum against it
   void* drow;             // [B, H, Tq]: rowsum(dO O)
   void *po, *pm, *pl;     // partial results of a split loop
+  void* ds;               // dS for the dQ pass, or NULL: 16 x 16 tiles [B, Hk][rows / 16][keys / 16], each [key][row]
+  int64_t rt, kt;         // its tiles of rows and keys
   const int64_t* lengths;
   HT sq, sk, sv, so, sdo, sdq, sdk, sdv;
   int64_t B, H, Hk, G, Tq, Tk, D, R;  // G: heads per group, H / Hk; R: rows, G Tq
   double scale;
   FastDiv by_tq;  // rows to heads
-  int nsplit;   // parts of the loop
+  int nsplit;   // parts of the loop, at most
+  int per, parts, least;  // positions per part; with lengths: parts of all sequences, positions to a part at least
   int ntile;    // blocks along the owned axis
   int vec;      // 16-byte loads and stores allowed for every operand, positions less than 2^23 elements apart
 };
@@ -240,6 +243,13 @@ __device__ __forceinline__ void mul_cols(typename XM<T>::acc_t (&out)[N], const 
 #pragma unroll
     for (int t = 0; t < N; ++t) out[t] = XM<T>::mma(x[i][t], p[i], out[t]);
 }
+// float64 products' operands are read when the ones before are done with: read
+// ahead, as the compiler prefers, they spill. float32 has the registers.
+template <typename T>
+__device__ __forceinline__ void phase() {
+  if constexpr (sizeof(T) == 8) __builtin_amdgcn_sched_barrier(0);
+}
+
 // The lane's part of a result row: registers (t, i) are d = N row(i, g) + t
 template <typename T, int DP>
 __device__ __forceinline__ void put_row(T* __restrict__ row, const typename XM<T>::acc_t (&x)[DP / 16], T mul, int D,
@@ -281,14 +291,27 @@ __device__ __forceinline__ T over_groups_sum(T x) {
 struct XBlock {
   int64_t b, kh;
   int tile, split;
-  // this block's part of a loop over n positions, whole tiles of `tile`
-  __device__ __forceinline__ void part(const XArgs& a, int n, int step, int& lo, int& hi) const {
-    const int per = ((n + a.nsplit - 1) / a.nsplit + step - 1) / step * step;
+  // this block's part of a loop over n positions, `per` to a part
+  __device__ __forceinline__ bool part(int per, int n, int& lo, int& hi) const {
     const int64_t from = (int64_t)split * per;
     lo = from < n ? (int)from : n;
     hi = n - lo > per ? lo + per : n;
+    return lo < hi || split == 0;
   }
 };
+// Keys per part of a loop over keys: the host's, or with lengths such that all
+// sequences' parts together number a.parts per key/value head, so that a long
+// sequence gets more blocks and not longer ones (every wave sums the lengths).
+__device__ __forceinline__ int keys_per_part(const XArgs& a) {
+  if (!a.lengths || a.nsplit == 1) return a.per;
+  int64_t total = 0;
+  for (int64_t b = threadIdx.x & 63; b < a.B; b += 64) total += key_count(a, b);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) total += __shfl_xor((long long)total, x, 64);
+  const int64_t fair = (total + a.parts - 1) / a.parts;
+  const int per = (int)(fair > a.least ? fair : a.least), least = (int)((a.Tk + a.nsplit - 1) / a.nsplit);
+  return ((per > least ? per : least) + 63) & ~63;
+}
 __device__ __forceinline__ XBlock x_block(const XArgs& a) {
   // blocks are dealt to the eight XCDs in turn: XCD x takes the x-th eighth of
   // the blocks, so that those sharing a head's keys share an L2; not with
@@ -320,11 +343,11 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
   typedef typename M::acc_t AT;
   constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys;
   __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b);
   int lo, hi;
-  k.part(a, len, KT, lo, hi);
+  if (!k.part(keys_per_part(a), len, lo, hi)) return;
   const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
   typename M::vec_t qf[DP / (4 * M::VEC)];
@@ -362,9 +385,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
       AT p0, p1;
       lds_slice<T, DP>(x0, Ks, 0, g, c);
       lds_slice<T, DP>(x1, Ks, 16, g, c);
-      lds_cols<T, DP>(v0, Vs, 0, g, c);
-      lds_cols<T, DP>(v1, Vs, 16, g, c);
       mul_slices<T, NF>(p0, x0, qf, p1, x1, qf);
+      phase<T>();
+      lds_cols<T, DP>(v0, Vs, 0, g, c);
       p0 *= sl2;
       p1 *= sl2;
       if (!more)
@@ -391,6 +414,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
         l = l + (p0[i] + p1[i]);
       }
       mul_cols<T, N>(o, v0, p0);
+      phase<T>();
+      lds_cols<T, DP>(v1, Vs, 16, g, c);
       mul_cols<T, N>(o, v1, p1);
     }
     __syncthreads();
@@ -431,11 +456,11 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
   constexpr int N = DP / 16, NF = DP / (4 * M::VEC), VW = N % M::VEC == 0 ? M::VEC : 2;
   typedef T vw __attribute__((ext_vector_type(VW)));
   __shared__ T so[4][16][DP + 1], sm[4][16], sl[4][16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D, R = (int)a.R;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D, R = (int)a.R;
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b);
   int lo, hi;
-  k.part(a, len, 64, lo, hi);
+  if (!k.part(keys_per_part(a), len, lo, hi)) return;
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
   VT qf[NF];
   load_slice<T, DP>(qf, Qb + (c < R ? row_at(a, a.sq, c) : 0), c < R, D, g, VEC);
@@ -541,15 +566,79 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
   }
 }
 
-// Joins the forward's parts (at most 64): a wave per row. Lane s weighs part s;
-// then the lanes go over d, eight parts' loads in flight.
+// Parts of a sequence's keys (0 keys: one, of zeros).
+__device__ __forceinline__ int part_count(const XArgs& a, int64_t b) {
+  const int per = keys_per_part(a), len = (int)key_count(a, b);
+  return len > per ? (len + per - 1) / per : 1;
+}
+
+// Joins the forward's parts (at most 64) of few rows: a block per row. Lane s
+// weighs part s; then 256 / DP groups of threads over d add every so many parts
+// each, eight loads in flight, and their sums are added in order. (32 parts of
+// 128 rows: 4.0 us, a wave per row 7.8; of 10656 rows 17.5 and 9.9.)
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) xattn_join_few_kernel(XArgs a) {
+  constexpr int G = DP <= 32 ? 8 : DP <= 64 ? 4 : 2;
+  __shared__ T swt[64], ssum, part[G][DP];
+  const int64_t bh = blockIdx.x / (unsigned)a.R;
+  const int r = (int)(blockIdx.x % (unsigned)a.R), lane = threadIdx.x & 63;
+  const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * a.nsplit * a.R + r;
+  const int n = part_count(a, b);
+  if (threadIdx.x < 64) {
+    const bool mine = lane < n;
+    const T m = mine ? ((const T*)a.pm)[at + lane * a.R] : XM<T>::lowest;
+    T top = m;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = fmax(top, __shfl_xor(top, x, 64));
+    const T wt = m == top ? T(1) : XM<T>::ex2(m - top);
+    T sum = mine ? ((const T*)a.pl)[at + lane * a.R] * wt : T(0);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) sum = sum + __shfl_xor(sum, x, 64);
+    swt[lane] = wt;
+    if (lane == 0) {
+      ssum = sum;
+      if (a.rowmax) {
+        ((T*)a.rowmax)[stat_at(a, b, kh, r)] = top;
+        ((T*)a.rowsum)[stat_at(a, b, kh, r)] = sum;
+      }
+    }
+  }
+  const int d = threadIdx.x % DP, grp = threadIdx.x / DP;
+  const T* p = (const T*)a.po + at * DP + d;
+  T y = T(0), x[8];
+  auto load = [&](int s) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = p[(int64_t)(s + G * u < n ? s + G * u : n - 1) * a.R * DP];
+  };
+  load(grp);  // ahead of the weights
+  __syncthreads();
+  if (grp < G) {
+    for (int s = grp; s < n; s += 8 * G) {
+      if (s != grp) load(s);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s + G * u < n) y = fma(x[u], swt[s + G * u], y);
+    }
+    part[grp][d] = y;
+  }
+  __syncthreads();
+  if (grp == 0 && d < a.D) {
+    y = T(0);
+#pragma unroll
+    for (int u = 0; u < G; ++u) y = y + part[u][d];
+    (group_of<T>(a, a.out, a.so, b, kh) + row_at(a, a.so, r))[d] = ssum == T(0) ? T(0) : y / ssum;
+  }
+}
+
+// The same for many rows: a wave per row.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), bh = id / a.R;
   const int r = (int)(id % a.R);
   if (bh >= a.B * a.Hk) return;
-  const int lane = threadIdx.x & 63, n = a.nsplit;
-  const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * n * a.R + r;
+  const int lane = threadIdx.x & 63;
+  const int64_t b = bh / a.Hk, kh = bh % a.Hk, at = bh * a.nsplit * a.R + r;
+  const int n = part_count(a, b);
   const bool mine = lane < n;
   const T m = mine ? ((const T*)a.pm)[at + lane * a.R] : XM<T>::lowest;
   T top = m;
@@ -609,11 +698,11 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
   typedef typename M::acc_t AT;
   constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys, NF = DP / (4 * M::VEC);
   __shared__ __attribute__((aligned(16))) T Ks[KT * LD], Vs[KT * LD];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b);
   int lo, hi;
-  k.part(a, len, KT, lo, hi);
+  if (!k.part(keys_per_part(a), len, lo, hi)) return;
   const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
   const bool in = r < R;
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
@@ -656,13 +745,10 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
       lds_slice<T, DP>(xv, Vs, 0, g, c);
 #pragma unroll
       for (int kt = 0; kt < KT / 16; ++kt) {
-        lds_cols<T, DP>(kc, Ks, 16 * kt, g, c);
         AT s, dp, ds;
         mul_slices<T, NF>(s, xk, qf, dp, xv, gf);
-        if (kt + 1 < KT / 16) {
-          lds_slice<T, DP>(xk, Ks, 16 * (kt + 1), g, c);
-          lds_slice<T, DP>(xv, Vs, 16 * (kt + 1), g, c);
-        }
+        phase<T>();
+        lds_cols<T, DP>(kc, Ks, 16 * kt, g, c);
         s *= sl2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -671,6 +757,11 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
           ds[i] = on ? d : T(0);
         }
         mul_cols<T, N>(dq, kc, ds);
+        phase<T>();
+        if (kt + 1 < KT / 16) {
+          lds_slice<T, DP>(xk, Ks, 16 * (kt + 1), g, c);
+          lds_slice<T, DP>(xv, Vs, 16 * (kt + 1), g, c);
+        }
       }
     }
     __syncthreads();
@@ -697,11 +788,11 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
   constexpr int N = DP / 16, LD = DP + M::PAD, QT = kKeys, NF = DP / (4 * M::VEC);
   __shared__ __attribute__((aligned(16))) T Qs[QT * LD], Gs[QT * LD];
   __shared__ __attribute__((aligned(16))) T sm[QT], si[QT], sr[QT];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b), R = (int)a.R;
   int lo, hi;
-  k.part(a, R, QT, lo, hi);
+  k.part(a.per, R, lo, hi);
   const int j0 = (k.tile * 4 + w) * 16, j = j0 + c;
   const bool in = j < len;
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
@@ -739,6 +830,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
   AT dk[N], dv[N];
 #pragma unroll
   for (int t = 0; t < N; ++t) dk[t] = dv[t] = AT(0);
+  const T* dsp = (const T*)a.ds + ((k.b * a.Hk + k.kh) * a.rt * a.kt + (j0 >> 4)) * 256;
   // a block past the sequence's keys has only zeros to write
   const bool any = k.tile * 64 < len, busy = j0 < len;
   if (any && lo < hi) {
@@ -764,14 +856,10 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
           inv[i] = si[r];
           dr[i] = sr[r];
         }
-        lds_cols<T, DP>(gc, Gs, 16 * qt, g, c);
         AT s, dp, p, ds;
         mul_slices<T, NF>(s, xq, kf, dp, xg, vf);
-        lds_cols<T, DP>(qc, Qs, 16 * qt, g, c);
-        if (qt + 1 < QT / 16) {
-          lds_slice<T, DP>(xq, Qs, 16 * (qt + 1), g, c);
-          lds_slice<T, DP>(xg, Gs, 16 * (qt + 1), g, c);
-        }
+        phase<T>();
+        lds_cols<T, DP>(gc, Gs, 16 * qt, g, c);
         s *= sl2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -780,8 +868,26 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
           p[i] = on ? e : T(0);
           ds[i] = on ? d : T(0);
         }
+        // (an empty buffer where dS is not kept: no branch)
+        const Rsrc tile = make_rsrc(dsp + (int64_t)((r0 >> 4) + qt) * a.kt * 256, a.ds ? 256 * sizeof(T) : 0);
+        if constexpr (sizeof(T) == 4)
+          buf_store4(ds, tile, (c * 16 + 4 * g) * 4, 0);
+        else
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            typedef int i2 __attribute__((ext_vector_type(2)));
+            const T x = ds[i];  // (a bit cast of the element itself takes element 0)
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i2, x), tile, (c * 16 + M::row(i, g)) * 8, 0, 0);
+          }
         mul_cols<T, N>(dv, gc, p);
+        phase<T>();
+        lds_cols<T, DP>(qc, Qs, 16 * qt, g, c);
         mul_cols<T, N>(dk, qc, ds);
+        phase<T>();
+        if (qt + 1 < QT / 16) {
+          lds_slice<T, DP>(xq, Qs, 16 * (qt + 1), g, c);
+          lds_slice<T, DP>(xg, Gs, 16 * (qt + 1), g, c);
+        }
       }
     }
     __syncthreads();
@@ -799,16 +905,84 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
   }
 }
 
+// dQ from the dS that the dK/dV pass left: one product, bound by reading dS.
+template <typename T, int DP, bool VEC>
+__global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs a) {
+  using M = XM<T>;
+  typedef typename M::acc_t AT;
+  constexpr int N = DP / 16, LD = DP + M::PAD, KT = kKeys;
+  __shared__ __attribute__((aligned(16))) T Ks[KT * LD];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D;
+  const XBlock k = x_block(a);
+  const int len = (int)key_count(a, k.b);
+  int lo, hi;
+  if (!k.part(keys_per_part(a), len, lo, hi)) return;
+  const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
+  const bool busy = r0 < R;
+  // lane (g, c): keys row(i, g) of row c
+  const T* dsp = (const T*)a.ds + ((k.b * a.Hk + k.kh) * a.rt + (busy ? r0 >> 4 : 0)) * a.kt * 256 + c;
+  const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
+  Rows<T, KT, DP, VEC> fk;
+  if constexpr (VEC) fk.start(a.sk.t, D);
+  T nx[2][4];
+  auto fetch = [&](int j0) {
+    fk.fetch(Kb + j0 * a.sk.t, a.sk.t, hi - j0, D);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int kt = (j0 >> 4) + s;  // a tile of keys past the sequence was not written
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        nx[s][i] = j0 + 16 * s < hi ? dsp[(int64_t)kt * 256 + M::row(i, g) * 16] : T(0);
+    }
+  };
+  AT dq[N];
+#pragma unroll
+  for (int t = 0; t < N; ++t) dq[t] = AT(0);
+  if (lo < hi) {
+    fetch(lo);
+    fk.put(Ks);
+  }
+  __syncthreads();
+  for (int j0 = lo; j0 < hi; j0 += KT) {
+    const bool more = j0 + KT < hi;
+    AT ds[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ds[s][i] = nx[s][i];
+    if (more) fetch(j0 + KT);
+    if (busy)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        T kc[4][N];
+        lds_cols<T, DP>(kc, Ks, 16 * s, g, c);
+        mul_cols<T, N>(dq, kc, ds[s]);
+      }
+    __syncthreads();
+    if (more) fk.put(Ks);
+    __syncthreads();
+  }
+  if (r >= R) return;
+  if (a.nsplit > 1) {
+    const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
+    put_row<T, DP>((T*)a.po + at * DP, dq, (T)a.scale, DP, g, true);
+  } else {
+    put_row<T, DP>(group_of<T>(a, a.dq, a.sdq, k.b, k.kh) + row_at(a, a.sdq, r), dq, (T)a.scale, D, g, VEC);
+  }
+}
+
 // Sums the parts of dQ (rows: the group's) or of dK and dV (blockIdx.y 0, 1; rows: keys).
 template <typename T, int DP, bool KV>
 __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
   const int64_t rows = KV ? a.Tk : a.R, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t d = id % DP, r = id / DP % rows, bh = id / DP / rows;
-  if (bh >= a.B * a.Hk || d >= a.D) return;
-  const int64_t b = bh / a.Hk, kh = bh % a.Hk;
+  // (every lane stays for the sum over lengths)
+  const int64_t b = bh < a.B * a.Hk ? bh / a.Hk : 0, kh = bh % a.Hk;
   const T* p = (const T*)(KV && blockIdx.y ? a.pm : a.po) + (bh * a.nsplit * rows + r) * DP + d;
+  const int n = KV ? a.nsplit : part_count(a, b);
+  if (bh >= a.B * a.Hk || d >= a.D) return;
   T s = T(0);
-  for (int i = 0; i < a.nsplit; ++i) s = s + p[(int64_t)i * rows * DP];
+  for (int i = 0; i < n; ++i) s = s + p[(int64_t)i * rows * DP];
   if constexpr (KV) {
     if (blockIdx.y)
       ((T*)a.dv)[b * a.sdv.b + kh * a.sdv.h + r * a.sdv.t + d] = s;
@@ -821,12 +995,19 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
 
 // Blocks along the owned axis, `per_block` of it each, and the parts of the loop
 // over `loop` positions: more than one where the card would have fewer than
-// `per_cu` blocks per CU, of at least `least` positions each, at most 64.
-static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int least) {
+// `per_cu` blocks per CU, of at least `least` positions each (a multiple of
+// 64), at most 64. With lengths (`ragged`) the longest sequence may take up to
+// four times its share of the parts.
+static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int least, bool ragged) {
   const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = per_cu * (int64_t)num_cus();
   int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
+  if (ragged && s > 1) s *= 4;
   if (s > loop / least) s = loop / least;
-  a.nsplit = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  s = s < 1 ? 1 : s > 64 ? 64 : s;
+  a.per = (int)(cdiv(cdiv(loop > 0 ? loop : 1, s), 64) * 64);
+  a.nsplit = loop > 0 ? (int)cdiv(loop, a.per) : 1;
+  a.parts = (int)cdiv(want, a.Hk * tiles);
+  a.least = least;
   DTMI_CHECK(tiles <= 0x7fffffff && blocks * a.nsplit <= 0x7fffffff, "cross attention: too many elements");
   a.ntile = (int)tiles;
   return DTMI_OK;
@@ -844,7 +1025,7 @@ static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu
 template <typename T, int DP>
 static int x_fwd(XArgs& a) {
   const bool few = a.R <= 16;
-  if (int rc = few ? plan(a, a.R, 16, a.Tk, 4, 64) : plan(a, a.R, 64, a.Tk, 2, 2 * kKeys)) return rc;
+  if (int rc = few ? plan(a, a.R, 16, a.Tk, 2, 64, a.lengths) : plan(a, a.R, 64, a.Tk, 3, 64, a.lengths)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.R;
@@ -857,7 +1038,13 @@ static int x_fwd(XArgs& a) {
     X_LAUNCH(xattn_rows_kernel)
   else
     X_LAUNCH(xattn_fwd_kernel)
-  if (a.nsplit > 1) xattn_join_kernel<T, DP><<<(unsigned)cdiv(a.B * a.Hk * a.R, 4), 256, 0, stream()>>>(a);
+  if (a.nsplit > 1) {
+    const int64_t rows = a.B * a.Hk * a.R;
+    if (rows <= 2048)
+      xattn_join_few_kernel<T, DP><<<(unsigned)rows, 256, 0, stream()>>>(a);
+    else
+      xattn_join_kernel<T, DP><<<(unsigned)cdiv(rows, 4), 256, 0, stream()>>>(a);
+  }
   const hipError_t e = hipGetLastError();
   if (ws) pool_free(ws);
   return e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_fwd", __FILE__, __LINE__);
@@ -865,7 +1052,7 @@ static int x_fwd(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_kv(XArgs& a) {
-  if (int rc = plan(a, a.Tk, 64, a.R, 2, 2 * kKeys)) return rc;
+  if (int rc = plan(a, a.Tk, 64, a.R, 2, 64, false)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.Tk * DP;
@@ -884,13 +1071,16 @@ static int x_bwd_kv(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_q(XArgs& a) {
-  if (int rc = plan(a, a.R, 64, a.Tk, 2, 2 * kKeys)) return rc;
+  if (int rc = plan(a, a.R, 64, a.Tk, 2, 64, a.lengths)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     if (int rc = pool_alloc(&ws, (size_t)a.B * a.Hk * a.nsplit * a.R * DP * sizeof(T))) return rc;
     a.po = ws;
   }
-  X_LAUNCH(xattn_bwd_q_kernel)
+  if (a.ds)
+    X_LAUNCH(xattn_bwd_ds_kernel)
+  else
+    X_LAUNCH(xattn_bwd_q_kernel)
   if (a.nsplit > 1)
     xattn_sum_kernel<T, DP, false><<<(unsigned)cdiv(a.B * a.Hk * a.R * DP, 256), 256, 0, stream()>>>(a);
   const hipError_t e = hipGetLastError();
@@ -907,8 +1097,15 @@ static int x_bwd(XArgs& a) {
   xattn_drow_kernel<T><<<(unsigned)cdiv(a.B * a.Hk * a.R, 16), 256, 0, stream()>>>(a);
   const hipError_t e = hipGetLastError();
   int rc = e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_bwd: row dots", __FILE__, __LINE__);
+  // dS handed from the one pass to the other: 16 bytes of traffic per two
+  // scores against two products of the three that the dQ pass would take
+  a.rt = cdiv(a.R, kKeys) * (kKeys / 16);
+  a.kt = cdiv(a.Tk, 16);
+  const int64_t bytes = a.B * a.Hk * a.rt * a.kt * 256 * (int64_t)sizeof(T);
+  if (rc == DTMI_OK && DP > 32 && bytes <= ds_limit() && pool_alloc(&a.ds, bytes) != DTMI_OK) a.ds = nullptr;
   if (rc == DTMI_OK) rc = x_bwd_kv<T, DP>(a);
   if (rc == DTMI_OK) rc = x_bwd_q<T, DP>(a);
+  if (a.ds) pool_free(a.ds);
   pool_free(dr);
   return rc;
 }
