@@ -52,8 +52,12 @@ __host__ __device__ constexpr int held_len(int W) {
   return (sizeof(T) == 4 ? 8 : 4) / (W <= 8 ? 1 : 2);
 }
 // Waves per SIMD the backward's registers are cut to: two of 219 (float32, 9 to
-// 16 states). Three of 168 spill, and a spill's store counts as one to wait for.
-__host__ __device__ constexpr int bwd_waves(int W) { return W == 16 ? 4 : 2; }
+// 16 states; three of 168 spill, and a spill's store counts as one to wait for),
+// one in float64 and for up to 4 states (a wave then stages all of a tile), where two spill.
+template <typename T>
+__host__ __device__ constexpr int bwd_waves(int W) {
+  return W == 16 ? 4 : W == 8 ? 2 : sizeof(T) == 4 && W > 1 ? 2 : 1;
+}
 // Positions per state kept for the backward, which rebuilds the states in
 // between. float32 keeps one per part (16 states: two activations' memory,
 // 5 us more traffic against 10 us of exponentials at 4 x 1024 x 1536 x 16);
@@ -447,7 +451,7 @@ __device__ __forceinline__ T sum8(const T (&v)[8], bool upper8) {
 // step together, and eight steps' results leave a wave as one LDS write.
 // CARRY: only dh over the segment, and its sum of d.
 template <typename T, int W, bool CARRY>
-__global__ void __launch_bounds__(64 * W, bwd_waves(W)) scan_bwd_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanArgs a) {
   constexpr int NS = kStates, TT = tile_len<T>(), HT = held_len<T>(W), KT = keep_len<T>(W);
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP, RB = HT < 8 ? HT : 8;
@@ -736,7 +740,13 @@ __global__ void __launch_bounds__(256) scan_param_kernel(const T* __restrict__ p
   if (id >= (N + 2) * C) return;
   const int64_t n = id / C, c = id % C;
   T s = T(0);
-  for (int64_t p = 0; p < parts; ++p) s = s + prm[p * (N + 2) * C + id];
+  for (int64_t p = 0; p < parts; p += 8) {  // eight terms' loads in flight
+    T x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = prm[(p + u < parts ? p + u : parts - 1) * (N + 2) * C + id];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s = p + u < parts ? s + x[u] : s;
+  }
   if (n < N)
     dA[c * N + n] = s;
   else if (n == N && dD)
@@ -753,9 +763,19 @@ __global__ void __launch_bounds__(256) scan_map_kernel(ScanArgs a, T* __restrict
   if (id >= n1) return;
   const int64_t n = id % a.N, row = id / a.N, g = row % a.G, bt = row / a.G, t = bt % a.T, b = bt / a.T;
   T x = T(0), y = T(0);
-  for (int p = 0; p < a.tpg; ++p) {
-    x = x + ((const T*)a.dBp)[p * n1 + id];
-    y = y + ((const T*)a.dCp)[p * n1 + id];
+  for (int p = 0; p < a.tpg; p += 8) {  // sixteen loads in flight
+    T vx[8], vy[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t at = (p + u < a.tpg ? p + u : a.tpg - 1) * n1 + id;
+      vx[u] = ((const T*)a.dBp)[at];
+      vy[u] = ((const T*)a.dCp)[at];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      x = p + u < a.tpg ? x + vx[u] : x;
+      y = p + u < a.tpg ? y + vy[u] : y;
+    }
   }
   dB[b * sB.b + t * sB.t + g * gB + n] = x;
   dC[b * sC.b + t * sC.t + g * gC + n] = y;

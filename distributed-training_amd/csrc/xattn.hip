@@ -91,7 +91,8 @@ struct XArgs {
   double scale;
   FastDiv by_tq;  // rows to heads
   int nsplit;   // parts of the loop, at most
-  int per, parts, least;  // positions per part; with lengths: parts of all sequences, positions to a part at least
+  int per, step;  // positions per part, a multiple of step
+  int parts;      // with lengths: parts of all sequences together
   int ntile;    // blocks along the owned axis
   int vec;      // 16-byte loads and stores allowed for every operand, positions less than 2^23 elements apart
 };
@@ -309,8 +310,8 @@ __device__ __forceinline__ int keys_per_part(const XArgs& a) {
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) total += __shfl_xor((long long)total, x, 64);
   const int64_t fair = (total + a.parts - 1) / a.parts;
-  const int per = (int)(fair > a.least ? fair : a.least), least = (int)((a.Tk + a.nsplit - 1) / a.nsplit);
-  return ((per > least ? per : least) + 63) & ~63;
+  const int64_t least = (a.Tk + a.nsplit - 1) / a.nsplit, per = fair > least ? fair : least;
+  return (int)((per + a.step - 1) / a.step) * a.step;
 }
 __device__ __forceinline__ XBlock x_block(const XArgs& a) {
   // blocks are dealt to the eight XCDs in turn: XCD x takes the x-th eighth of
@@ -982,7 +983,13 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
   const int n = KV ? a.nsplit : part_count(a, b);
   if (bh >= a.B * a.Hk || d >= a.D) return;
   T s = T(0);
-  for (int i = 0; i < n; ++i) s = s + p[(int64_t)i * rows * DP];
+  for (int i = 0; i < n; i += 8) {  // eight parts' loads in flight
+    T x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = p[(int64_t)(i + u < n ? i + u : n - 1) * rows * DP];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s = i + u < n ? s + x[u] : s;
+  }
   if constexpr (KV) {
     if (blockIdx.y)
       ((T*)a.dv)[b * a.sdv.b + kh * a.sdv.h + r * a.sdv.t + d] = s;
@@ -995,19 +1002,18 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
 
 // Blocks along the owned axis, `per_block` of it each, and the parts of the loop
 // over `loop` positions: more than one where the card would have fewer than
-// `per_cu` blocks per CU, of at least `least` positions each (a multiple of
-// 64), at most 64. With lengths (`ragged`) the longest sequence may take up to
-// four times its share of the parts.
-static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int least, bool ragged) {
+// `per_cu` blocks per CU, of at least two steps each, at most 64. With lengths
+// (`ragged`) the longest sequence may take up to four times its share of the parts.
+static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int step, bool ragged) {
   const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = per_cu * (int64_t)num_cus();
   int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
   if (ragged && s > 1) s *= 4;
-  if (s > loop / least) s = loop / least;
+  if (s > loop / (2 * step)) s = loop / (2 * step);
   s = s < 1 ? 1 : s > 64 ? 64 : s;
-  a.per = (int)(cdiv(cdiv(loop > 0 ? loop : 1, s), 64) * 64);
+  a.step = step;
+  a.per = (int)(cdiv(cdiv(loop > 0 ? loop : 1, s), step) * step);
   a.nsplit = loop > 0 ? (int)cdiv(loop, a.per) : 1;
   a.parts = (int)cdiv(want, a.Hk * tiles);
-  a.least = least;
   DTMI_CHECK(tiles <= 0x7fffffff && blocks * a.nsplit <= 0x7fffffff, "cross attention: too many elements");
   a.ntile = (int)tiles;
   return DTMI_OK;
@@ -1025,7 +1031,7 @@ static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu
 template <typename T, int DP>
 static int x_fwd(XArgs& a) {
   const bool few = a.R <= 16;
-  if (int rc = few ? plan(a, a.R, 16, a.Tk, 2, 64, a.lengths) : plan(a, a.R, 64, a.Tk, 3, 64, a.lengths)) return rc;
+  if (int rc = few ? plan(a, a.R, 16, a.Tk, 2, 64, a.lengths) : plan(a, a.R, 64, a.Tk, 3, kKeys, a.lengths)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.R;
@@ -1052,7 +1058,7 @@ static int x_fwd(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_kv(XArgs& a) {
-  if (int rc = plan(a, a.Tk, 64, a.R, 2, 64, false)) return rc;
+  if (int rc = plan(a, a.Tk, 64, a.R, 3, kKeys, false)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.Tk * DP;
@@ -1071,7 +1077,7 @@ static int x_bwd_kv(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_q(XArgs& a) {
-  if (int rc = plan(a, a.R, 64, a.Tk, 2, 64, a.lengths)) return rc;
+  if (int rc = plan(a, a.R, 64, a.Tk, 3, kKeys, a.lengths)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     if (int rc = pool_alloc(&ws, (size_t)a.B * a.Hk * a.nsplit * a.R * DP * sizeof(T))) return rc;
