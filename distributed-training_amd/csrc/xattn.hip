@@ -17,7 +17,8 @@
 // row(i, g).
 //
 // Forward: scores in base 2, a reference maximum per query that moves only
-// when a score exceeds it by 2^8, sum and output rescaled then. Backward: the
+// when a score exceeds it by 2^8, sum and output rescaled then; a score is
+// scaled and the reference subtracted in one rounding. Backward: the
 // probabilities from the forward's reference and sum (the same products in the
 // same order, so the same scores), dV += P^T dO, dP = dO V^T, dS = P (dP -
 // rowsum(dO O)), dK += dS^T Q in the pass over keys; S, dP and dQ = dS K in
@@ -389,17 +390,12 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
       mul_slices<T, NF>(p0, x0, qf, p1, x1, qf);
       phase<T>();
       lds_cols<T, DP>(v0, Vs, 0, g, c);
-      p0 *= sl2;
-      p1 *= sl2;
-      if (!more)
+      T top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p0[i] = j0 + M::row(i, g) < hi ? p0[i] : -INFINITY;
-          p1[i] = j0 + 16 + M::row(i, g) < hi ? p1[i] : -INFINITY;
-        }
-      T top = fmax(p0[0], p1[0]);
-#pragma unroll
-      for (int i = 1; i < 4; ++i) top = fmax(top, fmax(p0[i], p1[i]));
+      for (int i = 0; i < 4; ++i) {
+        const bool in0 = more || j0 + M::row(i, g) < hi, in1 = more || j0 + 16 + M::row(i, g) < hi;
+        top = fmax(top, fmax(in0 ? p0[i] * sl2 : -INFINITY, in1 ? p1[i] * sl2 : -INFINITY));
+      }
       if (__any(top > mref + T(8))) {
         const T next = fmax(mref, over_groups_max(top));
         const T alpha = M::ex2(mref - next);
@@ -410,8 +406,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p0[i] = M::ex2(p0[i] - mref);
-        p1[i] = M::ex2(p1[i] - mref);
+        const bool in0 = more || j0 + M::row(i, g) < hi, in1 = more || j0 + 16 + M::row(i, g) < hi;
+        p0[i] = in0 ? M::ex2(fma(p0[i], sl2, -mref)) : T(0);
+        p1[i] = in1 ? M::ex2(fma(p1[i], sl2, -mref)) : T(0);
         l = l + (p0[i] + p1[i]);
       }
       mul_cols<T, N>(o, v0, p0);
@@ -503,10 +500,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
     for (int i = 0; i < NF; ++i)
 #pragma unroll
       for (int e = 0; e < M::VEC; ++e) s = M::mma(x[i][e], qf[i][e], s);
-    s *= sl2;
+    T top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = j + M::row(i, g) < hi ? s[i] : -INFINITY;
-    const T top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
+    for (int i = 0; i < 4; ++i) top = fmax(top, j + M::row(i, g) < hi ? s[i] * sl2 : -INFINITY);
     if (__any(top > mref + T(8))) {
       const T next = fmax(mref, over_groups_max(top));
       const T alpha = M::ex2(mref - next);
@@ -517,7 +513,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[i] = M::ex2(s[i] - mref);
+      s[i] = j + M::row(i, g) < hi ? M::ex2(fma(s[i], sl2, -mref)) : T(0);
       l = l + s[i];
     }
     mul_cols<T, N>(o, v, s);
@@ -750,11 +746,10 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
         mul_slices<T, NF>(s, xk, qf, dp, xv, gf);
         phase<T>();
         lds_cols<T, DP>(kc, Ks, 16 * kt, g, c);
-        s *= sl2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool on = inv != T(0) && (more || j0 + 16 * kt + M::row(i, g) < hi);
-          const T d = M::ex2(s[i] - m) * inv * (dp[i] - dr);
+          const T d = M::ex2(fma(s[i], sl2, -m)) * inv * (dp[i] - dr);
           ds[i] = on ? d : T(0);
         }
         mul_cols<T, N>(dq, kc, ds);
@@ -861,11 +856,10 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
         mul_slices<T, NF>(s, xq, kf, dp, xg, vf);
         phase<T>();
         lds_cols<T, DP>(gc, Gs, 16 * qt, g, c);
-        s *= sl2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool on = in && inv[i] != T(0);
-          const T e = M::ex2(s[i] - m[i]) * inv[i], d = e * (dp[i] - dr[i]);
+          const T e = M::ex2(fma(s[i], sl2, -m[i])) * inv[i], d = e * (dp[i] - dr[i]);
           p[i] = on ? e : T(0);
           ds[i] = on ? d : T(0);
         }
