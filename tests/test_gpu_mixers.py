@@ -174,6 +174,9 @@ SCAN = [  # B, T, C, N, G, lengths, fused, has (D, z, bias, state, softplus)
     (2, 50, 20, 64, 1, [50, 31], False, (1, 1, 1, 1, 1)),
     (1, 700, 66, 16, 1, None, True, (1, 1, 1, 1, 1)),     # segments of the sequence
     (3, 410, 16, 3, 1, [0, 410, 130], False, (1, 1, 1, 1, 1)),  # with ends inside and before them
+    (2, 300, 70, 48, 2, [300, 129], True, (1, 1, 1, 1, 1)),
+    (1, 230, 200, 8, 1, None, False, (1, 1, 1, 0, 1)),
+    (300, 20, 64, 2, 1, None, False, (1, 1, 1, 1, 1)),    # enough blocks for one segment
 ]
 
 
@@ -293,6 +296,10 @@ CROSS = [  # B, H, Hk, Tq, Tk, D, lengths, strided
     (1, 1, 1, 600, 3, 40, None, False),
     (1, 1, 1, 3, 3000, 48, None, True),
     (1, 12, 12, 200, 160, 64, None, True),
+    (2, 4, 1, 1, 900, 128, [900, 130], True),   # up to 16 rows per key/value head
+    (1, 6, 2, 5, 210, 100, None, False),
+    (4, 16, 1, 1, 70, 96, [1, 0, 70, 16], False),
+    (9, 1, 1, 90, 1100, 40, [0, 1, 1100, 64, 65, 600, 1099, 33, 2], False),  # parts by the lengths' sum
 ]
 
 
@@ -323,6 +330,35 @@ def test_cross_attention(dev, dt, case):
         close(x.grad, want, dt, 512, "d" + n)
     with A.no_grad():
         assert bits_equal(A.cross_attention(Q, Kt, V, lengths=lengths).numpy(), o.numpy())
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("case", [(2, 3, 3, 70, 65, 64, [65, 64]), (1, 4, 2, 90, 700, 96, None), (2, 2, 1, 40, 33, 128, [7, 33])],
+                         ids=lambda c: "-".join(str(v) for v in c[:6]))
+def test_cross_attention_backward_without_kept_ds(dev, dt, case):
+    """dS formed twice where its workspace is refused: the same dK and dV bits,
+    and dQ to the same bar."""
+    from dtmi import kernels as K
+    A, D = _mods()
+    B, H, Hk, Tq, Tk, Dh, lengths = case
+    rng = np.random.default_rng(Tq + Tk)
+    v = [rng.standard_normal(s).astype(dt) for s in ((B, H, Tq, Dh), (B, Hk, Tk, Dh), (B, Hk, Tk, Dh), (B, H, Tq, Dh))]
+
+    def grads():
+        L = [A.Tensor(D.from_numpy(x), requires_grad=True) for x in v[:3]]
+        A.cross_attention(*L, lengths=lengths).backward(D.from_numpy(v[3]))
+        return [x.grad.numpy() for x in L]
+    kept = grads()
+    before = K.attn_set_ds_limit(0)
+    try:
+        again = grads()
+    finally:
+        K.attn_set_ds_limit(before)
+    assert bits_equal(kept[1], again[1]) and bits_equal(kept[2], again[2])
+    R = [t64(x) for x in v[:3]]
+    want = torch.autograd.grad(cross_ref(*R, lengths, Dh ** -.5), R, t64(v[3], False))
+    close(kept[0], want[0], dt, 512, "dq, dS kept")
+    close(again[0], want[0], dt, 512, "dq, dS formed twice")
 
 
 def test_cross_attention_scale_and_large_scores(dev):
@@ -476,6 +512,80 @@ def test_results_repeat(dev):
     first = once()
     for a, b_ in zip(first, once()):
         assert bits_equal(a, b_)
+
+
+def test_gradients_land_and_accumulate(dev):
+    """Parameters with a place for their gradient get it written there; a second
+    backward adds; an upstream gradient may be a transposed view; one tensor may
+    be several operands; two graphs may be alive at once."""
+    A, D = _mods()
+    rng = np.random.default_rng(8)
+    B, T, C, N = 2, 30, 40, 6
+
+    def t(*s):
+        return rng.standard_normal(s)
+    x, w, b, Am, Dm, Bm = t(B, T, C), t(4, C), t(C), -rng.random((C, N)) - .5, t(C), t(B, T, N)
+    g = t(B, C, T)
+    flat = D.zeros((4 * C + C + C * N + C,), F64)
+    leaves = [A.Tensor(D.from_numpy(a), requires_grad=True) for a in (w, b, Am, Dm)]
+    off = 0
+    for p in leaves:
+        n = p.data.size
+        p.grad_dest = flat[off:off + n].reshape(p.shape)
+        off += n
+    W, bias, At, Dt = leaves
+    X, M = A.Tensor(D.from_numpy(x), requires_grad=True), A.Tensor(D.from_numpy(Bm), requires_grad=True)
+
+    def graph():
+        c = A.causal_conv(X, W, bias)
+        return A.ssm_scan(c, c, At, M, M, Dt, z=X)  # the maps one tensor, the convolution's output twice
+    y1, y2 = graph(), graph()
+    up = D.from_numpy(g).transpose(0, 2, 1)  # (B, T, C), C not contiguous
+    y1.backward(up)
+    once = flat.numpy()
+    for p in leaves:
+        assert p.grad.ptr == p.grad_dest.ptr
+    y2.backward(up)
+    assert bits_equal(flat.numpy(), once + once)
+    R = [t64(a) for a in (x, w, b, Am, Dm, Bm)]
+    zero = torch.zeros(B, 3, C, dtype=torch.float64)
+    rc, _ = conv_ref(R[0], R[1], R[2], zero, None, True)
+    m = R[5][:, :, None]
+    ry, _ = scan_ref(rc, rc, R[3], m, m, R[4], R[0], torch.zeros(C, dtype=torch.float64),
+                     torch.zeros(B, C, N, dtype=torch.float64), None, True)
+    want = torch.autograd.grad(ry, R, t64(g.transpose(0, 2, 1), False))
+    for p, r, n in zip([X] + leaves + [M], want, ("x", "w", "b", "A", "D", "B and C")):
+        close(p.grad.numpy() / 2, r, F64, 1024, "d" + n)
+
+
+@pytest.mark.parametrize("what", ["conv", "scan"])
+def test_lengths_uploaded_once_and_padding_left_out(dev, what):
+    """An Indices serves as lengths for several calls; every sequence of a padded
+    batch gives the bits it gives alone."""
+    A, D = _mods()
+    rng = np.random.default_rng(4)
+    B, T, C, N = 5, 70, 48, 16
+    ln = [70, 1, 0, 33, 64]
+    ix = A.Indices(ln)
+    x, m = rng.standard_normal((B, T, C)).astype(F32), rng.standard_normal((B, T, N)).astype(F32)
+    w, Am = rng.standard_normal((4, C)).astype(F32), (-rng.random((C, N))).astype(F32)
+
+    def run(x, m, ln):
+        X, M = A.Tensor(D.from_numpy(x)), A.Tensor(D.from_numpy(m))
+        if what == "conv":
+            return A.causal_conv(X, A.Tensor(D.from_numpy(w)), lengths=ln, return_state=True)
+        return A.ssm_scan(X, X, A.Tensor(D.from_numpy(Am)), M, M, lengths=ln, return_state=True)
+    with A.no_grad():
+        for _ in range(2):
+            y, s = run(hide(x, ln), hide(m, ln), ix)
+        for i, n in enumerate(ln):
+            y1, s1 = run(x[i:i + 1, :n], m[i:i + 1, :n], None)
+            assert (y.numpy()[i, n:] == 0).all()
+            if what == "conv":
+                assert bits_equal(y.numpy()[i, :n], y1.numpy()[0]) and bits_equal(s.numpy()[i], s1.numpy()[0])
+            else:  # a sequence alone may be split differently
+                close(y.numpy()[i, :n], y1.numpy()[0], F32, 64, "y")
+                close(s.numpy()[i], s1.numpy()[0], F32, 64, "state")
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
