@@ -14,6 +14,7 @@ arrays; `.contiguous()` materialises a strided view with one copy kernel.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from math import prod
 
 import numpy as np
@@ -41,12 +42,23 @@ class Block:
             self.ptr = None
 
 
-def _contig_strides(shape):
+@lru_cache(maxsize=4096)
+def _contig_strides(shape: tuple):
     st, acc = [], 1
     for s in reversed(shape):
         st.append(acc)
         acc *= int(s)
     return tuple(reversed(st))
+
+
+@lru_cache(maxsize=4096)
+def _is_contiguous(shape: tuple, strides: tuple) -> bool:
+    exp = 1
+    for s, st in zip(reversed(shape), reversed(strides)):
+        if s != 1 and st != exp:
+            return False
+        exp *= s
+    return True
 
 
 class DeviceArray:
@@ -83,12 +95,7 @@ class DeviceArray:
 
     @property
     def is_contiguous(self) -> bool:
-        exp = 1
-        for s, st in zip(reversed(self.shape), reversed(self.strides)):
-            if s != 1 and st != exp:
-                return False
-            exp *= s
-        return True
+        return _is_contiguous(self.shape, self.strides)
 
     def __len__(self):
         if not self.shape:

@@ -710,9 +710,9 @@ def _same(x: DeviceArray, shape: tuple, dtype, what: str, contiguous: bool = Tru
 
 def _conv_check(x, w, b, state, what):
     C_ = x.shape[-1]
-    if w.ndim != 2 or w.shape[1] != C_ or not 1 <= w.shape[0] <= 8:
+    K = w.shape[0] if len(w.shape) == 2 and w.shape[1] == C_ else 0
+    if not 1 <= K <= 8:
         raise ValueError(f"{what}: w must be [taps, {C_}] with 1 to 8 taps, not {w.shape}")
-    K = w.shape[0]
     _same(w, (K, C_), x.dtype, f"{what}: w")
     if b is not None:
         _same(b, (C_,), x.dtype, f"{what}: b")
