@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backwar
   if (b >= a.B) return;
   const T A2 = ((const T*)a.A)[c * a.N + n] * T(kLog2e);
   T in = !backward && a.h0 ? ((const T*)a.h0)[(b * a.C + c) * a.N + n] : T(0);
-  // the loads do not wait for the chain: eight segments' at a time
-  constexpr int U = 8;
+  // the loads do not wait for the chain: sixteen segments' at a time
+  constexpr int U = 16;
   const int64_t step = backward ? -1 : 1, from = b * a.nseg + (backward ? a.nseg - 1 : 0);
   T* p = (T*)a.carry + (from * a.N + n) * a.C + c;
   const T* d = (const T*)a.dsum + from * a.C + c;
