@@ -316,8 +316,10 @@ __device__ __forceinline__ int keys_per_part(const XArgs& a) {
 }
 __device__ __forceinline__ XBlock x_block(const XArgs& a) {
   // blocks are dealt to the eight XCDs in turn: XCD x takes the x-th eighth of
-  // the blocks, so that those sharing a head's keys share an L2; not with
-  // lengths, where an eighth may hold the long sequences
+  // the blocks, so that those sharing a head's keys share an L2 (forward of 8 x 12
+  // heads x 1024 x 2048 x 64: 457 us, in the dealt order 463); not with lengths,
+  // where an eighth may hold the long sequences (4 x 8 / 2 heads x 333 x 777 x 72,
+  // forward and backward: 427 us so and 314 dealt, when this was chosen)
   const unsigned n = gridDim.x, xcd = blockIdx.x & 7, more = n & 7;
   const unsigned id = a.lengths ? blockIdx.x : xcd * (n >> 3) + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
   XBlock k;
@@ -331,7 +333,8 @@ __device__ __forceinline__ XBlock x_block(const XArgs& a) {
 
 // Waves per SIMD the registers are cut to: more than two would spill, and the
 // wide float64 tiles do at two. (With no bound the accumulators go to the
-// accumulation registers and every use of a score is a move more.)
+// accumulation registers and every use of a score is a move more: forward and
+// backward of 8 x 12 heads x 1024 x 512 x 64 took 671 us so, and 582 bounded.)
 template <typename T>
 constexpr int x_waves(int DP) {
   return sizeof(T) == 8 && DP >= 96 ? 1 : 2;
@@ -339,6 +342,11 @@ constexpr int x_waves(int DP) {
 
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 
+// The forward for more than 16 rows: a wave owns 16 of them. Bound by the MFMAs:
+// two products, 4 D per score. float32, 32 x 12 heads x 1024 x 2048 x 64: 130
+// TFLOP/s (a large library product: 154); 8 x 12 x 1024 x 512: 125 us, 103, one
+// and a half rounds of blocks. Five or six waves per SIMD spill, a second LDS
+// buffer and 32 rows per wave gave nothing.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a) {
   using M = XM<T>;
@@ -445,7 +453,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
 // Up to 16 rows per key/value head (one query token with shared heads): bound
 // by reading k and v once. Each wave takes every fourth 16 keys of the block's
 // part and loads them straight into the products' operand registers, the next
-// 16 while it works; the waves' results are joined through LDS.
+// 16 while it works; the waves' results are joined through LDS. One query of
+// 64 x 12 heads x 1024 keys x 64, 403 MB: 74 us, 5.4 TB/s (the kernel for more
+// rows, three of its waves idle: 84); of 8 x 16 / 4 heads x 4999 x 128: 34 and 56.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a) {
   using M = XM<T>;
@@ -670,7 +680,7 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
   }
 }
 
-// rowsum(dO O): 16 lanes per row
+// rowsum(dO O): 16 lanes per row; reads both once (8 x 12 x 1024 x 64 float32: 12 us, 4.2 TB/s)
 template <typename T>
 __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), bh = id / a.R;
@@ -688,7 +698,9 @@ __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
   if (on && (threadIdx.x & 15) == 0) ((T*)a.drow)[stat_at(a, bh / a.Hk, bh % a.Hk, r)] = s;
 }
 
-// dQ: a wave owns 16 rows and loops over the keys of its part.
+// dQ where dS is not kept: a wave owns 16 rows and loops over the keys of its
+// part. Bound by the MFMAs (three products): float32, 32 x 12 heads x 1024 x 2048 x
+// 64, 131 TFLOP/s.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs a) {
   using M = XM<T>;
@@ -776,7 +788,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
   }
 }
 
-// dK and dV: a wave owns 16 keys and loops over the rows of its part.
+// dK and dV: a wave owns 16 keys and loops over the rows of its part. Bound by
+// the MFMAs (four products): float32, 32 x 12 heads x 1024 x 2048 x 64, 124
+// TFLOP/s; 8 x 12 x 1024 x 512, 768 blocks: 250 us, 103.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs a) {
   using M = XM<T>;
@@ -900,7 +914,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
   }
 }
 
-// dQ from the dS that the dK/dV pass left: one product, bound by reading dS.
+// dQ from the dS that the dK/dV pass left: one product, bound by reading dS
+// (8 x 12 heads x 1024 x 512 x 64 float32, 201 MB: 60 to 75 us).
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs a) {
   using M = XM<T>;
@@ -966,7 +981,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs
   }
 }
 
-// Sums the parts of dQ (rows: the group's) or of dK and dV (blockIdx.y 0, 1; rows: keys).
+// Sums the parts of dQ (rows: the group's) or of dK and dV (blockIdx.y 0, 1; rows:
+// keys): launch and one round of loads (4 x 8 / 2 heads x 333 x 777 x 72: 12 us each).
 template <typename T, int DP, bool KV>
 __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
   const int64_t rows = KV ? a.Tk : a.R, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -998,6 +1014,10 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
 // over `loop` positions: more than one where the card would have fewer than
 // `per_cu` blocks per CU, of at least two steps each, at most 64. With lengths
 // (`ragged`) the longest sequence may take up to four times its share of the parts.
+// per_cu 3 (2 for up to 16 rows) was taken from sweeps of 1, 2, 3, 5: backward of
+// 4 x 8 / 2 heads x 333 x 777 x 72, padded, 155 / 115 / 100 / 107 us, of 2 x 12 x
+// 300 x 257 x 64 51 / 48 / 47 / 47; one query of 8 x 16 / 4 heads x 4999 x 128
+// 39 / 34 / 44 / 41.
 static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int step, bool ragged) {
   const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = per_cu * (int64_t)num_cus();
   int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
@@ -1097,12 +1117,14 @@ static int x_bwd(XArgs& a) {
   xattn_drow_kernel<T><<<(unsigned)cdiv(a.B * a.Hk * a.R, 16), 256, 0, stream()>>>(a);
   const hipError_t e = hipGetLastError();
   int rc = e == hipSuccess ? DTMI_OK : fail_hip(e, "dtmi_xattn_bwd: row dots", __FILE__, __LINE__);
-  // dS handed from the one pass to the other: 16 bytes of traffic per two
-  // scores against two products of the three that the dQ pass would take
+  // dS handed from the one pass to the other, where it may be kept: 8 bytes of
+  // traffic per score (float32) against two of the three products that the dQ pass
+  // would take. Backward of 8 x 12 heads x 1024 queries, us without and with: 512
+  // keys x 32 237 / 195, 512 x 64 400 / 312, 2048 x 32 824 / 697, 2048 x 64 1492 / 1127.
   a.rt = cdiv(a.R, kKeys) * (kKeys / 16);
   a.kt = cdiv(a.Tk, 16);
   const int64_t bytes = a.B * a.Hk * a.rt * a.kt * 256 * (int64_t)sizeof(T);
-  if (rc == DTMI_OK && DP > 32 && bytes <= ds_limit() && pool_alloc(&a.ds, bytes) != DTMI_OK) a.ds = nullptr;
+  if (rc == DTMI_OK && bytes <= ds_limit() && pool_alloc(&a.ds, bytes) != DTMI_OK) a.ds = nullptr;
   if (rc == DTMI_OK) rc = x_bwd_kv<T, DP>(a);
   if (rc == DTMI_OK) rc = x_bwd_q<T, DP>(a);
   if (a.ds) pool_free(a.ds);
@@ -1125,7 +1147,7 @@ static int x_shape(const char* what, int dtype, int64_t B, int64_t H, int64_t Hk
              (long long)Hk);
   DTMI_CHECK(D >= 1 && D <= 128, "%s: head dimension 1 to 128 (got %lld)", what, (long long)D);
   DTMI_CHECK(Tk < ((int64_t)1 << 31) - 4096, "%s: too many keys", what);
-  DTMI_CHECK(B * H * Tq < ((int64_t)1 << 31) && B * Hk * Tk * 128 < ((int64_t)1 << 38), "%s: too many elements", what);
+  DTMI_CHECK(B * H * Tq < ((int64_t)1 << 31) - 4096 && B * Hk * Tk * 128 < ((int64_t)1 << 38), "%s: too many elements", what);
   return DTMI_OK;
 }
 

@@ -333,7 +333,8 @@ def test_cross_attention(dev, dt, case):
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
-@pytest.mark.parametrize("case", [(2, 3, 3, 70, 65, 64, [65, 64]), (1, 4, 2, 90, 700, 96, None), (2, 2, 1, 40, 33, 128, [7, 33])],
+@pytest.mark.parametrize("case", [(2, 3, 3, 70, 65, 64, [65, 64]), (1, 4, 2, 90, 700, 96, None), (2, 2, 1, 40, 33, 128, [7, 33]),
+                                  (2, 3, 1, 50, 47, 20, [3, 47])],
                          ids=lambda c: "-".join(str(v) for v in c[:6]))
 def test_cross_attention_backward_without_kept_ds(dev, dt, case):
     """dS formed twice where its workspace is refused: the same dK and dV bits,
