@@ -4,6 +4,8 @@ Mirrors dtrain/autograd.py: `Tensor(data, requires_grad, name)`, `.grad`,
 `.backward(grad=None)`, `.register_grad_ready_hook(fn)`, the operators
 `+ - * @`, `.sum .mean .reshape .transpose .gelu .relu`, and the functional ops
 `embedding`, `layer_norm`, `causal_attention`, `cross_entropy`, `no_grad`.
+Beside causal_attention, without a counterpart there: `causal_conv`, `ssm_scan`,
+`cross_attention` and the single-token `causal_conv_step`, `ssm_scan_step`.
 
 Differences from dtrain are in where the numbers live, not in semantics:
 `.data` and `.grad` are DeviceArrays (HBM buffers owned by libdtmi; `.numpy()`
