@@ -84,7 +84,7 @@ struct XArgs {
   void *rowmax, *rowsum;  // [B, H, Tq]: the reference maximum (base 2) and the sum against it
   void* drow;             // [B, H, Tq]: rowsum(dO O)
   void *po, *pm, *pl;     // partial results of a split loop
-  void* ds;               // dS for the dQ pass, or NULL: 16 x 16 tiles [B, Hk][rows / 16][keys / 16], each [key][row]
+  void* ds;               // dS for the dQ pass, or NULL: 16 x 16 tiles [B, Hk][rows / 16][keys / 16], each [key][4 g + i] for row(i, g)
   int64_t rt, kt;         // its tiles of rows and keys
   const int64_t* lengths;
   HT sq, sk, sv, so, sdo, sdq, sdk, sdv;
@@ -332,12 +332,14 @@ __device__ __forceinline__ XBlock x_block(const XArgs& a) {
 }
 
 // Waves per SIMD the registers are cut to: more than two would spill, and the
-// wide float64 tiles do at two. (With no bound the accumulators go to the
-// accumulation registers and every use of a score is a move more: forward and
-// backward of 8 x 12 heads x 1024 x 512 x 64 took 671 us so, and 582 bounded.)
+// wide float64 tiles do at two, those of the pass that owns two operands (kv) from
+// 64 elements on (backward of 8 x 12 heads x 1024 x 512 x 64: 937 us at two, 735).
+// (With no bound the accumulators go to the accumulation registers and every use
+// of a score is a move more: forward and backward of the same in float32 took 671
+// us so, and 582 bounded.)
 template <typename T>
-constexpr int x_waves(int DP) {
-  return sizeof(T) == 8 && DP >= 96 ? 1 : 2;
+constexpr int x_waves(int DP, bool kv = false) {
+  return sizeof(T) == 8 && DP >= (kv ? 64 : 96) ? 1 : 2;
 }
 
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
@@ -792,7 +794,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
 // the MFMAs (four products): float32, 32 x 12 heads x 1024 x 2048 x 64, 124
 // TFLOP/s; 8 x 12 x 1024 x 512, 768 blocks: 250 us, 103.
 template <typename T, int DP, bool VEC>
-__global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs a) {
+__global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel(XArgs a) {
   using M = XM<T>;
   typedef typename M::acc_t AT;
   constexpr int N = DP / 16, LD = DP + M::PAD, QT = kKeys, NF = DP / (4 * M::VEC);
@@ -879,15 +881,14 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_kv_kernel(XArgs
         }
         // (an empty buffer where dS is not kept: no branch)
         const Rsrc tile = make_rsrc(dsp + (int64_t)((r0 >> 4) + qt) * a.kt * 256, a.ds ? 256 * sizeof(T) : 0);
-        if constexpr (sizeof(T) == 4)
-          buf_store4(ds, tile, (c * 16 + 4 * g) * 4, 0);
-        else
+        typedef int i4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            typedef int i2 __attribute__((ext_vector_type(2)));
-            const T x = ds[i];  // (a bit cast of the element itself takes element 0)
-            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(i2, x), tile, (c * 16 + M::row(i, g)) * 8, 0, 0);
-          }
+        for (int i = 0; i < 4; i += M::VEC) {
+          typename M::vec_t y;
+#pragma unroll
+          for (int e = 0; e < M::VEC; ++e) y[e] = ds[i + e];
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i4, y), tile, (c * 16 + 4 * g + i) * (int)sizeof(T), 0, 0);
+        }
         mul_cols<T, N>(dv, gc, p);
         phase<T>();
         lds_cols<T, DP>(qc, Qs, 16 * qt, g, c);
@@ -929,8 +930,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs
   if (!k.part(keys_per_part(a), len, lo, hi)) return;
   const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
   const bool busy = r0 < R;
-  // lane (g, c): keys row(i, g) of row c
-  const T* dsp = (const T*)a.ds + ((k.b * a.Hk + k.kh) * a.rt + (busy ? r0 >> 4 : 0)) * a.kt * 256 + c;
+  // lane (g, c): keys row(i, g) of row c, which stands where its writer's registers put it
+  const int cp = M::row(1, 0) == 1 ? c : 4 * (c & 3) + (c >> 2);
+  const T* dsp = (const T*)a.ds + ((k.b * a.Hk + k.kh) * a.rt + (busy ? r0 >> 4 : 0)) * a.kt * 256 + cp;
   const T* Kb = (const T*)a.k + k.b * a.sk.b + k.kh * a.sk.h;
   Rows<T, KT, DP, VEC> fk;
   if constexpr (VEC) fk.start(a.sk.t, D);
