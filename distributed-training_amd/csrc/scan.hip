@@ -32,15 +32,16 @@ namespace dtmi {
 constexpr int kStates = 4;  // states per lane
 constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
-// Positions per tile.
+// Positions per tile. The backward's sixteen waves have 128 registers a lane, which
+// hold half a float32 tile (4 x 1024 x 1536 x 64: 16 positions spill, 732 us, 8: 472).
 template <typename T>
-__host__ __device__ constexpr int tile_len() {
-  return sizeof(T) == 4 ? 16 : 8;
+__host__ __device__ constexpr int tile_len(int W, bool bwd) {
+  return sizeof(T) == 4 && !(bwd && W == 16) ? 16 : 8;
 }
 // Positions whose per-wave sums pass through LDS together in the forward.
 template <typename T>
 __host__ __device__ constexpr int sum_len(int W) {
-  const int n = (sizeof(T) == 4 ? 64 : 32) / W, t = tile_len<T>();
+  const int n = (sizeof(T) == 4 ? 64 : 32) / W, t = tile_len<T>(W, false);
   return n < t ? n : t;
 }
 // Positions whose states and decays a backward wave holds in registers at a
@@ -64,7 +65,7 @@ __host__ __device__ constexpr int bwd_waves(int W) {
 // from 33 states on, and in float64, memory counts for more: one per tile.
 template <typename T>
 __host__ __device__ constexpr int keep_len(int W) {
-  return sizeof(T) == 4 && W <= 8 ? held_len<T>(W) : tile_len<T>();
+  return sizeof(T) == 4 && W <= 8 ? held_len<T>(W) : tile_len<T>(W, true);
 }
 static int waves_for(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
@@ -208,6 +209,14 @@ template <typename T>
 struct Step {
   T d, x, g, b[kStates], c[kStates];
 };
+// Not where many waves share a SIMD's registers: there they cover each other's reads
+// and the positions ahead would spill (4 x 1024 x 1536, us with and without: backward
+// of 64 states 826 / 732 in float32, 3285 / 3015 in float64, of 32 in float64 1041 /
+// 890; small, the forward and the segments' passes: 64 states in float64 1516 / 912).
+template <typename T>
+constexpr bool reads_ahead(int W, bool small) {
+  return sizeof(T) == 4 ? small || W < 16 : W < (small ? 16 : 8);
+}
 
 // 4 x 1024 x 1536 x 16 float32: 100.7 M states and steps at 6 issue slots are 15
 // us of vector instructions, the bytes 19; measured 39, and 27 for CARRY: the
@@ -216,9 +225,10 @@ struct Step {
 // CARRY: only the segment's end state from a zero start, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(), YT = sum_len<T>(W), KT = keep_len<T>(W);
+  constexpr int NS = kStates, TT = tile_len<T>(W, false), YT = sum_len<T>(W), KT = keep_len<T>(W);
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP;
+  constexpr bool AHEAD = reads_ahead<T>(W, true);
   __shared__ __attribute__((aligned(16))) T sB[TT * NP], sC[CARRY ? 1 : TT * NP];
   __shared__ T sd[TT][64], sx[TT][64], yp[CARRY ? 1 : W][CARRY ? 1 : YT][64];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
     if constexpr (!CARRY) In::put_map(sC, in.c, t0, k.len, N);
     __syncthreads();
     fetch(t0 + TT);
-    constexpr int PF = 2;  // positions read ahead
+    constexpr int PF = AHEAD ? 2 : 1;  // positions read together
     Step<T> at[PF], next[PF];
     auto read = [&](Step<T>(&x)[PF], int r) {
 #pragma unroll
@@ -290,12 +300,15 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
         }
       }
     };
-    read(at, 0);
+    if (AHEAD) read(at, 0);
 #pragma unroll
     for (int s = 0; s < TT / YT; ++s) {
 #pragma unroll
       for (int q = 0; q < YT; q += PF) {
-        if (s * YT + q + PF < TT) read(next, s * YT + q + PF);
+        if (!AHEAD)
+          read(at, s * YT + q);
+        else if (s * YT + q + PF < TT)
+          read(next, s * YT + q + PF);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < PF; ++i) at[i] = next[i];
+        for (int i = 0; i < (AHEAD ? PF : 0); ++i) at[i] = next[i];
       }
       __syncthreads();
       if constexpr (!CARRY) {
@@ -459,9 +472,10 @@ __device__ __forceinline__ T sum8(const T (&v)[8], bool upper8) {
 // CARRY: only dh over the segment, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(), HT = held_len<T>(W), KT = keep_len<T>(W);
+  constexpr int NS = kStates, TT = tile_len<T>(W, true), HT = held_len<T>(W), KT = keep_len<T>(W);
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP, RB = HT < 8 ? HT : 8;
+  constexpr bool AHEAD = reads_ahead<T>(W, CARRY);
   __shared__ T sd[TT][64], sx[CARRY ? 1 : TT][64], sy[TT][64], yp[CARRY ? 1 : 3][CARRY ? 1 : W][CARRY ? 1 : HT][64];
   __shared__ __attribute__((aligned(16))) T sB[CARRY ? 1 : TT * NP], sC[TT * NP];
   __shared__ T sg[CARRY ? 1 : TT][CARRY ? 1 : 2 * NP];
@@ -556,7 +570,7 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
     if constexpr (CARRY) {
       __syncthreads();
       fetch(t0 - TT);
-      constexpr int PF = 2;  // positions read ahead
+      constexpr int PF = AHEAD ? 2 : 1;  // positions read together
       Step<T> at[PF], next[PF];
       auto read = [&](Step<T>(&x)[PF], int r) {
 #pragma unroll
@@ -567,10 +581,13 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
           for (int j = 0; j < NS; ++j) x[i].c[j] = sC[(r + i) * NP + n0 + j];
         }
       };
-      read(at, TT - PF);
+      if (AHEAD) read(at, TT - PF);
 #pragma unroll
       for (int r = TT - PF; r >= 0; r -= PF) {
-        if (r > 0) read(next, r - PF);
+        if (!AHEAD)
+          read(at, r);
+        else if (r > 0)
+          read(next, r - PF);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = PF - 1; i >= 0; --i) {
@@ -580,7 +597,7 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < PF; ++i) at[i] = next[i];
+        for (int i = 0; i < (AHEAD ? PF : 0); ++i) at[i] = next[i];
       }
     } else {
       In::put_map(sB, in.b, t0, k.len, N);
@@ -626,10 +643,15 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
           }
           return x;
         };
-        Step<T> at = read(s * HT, false);
+        Step<T> at;
+        if (AHEAD) at = read(s * HT, false);
 #pragma unroll
         for (int q = 0; q < HT; ++q) {
-          const Step<T> next = q + 1 < HT ? read(s * HT + q + 1, false) : read(s * HT + q, true);
+          Step<T> next;
+          if (AHEAD)
+            next = q + 1 < HT ? read(s * HT + q + 1, false) : read(s * HT + q, true);
+          else
+            at = read(s * HT + q, false);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int j = 0; j < NS; ++j) {
@@ -637,12 +659,16 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
             h[q + 1][j] = fma(dec[q][j], h[q][j], at.x * at.b[j]);
           }
           __builtin_amdgcn_sched_barrier(0);
-          at = next;
+          if (AHEAD) at = next;
         }
 #pragma unroll
         for (int q = HT - 1; q >= 0; --q) {
           const int r = s * HT + q;
-          const Step<T> next = q > 0 ? read(r - 1, true) : at;
+          Step<T> next;
+          if (AHEAD)
+            next = q > 0 ? read(r - 1, true) : at;
+          else
+            at = read(r, true);
           __builtin_amdgcn_sched_barrier(0);
           T dx = T(0), e = T(0), y = T(0), v[8];
 #pragma unroll
@@ -657,7 +683,7 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
             e = fma(A2[j], p, e);
             dA[j] = fma(at.d, p, dA[j]);
           }
-          at = next;
+          if (AHEAD) at = next;
           yp[0][w][q][lane] = y;
           yp[1][w][q][lane] = dx;
           yp[2][w][q][lane] = e;
@@ -904,7 +930,7 @@ static int scan_chain(ScanArgs& a, int W, bool backward) {
 template <typename T>
 static int scan_fwd(ScanArgs& a) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(), W);
+  scan_segments(a, tile_len<T>(W, false), W);
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256,
              "dtmi_scan_fwd: too many elements");
   void* ws = nullptr;
@@ -930,7 +956,7 @@ template <typename T>
 static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* dC, BT sdC, int64_t gdC, void* dD,
                     void* dbias) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(), W);
+  scan_segments(a, tile_len<T>(W, true), W);
   const int64_t maps = a.B * a.T * a.G * a.N;
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256 &&
                  maps <= (int64_t)0x7fffffff * 256,

@@ -177,6 +177,7 @@ SCAN = [  # B, T, C, N, G, lengths, fused, has (D, z, bias, state, softplus)
     (2, 300, 70, 48, 2, [300, 129], True, (1, 1, 1, 1, 1)),
     (1, 230, 200, 8, 1, None, False, (1, 1, 1, 0, 1)),
     (300, 20, 64, 2, 1, None, False, (1, 1, 1, 1, 1)),    # enough blocks for one segment
+    (257, 19, 8, 40, 1, None, False, (1, 1, 1, 1, 1)),    # of sixteen waves
 ]
 
 
