@@ -117,6 +117,18 @@ __device__ __forceinline__ int64_t stat_at(const XArgs& a, int64_t b, int64_t kh
   return (b * a.H + kh * a.G) * a.Tq + r;
 }
 
+// The d that tile column m of 16 stands for in the N products along D: chunks of
+// products as wide as a vector allows (5: 4 + 1), each 16 vectors of the row in
+// order, so that the lanes' reads are contiguous (6 as 4 + 2: forward and backward
+// of 8 x 12 heads x 1024 x 512 x 96 672 us, as 6 elements a lane 738).
+template <typename T, int N>
+struct Cols {
+  static constexpr int V = XM<T>::VEC, FULL = N / V * V, TWO = FULL + ((N - FULL) & 2);
+  static __device__ constexpr int width(int t) { return t < FULL ? V : t < TWO ? 2 : 1; }
+  static __device__ constexpr int first(int t) { return t < FULL ? t / V * V : t < TWO ? FULL : TWO; }  // product of t's chunk
+  static __device__ __forceinline__ int d(int t, int m) { return 16 * first(t) + width(t) * m + (t - first(t)); }
+};
+
 // A lane's slice of one row as MFMA operand: element e of vector f is
 // d = 4 VEC f + VEC g + e, so the lane groups' reads of a row are contiguous.
 template <typename T, int DP>
@@ -145,15 +157,15 @@ __device__ __forceinline__ void load_slice(typename XM<T>::vec_t (&f)[DP / (4 * 
 template <typename T, int NR, int DP, bool VEC>
 struct Rows {
   typedef typename XM<T>::vec_t VT;
-  static constexpr int V = XM<T>::VEC, LD = DP + XM<T>::PAD, NV = NR * DP / V / 256;
-  static_assert(NR * DP % (V * 256) == 0, "whole vectors per thread");
+  static constexpr int V = XM<T>::VEC, LD = DP + XM<T>::PAD, ALL = NR * DP / V, NV = (ALL + 255) / 256;
   VT x[NV];
   uint32_t off[NV];  // bytes from the tile's first row; past every buffer's end in columns from D on
   static __device__ __forceinline__ int row(int i) { return (threadIdx.x + 256 * i) / (DP / V); }
   static __device__ __forceinline__ int col(int i) { return (threadIdx.x + 256 * i) % (DP / V) * V; }
+  static __device__ __forceinline__ bool mine(int i) { return ALL % 256 == 0 || threadIdx.x + 256 * i < ALL; }
   __device__ __forceinline__ void start(int64_t st, int D) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) off[i] = col(i) < D ? (uint32_t)((row(i) * st + col(i)) * sizeof(T)) : 0x80000000u;
+    for (int i = 0; i < NV; ++i) off[i] = mine(i) && col(i) < D ? (uint32_t)((row(i) * st + col(i)) * sizeof(T)) : 0x80000000u;
   }
   // `n` rows from p on, `st` elements apart (start()): the buffer ends with the
   // last of them, so the address work of a tile is scalar
@@ -173,7 +185,7 @@ struct Rows {
   __device__ __forceinline__ void gather(const F& base, int D) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const T* p = base(row(i));
+      const T* p = mine(i) ? base(row(i)) : nullptr;
       const int d = col(i);
       VT v = VT(0);
       if (VEC) {
@@ -188,12 +200,37 @@ struct Rows {
   }
   __device__ __forceinline__ void put(T* __restrict__ lds) const {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) *reinterpret_cast<VT*>(lds + row(i) * LD + col(i)) = x[i];
+    for (int i = 0; i < NV; ++i)
+      if (mine(i)) *reinterpret_cast<VT*>(lds + row(i) * LD + col(i)) = x[i];
   }
 };
 
-// A lane's slice of row r0 + c of an LDS tile, and its N columns N c .. of the
-// rows row(i, g): the two ways a tile's rows enter a product.
+// A row's elements Cols::d(t, c), as vectors; f (of a vector's first d): whether it is there
+template <typename T, int N, typename F>
+__device__ __forceinline__ void row_cols(T (&x)[N], const T* __restrict__ row, int c, const F& f) {
+  using L = Cols<T, N>;
+#pragma unroll
+  for (int t = 0; t < N; ++t) {
+    if (t != L::first(t)) continue;
+    const int d = L::d(t, c);
+    if (L::width(t) == XM<T>::VEC) {
+      typename XM<T>::vec_t y = typename XM<T>::vec_t(0);
+      if (f(d)) y = *reinterpret_cast<const typename XM<T>::vec_t*>(row + d);
+#pragma unroll
+      for (int e = 0; e < XM<T>::VEC; ++e) x[t + e] = y[e];
+    } else if (L::width(t) == 2) {
+      typedef T v2 __attribute__((ext_vector_type(2)));
+      v2 y = v2(0);
+      if (f(d)) y = *reinterpret_cast<const v2*>(row + d);
+      x[t] = y[0];
+      if (t + 1 < N) x[t + 1] = y[1];
+    } else {
+      x[t] = f(d) ? row[d] : T(0);
+    }
+  }
+}
+// A lane's slice of row r0 + c of an LDS tile, and its columns Cols::d(t, c) of
+// the rows row(i, g): the two ways a tile's rows enter a product.
 template <typename T, int DP>
 __device__ __forceinline__ void lds_slice(typename XM<T>::vec_t (&x)[DP / (4 * XM<T>::VEC)], const T* __restrict__ lds, int r0,
                                           int g, int c) {
@@ -204,23 +241,9 @@ __device__ __forceinline__ void lds_slice(typename XM<T>::vec_t (&x)[DP / (4 * X
 }
 template <typename T, int DP>
 __device__ __forceinline__ void lds_cols(T (&x)[4][DP / 16], const T* __restrict__ lds, int r0, int g, int c) {
-  constexpr int N = DP / 16, LD = DP + XM<T>::PAD, VW = N % XM<T>::VEC == 0 ? XM<T>::VEC : N % 2 == 0 ? 2 : 1;
-  typedef T vt __attribute__((ext_vector_type(VW == 1 ? 2 : VW)));
+  constexpr int N = DP / 16, LD = DP + XM<T>::PAD;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const T* row = lds + (r0 + XM<T>::row(i, g)) * LD + N * c;
-    if constexpr (VW > 1) {
-#pragma unroll
-      for (int v = 0; v < N / VW; ++v) {
-        const vt y = *reinterpret_cast<const vt*>(row + VW * v);
-#pragma unroll
-        for (int e = 0; e < VW; ++e) x[i][VW * v + e] = y[e];
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < N; ++t) x[i][t] = row[t];
-    }
-  }
+  for (int i = 0; i < 4; ++i) row_cols<T, N>(x[i], lds + (r0 + XM<T>::row(i, g)) * LD, c, [](int) { return true; });
 }
 // Two 16 x 16 tiles of products of slices, their chains of dependent MFMAs interleaved
 template <typename T, int NF>
@@ -236,7 +259,7 @@ __device__ __forceinline__ void mul_slices(typename XM<T>::acc_t& p, const typen
       q = XM<T>::mma(xq[i][e], fq[i][e], q);
     }
 }
-// out^T (d = N m + t by column) += sum over a tile's 16 rows of x(row, d) p(row, column)
+// out^T (d by column) += sum over a tile's 16 rows of x(row, d) p(row, column)
 template <typename T, int N>
 __device__ __forceinline__ void mul_cols(typename XM<T>::acc_t (&out)[N], const T (&x)[4][N],
                                          const typename XM<T>::acc_t& p) {
@@ -252,31 +275,28 @@ __device__ __forceinline__ void phase() {
   if constexpr (sizeof(T) == 8) __builtin_amdgcn_sched_barrier(0);
 }
 
-// The lane's part of a result row: registers (t, i) are d = N row(i, g) + t
+// The lane's part of a result row: registers (t, i) are Cols::d(t, row(i, g))
 template <typename T, int DP>
 __device__ __forceinline__ void put_row(T* __restrict__ row, const typename XM<T>::acc_t (&x)[DP / 16], T mul, int D,
                                         int g, bool vec) {
-  constexpr int N = DP / 16, VEC = XM<T>::VEC;
+  constexpr int N = DP / 16;
+  using L = Cols<T, N>;
   typedef typename XM<T>::vec_t VT;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = N * XM<T>::row(i, g);
-    if constexpr (N % VEC == 0) {
-      if (vec) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int v = 0; v < N / VEC; ++v) {
-          VT y;
+    for (int t = 0; t < N; ++t) {
+      const int d = L::d(t, XM<T>::row(i, g));
+      if (vec && L::width(t) == XM<T>::VEC) {
+        if (t % XM<T>::VEC != 0) continue;
+        VT y;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) y[e] = x[VEC * v + e][i] * mul;
-          if (d + VEC * v < D) *reinterpret_cast<VT*>(row + d + VEC * v) = y;
-        }
-        continue;
+        for (int e = 0; e < XM<T>::VEC; ++e) y[e] = x[t + e][i] * mul;
+        if (d < D) *reinterpret_cast<VT*>(row + d) = y;
+      } else if (d < D) {
+        row[d] = x[t][i] * mul;
       }
     }
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-      if (d + t < D) row[d + t] = x[t][i] * mul;
-  }
 }
 
 template <typename T>
@@ -339,7 +359,7 @@ __device__ __forceinline__ XBlock x_block(const XArgs& a) {
 // us so, and 582 bounded.)
 template <typename T>
 constexpr int x_waves(int DP, bool kv = false) {
-  return sizeof(T) == 8 && DP >= (kv ? 64 : 96) ? 1 : 2;
+  return sizeof(T) == 8 && DP >= (kv ? 64 : 80) ? 1 : 2;
 }
 
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
@@ -463,8 +483,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
   using M = XM<T>;
   typedef typename M::acc_t AT;
   typedef typename M::vec_t VT;
-  constexpr int N = DP / 16, NF = DP / (4 * M::VEC), VW = N % M::VEC == 0 ? M::VEC : 2;
-  typedef T vw __attribute__((ext_vector_type(VW)));
+  constexpr int N = DP / 16, NF = DP / (4 * M::VEC);
   __shared__ T so[4][16][DP + 1], sm[4][16], sl[4][16];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D, R = (int)a.R;
   const XBlock k = x_block(a);
@@ -481,19 +500,15 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = j + M::row(i, g);
-      const T* row = Vb + (int64_t)(r < hi ? r : 0) * a.sv.t + N * c;
+      const T* row = Vb + (int64_t)(r < hi ? r : 0) * a.sv.t;
+      if (VEC) {
+        row_cols<T, N>(v[i], row, c, [&](int d) { return r < hi && d < D; });
+      } else {
 #pragma unroll
-      for (int u = 0; u < N / VW; ++u) {
-        vw y = vw(0);
-        if (VEC) {
-          if (r < hi && N * c + VW * u < D) y = *reinterpret_cast<const vw*>(row + VW * u);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VW; ++e)
-            if (r < hi && N * c + VW * u + e < D) y[e] = row[VW * u + e];
+        for (int t = 0; t < N; ++t) {
+          const int d = Cols<T, N>::d(t, c);
+          v[i][t] = r < hi && d < D ? row[d] : T(0);
         }
-#pragma unroll
-        for (int e = 0; e < VW; ++e) v[i][VW * u + e] = y[e];
       }
     }
   };
@@ -540,7 +555,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int t = 0; t < N; ++t) so[w][c][N * M::row(i, g) + t] = o[t][i];
+    for (int t = 0; t < N; ++t) so[w][c][Cols<T, N>::d(t, M::row(i, g))] = o[t][i];
   if (g == 0) {
     sm[w][c] = mref;
     sl[w][c] = sum;
@@ -1017,8 +1032,8 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
 // `per_cu` blocks per CU, of at least two steps each, at most 64. With lengths
 // (`ragged`) the longest sequence may take up to four times its share of the parts.
 // per_cu 3 (2 for up to 16 rows) was taken from sweeps of 1, 2, 3, 5: backward of
-// 4 x 8 / 2 heads x 333 x 777 x 72, padded, 155 / 115 / 100 / 107 us, of 2 x 12 x
-// 300 x 257 x 64 51 / 48 / 47 / 47; one query of 8 x 16 / 4 heads x 4999 x 128
+// 4 x 8 / 2 heads x 333 x 777 x 72, padded, 155 / 115 / 100 / 107 us (in 96 columns,
+// as 65 to 96 then were), of 2 x 12 x 300 x 257 x 64 51 / 48 / 47 / 47; one query of 8 x 16 / 4 heads x 4999 x 128
 // 39 / 34 / 44 / 41.
 static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int step, bool ragged) {
   const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = per_cu * (int64_t)num_cus();
@@ -1134,10 +1149,15 @@ static int x_bwd(XArgs& a) {
   return rc;
 }
 
+// Columns that a head is padded to. 48 and 80 beside the multiples of 32: forward /
+// backward of 8 x 12 heads x 1024 x 512 x 40 124 / 304 us in 64 columns, 105 / 253
+// in 48; x 72 188 / 510 in 96, 154 / 440 in 80.
 template <typename T>
 static int x_dispatch(XArgs& a, bool bwd) {
   if (a.D <= 32) return bwd ? x_bwd<T, 32>(a) : x_fwd<T, 32>(a);
+  if (a.D <= 48) return bwd ? x_bwd<T, 48>(a) : x_fwd<T, 48>(a);
   if (a.D <= 64) return bwd ? x_bwd<T, 64>(a) : x_fwd<T, 64>(a);
+  if (a.D <= 80) return bwd ? x_bwd<T, 80>(a) : x_fwd<T, 80>(a);
   if (a.D <= 96) return bwd ? x_bwd<T, 96>(a) : x_fwd<T, 96>(a);
   return bwd ? x_bwd<T, 128>(a) : x_fwd<T, 128>(a);
 }

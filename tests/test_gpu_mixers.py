@@ -300,6 +300,13 @@ CROSS = [  # B, H, Hk, Tq, Tk, D, lengths, strided
     (2, 4, 1, 1, 900, 128, [900, 130], True),   # up to 16 rows per key/value head
     (1, 6, 2, 5, 210, 100, None, False),
     (4, 16, 1, 1, 70, 96, [1, 0, 70, 16], False),
+    (2, 4, 2, 3, 150, 80, [150, 20], True),     # widths between the powers of two
+    (1, 4, 1, 60, 90, 80, None, True),
+    (2, 2, 2, 40, 70, 44, None, False),
+    (1, 4, 2, 5, 70, 76, None, False),
+    (1, 2, 2, 30, 60, 77, None, False),
+    (1, 2, 1, 8, 130, 37, [120], True),
+    (1, 3, 3, 45, 40, 120, None, True),
     (9, 1, 1, 90, 1100, 40, [0, 1, 1100, 64, 65, 600, 1099, 33, 2], False),  # parts by the lengths' sum
 ]
 
@@ -335,7 +342,8 @@ def test_cross_attention(dev, dt, case):
 
 @pytest.mark.parametrize("dt", [F32, F64])
 @pytest.mark.parametrize("case", [(2, 3, 3, 70, 65, 64, [65, 64]), (1, 4, 2, 90, 700, 96, None), (2, 2, 1, 40, 33, 128, [7, 33]),
-                                  (2, 3, 1, 50, 47, 20, [3, 47])],
+                                  (2, 3, 1, 50, 47, 20, [3, 47]), (1, 2, 1, 40, 50, 72, None),
+                                  (1, 2, 2, 33, 40, 45, [31])],
                          ids=lambda c: "-".join(str(v) for v in c[:6]))
 def test_cross_attention_backward_without_kept_ds(dev, dt, case):
     """dS formed twice where its workspace is refused: the same dK and dV bits,
