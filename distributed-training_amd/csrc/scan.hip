@@ -60,13 +60,10 @@ __host__ __device__ constexpr int bwd_waves(int W) {
   return W == 16 ? 4 : W == 8 ? 2 : sizeof(T) == 4 && W > 1 ? 2 : 1;
 }
 // Positions per state kept for the backward, which rebuilds the states in
-// between. float32 keeps one per part (16 states: two activations' memory,
-// 5 us more traffic against 10 us of exponentials at 4 x 1024 x 1536 x 16);
-// from 33 states on, and in float64, memory counts for more: one per tile.
-template <typename T>
-__host__ __device__ constexpr int keep_len(int W) {
-  return sizeof(T) == 4 && W <= 8 ? held_len<T>(W) : tile_len<T>(W, true);
-}
+// between (16 states: two activations' memory). One per float32 part: at one per
+// 16 positions 5 us less traffic and 10 us more of exponentials at 4 x 1024 x 1536 x
+// 16. One per tile of eight where a part is shorter: there memory counts for more.
+constexpr int kKeep = 8;
 static int waves_for(int64_t N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 // Element strides of the batch axis and of positions (below 2^31, checked on the host).
@@ -225,7 +222,7 @@ constexpr bool reads_ahead(int W, bool small) {
 // CARRY: only the segment's end state from a zero start, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(W, false), YT = sum_len<T>(W), KT = keep_len<T>(W);
+  constexpr int NS = kStates, TT = tile_len<T>(W, false), YT = sum_len<T>(W), KT = kKeep;
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP;
   constexpr bool AHEAD = reads_ahead<T>(W, true);
@@ -472,7 +469,7 @@ __device__ __forceinline__ T sum8(const T (&v)[8], bool upper8) {
 // CARRY: only dh over the segment, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanArgs a) {
-  constexpr int NS = kStates, TT = tile_len<T>(W, true), HT = held_len<T>(W), KT = keep_len<T>(W);
+  constexpr int NS = kStates, TT = tile_len<T>(W, true), HT = held_len<T>(W), KT = kKeep;
   using In = Tile<T, W, TT>;
   constexpr int RPW = In::RPW, NP = In::NP, RB = HT < 8 ? HT : 8;
   constexpr bool AHEAD = reads_ahead<T>(W, CARRY);
@@ -885,11 +882,6 @@ static void scan_launch(const ScanArgs& a, int W) {
 #undef SCAN_W
 }
 
-static int scan_keep(int dtype, int64_t N) {
-  const int W = waves_for(N);
-  return dtype == DTMI_F32 ? keep_len<float>(W) : keep_len<double>(W);
-}
-
 // Segments of T: one where B * C / 64 blocks already occupy the card. A split
 // costs the exponentials a second time, so it pays while less than a block per
 // CU would run (float32, 1536 channels x 16 states x 1024 positions, forward
@@ -1009,7 +1001,7 @@ DTMI_EXPORT int dtmi_scan_kept(int dtype, int64_t B, int64_t T, int64_t C, int64
   DTMI_BODY_BEGIN
   if (int rc = scan_shape("dtmi_scan_kept", dtype, B, T, C, N, 1)) return rc;
   DTMI_CHECK(count, "dtmi_scan_kept: NULL result");
-  *count = B * cdiv(T, scan_keep(dtype, N)) * N * C;
+  *count = B * cdiv(T, kKeep) * N * C;
   return DTMI_OK;
   DTMI_BODY_END
 }

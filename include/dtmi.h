@@ -448,7 +448,7 @@ int dtmi_conv_step(int dtype, int64_t B, int64_t C, int64_t K, const void* x, in
  *   out = y silu(z), or y without z
  * A [C, N]; D, dt_bias [C], z [B, T, C], state [B, C, N] may be NULL (0; no gate);
  * state_out [B, C, N] or NULL. `kept`, for the backward: dtmi_scan_kept() elements
- * that the forward fills with the states before each tile of positions (NULL: not
+ * that the forward fills with the states before every eighth position (NULL: not
  * kept). The backward writes every gradient it is given room for; dD, ddt_bias and
  * dstate may be NULL. The step takes one position per sequence (u, dt, z, out
  * [B, C], b strides; maps [B, G, N], (b, g) strides) and updates the state in place. */
