@@ -324,15 +324,19 @@ struct XBlock {
 // Keys per part of a loop over keys: the host's, or with lengths such that all
 // sequences' parts together number a.parts per key/value head, so that a long
 // sequence gets more blocks and not longer ones (every wave sums the lengths).
+// In 32 bits (the host checks that the lengths' sum fits) and known to be one value:
+// as lanes' 64-bit numbers they kept the loop's bounds in vector registers and cost
+// the forward of 4 x 8 / 2 heads x 333 x 1501 x 72, padded, 4 us of 57.
 __device__ __forceinline__ int keys_per_part(const XArgs& a) {
   if (!a.lengths || a.nsplit == 1) return a.per;
-  int64_t total = 0;
-  for (int64_t b = threadIdx.x & 63; b < a.B; b += 64) total += key_count(a, b);
+  uint32_t total = 0;
+  for (int b = threadIdx.x & 63; b < (int)a.B; b += 64) total += (uint32_t)key_count(a, b);
 #pragma unroll
-  for (int x = 1; x < 64; x <<= 1) total += __shfl_xor((long long)total, x, 64);
-  const int64_t fair = (total + a.parts - 1) / a.parts;
-  const int64_t least = (a.Tk + a.nsplit - 1) / a.nsplit, per = fair > least ? fair : least;
-  return (int)((per + a.step - 1) / a.step) * a.step;
+  for (int x = 1; x < 64; x <<= 1) total += __shfl_xor(total, x, 64);
+  total = (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+  const uint32_t parts = (uint32_t)a.parts, split = (uint32_t)a.nsplit, step = (uint32_t)a.step;
+  const uint32_t fair = (total + parts - 1) / parts, least = ((uint32_t)a.Tk + split - 1) / split;
+  return (int)(((fair > least ? fair : least) + step - 1) / step * step);
 }
 __device__ __forceinline__ XBlock x_block(const XArgs& a) {
   // blocks are dealt to the eight XCDs in turn: XCD x takes the x-th eighth of
@@ -366,7 +370,7 @@ constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 
 // The forward for more than 16 rows: a wave owns 16 of them. Bound by the MFMAs:
 // two products, 4 D per score. float32, 32 x 12 heads x 1024 x 2048 x 64: 130
-// TFLOP/s (a large library product: 154); 8 x 12 x 1024 x 512: 125 us, 103, one
+// TFLOP/s (a large library product: 154); 8 x 12 x 1024 x 512: 120 us, 107, one
 // and a half rounds of blocks. Five or six waves per SIMD spill, a second LDS
 // buffer and 32 rows per wave gave nothing.
 template <typename T, int DP, bool VEC>
@@ -818,6 +822,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15, D = (int)a.D;
   const XBlock k = x_block(a);
   const int len = (int)key_count(a, k.b), R = (int)a.R;
+  // a block past the sequence's keys has only zeros to write
+  const bool any = k.tile * 64 < len;
   int lo, hi;
   k.part(a.per, R, lo, hi);
   const int j0 = (k.tile * 4 + w) * 16, j = j0 + c;
@@ -858,8 +864,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel
 #pragma unroll
   for (int t = 0; t < N; ++t) dk[t] = dv[t] = AT(0);
   const T* dsp = (const T*)a.ds + ((k.b * a.Hk + k.kh) * a.rt * a.kt + (j0 >> 4)) * 256;
-  // a block past the sequence's keys has only zeros to write
-  const bool any = k.tile * 64 < len, busy = j0 < len;
+  const bool busy = j0 < len;
   if (any && lo < hi) {
     fetch(lo);
     put();
@@ -1029,16 +1034,16 @@ __global__ void __launch_bounds__(256) xattn_sum_kernel(XArgs a) {
 
 // Blocks along the owned axis, `per_block` of it each, and the parts of the loop
 // over `loop` positions: more than one where the card would have fewer than
-// `per_cu` blocks per CU, of at least two steps each, at most 64. With lengths
-// (`ragged`) the longest sequence may take up to four times its share of the parts.
+// `per_cu` blocks per CU, of at least two steps each, at most 64; with lengths up to
+// `ragged` times as many, of which a block finds by the lengths how many are used.
 // per_cu 3 (2 for up to 16 rows) was taken from sweeps of 1, 2, 3, 5: backward of
 // 4 x 8 / 2 heads x 333 x 777 x 72, padded, 155 / 115 / 100 / 107 us (in 96 columns,
 // as 65 to 96 then were), of 2 x 12 x 300 x 257 x 64 51 / 48 / 47 / 47; one query of 8 x 16 / 4 heads x 4999 x 128
 // 39 / 34 / 44 / 41.
-static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int step, bool ragged) {
+static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu, int step, int ragged) {
   const int64_t tiles = cdiv(owned, per_block), blocks = a.B * a.Hk * tiles, want = per_cu * (int64_t)num_cus();
   int64_t s = blocks >= want ? 1 : cdiv(want, blocks);
-  if (ragged && s > 1) s *= 4;
+  if (a.lengths && s > 1) s *= ragged;
   if (s > loop / (2 * step)) s = loop / (2 * step);
   s = s < 1 ? 1 : s > 64 ? 64 : s;
   a.step = step;
@@ -1062,7 +1067,7 @@ static int plan(XArgs& a, int64_t owned, int per_block, int64_t loop, int per_cu
 template <typename T, int DP>
 static int x_fwd(XArgs& a) {
   const bool few = a.R <= 16;
-  if (int rc = few ? plan(a, a.R, 16, a.Tk, 2, 64, a.lengths) : plan(a, a.R, 64, a.Tk, 3, kKeys, a.lengths)) return rc;
+  if (int rc = few ? plan(a, a.R, 16, a.Tk, 2, 64, 4) : plan(a, a.R, 64, a.Tk, 3, kKeys, 4)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.R;
@@ -1089,7 +1094,7 @@ static int x_fwd(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_kv(XArgs& a) {
-  if (int rc = plan(a, a.Tk, 64, a.R, 3, kKeys, false)) return rc;
+  if (int rc = plan(a, a.Tk, 64, a.R, 3, kKeys, 1)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     const size_t n = (size_t)a.B * a.Hk * a.nsplit * a.Tk * DP;
@@ -1108,7 +1113,7 @@ static int x_bwd_kv(XArgs& a) {
 
 template <typename T, int DP>
 static int x_bwd_q(XArgs& a) {
-  if (int rc = plan(a, a.R, 64, a.Tk, 3, kKeys, a.lengths)) return rc;
+  if (int rc = plan(a, a.R, 64, a.Tk, 3, kKeys, 4)) return rc;
   void* ws = nullptr;
   if (a.nsplit > 1) {
     if (int rc = pool_alloc(&ws, (size_t)a.B * a.Hk * a.nsplit * a.R * DP * sizeof(T))) return rc;
