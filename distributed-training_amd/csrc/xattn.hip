@@ -371,8 +371,8 @@ constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 // The forward for more than 16 rows: a wave owns 16 of them. Bound by the MFMAs:
 // two products, 4 D per score. float32, 32 x 12 heads x 1024 x 2048 x 64: 130
 // TFLOP/s (a large library product: 154); 8 x 12 x 1024 x 512: 120 us, 107, all
-// blocks at once. Five or six waves per SIMD spill, a second LDS
-// buffer and 32 rows per wave gave nothing.
+// blocks at once. Five or six waves per SIMD spill; a second LDS buffer and 32 rows
+// per wave gave nothing.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a) {
   using M = XM<T>;
