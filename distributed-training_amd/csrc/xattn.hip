@@ -22,7 +22,9 @@
 // probabilities from the forward's reference and sum (the same products in the
 // same order, so the same scores), dV += P^T dO, dP = dO V^T, dS = P (dP -
 // rowsum(dO O)), dK += dS^T Q in the pass over keys; S, dP and dQ = dS K in
-// the pass over queries.
+// the pass over queries. A memory of one key has P = 1 whatever the score, so dS,
+// dQ and dK are 0: dP and rowsum(dO O), the same sum in two orders, would leave
+// their rounding.
 //
 // Few rows or few keys give few blocks: the loop (over keys in the forward and
 // the dQ pass, over rows in the dK/dV pass) is then split over blocks, whose
@@ -733,6 +735,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
   const int len = (int)key_count(a, k.b);
   int lo, hi;
   if (!k.part(keys_per_part(a), len, lo, hi)) return;
+  if (len == 1) hi = lo;  // dS is 0
   const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
   const bool in = r < R;
   const T* Qb = group_of<const T>(a, a.q, a.sq, k.b, k.kh);
@@ -925,6 +928,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel
     __syncthreads();
   }
   if (j >= a.Tk) return;
+  if (len == 1)  // dS is 0
+#pragma unroll
+    for (int t = 0; t < N; ++t) dk[t] = AT(0);
   if (a.nsplit > 1) {
     const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.Tk + j;
     put_row<T, DP>((T*)a.po + at * DP, dk, (T)a.scale, DP, g, true);
@@ -948,6 +954,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs
   const int len = (int)key_count(a, k.b);
   int lo, hi;
   if (!k.part(keys_per_part(a), len, lo, hi)) return;
+  if (len == 1) hi = lo;  // dS is 0
   const int r0 = (k.tile * 4 + w) * 16, R = (int)a.R, r = r0 + c;
   const bool busy = r0 < R;
   // lane (g, c): keys row(i, g) of row c, which stands where its writer's registers put it

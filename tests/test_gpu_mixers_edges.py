@@ -1,0 +1,65 @@
+"""Sequence mixers on the GPU at the edges of their ranges, against their
+definitions in float64: memories of one key, scores and decays that leave the
+types' range on the way to a finite value, operands without elements, states
+moved on between the passes. Bars count roundings of half a step u as in
+test_gpu_mixers; a bar that differs has its own count beside it."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import bits_equal
+from test_gpu_mixers import F32, F64, U, _mods, bthd, close, conv_ref, cross_ref, scan_ref, t64
+
+pytestmark = pytest.mark.gpu
+
+
+def cross_grads(q, k, v, g, lengths=None, scale=None, strided=False, kept=True):
+    """o, dq, dk, dv of cross_attention, dS kept for the dQ pass or formed twice."""
+    from dtmi import kernels as K
+    A, _ = _mods()
+    L = [A.Tensor(bthd(x, strided), requires_grad=True) for x in (q, k, v)]
+    before = K.attn_set_ds_limit(0 if not kept else 1 << 32)
+    try:
+        o = A.cross_attention(*L, lengths=lengths, scale=scale)
+        o.backward(bthd(g, strided))
+    finally:
+        K.attn_set_ds_limit(before)
+    return [o.numpy()] + [x.grad.numpy() for x in L]
+
+
+ONE_KEY = [  # B, H, Hk, Tq, Tk, D, lengths
+    (1, 1, 1, 1, 1, 64, None),
+    (2, 4, 2, 9, 1, 32, None),
+    (2, 3, 3, 70, 1, 72, None),
+    (1, 2, 1, 40, 1, 128, None),
+    (3, 2, 2, 33, 40, 64, [1, 1, 1]),
+    (2, 4, 1, 5, 300, 96, [1, 1]),
+    (4, 2, 1, 50, 700, 40, [1, 700, 0, 1]),
+]
+
+
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("case", ONE_KEY, ids=lambda c: "-".join(str(v) for v in c[:6]))
+def test_cross_attention_of_one_key(dev, dt, case, kept):
+    """With one key the probability is 1 whatever the score: o is its value, and
+    dQ and dK are 0, not what rounding leaves of a difference. Each sequence is
+    judged by itself."""
+    B, H, Hk, Tq, Tk, Dh, lengths = case
+    rng = np.random.default_rng(Tq + Tk + Dh)
+    q, g = (rng.standard_normal((B, H, Tq, Dh)).astype(dt) for _ in range(2))
+    k, v = (rng.standard_normal((B, Hk, Tk, Dh)).astype(dt) for _ in range(2))
+    o, dq, dk, dv = cross_grads(q, k, v, g, lengths, kept=kept)
+    R = [t64(x) for x in (q, k, v)]
+    ro = cross_ref(*R, lengths, Dh ** -.5)
+    want = torch.autograd.grad(ro, R, t64(g, False))
+    for i in range(B):
+        n = Tk if lengths is None else lengths[i]
+        close(o[i], ro[i], dt, 4 if n == 1 else 512, f"o {i}")
+        if n > 1:
+            for got, w, name in zip((dq, dk, dv), want, ("dq", "dk", "dv")):
+                close(got[i], w[i], dt, 512, f"{name} {i}")
+            continue
+        assert not dq[i].any() and not dk[i].any(), i
+        # a sum over the group's rows, each term with its probability's roundings
+        close(dv[i], want[2][i], dt, H // Hk * Tq + 8, f"dv {i}")
