@@ -17,8 +17,10 @@
 // row(i, g).
 //
 // Forward: scores in base 2, a reference maximum per query that moves only
-// when a score exceeds it by 2^8, sum and output rescaled then; a score is
-// scaled and the reference subtracted in one rounding. Backward: the
+// when a score exceeds it by 2^8, sum and output rescaled then. A score is scaled
+// and rounded as the reference was before it is subtracted: in one rounding with
+// the difference, scores of 2^32 and more would leave the reference's own
+// rounding, hundreds, in the exponent. Backward: the
 // probabilities from the forward's reference and sum (the same products in the
 // same order, so the same scores), dV += P^T dO, dP = dO V^T, dS = P (dP -
 // rowsum(dO O)), dK += dS^T Q in the pass over keys; S, dP and dQ = dS K in
@@ -430,7 +432,9 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool in0 = more || j0 + M::row(i, g) < hi, in1 = more || j0 + 16 + M::row(i, g) < hi;
-        top = fmax(top, fmax(in0 ? p0[i] * sl2 : -INFINITY, in1 ? p1[i] * sl2 : -INFINITY));
+        p0[i] = in0 ? p0[i] * sl2 : -INFINITY;
+        p1[i] = in1 ? p1[i] * sl2 : -INFINITY;
+        top = fmax(top, fmax(p0[i], p1[i]));
       }
       if (__any(top > mref + T(8))) {
         const T next = fmax(mref, over_groups_max(top));
@@ -442,9 +446,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool in0 = more || j0 + M::row(i, g) < hi, in1 = more || j0 + 16 + M::row(i, g) < hi;
-        p0[i] = in0 ? M::ex2(fma(p0[i], sl2, -mref)) : T(0);
-        p1[i] = in1 ? M::ex2(fma(p1[i], sl2, -mref)) : T(0);
+        p0[i] = M::ex2(p0[i] - mref);
+        p1[i] = M::ex2(p1[i] - mref);
         l = l + (p0[i] + p1[i]);
       }
       mul_cols<T, N>(o, v0, p0);
@@ -535,7 +538,10 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
       for (int e = 0; e < M::VEC; ++e) s = M::mma(x[i][e], qf[i][e], s);
     T top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmax(top, j + M::row(i, g) < hi ? s[i] * sl2 : -INFINITY);
+    for (int i = 0; i < 4; ++i) {
+      s[i] = j + M::row(i, g) < hi ? s[i] * sl2 : -INFINITY;
+      top = fmax(top, s[i]);
+    }
     if (__any(top > mref + T(8))) {
       const T next = fmax(mref, over_groups_max(top));
       const T alpha = M::ex2(mref - next);
@@ -546,7 +552,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      s[i] = j + M::row(i, g) < hi ? M::ex2(fma(s[i], sl2, -mref)) : T(0);
+      s[i] = M::ex2(s[i] - mref);
       l = l + s[i];
     }
     mul_cols<T, N>(o, v, s);
@@ -785,7 +791,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool on = inv != T(0) && (more || j0 + 16 * kt + M::row(i, g) < hi);
-          const T d = M::ex2(fma(s[i], sl2, -m)) * inv * (dp[i] - dr);
+          const T d = M::ex2(s[i] * sl2 - m) * inv * (dp[i] - dr);
           ds[i] = on ? d : T(0);
         }
         mul_cols<T, N>(dq, kc, ds);
@@ -898,7 +904,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool on = in && inv[i] != T(0);
-          const T e = M::ex2(fma(s[i], sl2, -m[i])) * inv[i], d = e * (dp[i] - dr[i]);
+          const T e = M::ex2(s[i] * sl2 - m[i]) * inv[i], d = e * (dp[i] - dr[i]);
           p[i] = on ? e : T(0);
           ds[i] = on ? d : T(0);
         }

@@ -63,3 +63,31 @@ def test_cross_attention_of_one_key(dev, dt, case, kept):
         assert not dq[i].any() and not dk[i].any(), i
         # a sum over the group's rows, each term with its probability's roundings
         close(dv[i], want[2][i], dt, H // Hk * Tq + 8, f"dv {i}")
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("case", [(1, 1, 1, 3, 40, 8), (1, 2, 2, 40, 300, 16), (1, 2, 1, 130, 20, 64), (2, 2, 2, 1, 900, 32)],
+                         ids=lambda c: "-".join(str(v) for v in c))
+def test_cross_attention_of_scores_whose_rounding_is_large(dev, dt, case):
+    """Scores of 1e11 (float64: 1e25), finite: a step of them is far above 1, and
+    the largest takes all the weight. o is its value to the bit."""
+    B, H, Hk, Tq, Tk, Dh = case
+    rng = np.random.default_rng(Tk)
+    size = 1e5 if dt is F32 else 1e12
+    q, g = (rng.standard_normal((B, H, Tq, Dh)).astype(dt) for _ in range(2))
+    k, v = (rng.standard_normal((B, Hk, Tk, Dh)).astype(dt) for _ in range(2))
+    q, k = q * dt(size), k * dt(size)
+    s = np.repeat(k, H // Hk, 1).astype(F64) @ np.swapaxes(q, 2, 3).astype(F64)  # [B, H, Tk, Tq]
+    top = np.sort(s, 2)
+    # the winner is clear of every score's rounding (D of them, and one of the scaling)
+    assert (top[:, :, -1] - top[:, :, -2] > 4 * (Dh + 2) * U[dt] * np.abs(s).max()).all()
+    best = s.argmax(2)  # [B, H, Tq]
+    want = np.take_along_axis(np.repeat(v, H // Hk, 1), best[..., None], 2)
+    o, dq, dk, dv = cross_grads(q, k, v, g, scale=1.0)
+    assert bits_equal(o, want)
+    assert np.isfinite(dq).all() and np.isfinite(dk).all()
+    sums = np.zeros((B, H, Tk, Dh))
+    for b in range(B):
+        for h in range(H):
+            np.add.at(sums[b, h], best[b, h], g[b, h].astype(F64))
+    close(dv, sums.reshape(B, Hk, H // Hk, Tk, Dh).sum(2), dt, H // Hk * Tq + 8, "dv")
