@@ -303,6 +303,15 @@ __device__ __forceinline__ void put_row(T* __restrict__ row, const typename XM<T
     }
 }
 
+// The result and the gradient of a row without a finite score (weight 0) are 0,
+// whatever infinite keys or values made of its products
+template <typename T, int N>
+__device__ __forceinline__ void none_without(typename XM<T>::acc_t (&x)[N], T weight) {
+  if (weight == T(0))
+#pragma unroll
+    for (int t = 0; t < N; ++t) x[t] = typename XM<T>::acc_t(0);
+}
+
 template <typename T>
 __device__ __forceinline__ T over_groups_max(T x) {
   x = fmax(x, __shfl_xor(x, 16, 64));
@@ -473,6 +482,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
     }
     return;
   }
+  none_without<T, N>(o, sum);
   put_row<T, DP>(group_of<T>(a, a.out, a.so, k.b, k.kh) + row_at(a, a.so, r), o, sum == T(0) ? T(0) : T(1) / sum, D, g, VEC);
   if (g == 0 && a.rowmax) {
     const int64_t at = stat_at(a, k.b, k.kh, r);
@@ -701,7 +711,7 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
         if (s + u < n) y = fma(x[u], f, y);
       }
     }
-    if (lane + 64 * e < a.D) out[lane + 64 * e] = y * inv;
+    if (lane + 64 * e < a.D) out[lane + 64 * e] = sum == T(0) ? T(0) : y * inv;
   }
   if (lane == 0 && a.rowmax) {
     ((T*)a.rowmax)[stat_at(a, b, kh, r)] = top;
@@ -810,6 +820,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
     __syncthreads();
   }
   if (!in) return;
+  none_without<T, N>(dq, inv);
   if (a.nsplit > 1) {
     const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
     put_row<T, DP>((T*)a.po + at * DP, dq, (T)a.scale, DP, g, true);
@@ -881,6 +892,17 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel
   __syncthreads();
   for (int r0 = lo; any && r0 < hi; r0 += QT) {
     const bool more = r0 + QT < hi;
+    // A row without a finite score passes nothing on: its products with 0 would,
+    // where it is infinite. (Every wave finds the same. The index is taken as new so
+    // that nothing of this is kept in registers over the loop.)
+    if (__any(si[lane % QT] == T(0))) {
+      int f = threadIdx.x;
+      asm volatile("" : "+v"(f));
+#pragma unroll 1
+      for (; f < QT * DP; f += 256)
+        if (si[f / DP] == T(0)) Qs[f / DP * LD + f % DP] = Gs[f / DP * LD + f % DP] = T(0);
+      __syncthreads();
+    }
     if (more) fetch(r0 + QT);
     if (busy) {
       typename M::vec_t xq[NF], xg[NF];
@@ -1008,6 +1030,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs
     __syncthreads();
   }
   if (r >= R) return;
+  none_without<T, N>(dq, ((const T*)a.rowsum)[stat_at(a, k.b, k.kh, r)]);
   if (a.nsplit > 1) {
     const int64_t at = ((k.b * a.Hk + k.kh) * a.nsplit + k.split) * a.R + r;
     put_row<T, DP>((T*)a.po + at * DP, dq, (T)a.scale, DP, g, true);

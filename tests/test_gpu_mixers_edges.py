@@ -91,3 +91,36 @@ def test_cross_attention_of_scores_whose_rounding_is_large(dev, dt, case):
         for h in range(H):
             np.add.at(sums[b, h], best[b, h], g[b, h].astype(F64))
     close(dv, sums.reshape(B, Hk, H // Hk, Tk, Dh).sum(2), dt, H // Hk * Tq + 8, "dv")
+
+
+@pytest.mark.parametrize("kept", [True, False])
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("case", [(1, 1, 1, 3, 40, 1), (1, 2, 2, 70, 300, 20), (2, 4, 2, 40, 33, 64), (1, 2, 1, 5, 2000, 72),
+                                  (1, 12, 12, 200, 160, 40)],
+                         ids=lambda c: "-".join(str(v) for v in c))
+def test_rows_without_a_finite_score_pass_no_gradient(dev, dt, case, kept):
+    """Scores of -inf from infinite keys or from infinite queries: such a row is 0,
+    its dq is 0 and it adds nothing to dk and dv."""
+    B, H, Hk, Tq, Tk, Dh = case
+    rng = np.random.default_rng(Tk)
+    q, k = (np.abs(rng.standard_normal(s)).astype(dt) + dt(.1) for s in ((B, H, Tq, Dh), (B, Hk, Tk, Dh)))
+    v, g = (rng.standard_normal(s).astype(dt) for s in ((B, Hk, Tk, Dh), (B, H, Tq, Dh)))
+    beyond = v.copy()
+    beyond[..., 0, 0] = np.inf
+    for values in (v, beyond):
+        for got in cross_grads(q, np.full_like(k, -np.inf), values, g, kept=kept):
+            assert (got == 0).all()
+    dead = (0, H - 1, Tq // 2)
+    qi = q.copy()
+    qi[dead] = -np.inf
+    o, dq, dk, dv = cross_grads(qi, k, v, g, kept=kept)
+    assert (o[dead] == 0).all() and (dq[dead] == 0).all()
+    R, live = [t64(x) for x in (q, k, v)], np.ones((B, H, Tq, 1))
+    live[dead] = 0
+    ro = cross_ref(*R, None, Dh ** -.5) * torch.tensor(live)
+    want = torch.autograd.grad(ro, R, t64(g, False))
+    close(o, ro, dt, 512, "o")
+    # dS sums to 0 along the keys, whose elements have a mean of 1.5 times their spread: of
+    # dq's terms less than half is left
+    for got, w, name, bar in zip((dq, dk, dv), want, ("dq", "dk", "dv"), (1024, 512, 512)):
+        close(got, w, dt, bar, name)
