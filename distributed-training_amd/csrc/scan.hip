@@ -371,7 +371,9 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
 
 // Chains the segments in place: carry[s] becomes what enters segment s, in
 // the order of time (forward: from h0) or against it (backward: from zero;
-// what leaves the first segment is the gradient of h0). Bound by the latency of
+// what leaves the first segment is the gradient of h0). States that grow may do so
+// beyond the type's range over a segment while their own value stays in it: 0 stays
+// 0, and the growth is applied in two halves. Bound by the latency of
 // its rounds of loads (64 segments of 1 x 768 x 16: 8.5 us).
 template <typename T>
 __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backward) {
@@ -397,7 +399,8 @@ __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backwar
     for (int v = 0; v < U; ++v) {
       if (i + v >= a.nseg) break;
       p[step * (i + v) * a.N * a.C] = in;
-      in = fma(exp2_of(A2 * sum[v]), in, local[v]);
+      const T half = exp2_of(T(.5) * A2 * sum[v]);
+      in = in == T(0) ? local[v] : fma(in * half, half, local[v]);
     }
   }
 }

@@ -124,3 +124,72 @@ def test_rows_without_a_finite_score_pass_no_gradient(dev, dt, case, kept):
     # dq's terms less than half is left
     for got, w, name, bar in zip((dq, dk, dv), want, ("dq", "dk", "dv"), (1024, 512, 512)):
         close(got, w, dt, bar, name)
+
+
+def scan_all(v, dt, lengths=None, softplus=True, steps=False):
+    """out, state and gradients of ssm_scan for arrays by name, and the reference's."""
+    A, D = _mods()
+    names = [n for n in ("u", "dt", "A", "B", "C", "D", "z", "bias", "h") if n in v]
+    L = {n: A.Tensor(D.from_numpy(v[n].astype(dt)), requires_grad=True) for n in names}
+    y, state = A.ssm_scan(*(L[n] for n in ("u", "dt", "A", "B", "C")), D=L.get("D"), z=L.get("z"), dt_bias=L.get("bias"),
+                          state=L.get("h"), lengths=lengths, return_state=True, softplus=softplus)
+    y.backward(D.from_numpy(v["g"].astype(dt)))
+    # where A has no finite value the reference takes one whose decay is 0 all the same
+    R = {n: t64(np.maximum(v[n].astype(dt).astype(F64), -1e30)) for n in names}
+    B, T, C = v["u"].shape
+    N = v["A"].shape[1]
+    zero = {n: torch.zeros(s, dtype=torch.float64) for n, s in (("D", C), ("bias", C), ("h", (B, C, N)))}
+    Bm, Cm = (R[n] if R[n].ndim == 4 else R[n][:, :, None] for n in "BC")
+    ry, rs = scan_ref(R["u"], R["dt"], R["A"], Bm, Cm, R.get("D", zero["D"]), R.get("z"), R.get("bias", zero["bias"]),
+                      R.get("h", zero["h"]), lengths, softplus)
+    want = torch.autograd.grad(ry, [R[n] for n in names], t64(v["g"].astype(dt), False))
+    return y, state, {n: L[n].grad for n in names}, ry, rs, dict(zip(names, want))
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+def test_scan_growth_of_a_zero_state(dev, dt):
+    """Steps of a negative size make states grow; a state of 0, and a gradient of
+    0, stay 0 over any growth, also where a segment's decay alone leaves the type's range."""
+    rng = np.random.default_rng(6)
+    B, T, C, N = 1, 300, 3, 4
+    v = {n: rng.standard_normal((B, T, C)) for n in ("u", "g")}
+    v.update(A=np.full((C, N), -1.0), B=rng.standard_normal((B, T, N)), C=rng.standard_normal((B, T, N)),
+             D=rng.standard_normal(C), h=rng.standard_normal((B, C, N)), dt=.1 + rng.random((B, T, C)) * .1)
+    v["u"][:, 40:200] = v["g"][:, 40:200] = 0
+    v["dt"][:, 41:199] = -3 if dt is F32 else -60
+    v["dt"][:, [40, 199]] = 20000  # exp(-20000) leaves nothing that exp(158 x 60) could bring back
+    y, state, got, ry, rs, want = scan_all(v, dt, softplus=False)
+    # decays of 0.1 and more: 10 steps' worth of 4 roundings, and the products around them, as in test_scan
+    close(y, ry, dt, 256, "y")
+    close(state, rs, dt, 256, "state")
+    for n in got:
+        close(got[n], want[n], dt, 512, "d" + n)
+
+
+@pytest.mark.parametrize("dt,size,rate,n,bar", [
+    (F32, 1e-30, 2.0, 48, 512),     # e^96 times 1e-30
+    (F64, 1e-300, 48.0, 16, 4096),  # e^768 times 1e-300
+])
+def test_scan_growth_of_a_small_state(dev, dt, size, rate, n, bar):
+    """A state whose product with a segment's growth is in range where the growth
+    is not. The exponent's relative roundings count by its size: 96 and 768, two of
+    them in one product over the segment, and as much again step by step."""
+    A, D = _mods()
+    T, C, N = 300, 2, 3
+    rng = np.random.default_rng(7)
+    h = (1 + rng.random((1, C, N))) * size
+    step, u = np.full((1, T, C), .1), np.zeros((1, T, C))
+    step[:, :n], step[:, n] = -rate, 800
+    step[:, n + 1:] = .1 + rng.random((1, T - n - 1, C)) * .1
+    u[:, n + 1:] = rng.standard_normal((1, T - n - 1, C))
+    Bm, Cm = rng.standard_normal((2, 1, T, N)).astype(dt)
+    a = [x.astype(dt) for x in (u, step, -np.ones((C, N)), Bm, Cm)]
+    with A.no_grad():
+        y, state = A.ssm_scan(*(A.Tensor(D.from_numpy(x)) for x in a), state=D.from_numpy(h.astype(dt)), return_state=True,
+                              softplus=False)
+    z = torch.zeros((), dtype=torch.float64)
+    r = [t64(x, False) for x in a]
+    ry, rs = scan_ref(r[0], r[1], r[2], r[3][:, :, None], r[4][:, :, None], z, None, z, t64(h.astype(dt), False), None, False)
+    close(y.numpy()[:, :n], ry[:, :n], dt, bar, "y while it grows")
+    close(y.numpy()[:, n:], ry[:, n:], dt, 256, "y after")
+    close(state, rs, dt, 256, "state")
