@@ -32,6 +32,15 @@ namespace dtmi {
 constexpr int kStates = 4;  // states per lane
 constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
+// A in base 2, at least the type's lowest value: an A of -inf (-exp(log rate), when
+// it overflows) forgets a state at once, but not where the step is 0
+template <typename T>
+__device__ __forceinline__ T decay_rate(T a) {
+  constexpr T lowest = sizeof(T) == 4 ? T(-3.40282347e38f) : T(-1.7976931348623157e308);
+  const T x = a * T(kLog2e);
+  return x < lowest ? lowest : x;
+}
+
 // Positions per tile. The backward's sixteen waves have 128 registers a lane, which
 // hold half a float32 tile (4 x 1024 x 1536 x 64: 16 positions spill, 732 us, 8: 472).
 template <typename T>
@@ -243,7 +252,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
   T A2[NS], h[NS], total = T(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    A2[j] = k.on && n0 + j < N ? ((const T*)a.A)[k.c * N + n0 + j] * T(kLog2e) : T(0);
+    A2[j] = k.on && n0 + j < N ? decay_rate(((const T*)a.A)[k.c * N + n0 + j]) : T(0);
     h[j] = T(0);
     if (!CARRY && k.on && n0 + j < N) {
       if (a.nseg > 1)
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backwar
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t c = id % a.C, bn = id / a.C, n = bn % a.N, b = bn / a.N;
   if (b >= a.B) return;
-  const T A2 = ((const T*)a.A)[c * a.N + n] * T(kLog2e);
+  const T A2 = decay_rate(((const T*)a.A)[c * a.N + n]);
   T in = !backward && a.h0 ? ((const T*)a.h0)[(b * a.C + c) * a.N + n] : T(0);
   // the loads do not wait for the chain: sixteen segments' at a time
   constexpr int U = 16;
@@ -494,7 +503,7 @@ __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanA
   T A2[NS], dh[NS], dA[NS], total = T(0), dD = T(0), dbias = T(0);
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
-    A2[j] = k.on && n0 + j < N ? ((const T*)a.A)[k.c * N + n0 + j] * T(kLog2e) : T(0);
+    A2[j] = k.on && n0 + j < N ? decay_rate(((const T*)a.A)[k.c * N + n0 + j]) : T(0);
     dA[j] = dh[j] = T(0);
     if (!CARRY && a.nseg > 1 && k.on && n0 + j < N)
       dh[j] = ((const T*)a.carry)[((k.b * a.nseg + k.seg) * N + n0 + j) * a.C + k.c];
@@ -843,7 +852,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs a) {
         vt h = *(const vt*)hp;
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-          h[j] = fma(exp2_of(d * (A[j] * T(kLog2e))), h[j], x * Bp[j]);
+          h[j] = fma(exp2_of(d * decay_rate(T(A[j]))), h[j], x * Bp[j]);
           y = fma(Cp[j], h[j], y);
         }
         *(vt*)hp = h;
@@ -852,7 +861,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs a) {
 #pragma unroll
       for (int j = 0; j < NS; ++j)
         if (n0 + j < N) {
-          const T h = fma(exp2_of(d * (Ap[j] * T(kLog2e))), hp[j], x * Bp[j]);
+          const T h = fma(exp2_of(d * decay_rate(Ap[j])), hp[j], x * Bp[j]);
           hp[j] = h;
           y = fma(Cp[j], h, y);
         }

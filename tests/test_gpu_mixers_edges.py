@@ -193,3 +193,23 @@ def test_scan_growth_of_a_small_state(dev, dt, size, rate, n, bar):
     close(y.numpy()[:, :n], ry[:, :n], dt, bar, "y while it grows")
     close(y.numpy()[:, n:], ry[:, n:], dt, 256, "y after")
     close(state, rs, dt, 256, "state")
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("B,T,C,N,lengths", [(1, 19, 5, 4, None), (2, 40, 70, 16, [40, 13]), (1, 700, 33, 5, None),
+                                             (3, 33, 20, 33, [0, 1, 33])],
+                         ids=lambda v: str(v) if isinstance(v, int) else "")
+def test_scan_of_states_that_are_forgotten_at_once(dev, dt, B, T, C, N, lengths):
+    """A of -inf, as -exp(log rate) gives when it overflows (or a finite one that
+    does in base 2): the decay is 0 at every position and 1 where there is none."""
+    rng = np.random.default_rng(T)
+    v = {n: rng.standard_normal((B, T, C)) for n in ("u", "g", "z")}
+    v.update(A=-0.5 - rng.random((C, N)) * 8, B=rng.standard_normal((B, T, N)), C=rng.standard_normal((B, T, N)),
+             D=rng.standard_normal(C), h=rng.standard_normal((B, C, N)), dt=rng.standard_normal((B, T, C)) * .5)
+    v["A"][rng.random((C, N)) < .3] = -np.inf
+    v["A"][0, 0], v["A"][-1, -1] = -np.inf, -.9 * float(np.finfo(dt).max)
+    y, state, got, ry, rs, want = scan_all(v, dt, lengths)
+    close(y, ry, dt, 256, "y")
+    close(state, rs, dt, 256, "state")
+    for n in got:
+        close(got[n], want[n], dt, 512, "d" + n)
