@@ -956,6 +956,15 @@ static int scan_fwd(ScanArgs& a) {
   return rc;
 }
 
+// The gradients of the maps from their channel tiles' terms (a.tpg tiles; none: zeros).
+template <typename T>
+static int scan_maps(const ScanArgs& a, void* dB, BT sdB, int64_t gdB, void* dC, BT sdC, int64_t gdC) {
+  scan_map_kernel<T><<<(unsigned)cdiv(a.B * a.T * a.G * a.N, 256), 256, 0, stream()>>>(a, (T*)dB, sdB, gdB, (T*)dC, sdC,
+                                                                                      gdC);
+  LAUNCH_CHECK("scan: map gradients");
+  return DTMI_OK;
+}
+
 template <typename T>
 static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* dC, BT sdC, int64_t gdC, void* dD,
                     void* dbias) {
@@ -984,9 +993,8 @@ static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* 
     scan_launch<T, true, false>(a, W);
     scan_param_kernel<T><<<(unsigned)cdiv((a.N + 2) * a.C, 256), 256, 0, stream()>>>(
         (const T*)a.prm, a.B * a.nseg, a.N, a.C, (T*)dA, (T*)dD, (T*)dbias);
-    scan_map_kernel<T><<<(unsigned)cdiv(maps, 256), 256, 0, stream()>>>(a, (T*)dB, sdB, gdB, (T*)dC, sdC, gdC);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) rc = fail_hip(e, "dtmi_scan_bwd", __FILE__, __LINE__);
+    rc = e == hipSuccess ? scan_maps<T>(a, dB, sdB, gdB, dC, sdC, gdC) : fail_hip(e, "dtmi_scan_bwd", __FILE__, __LINE__);
   }
   pool_free(ws);
   return rc;
@@ -1062,8 +1070,17 @@ DTMI_EXPORT int dtmi_scan_bwd(int dtype, int64_t B, int64_t T, int64_t C, int64_
   DTMI_BODY_BEGIN
   DTMI_REQUIRE_INIT();
   if (int rc = scan_shape("dtmi_scan_bwd", dtype, B, T, C, N, G)) return rc;
-  if (C == 0) return DTMI_OK;
   const size_t es = dtype == DTMI_F32 ? 4 : 8;
+  if (C == 0) {  // the maps alone have gradients, of no terms
+    if (B == 0 || T == 0) return DTMI_OK;
+    DTMI_CHECK(dB && dC && dB_strides && dC_strides, "dtmi_scan_bwd: NULL operand");
+    DTMI_CHECK(B * T * G * N <= (int64_t)0x7fffffff * 256, "dtmi_scan_bwd: too many elements");
+    ScanArgs a{};
+    a.B = B, a.T = T, a.N = N, a.G = G;
+    const BT sdB = bt(dB_strides), sdC = bt(dC_strides);
+    return dtype == DTMI_F32 ? scan_maps<float>(a, dB, sdB, dB_strides[2], dC, sdC, dC_strides[2])
+                             : scan_maps<double>(a, dB, sdB, dB_strides[2], dC, sdC, dC_strides[2]);
+  }
   DTMI_CHECK(dA, "dtmi_scan_bwd: NULL operand");
   if (B == 0 || T == 0) {
     int rc = dtmi_zero_bytes(dA, (size_t)C * N * es);

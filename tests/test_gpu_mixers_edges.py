@@ -213,3 +213,22 @@ def test_scan_of_states_that_are_forgotten_at_once(dev, dt, B, T, C, N, lengths)
     close(state, rs, dt, 256, "state")
     for n in got:
         close(got[n], want[n], dt, 512, "d" + n)
+
+
+def leave_sevens():
+    """Sevens in the memory that the next arrays of up to 512 bytes are made of."""
+    _, D = _mods()
+    held = [D.full((n,), 7.0, F32) for n in (64, 128) for _ in range(64)]
+    del held
+
+
+def test_scan_without_channels_has_zero_map_gradients(dev):
+    A, D = _mods()
+    for G in (1, 2):
+        L = [A.Tensor(D.full(s, 1.0, F32), requires_grad=True)
+             for s in ((2, 3, 0), (2, 3, 0), (0, 5), (2, 3, G, 5), (2, 3, G, 5))]
+        y = A.ssm_scan(*L)
+        leave_sevens()
+        y.backward(D.full(y.shape, 1.0, F32))
+        for x in L:
+            assert x.grad.shape == x.shape and (x.grad.numpy() == 0).all()
