@@ -1271,7 +1271,7 @@ DTMI_EXPORT int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   a.q = q, a.k = k, a.v = v, a.out = o, a.lengths = lengths, a.rowmax = rowmax, a.rowsum = rowsum;
   a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides);
   a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.G = H / Hk, a.R = a.G * Tq, a.scale = scale;
-  a.by_tq = FastDiv((uint32_t)(Tq > 0 ? Tq : 1));
+  a.by_tq = FastDiv((uint32_t)(a.R > 0 ? Tq : 1));
   TimedLaunch tl(DTMI_FAM_OTHER, 4.0 * B * H * Tq * Tk * D);
   return dtype == DTMI_F32 ? xattn_fwd<float>(a) : xattn_fwd<double>(a);
   DTMI_BODY_END
@@ -1287,8 +1287,8 @@ DTMI_EXPORT int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   DTMI_BODY_BEGIN
   DTMI_REQUIRE_INIT();
   if (int rc = x_shape("dtmi_xattn_bwd", dtype, B, H, Hk, Tq, Tk, D)) return rc;
-  if (B == 0 || H == 0) return DTMI_OK;
-  DTMI_CHECK((Tq == 0 || (q && o && dO && dq && rowmax && rowsum && q_strides && o_strides && dO_strides && dq_strides)) &&
+  if (B == 0) return DTMI_OK;
+  DTMI_CHECK((H == 0 || Tq == 0 || (q && o && dO && dq && rowmax && rowsum && q_strides && o_strides && dO_strides && dq_strides)) &&
                  (Tk == 0 || (k && v && dk && dv && k_strides && v_strides && dk_strides && dv_strides)),
              "dtmi_xattn_bwd: NULL operand");
   XArgs a{};
@@ -1297,7 +1297,7 @@ DTMI_EXPORT int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int6
   a.sq = ht(q_strides), a.sk = ht(k_strides), a.sv = ht(v_strides), a.so = ht(o_strides), a.sdo = ht(dO_strides);
   a.sdq = ht(dq_strides), a.sdk = ht(dk_strides), a.sdv = ht(dv_strides);
   a.B = B, a.H = H, a.Hk = Hk, a.Tq = Tq, a.Tk = Tk, a.D = D, a.G = H / Hk, a.R = a.G * Tq, a.scale = scale;
-  a.by_tq = FastDiv((uint32_t)(Tq > 0 ? Tq : 1));
+  a.by_tq = FastDiv((uint32_t)(a.R > 0 ? Tq : 1));
   TimedLaunch tl(DTMI_FAM_OTHER, 14.0 * B * H * Tq * Tk * D);
   return dtype == DTMI_F32 ? xattn_bwd<float>(a) : xattn_bwd<double>(a);
   DTMI_BODY_END

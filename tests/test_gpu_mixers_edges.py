@@ -232,3 +232,13 @@ def test_scan_without_channels_has_zero_map_gradients(dev):
         y.backward(D.full(y.shape, 1.0, F32))
         for x in L:
             assert x.grad.shape == x.shape and (x.grad.numpy() == 0).all()
+
+
+def test_cross_attention_without_heads_has_zero_memory_gradients(dev):
+    A, D = _mods()
+    L = [A.Tensor(D.full(s, 1.0, F32), requires_grad=True) for s in ((2, 0, 3, 8), (2, 2, 4, 8), (2, 2, 4, 8))]
+    o = A.cross_attention(*L)
+    leave_sevens()
+    o.backward(D.full(o.shape, 1.0, F32))
+    for x in L:
+        assert x.grad.shape == x.shape and (x.grad.numpy() == 0).all()
