@@ -490,6 +490,8 @@ def causal_conv(x: Tensor, w: Tensor, b: Tensor | None = None, silu: bool = True
     ln = _lengths_of(lengths, X.shape[0], X.shape[1])
     st = _state_of(state)
     W, bd, S = _contig(w.data), _contig(b.data) if b is not None else None, _contig(st.data) if st is not None else None
+    if S is not None and S is st.data and _grad_enabled and any(p is not None and p.requires_grad for p in (x, w, b, st)):
+        S = S.copy()  # the backward reads it again; causal_conv_step may have moved the caller's on by then
     y, new = K.conv_fwd(X, W, bd, S, ln, silu, return_state)
 
     def bw(g):

@@ -242,3 +242,25 @@ def test_cross_attention_without_heads_has_zero_memory_gradients(dev):
     o.backward(D.full(o.shape, 1.0, F32))
     for x in L:
         assert x.grad.shape == x.shape and (x.grad.numpy() == 0).all()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_conv_gradient_after_its_state_moved_on(dev, grad):
+    """The state handed to causal_conv may be moved on in place before backward."""
+    A, D = _mods()
+    rng = np.random.default_rng(9)
+    B, T, C, K = 2, 6, 20, 4
+    x, g = rng.standard_normal((2, B, T, C))
+    w, st = rng.standard_normal((K, C)), rng.standard_normal((B, K - 1, C))
+    X, W = (A.Tensor(D.from_numpy(a), requires_grad=True) for a in (x, w))
+    state = D.from_numpy(st)
+    y = A.causal_conv(X, W, state=A.Tensor(state, requires_grad=True) if grad else state)
+    with A.no_grad():
+        A.causal_conv_step(A.Tensor(D.from_numpy(x[:, 0])), W, None, state)
+    y.backward(D.from_numpy(g))
+    rx, rw = t64(x), t64(w)
+    ry, _ = conv_ref(rx, rw, torch.zeros(C, dtype=torch.float64), t64(st, False), None, True)
+    want = torch.autograd.grad(ry, (rx, rw), t64(g, False))
+    close(y, ry, F64, K + 16, "y")
+    close(X.grad, want[0], F64, 2 * K + 32, "dx")
+    close(W.grad, want[1], F64, 2 * K + 160, "dw")
