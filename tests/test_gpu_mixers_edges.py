@@ -264,3 +264,126 @@ def test_conv_gradient_after_its_state_moved_on(dev, grad):
     close(y, ry, F64, K + 16, "y")
     close(X.grad, want[0], F64, 2 * K + 32, "dx")
     close(W.grad, want[1], F64, 2 * K + 160, "dw")
+
+
+# ------------------------------------------------ configurations without a fault
+JOIN = [  # more than 2048 rows of a split loop, B, H, Hk, Tq, Tk, D, lengths
+    (2, 4, 2, 300, 1500, 40, None),
+    (1, 12, 12, 200, 1500, 128, None),
+    (2, 2, 1, 520, 700, 20, None),
+    (1, 3, 3, 700, 900, 90, None),
+    (5, 2, 1, 210, 1500, 72, [1500, 0, 97, 1024, 1025]),
+    (4, 4, 2, 140, 800, 128, [1, 800, 65, 0]),
+    (3, 2, 2, 350, 600, 48, [33, 600, 577]),
+]
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("case", JOIN, ids=lambda c: "-".join(str(v) for v in c[:6]))
+def test_cross_attention_joins_many_rows(dev, dt, case):
+    B, H, Hk, Tq, Tk, Dh, lengths = case
+    rng = np.random.default_rng(Tq + Dh)
+    q, g = (rng.standard_normal((B, H, Tq, Dh)).astype(dt) for _ in range(2))
+    k, v = (rng.standard_normal((B, Hk, Tk, Dh)).astype(dt) for _ in range(2))
+    got = cross_grads(q, k, v, g, lengths, strided=Tq % 4 == 0)
+    R = [t64(x) for x in (q, k, v)]
+    ro = cross_ref(*R, lengths, Dh ** -.5)
+    for i in range(B):  # each sequence by itself
+        close(got[0][i], ro[i], dt, 512, f"o {i}")
+    for x, w, name in zip(got[1:], torch.autograd.grad(ro, R, t64(g, False)), ("dq", "dk", "dv")):
+        close(x, w, dt, 512, name)
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+def test_step_sizes_keep_their_relative_accuracy(dev, dt):
+    """One position, one state, operands of 1: the state is softplus(dt) and the
+    gradient of dt its sigmoid, each judged by itself from 1e-35 to 80. float32
+    takes exp(x) as a power of two whose exponent carries two roundings of its size,
+    2 |x| u of the value; beside that exponential, reciprocal, series and sums: 16."""
+    A, D = _mods()
+    x = np.concatenate([np.linspace(-80, 80, 3201), np.linspace(-9, -3, 801), [0.0]]).astype(dt)
+    C = len(x)
+    one = lambda *s: A.Tensor(D.full(s, 1.0, dt), requires_grad=True)  # noqa: E731
+    X = A.Tensor(D.from_numpy(x[None, None]), requires_grad=True)
+    y, state = A.ssm_scan(one(1, 1, C), X, A.Tensor(D.full((C, 1), -1.0, dt)), one(1, 1, 1), one(1, 1, 1), return_state=True)
+    y.backward(D.full((1, 1, C), 1.0, dt))
+    x = x.astype(F64)
+    bar = (16 + (2 * np.abs(x) if dt is F32 else 0)) * U[dt]
+    for got, want, what in ((state, np.maximum(x, 0) + np.log1p(np.exp(-np.abs(x))), "softplus"),
+                            (X.grad, 1 / (1 + np.exp(-x)), "sigmoid")):
+        off = np.abs(got.numpy().reshape(-1).astype(F64) - want) / want / bar
+        assert off.max() <= 1, (what, x[off.argmax()], off.max())
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("B,T,C,N,lengths", [(1, 300, 70, 16, None), (2, 260, 40, 4, [260, 131]), (1, 200, 24, 40, None)],
+                         ids=lambda v: str(v) if isinstance(v, int) else "")
+def test_scan_of_slow_decays(dev, dt, B, T, C, N, lengths):
+    """Rates of 1..N and steps of 1e-3 to 1e-1, as such layers start with: a
+    segment leaves most of the state that enters it. A value carries 4 roundings a
+    step over up to T steps, its gradients those of both ways: 4 T and 8 T, and 512."""
+    rng = np.random.default_rng(T)
+    v = {n: rng.standard_normal((B, T, C)) for n in ("u", "g", "z")}
+    size = np.exp(rng.random(C) * np.log(100) + np.log(1e-3))
+    v.update(A=-np.broadcast_to(np.arange(1, N + 1), (C, N)) * np.exp(.1 * rng.standard_normal((C, N))),
+             B=rng.standard_normal((B, T, N)), C=rng.standard_normal((B, T, N)), D=1 + .1 * rng.standard_normal(C),
+             bias=size + np.log(-np.expm1(-size)), h=rng.standard_normal((B, C, N)), dt=rng.standard_normal((B, T, C)) * .5)
+    y, state, got, ry, rs, want = scan_all(v, dt, lengths)
+    close(y, ry, dt, 4 * T, "y")
+    close(state, rs, dt, 4 * T, "state")
+    for n in got:
+        close(got[n], want[n], dt, 8 * T + 512, "d" + n)
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+def test_steps_take_views(dev, dt):
+    """Single positions out of fused projections: the bits of contiguous operands."""
+    A, D = _mods()
+    rng = np.random.default_rng(3)
+    B, C, N, G, K = 3, 36, 8, 2, 4
+
+    def fused(a):
+        """a [B, ...] as the second of two arrays that one projection leaves side by side."""
+        both = np.full((B, 2) + a.shape[1:], np.nan, dt)
+        both[:, 1] = a
+        return A.Tensor(D.from_numpy(both).transpose(1, 0, *range(2, a.ndim + 1))[1])
+
+    def whole(a):
+        return A.Tensor(D.from_numpy(a))
+    x, step, z = rng.standard_normal((3, B, C)).astype(dt)
+    Bm, Cm = rng.standard_normal((2, B, G, N)).astype(dt)
+    w, b, Am, Dm, bias = (whole(rng.standard_normal(s).astype(dt)) for s in ((K, C), C, (C, N), C, C))
+    cs, hs = rng.standard_normal((B, K - 1, C)).astype(dt), rng.standard_normal((B, C, N)).astype(dt)
+    out = []
+    for of in (whole, fused):
+        c, h = D.from_numpy(cs), D.from_numpy(hs)
+        y = A.causal_conv_step(of(x), w, b, c)
+        s = A.ssm_scan_step(of(x), of(step), Am, of(Bm), of(Cm), Dm, of(z), bias, h)
+        out.append([t.numpy() for t in (y, s, c, h)])
+    for a, b_ in zip(*out):
+        assert np.isfinite(a).all() and bits_equal(a, b_)
+
+
+@pytest.mark.parametrize("D_", [64, 45])
+def test_cross_attention_results_in_views(dev, D_):
+    """Output and gradients written into parts of larger arrays, nothing beside them."""
+    from dtmi import kernels as K
+    _, D = _mods()
+    rng = np.random.default_rng(D_)
+    B, H, Hk, Tq, Tk = 2, 4, 2, 37, 50
+    q, g = (D.from_numpy(rng.standard_normal((B, H, Tq, D_)).astype(F32)) for _ in range(2))
+    k, v = (D.from_numpy(rng.standard_normal((B, Hk, Tk, D_)).astype(F32)) for _ in range(2))
+
+    def room(T, heads):
+        """Three arrays [B, T, 3, heads, D] in one of sevens; the view is the middle one."""
+        a = D.full((B, T, 3, heads, D_), 7.0, F32)
+        return a, a.transpose(2, 0, 3, 1, 4)[1]
+    o, m, l = K.xattn_fwd(q, k, v)
+    grads = K.xattn_bwd(q, k, v, o, g, m, l)
+    rooms = [room(Tq, H), room(Tq, H), room(Tk, Hk), room(Tk, Hk)]
+    o2, m2, l2 = K.xattn_fwd(q, k, v, out=rooms[0][1])
+    K.xattn_bwd(q, k, v, o2, g, m2, l2, dq=rooms[1][1], dk=rooms[2][1], dv=rooms[3][1])
+    for want, (whole, view) in zip((o,) + tuple(grads), rooms):
+        assert bits_equal(view.numpy(), want.numpy())
+        rest = whole.numpy()
+        assert (rest[:, :, [0, 2]] == 7).all()
