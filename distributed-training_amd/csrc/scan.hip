@@ -894,15 +894,24 @@ static void scan_launch(const ScanArgs& a, int W) {
 #undef SCAN_W
 }
 
-// Segments of T: one where B * C / 64 blocks already occupy the card. A split
-// costs the exponentials a second time, so it pays while less than a block per
-// CU would run (float32, 1536 channels x 16 states x 1024 positions, forward
-// and backward without and with: 96 blocks 498 / 208 us, 192 blocks 516 / 410,
-// at 256 blocks equal); then enough segments for 12 waves per CU (three blocks
-// at 16 states), of at least two tiles each.
+// Segments of T: one where the blocks (B * C / 64, of W waves) occupy the card. A
+// split costs the exponentials a second time, so it pays while the card would run
+// fewer than about four waves per CU (float64 three, whose exponentials cost
+// more), but not beyond half a block per CU (sixteen waves fill one; the segments
+// have to run at once) or two. Forward and backward of 1024 positions x 1536
+// channels, us in one piece and cut, float32: 4 states, 384 blocks 917 / 504, 672
+// blocks 921 / 892, 960 blocks 937 / 1222; 8 states, 288 blocks 785 / 459, 504
+// blocks 800 / 751, 768 blocks 812 / 1106; 16 states, 192 blocks 503 / 376, 240
+// blocks 506 / 495, 264 blocks 650 / 686; 32 states, 120 blocks 607 / 421, 192 blocks
+// 612 / 789; 64 states, 120 blocks 1179 / 820, 192 blocks 1203 / 1568. float64: 8
+// states, 384 blocks 1826 / 1798, 432 blocks 1830 / 2188; 16 states, 144 blocks 1296
+// / 1093, 192 blocks 1302 / 1348; 64 states, 120 blocks 6957 / 4858. Then enough
+// segments for 12 waves per CU (three blocks at 16 states), of at least two tiles each.
+template <typename T>
 static void scan_segments(ScanArgs& a, int TT, int W) {
-  const int64_t blocks = a.B * a.ct, want = (W <= 4 ? 12 / W : 2) * (int64_t)num_cus(), tiles = cdiv(a.T, TT);
-  int64_t s = blocks >= num_cus() ? 1 : want / blocks;
+  const int64_t cus = num_cus(), blocks = a.B * a.ct, want = (W <= 4 ? 12 / W : 2) * cus, tiles = cdiv(a.T, TT);
+  const int64_t waves = (sizeof(T) == 4 ? 4 : 3) * cus / W, full = waves < cus / 2 ? cus / 2 : waves > 2 * cus ? 2 * cus : waves;
+  int64_t s = blocks >= full ? 1 : want / blocks;
   if (s > tiles / 2) s = tiles / 2;
   if (s < 1) s = 1;
   a.seglen = (int)(cdiv(tiles, s) * TT);
@@ -934,7 +943,7 @@ static int scan_chain(ScanArgs& a, int W, bool backward) {
 template <typename T>
 static int scan_fwd(ScanArgs& a) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(W, false), W);
+  scan_segments<T>(a, tile_len<T>(W, false), W);
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256,
              "dtmi_scan_fwd: too many elements");
   void* ws = nullptr;
@@ -969,7 +978,7 @@ template <typename T>
 static int scan_bwd(ScanArgs& a, void* dA, void* dB, BT sdB, int64_t gdB, void* dC, BT sdC, int64_t gdC, void* dD,
                     void* dbias) {
   const int W = waves_for(a.N);
-  scan_segments(a, tile_len<T>(W, true), W);
+  scan_segments<T>(a, tile_len<T>(W, true), W);
   const int64_t maps = a.B * a.T * a.G * a.N;
   DTMI_CHECK(a.B * a.nseg * a.ct <= 0x7fffffff && a.B * a.N * a.C <= (int64_t)0x7fffffff * 256 &&
                  maps <= (int64_t)0x7fffffff * 256,

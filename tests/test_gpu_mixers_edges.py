@@ -316,7 +316,9 @@ def test_step_sizes_keep_their_relative_accuracy(dev, dt):
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
-@pytest.mark.parametrize("B,T,C,N,lengths", [(1, 300, 70, 16, None), (2, 260, 40, 4, [260, 131]), (1, 200, 24, 40, None)],
+@pytest.mark.parametrize("B,T,C,N,lengths", [(1, 300, 70, 16, None), (2, 260, 40, 4, [260, 131]), (1, 200, 24, 40, None),
+                                             (100, 80, 130, 4, None), (130, 70, 130, 7, None),  # more blocks than CUs, cut
+                                             (130, 70, 65, 13, None), (140, 70, 20, 20, None)],   # in one piece
                          ids=lambda v: str(v) if isinstance(v, int) else "")
 def test_scan_of_slow_decays(dev, dt, B, T, C, N, lengths):
     """Rates of 1..N and steps of 1e-3 to 1e-1, as such layers start with: a
