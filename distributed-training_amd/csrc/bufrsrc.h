@@ -1,11 +1,11 @@
 // Raw buffer accesses: a wave-uniform resource (base address and byte range),
 // a per-lane byte offset that stays fixed over a loop and a wave-uniform byte
-// offset, so addressing takes no vector instructions. The range check covers
-// the per-lane offset only: an access whose lane offset is at or past the
-// range reads 0 and writes nothing, while the wave-uniform offset is added
-// unchecked -- every caller that relies on the check puts the whole offset in
-// the lane offset. Shared by the attention, GEMM-epilogue and cross-entropy
-// kernels.
+// offset, so addressing takes no vector instructions. An access whose offset is at
+// or past the range reads 0 and writes nothing. The wave-uniform offset counts
+// for that check on gfx950 (a range of 256 bytes, read at 1024 + lane: 0); callers
+// that rely on the check put the whole offset in the lane offset all the same, and
+// the others' ranges hold both. Shared by the attention, GEMM-epilogue,
+// cross-entropy, scan and cross-attention kernels.
 #pragma once
 
 #include <hip/hip_runtime.h>

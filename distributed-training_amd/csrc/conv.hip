@@ -38,8 +38,8 @@ __device__ __forceinline__ void conv_row(T (&r)[VW], const ConvArgs& a, const T*
   }
 }
 
-// 8 x 1024 x 1536 float32, 4 taps: 19 us, 5.3 TB/s, the rate of a large copy; 5
-// padded prompts x 777 x 1001 (single elements: the rows are not 16-byte aligned), 3 taps: 9.
+// 8 x 1024 x 1536, 4 taps: float32 19 us, 5.3 TB/s, the rate of a large copy, float64
+// 41, 4.9; 5 padded prompts x 777 x 1001 (single elements, see conv_vectors), 3 taps: 8.
 template <typename T, int K, int VW>
 __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs a) {
   constexpr int U = kConvUnroll;
@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvArgs a) {
 // and the K - 1 after it, dx[t] = sum_k w[k] g'[t + K - 1 - k], and the
 // segment's own terms of dw[k] = sum_t g'[t] x[t - K + 1 + k] and db = sum_t g'[t],
 // summed over segments in a fixed order by a second kernel. The first segment
-// also owns the positions of the state. 8 x 1024 x 1536 float32, 4 taps: 32 us,
-// 4.7 TB/s, and 4 for the sums.
+// also owns the positions of the state. 8 x 1024 x 1536, 4 taps: float32 32 us,
+// 4.7 TB/s, and 4 for the sums; float64 99, 3.1 TB/s (a float64 exponential per element).
 template <typename T, int K, int VW>
 __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvArgs a) {
   constexpr int U = kConvUnroll;
@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(1024) conv_sum_kernel(const T* __restrict__ pa
 }
 
 // One position per sequence: the state's K - 1 rows and the new input give y,
-// and the state moves on by one row in place: a launch (4 x 256, 4 taps: 2.3 us).
+// and the state moves on by one row in place: a launch (4 x 256, 4 taps: 2.1 us;
+// 512 x 1536: 5.7, float64 8.2).
 template <typename T, int K, int VW>
 __global__ void __launch_bounds__(256) conv_step_kernel(ConvArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -282,8 +283,9 @@ static void conv_taps(ConvOp op, const ConvArgs& a, int K, unsigned grid) {
   }
 }
 
-// Vectors of channels per row: whole 16-byte ones where every row allows them,
-// else single elements.
+// Vectors of channels per row: whole 16-byte ones where every row is aligned to
+// them, as the vector type asks, else single elements. (The hardware asks for a
+// dword's alignment only: vectors for the bulk of such rows remain to be built.)
 template <typename T>
 static void conv_vectors(ConvArgs& a) {
   constexpr int VW = 16 / sizeof(T);

@@ -62,8 +62,10 @@ __host__ __device__ constexpr int held_len(int W) {
   return (sizeof(T) == 4 ? 8 : 4) / (W <= 8 ? 1 : 2);
 }
 // Waves per SIMD the backward's registers are cut to: two of 219 (float32, 9 to
-// 16 states; three of 168 spill, and a spill's store counts as one to wait for),
-// one in float64 and for up to 4 states (a wave then stages all of a tile), where two spill.
+// 16 states; three of 168 spill, and a spill's store counts as one to wait for), one
+// in float64 up to 16 states and for up to 4 states (a wave then stages all of a
+// tile), where two spill. A block of eight waves is two per SIMD and one of sixteen
+// four, whatever they need: float64 keeps 32 and 164 of a lane's values in memory there.
 template <typename T>
 __host__ __device__ constexpr int bwd_waves(int W) {
   return W == 16 ? 4 : W == 8 ? 2 : sizeof(T) == 4 && W > 1 ? 2 : 1;
@@ -225,9 +227,10 @@ constexpr bool reads_ahead(int W, bool small) {
 }
 
 // 4 x 1024 x 1536 x 16 float32: 100.7 M states and steps at 6 issue slots are 15
-// us of vector instructions, the bytes 19; measured 39, and 27 for CARRY: the
+// us of vector instructions, the bytes 19; measured 36, and 25 for CARRY: the
 // vector unit is busy for 77 % of the cycles (the stores of a tile, the sums over
-// waves and the staging are the rest). Maps as scalar loads: 68.
+// waves and the staging are the rest). Maps as scalar loads: 68 against 39 then.
+// float64: 130 and 99, the library's exponential.
 // CARRY: only the segment's end state from a zero start, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(64 * W) scan_fwd_kernel(ScanArgs a) {
 // what leaves the first segment is the gradient of h0). States that grow may do so
 // beyond the type's range over a segment while their own value stays in it: 0 stays
 // 0, and the growth is applied in two halves. Bound by the latency of
-// its rounds of loads (64 segments of 1 x 768 x 16: 8.5 us).
+// its rounds of loads (64 segments of 1 x 768 x 16: 8.2 us).
 template <typename T>
 __global__ void __launch_bounds__(256) scan_chain_kernel(ScanArgs a, int backward) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -476,8 +479,10 @@ __device__ __forceinline__ T sum8(const T (&v)[8], bool upper8) {
 // A tile's states are rebuilt in registers from the state kept before it. The
 // sums over a wave's channels (dB, dC) are taken as sum8, eight values of a
 // step together, and eight steps' results leave a wave as one LDS write.
-// 4 x 1024 x 1536 x 16 float32: 110 us, and 29 for CARRY; the vector unit is busy
-// for 61 to 70 % of the cycles, two waves per SIMD leave its chains in view.
+// 4 x 1024 x 1536 x 16 float32: 100 us, and 27 for CARRY (float64 339 and 107). Per
+// state and step 5 issue slots rebuild the state, 9 go back, 4.5 are the channel sums,
+// beside the tile's staging; the vector unit is busy for 61 to 70 % of the cycles, two
+// waves per SIMD leave its chains in view.
 // CARRY: only dh over the segment, and its sum of d.
 template <typename T, int W, bool CARRY>
 __global__ void __launch_bounds__(64 * W, bwd_waves<T>(W)) scan_bwd_kernel(ScanArgs a) {
@@ -825,7 +830,7 @@ __global__ void __launch_bounds__(256) scan_map_kernel(ScanArgs a, T* __restrict
 
 // One position per sequence, the states in place. A group of LPC lanes owns a
 // channel, four states each; bound by reading and writing the states once (64 x
-// 1536 x 16 float32, 14 MB: 5.4 us, launch included; the copy rate alone 2.7).
+// 1536 x 16 float32, 14 MB: 5.6 us, launch included; the copy rate alone 2.7; float64 9).
 template <typename T, int LPC, bool VEC>
 __global__ void __launch_bounds__(256) scan_step_kernel(ScanArgs a) {
   constexpr int NS = kStates;
@@ -910,7 +915,8 @@ static void scan_launch(const ScanArgs& a, int W) {
 template <typename T>
 static void scan_segments(ScanArgs& a, int TT, int W) {
   const int64_t cus = num_cus(), blocks = a.B * a.ct, want = (W <= 4 ? 12 / W : 2) * cus, tiles = cdiv(a.T, TT);
-  const int64_t waves = (sizeof(T) == 4 ? 4 : 3) * cus / W, full = waves < cus / 2 ? cus / 2 : waves > 2 * cus ? 2 * cus : waves;
+  const int64_t waves = (sizeof(T) == 4 ? 4 : 3) * cus / W;
+  const int64_t full = waves < cus / 2 ? cus / 2 : waves > 2 * cus ? 2 * cus : waves;
   int64_t s = blocks >= full ? 1 : want / blocks;
   if (s > tiles / 2) s = tiles / 2;
   if (s < 1) s = 1;

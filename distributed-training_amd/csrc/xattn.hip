@@ -382,10 +382,11 @@ constexpr int x_waves(int DP, bool kv = false) {
 constexpr int kKeys = 32;  // keys (rows, in the dK/dV pass) per tile
 
 // The forward for more than 16 rows: a wave owns 16 of them. Bound by the MFMAs:
-// two products, 4 D per score. float32, 32 x 12 heads x 1024 x 2048 x 64: 130
-// TFLOP/s (a large library product: 154); 8 x 12 x 1024 x 512: 120 us, 107, all
-// blocks at once. Five or six waves per SIMD spill; a second LDS buffer and 32 rows
-// per wave gave nothing.
+// two products, 4 D per score. float32, 32 x 12 heads x 1024 x 2048 x 64: 128
+// TFLOP/s (a large library product: 154); 8 x 12 x 1024 x 512: 115 us, 112: of 1536
+// blocks four waves per SIMD (103 registers) take 1024 at once, and the second round is
+// half empty. float64 263 us, 49 (a large product 73). Five or six waves per SIMD
+// spill; a second LDS buffer and 32 rows per wave gave nothing.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a) {
   using M = XM<T>;
@@ -496,7 +497,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_fwd_kernel(XArgs a)
 // part and loads them straight into the products' operand registers, the next
 // 16 while it works; the waves' results are joined through LDS. One query of
 // 64 x 12 heads x 1024 keys x 64, 403 MB: 74 us, 5.4 TB/s (the kernel for more
-// rows, three of its waves idle: 84); of 8 x 16 / 4 heads x 4999 x 128: 34 and 56.
+// rows, three of its waves idle: 84); of 8 x 16 / 4 heads x 4999 x 128: 34 and 56. In
+// float64 148 and 82.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_rows_kernel(XArgs a) {
   using M = XM<T>;
@@ -719,7 +721,7 @@ __global__ void __launch_bounds__(256) xattn_join_kernel(XArgs a) {
   }
 }
 
-// rowsum(dO O): 16 lanes per row; reads both once (8 x 12 x 1024 x 64 float32: 12 us, 4.2 TB/s)
+// rowsum(dO O): 16 lanes per row; reads both once (8 x 12 x 1024 x 64 float32: 13 us, 3.8 TB/s)
 template <typename T>
 __global__ void __launch_bounds__(256) xattn_drow_kernel(XArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), bh = id / a.R;
@@ -831,7 +833,8 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_q_kernel(XArgs 
 
 // dK and dV: a wave owns 16 keys and loops over the rows of its part. Bound by
 // the MFMAs (four products): float32, 32 x 12 heads x 1024 x 2048 x 64, 124
-// TFLOP/s; 8 x 12 x 1024 x 512, 768 blocks: 250 us, 103.
+// TFLOP/s; 8 x 12 x 1024 x 512: 232 us, 111, its 768 blocks all at once, three waves
+// per SIMD; float64 591 us, 44, one wave per SIMD.
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel(XArgs a) {
   using M = XM<T>;
@@ -970,7 +973,7 @@ __global__ void __launch_bounds__(256, x_waves<T>(DP, true)) xattn_bwd_kv_kernel
 }
 
 // dQ from the dS that the dK/dV pass left: one product, bound by reading dS
-// (8 x 12 heads x 1024 x 512 x 64 float32, 201 MB: 60 to 75 us).
+// (8 x 12 heads x 1024 x 512 x 64 float32, 201 MB: 66 us; float64 125).
 template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(256, x_waves<T>(DP)) xattn_bwd_ds_kernel(XArgs a) {
   using M = XM<T>;

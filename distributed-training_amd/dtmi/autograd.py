@@ -479,7 +479,8 @@ def causal_conv(x: Tensor, w: Tensor, b: Tensor | None = None, silu: bool = True
     SiLU (silu=False: none).
 
     `state` [B, K - 1, C] (a Tensor or DeviceArray) holds the inputs before the
-    first position, zeros without one. `lengths` (one per sequence, a host array
+    first position, zeros without one; it may be moved on in place once the call
+    returns. `lengths` (one per sequence, a host array
     or an Indices) marks a padded batch: y and the gradients are zero from a
     sequence's length on, and what lies there is not read. With `return_state`,
     returns (y, state): the last K - 1 inputs of every sequence as a DeviceArray,
@@ -522,7 +523,7 @@ def ssm_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor |
              dt_bias: Tensor | None = None, state=None, lengths=None, return_state: bool = False,
              softplus: bool = True):
     """Selective state space scan of u [B, T, C]: with d = softplus(dt + dt_bias)
-    (softplus=False: dt + dt_bias),
+    (softplus=False: dt + dt_bias; an A of -inf forgets its state at every position),
         h[c, n] = exp(d A[c, n]) h[c, n] + d u B[t, n],   y = sum_n C[t, n] h[c, n] + D u
     and the result y silu(z), or y without z. dt and z are [B, T, C], A is [C, N]
     (N up to 64), B and C are [B, T, N], or [B, T, G, N] for G groups of channels.

@@ -446,7 +446,8 @@ int dtmi_conv_step(int dtype, int64_t B, int64_t C, int64_t K, const void* x, in
  *   d = softplus(dt + dt_bias) (softplus != 0) or dt + dt_bias
  *   h[c, n] = exp(d A[c, n]) h[c, n] + d u Bm[t, g, n];  y = sum_n Cm[t, g, n] h[c, n] + D[c] u
  *   out = y silu(z), or y without z
- * A [C, N]; D, dt_bias [C], z [B, T, C], state [B, C, N] may be NULL (0; no gate);
+ * A [C, N] (-inf: the state is forgotten at every position with a d above 0); D,
+ * dt_bias [C], z [B, T, C], state [B, C, N] may be NULL (0; no gate);
  * state_out [B, C, N] or NULL. `kept`, for the backward: dtmi_scan_kept() elements
  * that the forward fills with the states before every eighth position (NULL: not
  * kept). The backward writes every gradient it is given room for; dD, ddt_bias and
@@ -475,10 +476,10 @@ int dtmi_scan_step(int dtype, int64_t B, int64_t C, int64_t N, int64_t G, const 
  * the first lengths[b] of k, v [B, Hk, Tk, D], H a multiple of Hk (head h reads
  * h / (H / Hk)), D = 1 to 128 contiguous, (b, h, t) strides as dtmi_attn_fwd takes
  * them. A row without keys, or whose scores are all -inf, is 0 and passes no
- * gradient. The forward writes the row statistics the backward reads (contiguous
- * [B, H, Tq], both or neither NULL): rowmax, a reference within 2^8 of the maximum
- * in base-2 units, and rowsum = sum_j 2^(log2(e) q . k_j scale - rowmax). The
- * backward keeps dS [B, H, Tq, Tk] for its dQ pass where that is within
+ * gradient, whatever its operands hold; with one key dq and dk are 0. The forward
+ * writes the row statistics the backward reads (contiguous [B, H, Tq], both or
+ * neither NULL): rowmax, a reference within 2^8 of the maximum in base-2 units, and
+ * rowsum = sum_j 2^(log2(e) q . k_j scale - rowmax). The backward keeps dS [B, H, Tq, Tk] for its dQ pass where that is within
  * dtmi_attn_set_ds_limit's bound and can be allocated, else forms it twice. */
 int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D, double scale,
                    const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
