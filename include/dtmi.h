@@ -479,8 +479,9 @@ int dtmi_scan_step(int dtype, int64_t B, int64_t C, int64_t N, int64_t G, const 
  * gradient, whatever its operands hold; with one key dq and dk are 0. The forward
  * writes the row statistics the backward reads (contiguous [B, H, Tq], both or
  * neither NULL): rowmax, a reference within 2^8 of the maximum in base-2 units, and
- * rowsum = sum_j 2^(log2(e) q . k_j scale - rowmax). The backward keeps dS [B, H, Tq, Tk] for its dQ pass where that is within
- * dtmi_attn_set_ds_limit's bound and can be allocated, else forms it twice. */
+ * rowsum = sum_j 2^(log2(e) q . k_j scale - rowmax). The backward keeps dS
+ * [B, H, Tq, Tk] for its dQ pass where that is within dtmi_attn_set_ds_limit's bound
+ * and can be allocated, else forms it twice. */
 int dtmi_xattn_fwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D, double scale,
                    const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                    const int64_t* v_strides, const int64_t* lengths, void* o, const int64_t* o_strides, void* rowmax,
