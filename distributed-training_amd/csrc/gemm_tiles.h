@@ -531,10 +531,20 @@ __device__ __forceinline__ void dma_tail_store(T* __restrict__ tile, const TileR
   }
 }
 
-// Block tile BM x BN (64 x 64, 128 x 128, or 256 x 128 in float32), 4 waves in a
-// 2 x 2 grid of (BM/2) x (BN/2) wave tiles.
+// The k loop of one block tile BM x BN (64 x 64, 128 x 128, or 256 x 128 in float32),
+// 4 waves in a 2 x 2 grid of (BM/2) x (BN/2) wave tiles: acc += A(m0.., k) B(k, n0..)
+// over kbeg <= k < kend. A and B are whole matrices (M, N: their edges, onto which
+// rows and columns past them are clamped); lds holds kDmaLds<T, BM, BN> elements, 1 KB
+// aligned. fold_groups as in GemmArgs; csum: this thread's column sum of B where
+// take_colsum.
+template <typename T, int BM, int BN>
+constexpr int kDmaLds = kDmaStages<BM, BN> * (BM + BN) * (64 / (int)sizeof(T));
+
 template <typename T, int BM, int BN, bool AKC, bool BKC, bool VECA, bool VECB>
-__global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(GemmArgs a) {
+__device__ __forceinline__ void dma_product(typename MF<T>::acc_t (&acc)[BM / 2 / MF<T>::MT][BN / 2 / MF<T>::MT],
+                                            T* lds, const T* A, int64_t lda, int64_t M, int64_t m0, const T* B,
+                                            int64_t ldb, int64_t N, int64_t n0, int64_t kbeg, int64_t kend,
+                                            int fold_groups, bool take_colsum, double& csum) {
   using MFT = MF<T>;
   constexpr int BK = 64 / (int)sizeof(T);
   constexpr int MT = MFT::MT, VEC = MFT::VEC, LV = VEC == 4 ? 2 : 1;  // VEC = 1 << LV
@@ -542,34 +552,15 @@ __global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(
   constexpr int TM = WM / MT, TN = WN / MT, NCH = BK / kKC;
   constexpr int TILE_A = BM * BK, TILE_B = BN * BK;  // elements per operand tile
   constexpr int NST = kDmaStages<BM, BN>;
-  __shared__ __attribute__((aligned(1024))) T lds[NST * (TILE_A + TILE_B)];
-
-  int tm, tn;
-  tile_coords(a, tm, tn);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int split = blockIdx.y;
-  const int64_t batch = blockIdx.z;
-  const int64_t kbeg = (int64_t)split * a.k_per_split;
-  const int64_t kend = kbeg + a.k_per_split < a.K ? kbeg + a.k_per_split : a.K;
-  const T* A = (const T*)a.A + batch * a.sA;
-  const T* B = (const T*)a.B + batch * a.sB;
-
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane / MT, c = lane % MT;
   const int wm0 = (wave >> 1) * WM, wn0 = (wave & 1) * WN;
-
-  typename MFT::acc_t acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = typename MFT::acc_t(0);
-
   const int ntiles = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
   const int nfull = kend > kbeg ? (int)((kend - kbeg) / BK) : 0;
   DmaSrc<T, AKC, BM, VECA> sa;
   DmaSrc<T, BKC, BN, VECB> sb;
-  dma_init(sa, A, a.lda, m0, a.M, kbeg, wave, lane);
-  dma_init(sb, B, a.ldb, n0, a.N, kbeg, wave, lane);
+  dma_init(sa, A, lda, m0, M, kbeg, wave, lane);
+  dma_init(sb, B, ldb, n0, N, kbeg, wave, lane);
   auto tileA = [&](int st) { return lds + st * (TILE_A + TILE_B); };
   auto tileB = [&](int st) { return lds + st * (TILE_A + TILE_B) + TILE_A; };
   // LDS byte address of this wave's first A chunk and first B chunk in stage
@@ -601,8 +592,6 @@ __global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(
     }
     return v;
   };
-  const bool take_colsum = a.colsum != nullptr && tm == 0 && (int)threadIdx.x < BN;
-  double csum = 0.0;
   auto compute = [&](int st) {
     const T* As = tileA(st);
     const T* Bs = tileB(st);  // st is a constant in the main loop: immediate LDS offsets
@@ -674,7 +663,7 @@ __global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(
       if (st < NST - 1 && st < nfull) issue(stc);
     });
   }
-  // A long range without a K split is summed in pieces (a.fold_groups): a chain
+  // A long range without a K split is summed in pieces (fold_groups): a chain
   // of thousands of float32 additions would lose what the splits of the 128-wide
   // tiles keep. 32 vector instructions per 192 k beside 96 MFMAs, no difference
   // in time that could be measured (1186 and 1188 us a block at 5 x 499 x 768).
@@ -705,7 +694,7 @@ __global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(
       each_stage([&](auto stc) { step(stc, kt + decltype(stc)::value); });
     }
     if constexpr (FOLD)
-      if (++grp == a.fold_groups) {
+      if (++grp == fold_groups) {
         fold();
         grp = 0;
       }
@@ -725,17 +714,17 @@ __global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(
     TileRegs<T, BKC, BN> rb;
     if constexpr (VECA) {
       TilePtr<T, AKC, BM> pa;
-      init_ptr<T, AKC, BM>(pa, A, a.lda, m0, a.M, k0);
-      load_tail<T, AKC, BM>(ra, pa, a.lda, k0, kend);
+      init_ptr<T, AKC, BM>(pa, A, lda, m0, M, k0);
+      load_tail<T, AKC, BM>(ra, pa, lda, k0, kend);
     } else {
-      load_tile<T, AKC, BM>(ra, A, a.lda, m0, a.M, k0, kend);
+      load_tile<T, AKC, BM>(ra, A, lda, m0, M, k0, kend);
     }
     if constexpr (VECB) {
       TilePtr<T, BKC, BN> pb;
-      init_ptr<T, BKC, BN>(pb, B, a.ldb, n0, a.N, k0);
-      load_tail<T, BKC, BN>(rb, pb, a.ldb, k0, kend);
+      init_ptr<T, BKC, BN>(pb, B, ldb, n0, N, k0);
+      load_tail<T, BKC, BN>(rb, pb, ldb, k0, kend);
     } else {
-      load_tile<T, BKC, BN>(rb, B, a.ldb, n0, a.N, k0, kend);
+      load_tile<T, BKC, BN>(rb, B, ldb, n0, N, k0, kend);
     }
     __syncthreads();  // every wave is done with the stage being refilled
     dma_tail_store<T, AKC, BM>(tileA(st), ra, k0, kend);
@@ -744,11 +733,45 @@ __global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(
     compute(st);
   }
   if constexpr (FOLD)
-    if (a.fold_groups > 0)
+    if (fold_groups > 0)
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] += tot[i][j];
+}
+
+template <typename T, int BM, int BN, bool AKC, bool BKC, bool VECA, bool VECB>
+__global__ void __launch_bounds__(256, (BM + BN > 384 ? 1 : 2)) gemm_dma_kernel(GemmArgs a) {
+  using MFT = MF<T>;
+  constexpr int MT = MFT::MT;
+  constexpr int WM = BM / 2, WN = BN / 2;
+  constexpr int TM = WM / MT, TN = WN / MT;
+  __shared__ __attribute__((aligned(1024))) T lds[kDmaLds<T, BM, BN>];
+
+  int tm, tn;
+  tile_coords(a, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int split = blockIdx.y;
+  const int64_t batch = blockIdx.z;
+  const int64_t kbeg = (int64_t)split * a.k_per_split;
+  const int64_t kend = kbeg + a.k_per_split < a.K ? kbeg + a.k_per_split : a.K;
+  const T* A = (const T*)a.A + batch * a.sA;
+  const T* B = (const T*)a.B + batch * a.sB;
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane / MT, c = lane % MT;
+  const int wm0 = (wave >> 1) * WM, wn0 = (wave & 1) * WN;
+
+  typename MFT::acc_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = typename MFT::acc_t(0);
+
+  const bool take_colsum = a.colsum != nullptr && tm == 0 && (int)threadIdx.x < BN;
+  double csum = 0.0;
+  dma_product<T, BM, BN, AKC, BKC, VECA, VECB>(acc, lds, A, a.lda, a.M, m0, B, a.ldb, a.N, n0, kbeg, kend,
+                                               a.fold_groups, take_colsum, csum);
   if (take_colsum) finish_colsum<T>(a, csum, n0 + threadIdx.x, split);
   write_acc<T, TM, TN, true>(a, acc, m0 + wm0, n0 + wn0, g, c, split, batch);
 }
