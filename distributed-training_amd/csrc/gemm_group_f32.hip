@@ -1,0 +1,9 @@
+// float32 group and statistics kernels on 128 x 128 block tiles.
+#include "gemm_group_tiles.h"
+
+namespace dtmi {
+
+template void launch_group<float, 128>(const GroupArgs&, int, int, bool);
+template void launch_stats<float, 128>(const StatsArgs&, int, bool);
+
+}  // namespace dtmi

@@ -4,8 +4,9 @@ Mirrors dtrain/autograd.py: `Tensor(data, requires_grad, name)`, `.grad`,
 `.backward(grad=None)`, `.register_grad_ready_hook(fn)`, the operators
 `+ - * @`, `.sum .mean .reshape .transpose .gelu .relu`, and the functional ops
 `embedding`, `layer_norm`, `causal_attention`, `cross_entropy`, `no_grad`.
-Beside causal_attention, without a counterpart there: `causal_conv`, `ssm_scan`,
-`cross_attention` and the single-token `causal_conv_step`, `ssm_scan_step`.
+Without a counterpart there: beside causal_attention, `causal_conv`, `ssm_scan`,
+`cross_attention` and the single-token `causal_conv_step`, `ssm_scan_step`; beside
+cross_entropy and linear, `linear_cross_entropy` and `expert_linear`.
 
 Differences from dtrain are in where the numbers live, not in semantics:
 `.data` and `.grad` are DeviceArrays (HBM buffers owned by libdtmi; `.numpy()`
@@ -444,6 +445,113 @@ def cross_entropy(logits: Tensor, targets) -> Tensor:
             return (K.xent_grad_scale(pending.pop(), g1),)
         return (K.xent_bwd(z, t.dev, rmax, rsum, g=g1),)
     return Tensor._make(loss, (logits,), bw)
+
+
+# --------------------------------------------- products of a training step
+# Beside linear and cross_entropy. dtrain has no counterpart.
+def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None, ignore: int | None = None,
+                         reduction: str = "mean") -> Tensor:
+    """cross_entropy(x @ w + b, targets) without the logits: x [..., C], w [C, V] (a
+    transposed embedding table [V, C] is read as it lies), b [V], `targets` a host
+    integer array or an Indices of x's leading shape.
+
+    Rows whose target is `ignore` do not count: their loss and gradients are 0 and x is
+    not read there. `reduction` "mean" gives the mean over the others (0 if there are
+    none), "none" the loss of every row, which without gradients (`no_grad()`) is minus
+    the log probability of its target: no logit is written then. The gradients of a mean
+    are computed by the forward pass, as cross_entropy's are, from the logits of up to
+    2048 rows at a time; those of single losses by backward, which forms the logits
+    again."""
+    if reduction not in ("mean", "none"):
+        raise ValueError(f"linear_cross_entropy: reduction must be 'mean' or 'none', not {reduction!r}")
+    X = _contig(x.data)
+    if X.ndim < 1 or len(w.shape) != 2 or w.shape[0] != X.shape[-1] or w.shape[1] < 1:
+        raise ValueError(f"linear_cross_entropy: x {x.shape} and w {w.shape} do not match")
+    lead, (C, V) = X.shape[:-1], w.shape
+    K.same_dtype(X, w.data)
+    if b is not None and (b.shape != (V,) or b.dtype != X.dtype):
+        raise ValueError(f"linear_cross_entropy: b must be {X.dtype} of shape {(V,)}, not {b.dtype} {b.shape}")
+    tied = not w.data.is_contiguous and w.data.transpose(1, 0).is_contiguous
+    W = w.data.transpose(1, 0) if tied else _contig(w.data)
+    bd = _contig(b.data) if b is not None else None
+    ix = targets if isinstance(targets, Indices) else None
+    host = ix.host if ix is not None else np.asarray(targets)
+    if host.size and not np.issubdtype(host.dtype, np.integer):
+        raise TypeError("indices must be integers")
+    if host.shape != lead:
+        raise ValueError(f"linear_cross_entropy: targets of shape {host.shape} for x {x.shape}")
+    host = host.reshape(-1)
+    rows = host.size
+    X2 = X.reshape(rows, C)
+    keep = None if ignore is None else host != ignore
+    sel = None
+    if keep is not None and not keep.all():
+        # the rows that count, by themselves
+        sel = dev.from_numpy(np.flatnonzero(keep).astype(np.int64))
+        host = host[keep]
+        X2 = K.embedding_fwd(X2, sel, (host.size,))
+    if host.size and (host.min() < 0 or host.max() >= V):
+        raise IndexError(f"target out of bounds for size {V}")
+    t = ix.dev if ix is not None and sel is None else dev.from_numpy(host.astype(np.int64))
+    n = host.size
+    mean = reduction == "mean"
+    coef = 1.0 / n if mean and n else 1.0
+    need = [_grad_enabled and p is not None and p.requires_grad for p in (x, w, b)]
+    grads = dict(need_dx=need[0], need_dw=need[1], need_db=need[2])
+    ls, total, *made = K.linear_xent(X2, W, bd, t, tied, coef, losses=not mean, mean=mean,
+                                     **(grads if mean else {}))
+
+    def spread(d, cols):
+        return d if sel is None else K.scatter_rows(d.reshape(n, cols), sel, rows)
+    pending = [made] if mean and any(need) else []
+
+    def scaled(d, g, dest):
+        if dest is None or d.shape != dest.shape:
+            return K.xent_grad_scale(d, g)
+        return K.scale(d, alpha_dev=g, out=dest)
+
+    def bw(g):
+        if mean:
+            g1 = _contig(g).reshape(1)
+            dest = None if tied else grad_out(w), grad_out(b) if b is not None else None
+            if pending:
+                dx, dw, db = pending.pop()
+                dx = K.xent_grad_scale(dx, g1) if dx is not None else None
+                dw = scaled(dw, g1, dest[0]) if dw is not None else None
+                db = scaled(db, g1, dest[1]) if db is not None else None
+            else:
+                dx, dw, db = K.linear_xent(X2, W, bd, t, tied, coef, g=g1, **grads)[2:]
+        else:
+            g1 = _contig(g).reshape(rows)
+            if sel is not None:
+                g1 = K.embedding_fwd(g1.reshape(rows, 1), sel, (n,)).reshape(n)
+            dx, dw, db = K.linear_xent(X2, W, bd, t, tied, g=g1, **grads)[2:]
+        dx = spread(dx, C).reshape(x.shape) if dx is not None else None
+        dw = dw.transpose(1, 0) if dw is not None and tied else dw
+        return (dx, dw) if b is None else (dx, dw, db)
+    out = total if mean else spread(ls, 1).reshape(lead)
+    return Tensor._make(out, (x, w) if b is None else (x, w, b), bw)
+
+
+def expert_linear(x: Tensor, w: Tensor, sizes, b: Tensor | None = None) -> Tensor:
+    """Products of experts that each take some of the rows: x [R, K] sorted by expert, the
+    first sizes[0] rows expert 0's, the next sizes[1] expert 1's, ...; y = x @ w[e] +
+    b[e] with w [E, K, N], b [E, N]. `sizes`: one whole number for each expert (a host
+    array or an Indices), adding up to R at most. Rows past the last expert's give 0 and
+    get no gradient, and are not read; an expert may have none (embedding() gathers rows
+    by expert, with a gradient)."""
+    X, W = _contig(x.data), _contig(w.data)
+    if X.ndim != 2:
+        raise ValueError(f"expert_linear: x must be [rows, {w.shape[1] if len(w.shape) == 3 else 'K'}], not {x.shape}")
+    n = sizes.host if isinstance(sizes, Indices) else np.array(sizes)
+    y = K.expert_linear_fwd(X, W, n, _contig(b.data) if b is not None else None)
+
+    def bw(g):
+        dx, dw, db = K.expert_linear_bwd(X, W, _contig(g), n, x.requires_grad, w.requires_grad,
+                                         b is not None and b.requires_grad, dw_out=grad_out(w),
+                                         db_out=grad_out(b) if b is not None else None)
+        return (dx, dw) if b is None else (dx, dw, db)
+    return Tensor._make(y, (x, w) if b is None else (x, w, b), bw)
 
 
 # --------------------------------------------------------- sequence mixers

@@ -25,6 +25,11 @@ def _dt(*arrays: DeviceArray) -> int:
     return _lib.dtype_code(d)
 
 
+def same_dtype(*arrays: DeviceArray):
+    """Raises TypeError unless the arrays share one type that libdtmi computes in."""
+    _dt(*arrays)
+
+
 def _contig(*arrays: DeviceArray):
     for a in arrays:
         if not a.is_contiguous:
@@ -901,3 +906,147 @@ def xattn_bwd(q, k, v, o, dO, rowmax, rowsum, lengths=None, scale=None, dq=None,
        _bht_strides(v), _lengths_ptr(lengths, B), o.ptr, _bht_strides(o), dO.ptr, _bht_strides(dO), rowmax.ptr,
        rowsum.ptr, dq.ptr, _bht_strides(dq), dk.ptr, _bht_strides(dk), dv.ptr, _bht_strides(dv))
     return dq, dk, dv
+
+
+# --------------------------------------------- products of a training step
+def linear_xent(x2: DeviceArray, w: DeviceArray, b: DeviceArray | None, targets: DeviceArray, tied: bool = False,
+                coef: float = 1.0, losses: bool = False, mean: bool = False, g: DeviceArray | None = None,
+                need_dx: bool = False, need_dw: bool = False, need_db: bool = False):
+    """Cross entropy of x2 [R, C] @ w [C, V] (tied: w is [V, C]) + b against int64
+    targets [R], without the logits. Returns (losses [R], mean, dx, dw, db), None where
+    not asked for; the mean is coef times the sum of the losses, the gradients are coef
+    times those of the sum, times g ([R], or one element for all) where given."""
+    _contig(x2, w, targets)
+    if x2.ndim != 2 or w.ndim != 2 or w.shape[1 if tied else 0] != x2.shape[1]:
+        raise ValueError(f"linear_xent: x {x2.shape} and w {w.shape} do not match")
+    R, C_ = x2.shape
+    V = w.shape[0 if tied else 1]
+    if V < 1:
+        raise ValueError("linear_xent: a vocabulary of at least one")
+    d = _dt(x2, w)
+    if targets.dtype != np.int64 or targets.size != R:
+        raise ValueError("linear_xent: targets must be int64 with one entry per row")
+    if b is not None:
+        _same(b, (V,), x2.dtype, "linear_xent: b")
+    if g is not None:
+        _same(g, (g.size,), x2.dtype, "linear_xent: g")
+        if g.size not in (1, R):
+            raise ValueError(f"linear_xent: g must have one entry or {R}, not {g.size}")
+    ls = empty((R,), x2.dtype) if losses else None
+    mn = empty((), x2.dtype) if mean else None
+    dx = empty(x2.shape, x2.dtype) if need_dx else None
+    dw = empty(w.shape, x2.dtype) if need_dw else None
+    db = empty((V,), x2.dtype) if need_db else None
+    _c("dtmi_linear_xent", d, R, C_, V, x2.ptr, w.ptr, 1 if tied else 0, _opt_ptr(b), targets.ptr, _opt_ptr(ls),
+       _opt_ptr(mn), _opt_ptr(g), 1 if g is not None and g.size == R and R > 1 else 0, float(coef), _opt_ptr(dx),
+       _opt_ptr(dw), _opt_ptr(db))
+    return ls, mn, dx, dw, db
+
+
+def scatter_rows(x2: DeviceArray, rows: DeviceArray, total: int) -> DeviceArray:
+    """[total, C] of zeros with row rows[i] = x2[i]; rows int64, each once."""
+    _contig(x2, rows)
+    if rows.dtype != np.int64 or rows.size != x2.shape[0]:
+        raise ValueError("scatter_rows: rows must be int64 with one entry per row")
+    out = empty((int(total), x2.shape[1]), x2.dtype)
+    _c("dtmi_scatter_rows", _dt(x2), out.ptr, x2.ptr, rows.ptr, x2.shape[0], int(total), x2.shape[1])
+    return out
+
+
+def _expert_check(what, rows, w, sizes, K, N):
+    """E and the sizes as int64_t[]; sizes: host whole numbers, one per expert."""
+    if w.ndim != 3 or (K is not None and w.shape[1] != K) or (N is not None and w.shape[2] != N):
+        raise ValueError(f"{what}: w must be [experts, {K}, {N}], not {w.shape}")
+    sizes = np.asarray(sizes)
+    if sizes.shape != (w.shape[0],):
+        raise ValueError(f"{what}: sizes must have one entry for each of the {w.shape[0]} experts, not shape {sizes.shape}")
+    if sizes.size and not np.issubdtype(sizes.dtype, np.integer):
+        raise TypeError(f"{what}: sizes must be integers")
+    sizes = sizes.astype(np.int64)
+    if sizes.size and sizes.min() < 0:
+        raise ValueError(f"{what}: negative size")
+    if sum(sizes.tolist()) > rows:
+        raise ValueError(f"{what}: sizes add up to {sum(sizes.tolist())}, more than the {rows} rows")
+    return _lib.i64_array(sizes)
+
+
+def expert_linear_fwd(x: DeviceArray, w: DeviceArray, sizes, b: DeviceArray | None = None) -> DeviceArray:
+    """y [R, N] = x [R, K] @ w[e] (+ b[e]), the first sizes[0] rows with expert 0's, ..."""
+    d = _dt(x, w)
+    _contig(x, w)
+    R, K_ = x.shape
+    s = _expert_check("expert_linear", R, w, sizes, K_, None)
+    E, _, N = w.shape
+    if b is not None:
+        _same(b, (E, N), x.dtype, "expert_linear: b")
+    y = empty((R, N), x.dtype)
+    _c("dtmi_expert_linear_fwd", d, E, R, K_, N, y.ptr, x.ptr, w.ptr, _opt_ptr(b), s)
+    return y
+
+
+def expert_linear_bwd(x: DeviceArray, w: DeviceArray, g: DeviceArray, sizes, need_dx=True, need_dw=True,
+                      need_db=True, dw_out: DeviceArray | None = None, db_out: DeviceArray | None = None):
+    """Returns (dx, dw, db), None where not asked for."""
+    _contig(x, w, g)
+    R, K_ = x.shape
+    E, _, N = w.shape
+    s = _expert_check("expert_linear", R, w, sizes, K_, N)
+    _same(g, (R, N), x.dtype, "expert_linear: g")
+    d = _dt(x, w, g)
+    dx = dw = db = None
+    if need_dx:
+        dx = empty(x.shape, x.dtype)
+        _c("dtmi_expert_linear_bwd_dx", d, E, R, K_, N, dx.ptr, g.ptr, w.ptr, s)
+    if need_dw or need_db:
+        dw = _out_or_new(dw_out, w.shape, x.dtype, "expert_linear")
+        db = _out_or_new(db_out, (E, N), x.dtype, "expert_linear") if need_db else None
+        _c("dtmi_expert_linear_bwd_dw", d, E, R, K_, N, dw.ptr, _opt_ptr(db), x.ptr, g.ptr, s)
+    return dx, dw if need_dw else None, db
+
+
+class Matrices:
+    """Pointers and sizes of a list of matrices ([..., m, n] arrays, each one or a stack
+    of them) as the library takes them."""
+
+    def __init__(self, arrays, what: str):
+        self.arrays, self.rows, self.cols, self.per = list(arrays), [], [], []
+        for a in self.arrays:
+            if a.ndim < 2:
+                raise ValueError(f"{what}: matrices are needed, not an array of shape {a.shape}")
+            _contig(a)
+            m, n = a.shape[-2:]
+            k = a.size // (m * n) if m * n else 0
+            self.per.append(k)
+            self.rows += [m] * k
+            self.cols += [n] * k
+        self.n = len(self.rows)
+        self.dtype = _dt(*self.arrays) if self.arrays else 0
+        self.c_rows, self.c_cols = _lib.i64_array(self.rows), _lib.i64_array(self.cols)
+        self.c_ptrs = self.pointers(self.arrays)
+
+    def pointers(self, arrays):
+        """One pointer per matrix of arrays that are shaped as these."""
+        ptrs = []
+        for a, k in zip(arrays, self.per):
+            step = a.nbytes // k if k else 0
+            ptrs += [a.ptr + i * step for i in range(k)]
+        return _lib.ptr_array(ptrs)
+
+
+def newton_schulz(ins: Matrices, outs, steps: int, coefficients, eps: float):
+    a, b, c = (float(x) for x in coefficients)
+    _c("dtmi_newton_schulz", ins.dtype, ins.n, ins.pointers(outs), ins.c_ptrs, ins.c_rows, ins.c_cols, int(steps), a, b,
+       c, float(eps))
+
+
+def muon(ps: Matrices, gs, ms, rates, keep: float, momentum: float, nesterov: bool, steps: int, coefficients,
+         eps: float, gscale: float = 1.0, gscale_dev: DeviceArray | None = None):
+    """p = keep p - rates[i] NS(u), see dtmi_muon; gs, ms: arrays shaped as ps's."""
+    for p, g, m in zip(ps.arrays, gs, ms):
+        _same(g, p.shape, p.dtype, "muon: gradient")
+        _same(m, p.shape, p.dtype, "muon: momentum")
+    a, b, c = (float(x) for x in coefficients)
+    rate = (C.c_double * max(1, ps.n))(*[float(r) for r in rates])
+    _c("dtmi_muon", ps.dtype, ps.n, ps.c_ptrs, ps.pointers(gs), ps.pointers(ms), ps.c_rows, ps.c_cols, rate, float(keep),
+       float(momentum), 1 if nesterov else 0, int(steps), a, b, c, float(eps), float(gscale),
+       gscale_dev.ptr if gscale_dev is not None else None)

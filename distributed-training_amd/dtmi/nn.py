@@ -27,7 +27,8 @@ import numpy as np
 
 from . import device as dev
 from . import kernels as K
-from .autograd import Indices, Tensor, _contig, as_indices, cross_entropy, embedding, grad_out, layer_norm
+from .autograd import (Indices, Tensor, _contig, as_indices, cross_entropy, embedding, grad_out, layer_norm,
+                       linear_cross_entropy)
 
 
 class Module:
@@ -307,14 +308,22 @@ class GPT(Module):
             cache[T] = Indices(np.arange(T))
         return cache[T]
 
-    def forward(self, idx, targets=None):
-        """idx, targets: host integer arrays or Indices (uploaded once)."""
+    def hidden(self, idx) -> Tensor:
+        """What the vocabulary head reads, [B, T, dim]."""
         idx = as_indices(idx)
         B, T = idx.shape
         x = embedding(self.tok, idx) + embedding(self.pos, self._positions(T))
         for i, b in enumerate(self.blocks):
             x = b(x, next_ln=self.blocks[i + 1].ln1 if i + 1 < len(self.blocks) else self.ln)
-        logits = self.head(self.ln(x))
+        return self.ln(x)
+
+    def loss(self, idx, targets, ignore: int | None = None, reduction: str = "mean") -> Tensor:
+        """The loss alone, without the [B, T, vocab] logits (linear_cross_entropy)."""
+        return linear_cross_entropy(self.hidden(idx), self.head.w, targets, self.head.b, ignore, reduction)
+
+    def forward(self, idx, targets=None):
+        """idx, targets: host integer arrays or Indices (uploaded once)."""
+        logits = self.head(self.hidden(idx))
         if targets is None:
             return logits
         return logits, cross_entropy(logits, targets)

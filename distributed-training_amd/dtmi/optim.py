@@ -85,6 +85,78 @@ class AdamW:
             dst.assign(src)
 
 
+# ------------------------------------------------------ orthogonalised updates
+# Beside AdamW. dtrain has no counterpart.
+# a, b, c of a Newton-Schulz step: from 0 the polynomial grows as fast as one that keeps
+# singular values of up to 1 within about 0.7 .. 1.2 can
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(arrays, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7):
+    """Matrices with (nearly) the singular vectors they had and singular values near 1, by
+    `steps` Newton-Schulz steps: X = G / (|G| + eps) with the Frobenius norm, then
+    X = a X + (b A + c A A) X with A = X X^T (on the right, with X^T X, where G has more
+    rows than columns). `arrays`: a contiguous DeviceArray [..., m, n], every matrix of a
+    stack by itself, or a list of such; all of them share the launches. Returns new
+    arrays of the same shapes."""
+    one = isinstance(arrays, DeviceArray)
+    ins = K.Matrices([arrays] if one else arrays, "orthogonalize")
+    outs = [dev.empty(a.shape, a.dtype) for a in ins.arrays]
+    if ins.n:
+        K.newton_schulz(ins, outs, steps, coefficients, eps)
+    return outs[0] if one else outs
+
+
+class Muon:
+    """Momentum whose update is orthogonalised, for weight matrices: per step
+        m = momentum m + g,  u = g + momentum m (nesterov) or m
+        p = (1 - lr weight_decay) p - lr sqrt(max(1, n / k)) orthogonalize(u)
+    for p [..., k, n] (x @ p maps k inputs to n outputs; a stack [E, k, n] holds a matrix
+    for each expert). `params`: DeviceArrays, updated in place. Biases, LayerNorms,
+    embeddings and the vocabulary head are AdamW's."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+                 coefficients=NEWTON_SCHULZ, eps=1e-7):
+        self.params = list(params)
+        self.lr, self.momentum, self.nesterov, self.wd = lr, momentum, nesterov, weight_decay
+        self.steps, self.coefficients, self.eps = steps, tuple(coefficients), eps
+        self._all = K.Matrices(self.params, "Muon")
+        self._mflat = dev.zeros((max(sum(p.size for p in self.params), 1),),
+                                self.params[0].dtype if self.params else np.float32)
+        self.m, off = [], 0
+        for p in self.params:
+            self.m.append(self._mflat[off:off + p.size].reshape(p.shape))
+            off += p.size
+
+    def step(self, grads, grad_scale=1.0):
+        """grads: a DeviceArray or None (the parameter stays as it is) per parameter;
+        grad_scale as AdamW's."""
+        grads = [None if g is None else (g if g.is_contiguous else g.contiguous()) for g in grads]
+        if len(grads) != len(self.params):
+            raise ValueError(f"Muon: {len(grads)} gradients for {len(self.params)} parameters")
+        gs_dev = grad_scale if isinstance(grad_scale, DeviceArray) else None
+        ps, ms = self._all, self.m
+        if any(g is None for g in grads):
+            live = [i for i, g in enumerate(grads) if g is not None]
+            ps = K.Matrices([self.params[i] for i in live], "Muon")
+            ms, grads = [self.m[i] for i in live], [grads[i] for i in live]
+        if not ps.n:
+            return
+        rates = [self.lr * max(1.0, n / k) ** 0.5 for k, n in zip(ps.rows, ps.cols)]
+        K.muon(ps, grads, ms, rates, 1.0 - self.lr * self.wd, self.momentum, self.nesterov, self.steps,
+               self.coefficients, self.eps, 1.0 if gs_dev is not None else float(grad_scale), gs_dev)
+
+    def state_bytes(self):
+        return sum(a.nbytes for a in self.m)
+
+    def state_dict(self):
+        return {"m": [a.numpy() for a in self.m]}
+
+    def load_state_dict(self, s):
+        for dst, src in zip(self.m, s["m"]):
+            dst.assign(src)
+
+
 def clip_scale(total_sq_norm: float, max_norm: float) -> float:
     """dtrain/optim.py:49-52."""
     n = float(np.sqrt(total_sq_norm))

@@ -493,6 +493,54 @@ int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int6
                    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
                    const int64_t* dv_strides);
 
+/* --------------------------------------------- products of a training step
+ * Beside the GEMM; dtrain has no counterpart. float32 products here run on the float32
+ * MFMA, but for the gradient products of dtmi_linear_xent, which dtmi_set_gemm_math
+ * selects as it does for dtmi_gemm. Matrices are contiguous, results do not overlap
+ * operands, scratch memory comes from the pool. Deterministic.
+ *
+ * Softmax cross entropy of z = X W + b over a large vocabulary without the logits:
+ * X [R, C], W [C, V] (tied != 0: [V, C], an embedding table), b [V] or NULL, targets
+ * int64 [R] in 0..V-1. With m_r the largest z of a row and s_r = sum_v exp(z - m_r),
+ *   losses[r] = log s_r + (m_r - z[r, t_r])    mean = coef * sum_r losses[r]
+ *   dz[r, v] = coef * g[r g_stride] * (exp(z - m_r) / s_r - [v = t_r])  (g NULL: 1)
+ *   dX = dz W^T, dW = X^T dz (tied: its transpose [V, C]), db = sum_r dz
+ * losses, mean, dX, dW and db may be NULL. Without gradients no logit is written; with
+ * any, those of up to 2048 rows at a time are, in a pooled workspace (fewer rows where
+ * it cannot be allocated). R = 0: mean, dW and db are 0. C and V below 2^22. */
+int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, const void* X, const void* W, int tied,
+                     const void* b, const int64_t* targets, void* losses, void* mean, const void* g,
+                     int64_t g_stride, double coef, void* dX, void* dW, void* db);
+/* out [total, cols] = 0, then row rows[i] = in[i] for i < n (in [n, cols], rows int64 in
+ * device memory, each once; those outside 0..total-1 are left out). */
+int dtmi_scatter_rows(int dtype, void* out, const void* in, const int64_t* rows, int64_t n, int64_t total,
+                      int64_t cols);
+
+/* Products of E experts with ragged sizes: the first sizes[0] rows of x [R, K] belong to
+ * expert 0, the next sizes[1] to expert 1, ... (sizes: host memory, their sum at most R);
+ *   y = x w[e] + b[e],  dx = g w[e]^T,  dw[e] = x^T g,  db[e] = sum of g over its rows
+ * w [E, K, N], b [E, N] or NULL, y and g [R, N]. Rows of y and dx past the last expert's
+ * are 0, and not read of x and g; an expert without rows has dw and db of 0. */
+int dtmi_expert_linear_fwd(int dtype, int64_t E, int64_t R, int64_t K, int64_t N, void* y, const void* x,
+                           const void* w, const void* b, const int64_t* sizes);
+int dtmi_expert_linear_bwd_dx(int dtype, int64_t E, int64_t R, int64_t K, int64_t N, void* dx, const void* g,
+                              const void* w, const int64_t* sizes);
+int dtmi_expert_linear_bwd_dw(int dtype, int64_t E, int64_t R, int64_t K, int64_t N, void* dw, void* db,
+                              const void* x, const void* g, const int64_t* sizes);
+
+/* Newton-Schulz orthogonalisation of n matrices in[i] [rows[i], cols[i]] (arrays of
+ * pointers and sizes in host memory): X = in / (|in|_F + eps), then 1 to 64 `steps` of
+ *   G = X X^T, X = a X + (b G + c G G) X      (X^T X on the right where rows > cols)
+ * into out[i], which may be in[i]. The norm is summed in float64. */
+int dtmi_newton_schulz(int dtype, int n, void* const* out, const void* const* in, const int64_t* rows,
+                       const int64_t* cols, int steps, double a, double b, double c, double eps);
+/* One optimizer step of n matrices: m = momentum m + s g, u = s g + momentum m (nesterov
+ * != 0) or m, p = keep p - rate[i] X with X the above of u. s is *gscale_dev (a device
+ * double) or gscale where that is NULL. */
+int dtmi_muon(int dtype, int n, void* const* p, const void* const* g, void* const* m, const int64_t* rows,
+              const int64_t* cols, const double* rate, double keep, double momentum, int nesterov, int steps,
+              double a, double b, double c, double eps, double gscale, const double* gscale_dev);
+
 #ifdef __cplusplus
 }
 #endif
