@@ -24,80 +24,9 @@
 #include "common.h"
 #include "gemm_common.h"
 #include "gemm_direct.h"
+#include "gemm_direct_tile.h"
 
 namespace dtmi {
-
-// 16-byte vector at an element-aligned address
-template <typename T>
-struct UVec;
-template <>
-struct UVec<float> {
-  typedef MF<float>::vec_t __attribute__((aligned(4))) type;
-};
-template <>
-struct UVec<double> {
-  typedef MF<double>::vec_t __attribute__((aligned(8))) type;
-};
-
-// One operand's share of a wave: R MFMA tiles of MT rows (columns) along m/n by
-// KB of k per batch.
-template <typename T, bool KCONTIG, int R, int KB>
-struct DirectSrc {
-  static constexpr int MT = MF<T>::MT, VEC = MF<T>::VEC, NCH = KB / 8;
-  typedef typename MF<T>::vec_t VT;
-  const char* base;  // wave-uniform: the current batch's first k
-  unsigned off[R];   // this lane's byte offset from it
-  int64_t ldb;       // bytes between k-rows (m/n-contiguous)
-
-  __device__ __forceinline__ void init(const T* __restrict__ P, int64_t ld, int64_t mn0, int64_t MN, int64_t k0, int g,
-                                       int c) {
-    base = reinterpret_cast<const char*>(KCONTIG ? P + mn0 * ld + k0 : P + k0 * ld + mn0);
-    ldb = ld * (int64_t)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      int64_t r = mn0 + i * MT + c;
-      r = (r < MN ? r : MN - 1) - mn0;
-      off[i] = (unsigned)((KCONTIG ? r * ld + VEC * g : (int64_t)VEC * g * ld + r) * (int64_t)sizeof(T));
-    }
-  }
-  __device__ __forceinline__ void load(VT (&v)[R][NCH]) {
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) {
-        if constexpr (KCONTIG) {
-          v[i][ch] = *reinterpret_cast<const typename UVec<T>::type*>(base + off[i] + 8 * ch * sizeof(T));
-        } else {
-#pragma unroll
-          for (int s = 0; s < VEC; ++s) v[i][ch][s] = *reinterpret_cast<const T*>(base + (8 * ch + s) * ldb + off[i]);
-        }
-      }
-    base += KCONTIG ? (int64_t)KB * (int64_t)sizeof(T) : (int64_t)KB * ldb;
-  }
-  // the last `left` (< KB) values of k: element loads clamped to k = left - 1,
-  // zeros from `left` on
-  __device__ __forceinline__ void load_tail(VT (&v)[R][NCH], int left, int g) {
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int ch = 0; ch < NCH; ++ch)
-#pragma unroll
-        for (int s = 0; s < VEC; ++s) {
-          const int k = 8 * ch + VEC * g + s;
-          const int64_t kc = (k < left ? k : left - 1) - VEC * g;  // relative to this lane's offset
-          const T x = *reinterpret_cast<const T*>(base + (int64_t)off[i] + kc * (KCONTIG ? (int64_t)sizeof(T) : ldb));
-          v[i][ch][s] = k < left ? x : T(0);
-        }
-  }
-};
-
-template <typename T>
-struct DirectTile {
-  static constexpr int EDGE = 32;                      // block tile
-  static constexpr int R = EDGE / MF<T>::MT;           // MFMA tiles per edge
-  static constexpr int REGS = R * R * MF<T>::NACC;     // accumulators per lane
-  static constexpr int KB = kDirectBatch<T>;
-};
 
 template <typename T, bool AKC, bool BKC>
 __global__ void __launch_bounds__(64 * kDirectMaxWaves<T>) gemm_direct_kernel(GemmArgs a) {

@@ -15,15 +15,15 @@ namespace dtmi {
 
 constexpr int kGroupTasks = 64;  // 56 bytes each: the arguments stay below 4 KB
 
-// Row-major matrices without gaps: A is [M, K] or, where m is contiguous, [K, M]; B is
-// [K, N] or, where k is contiguous, [N, K]; C is [M, N].
+// Row-major matrices: A is [M, K] or, where m is contiguous, [K, M]; B is [K, N] or,
+// where k is contiguous, [N, K]; C is [M, N]. See GroupArgs for their rows' lengths.
 struct GroupTask {
   const void* A;
   const void* B;
   void* C;
   void* D;
   int M, N, K;
-  int tile0;  // the launch's first tile of this task
+  int turned;  // C is written transposed, [N, M]
   double s;
 };
 
@@ -31,19 +31,37 @@ struct GroupTask {
 // column sums of B over k go ([N], the bias gradient of dW = X^T dY).
 enum GroupD { kDNone = 0, kDMatrix = 1, kDRow = 2, kDColsum = 3 };
 
+// The order of the blocks. At a launch's start the dispatcher goes round the CUs, one
+// block each; later it fills whatever slots are free, two on one CU if need be, without
+// regard to how long they will take. So the longest go first, and the pieces of split tiles
+// among them by their length. Blocks are dealt to the 8 XCDs in turn; where all tasks have
+// one k (`equal`), each XCD gets neighbouring tiles, an eighth of the launch, and shares
+// their operands in its L2; where they differ that would give one XCD all of the longest
+// task (8 experts' dw 305 us), and tiles go round as they are numbered.
 struct GroupArgs {
-  int count, tiles, splits, dmode;
-  int sym;    // A B is symmetric (M = N): tiles on and below the diagonal, the others mirrored
-  void* ws;   // split-K partials, [splits][tiles][BM * BN] (NULL when not split)
-  void* csws; // and the column sums' [splits][count][N]
+  int count, tiles, equal;
+  // the first `cut` tiles are split in `splits` along k, their partials added by a second
+  // kernel; `before` blocks of whole tiles run before them
+  int cut, splits, before;
+  // blocks turn .. turned - 1 in reverse (none: both 0): with one round and some of the
+  // next, the shortest then come to lie beside the longest
+  int turn, turned;
+  int dmode;
+  int sym;        // A B is symmetric (M = N): tiles on and below the diagonal, the others mirrored
+  // A, B and D have both dimensions rounded up to `pad`, with zeros there; C to padc, and
+  // the zeros are written where padc = pad. 1: matrices without gaps.
+  int pad, padc;
+  void* ws;       // [splits][cut][BM * BM] partials
+  void* csws;     // and the column sums' [splits][cut][BM]
   double alpha, beta, gamma;
+  int first[kGroupTasks];  // each task's first tile
   GroupTask t[kGroupTasks];
 };
 
 // Row statistics of Z = A B + bias over pieces of its columns, without Z (or with it,
-// where C is not NULL): part p of row m covers half a block tile's columns, pmax[p M +
-// m] is their maximum and psum[p M + m] the sum of exp(z - pmax) over them; zt[m] = Z[m,
-// targets[m]].
+// where C is not NULL): part p of row m covers some columns (half a block tile's), pmax[p
+// M + m] is their maximum and psum[p M + m] the sum of exp(z - pmax) over them; zt[m] =
+// Z[m, targets[m]]. Columns N .. nz - 1 of C are set to -inf.
 struct StatsArgs {
   const void* A;
   const void* B;
@@ -53,32 +71,36 @@ struct StatsArgs {
   void* psum;
   void* zt;
   const int64_t* targets;
-  int64_t M, N, K, lda, ldb, ldc;
+  int64_t M, N, K, lda, ldb, ldc, nz;
   int tiles_m, tiles_n;
 };
 
-// Block tile of a launch over these tasks (64 or 128) and its k splits, by the
-// estimate that gemm.hip makes of a single product.
-struct GroupPlan {
-  int tile, splits;
-};
-
-// gemm_group_f32.hip, gemm_group_f64.hip: one tile and type each
+// gemm_group_f32.hip, ...: one tile and type each; BM = 32: operands straight to
+// registers, k over the `nw` waves of a block (gemm_direct.hip)
 template <typename T, int BM>
 void launch_group(const GroupArgs& a, int akc, int bkc, bool vec);
 template <typename T, int BM>
 void launch_stats(const StatsArgs& a, int bkc, bool vec);
+template <typename T>
+void launch_group_direct(const GroupArgs& a, int akc, int bkc, int nw);
+template <typename T>
+void launch_stats_direct(const StatsArgs& a, int bkc, int nw);
+// tiles of 16 mr rows (gemm_rows.h), A k-contiguous
+template <typename T>
+void launch_group_rows(const GroupArgs& a, int bkc, int mr, int nw);
+template <typename T>
+void launch_stats_rows(const StatsArgs& a, int bkc, int mr, int nw);
 
-// The tasks (their tile0 unset) as one launch per 64 of them, with the sum pass of a
-// split. akc, bkc: which operands are k-contiguous (1, 0), (1, 1) or (0, 0).
+// Runs the tasks, longest k first, 64 to a launch. akc, bkc: which
+// operands are k-contiguous: (1, 0), (1, 1) or (0, 0).
 int run_group(int dtype, int akc, int bkc, GroupTask* tasks, int count, int dmode, int sym, double alpha, double beta,
-              double gamma);
+              double gamma, int pad = 1, int padc = 1);
 // The parts a row's statistics come in.
-int64_t stats_parts(int dtype, int64_t M, int64_t N, int64_t K);
+int64_t stats_parts(int dtype, int bkc, int64_t M, int64_t N, int64_t K);
 int run_stats(int dtype, int bkc, StatsArgs a);
 
 // Leading dimensions the tile kernels address (their byte offsets are 32 bits wide).
 template <typename T>
-constexpr int64_t kTileMaxLd = (1 << 24) / (int64_t)sizeof(T) - 1;
+constexpr int64_t kTileMaxLd = (1 << 24) / (int64_t)sizeof(T) - 4;
 
 }  // namespace dtmi

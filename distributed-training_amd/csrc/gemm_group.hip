@@ -1,62 +1,156 @@
 // Plans and launches of the group and statistics products (gemm_group.h).
 #include "gemm_group.h"
 
+#include <algorithm>
+
+#include "gemm_direct.h"
+#include "gemm_rows.h"
+
 namespace dtmi {
 
-// SIMD cycles of a launch, as tile_cost in gemm.hip (the same constants): rounds of
-// blocks x k x the MFMA time of a tile over the rate it reaches, the longest task's
-// own chain at least, and a split's partials and second launch.
-static double group_cost(const GroupTask* t, int count, int sym, int bm, int splits, int64_t cus, size_t es) {
-  const int64_t bk = 64 / (int64_t)es;
-  double work = 0, chain = 0;
-  int64_t tiles = 0;
-  for (int i = 0; i < count; ++i) {
-    const int64_t tm = cdiv(t[i].M, bm), tn = cdiv(t[i].N, bm), n = sym ? tm * (tm + 1) / 2 : tm * tn;
-    const double k = (double)(cdiv(cdiv(t[i].K, splits), bk) * bk);
-    tiles += n;
-    work += (double)n * k;
-    if (n && k > chain) chain = k;
-  }
-  if (!tiles) return 0;
-  const int64_t blocks = tiles * splits;
-  const double rounds = (double)cdiv(blocks, cus);
-  const double eff = bm == 64 ? (rounds > 1 ? 0.88 : 0.75) : rounds > 2 ? 0.97 : rounds > 1 ? 1.0 : 0.82;
-  const double per_k = (es == 4 ? 32.0 : 64.0) * (bm / 32) * (bm / 32) / 4.0;  // four waves
-  const double k = rounds * work / (double)tiles;
-  double c = 8800.0 + (k > chain ? k : chain) * per_k / eff;
-  if (splits > 1) c += 6600.0 + (double)tiles * bm * bm * (double)es * (splits + 1) / 2700.0;
-  return c;
+// Block tile (32: the small-product kernels, of nw waves), and how many tiles of a launch
+// are split along k (kAll: all).
+constexpr int kAll = 1 << 30;
+struct GroupPlan {
+  int tile, cut, splits, nw;
+};
+
+// Few rows: gemm_rows.h, up to 32 (the tile is then 16 or 32 rows).
+constexpr int kFewRows = 32;
+
+// Waves of a block of few rows: 16 per CU, each with at least a batch of k, and their
+// partial tiles within 64 KB.
+template <typename T>
+static int rows_waves(int64_t blocks, int64_t K, int64_t cus, int mr, int bkc) {
+  const int64_t bytes = 4 * mr * (bkc ? RowsTile<T, true>::NT : RowsTile<T, false>::NT) * 64 * (int64_t)sizeof(T);
+  int64_t w = 1;
+  while (w < kRowsMaxWaves && blocks * w < 16 * cus && 2 * w * bytes <= 64 * 1024) w *= 2;
+  const int64_t batches = cdiv(K > 0 ? K : 1, RowsTile<T, true>::BATCH);
+  return (int)(w < batches ? w : batches);
 }
 
-// The float32 sums of a 128-wide tile are one chain over its k range (64-wide tiles
-// fold theirs): at most 4096 k.
-static GroupPlan plan_group(const GroupTask* t, int count, int sym, int64_t cus, size_t es) {
-  int kmax = 0;
-  for (int i = 0; i < count; ++i) kmax = t[i].K > kmax ? t[i].K : kmax;
-  GroupPlan best{64, 1};
+// Waves of a small-product block: 16 per CU, each with at least a batch of k.
+template <typename T>
+static int direct_waves(int64_t tiles, int64_t K, int64_t cus) {
+  int64_t w = 4;
+  while (w < kDirectMaxWaves<T> && tiles * w < 16 * cus) w *= 2;
+  const int64_t batches = cdiv(K > 0 ? K : 1, kDirectBatch<T>);
+  return (int)(w < batches ? w : batches);
+}
+
+// SIMD cycles of a small-product launch: as direct_cost in gemm.hip.
+template <typename T>
+static double direct_cycles(int64_t tiles, double kavg, int64_t kmax, int nw, int64_t cus) {
+  const double kps = (double)(cdiv(cdiv(kmax, nw), kDirectBatch<T>) * kDirectBatch<T>);
+  const double rate = (double)cdiv(tiles, cus) * kavg * (sizeof(T) == 4 ? 8.0 / 0.45 : 16.0 / 0.55);
+  const double chain = 3500.0 + 1.35 * (sizeof(T) == 4 ? 32.0 : 64.0) * kps;
+  return 7700.0 + (rate > chain ? rate : chain);
+}
+
+// SIMD cycles of `units` blocks on BM-wide tiles, the busiest CU's k being `k`: as
+// tile_cost in gemm.hip (64-wide float32 tiles over several tasks reach less, 0.80 to
+// 0.89 of their MFMA rate).
+static double tile_cycles(int bm, double k, double units, int64_t cus, size_t es) {
+  const double eff = bm == 64 ? (units > cus ? (es == 4 ? 0.82 : 0.88) : 0.75) : units > 2.0 * cus ? 0.97 : units > cus ? 1.0 : 0.82;
+  return 8800.0 + k * (es == 4 ? 32.0 : 64.0) * (bm / 32) * (bm / 32) / 4.0 / eff;
+}
+// and what a split adds: its partials' traffic and a launch
+static double split_cycles(int bm, int64_t cut, int splits, size_t es) {
+  return splits > 1 ? 6600.0 + (double)cut * bm * bm * (double)es * (splits + 1) / 2700.0 : 0.0;
+}
+
+// How to run the tasks (longest k first). Blocks are dealt out as slots come free, so a
+// ragged last round, or a task that outlasts the others, leaves CUs idle:
+// - equal k: all tiles split (few tiles), or only as many as make the rest a whole
+//   number of rounds;
+// - unequal k: the tiles of the longest tasks split.
+template <typename T>
+static GroupPlan plan_group(const GroupTask* t, int count, int sym, int pad, int64_t cus) {
+  constexpr size_t es = sizeof(T);
+  constexpr int64_t bk = 64 / (int64_t)es;
+  int64_t k[kGroupTasks];
+  for (int i = 0; i < count; ++i) k[i] = cdiv(cdiv(t[i].K, pad) * pad, bk) * bk;
+  GroupPlan best{64, 0, 1, 0};
   double least = -1;
-  for (int bm = 64; bm <= 128; bm += 64)
-    for (int sp = 1; sp <= 16 && (sp == 1 || kmax / sp >= 128); ++sp) {
-      if (bm == 128 && es == 4 && kmax / sp > 4096 && sp < 16) continue;
-      const double c = group_cost(t, count, sym, bm, sp, cus, es);
-      if (least < 0 || c < least) {
-        least = c;
-        best = {bm, sp};
+  auto take = [&](double c, GroupPlan p) {
+    if (least < 0 || c < least) {
+      least = c;
+      best = p;
+    }
+  };
+  auto tiles_of = [&](int i, int bm) {
+    const int64_t tm = cdiv(t[i].M, bm), tn = cdiv(t[i].N, bm);
+    return sym ? tm * (tm + 1) / 2 : tm * tn;
+  };
+  for (int bm = 64; bm <= 128; bm += 64) {
+    int64_t n[kGroupTasks], total = 0;
+    double work = 0;
+    int last = 0;
+    for (int i = 0; i < count; ++i) {
+      n[i] = tiles_of(i, bm);
+      total += n[i];
+      work += (double)n[i] * (double)k[i];
+      if (n[i]) last = i;
+    }
+    if (!total) return best;
+    const bool equal = k[0] == k[last];
+    // one chain of float32 sums: at most 4096 k on 128-wide tiles (64-wide ones fold theirs)
+    const int64_t chain = bm == 128 && es == 4 ? 4096 : 1LL << 40;
+    const double even = work / (double)cus;
+    if (k[0] <= chain) {
+      const double busy = equal ? (double)cdiv(total, cus) * (double)k[0]
+                                : std::max((double)k[0], even + 0.5 * (double)k[last]);
+      take(tile_cycles(bm, busy, (double)total, cus, es), {bm, 0, 1, 0});
+    }
+    const int64_t rest = equal && total > cus ? total % cus : 0;
+    for (int sp = 2; sp <= 16 && k[0] / sp >= 128; ++sp) {
+      const double ks = (double)(cdiv(cdiv(k[0], sp), bk) * bk);
+      if (ks <= (double)chain || sp == 16) {
+        const double busy = equal ? (double)cdiv(total * sp, cus) * ks : std::max(ks, even + 0.5 * (double)k[last] / sp);
+        take(tile_cycles(bm, busy, (double)(total * sp), cus, es) + split_cycles(bm, total, sp, es), {bm, kAll, sp, 0});
+      }
+      if (rest && k[0] <= chain) {
+        // the last whole tiles run beside fewer and fewer pieces
+        const double busy = ((double)(total / cus) * (double)k[0] + (double)cdiv(rest * sp, cus) * ks) / 0.9;
+        take(tile_cycles(bm, busy, (double)(total + rest * (sp - 1)), cus, es) + split_cycles(bm, rest, sp, es),
+             {bm, (int)rest, sp, 0});
+      }
+      if (!equal && (sp <= 4 || sp % 4 == 0)) {
+        int64_t cut = 0;
+        for (int i = 0; i < last && i < 16; ++i) {
+          cut += n[i];
+          if (k[i] == k[i + 1] || !cut || k[i + 1] > chain || ks > (double)chain) continue;
+          const double busy = std::max(std::max(ks, (double)k[i + 1]), even + 0.5 * (double)k[last]);
+          take(tile_cycles(bm, busy, (double)(total + cut * (sp - 1)), cus, es) + split_cycles(bm, cut, sp, es),
+               {bm, (int)cut, sp, 0});
+        }
       }
     }
+  }
+  int64_t tiles = 0;
+  double work = 0;
+  for (int i = 0; i < count; ++i) {
+    tiles += tiles_of(i, 32);
+    work += (double)tiles_of(i, 32) * (double)k[i];
+  }
+  const int nw = direct_waves<T>(tiles, k[0], cus);
+  take(direct_cycles<T>(tiles, work / (double)tiles, k[0], nw, cus), {32, 0, 1, nw});
   return best;
 }
 
 template <typename T>
 static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmode, int sym, double alpha, double beta,
-                          double gamma) {
+                          double gamma, int pad, int padc) {
   constexpr int V = MF<T>::VEC;
   const int64_t cus = num_cus() > 0 ? num_cus() : 256;
+  std::stable_sort(tasks, tasks + count, [](const GroupTask& x, const GroupTask& y) { return x.K > y.K; });
   for (int lo = 0; lo < count; lo += kGroupTasks) {
     GroupArgs a{};
     a.count = count - lo < kGroupTasks ? count - lo : kGroupTasks;
     a.dmode = dmode;
     a.sym = sym;
+    a.pad = pad;
+    a.padc = padc;
     a.alpha = alpha;
     a.beta = beta;
     a.gamma = gamma;
@@ -65,36 +159,70 @@ static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmo
     for (int i = 0; i < a.count; ++i) {
       GroupTask& t = a.t[i];
       t = tasks[lo + i];
-      const int64_t lda = akc ? t.K : t.M, ldb = bkc ? t.K : t.N;
+      const int64_t lda = cdiv(akc ? t.K : t.M, pad) * pad, ldb = cdiv(bkc ? t.K : t.N, pad) * pad;
       DTMI_CHECK(lda <= kTileMaxLd<T> && ldb <= kTileMaxLd<T> && t.N <= kTileMaxLd<T>,
                  "group of products: rows of 2^24 bytes or more are not supported");
       vec = vec && lda % V == 0 && ldb % V == 0 && aligned(t.A, 16) && aligned(t.B, 16) &&
-            (!sym || (t.N % V == 0 && aligned(t.C, 16)));
+            (!sym || (cdiv(t.N, padc) * padc % V == 0 && aligned(t.C, 16)));
       flops += (sym ? 1.0 : 2.0) * (double)t.M * t.N * t.K;
     }
-    const GroupPlan p = plan_group(a.t, a.count, sym, cus, sizeof(T));
+    int rows = 0;
+    for (int i = 0; i < a.count; ++i) rows = a.t[i].M > rows ? a.t[i].M : rows;
+    if (rows <= kFewRows && akc && !sym && pad == 1 && dmode != kDColsum) {
+      const int mr = rows <= 16 ? 1 : 2, cols = bkc ? RowsTile<T, true>::COLS : RowsTile<T, false>::COLS;
+      int64_t tiles = 0, kmax = 0;
+      for (int i = 0; i < a.count; ++i) {
+        a.first[i] = (int)tiles;
+        tiles += cdiv(a.t[i].M, 16 * mr) * cdiv(a.t[i].N, cols);
+        kmax = a.t[i].K > kmax ? a.t[i].K : kmax;
+      }
+      if (!tiles) continue;
+      a.tiles = (int)tiles;
+      TimedLaunch tl(DTMI_FAM_GEMM, flops);
+      launch_group_rows<T>(a, bkc, mr, rows_waves<T>(tiles, kmax, cus, mr, bkc));
+      LAUNCH_CHECK("group_rows_kernel");
+      continue;
+    }
+    const GroupPlan p = plan_group<T>(a.t, a.count, sym, pad, cus);
+    a.equal = 1;
+    for (int i = 1; i < a.count; ++i) a.equal = a.equal && a.t[i].K == a.t[0].K;
     int64_t tiles = 0;
     for (int i = 0; i < a.count; ++i) {
       const int64_t tm = cdiv(a.t[i].M, p.tile), tn = cdiv(a.t[i].N, p.tile);
-      a.t[i].tile0 = (int)tiles;
+      a.first[i] = (int)tiles;
       tiles += sym ? tm * (tm + 1) / 2 : tm * tn;
-      DTMI_CHECK(tiles < (1LL << 30), "group of products: too large");
+      DTMI_CHECK(tiles < (1LL << 26), "group of products: too large");
     }
     if (!tiles) continue;
     a.tiles = (int)tiles;
+    a.cut = p.cut < a.tiles ? p.cut : a.tiles;
     a.splits = p.splits;
+    for (int i = 0; i < a.count && a.cut; ++i) {  // whole tiles that are longer than the pieces
+      const int end = i + 1 < a.count ? a.first[i + 1] : a.tiles;
+      if (end > a.cut && a.t[i].K >= cdiv(a.t[0].K, p.splits)) a.before = end - a.cut;
+    }
+    if (!a.equal && p.tile == 128) {  // the blocks that have something to do, longest first
+      int64_t units = a.tiles + (int64_t)a.cut * (p.splits - 1);
+      for (int i = a.count - 1; i >= 0 && a.t[i].K == 0; --i)
+        units -= (i + 1 < a.count ? a.first[i + 1] : a.tiles) - a.first[i];
+      if (units > cus && units <= 2 * cus) {
+        a.turn = (int)cus;
+        a.turned = (int)units;
+      }
+    }
     void* ws = nullptr;
-    if (p.splits > 1) {
-      const size_t main_bytes = (size_t)p.splits * tiles * p.tile * p.tile * sizeof(T);
-      const size_t cs_bytes = dmode == kDColsum ? (size_t)p.splits * a.count * a.t[0].N * sizeof(T) : 0;
-      int rc = pool_alloc(&ws, main_bytes + cs_bytes);
+    if (a.cut) {
+      const size_t slots = (size_t)p.splits * a.cut, main_bytes = slots * p.tile * p.tile * sizeof(T);
+      int rc = pool_alloc(&ws, main_bytes + slots * p.tile * sizeof(T));
       if (rc) return rc;
       a.ws = ws;
-      if (cs_bytes) a.csws = (char*)ws + main_bytes;
+      a.csws = (char*)ws + main_bytes;
     }
     {
       TimedLaunch tl(DTMI_FAM_GEMM, flops);
-      if (p.tile == 64)
+      if (p.tile == 32)
+        launch_group_direct<T>(a, akc, bkc, p.nw);
+      else if (p.tile == 64)
         launch_group<T, 64>(a, akc, bkc, vec);
       else
         launch_group<T, 128>(a, akc, bkc, vec);
@@ -107,47 +235,77 @@ static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmo
 }
 
 int run_group(int dtype, int akc, int bkc, GroupTask* tasks, int count, int dmode, int sym, double alpha, double beta,
-              double gamma) {
-  if (dtype == DTMI_F32) return group_launches<float>(akc, bkc, tasks, count, dmode, sym, alpha, beta, gamma);
-  return group_launches<double>(akc, bkc, tasks, count, dmode, sym, alpha, beta, gamma);
+              double gamma, int pad, int padc) {
+  if (dtype == DTMI_F32)
+    return group_launches<float>(akc, bkc, tasks, count, dmode, sym, alpha, beta, gamma, pad, padc);
+  return group_launches<double>(akc, bkc, tasks, count, dmode, sym, alpha, beta, gamma, pad, padc);
 }
 
-static int stats_tile(int dtype, int64_t M, int64_t N, int64_t K) {
-  GroupTask t{};
-  t.M = (int)M;
-  t.N = (int)N;
-  t.K = (int)K;
+// Tile and waves of a statistics product (tile 16: few rows).
+template <typename T>
+static GroupPlan plan_stats(int bkc, int64_t M, int64_t N, int64_t K) {
   const int64_t cus = num_cus() > 0 ? num_cus() : 256;
-  const size_t es = dtype == DTMI_F32 ? 4 : 8;
-  return group_cost(&t, 1, 0, 64, 1, cus, es) < group_cost(&t, 1, 0, 128, 1, cus, es) ? 64 : 128;
+  if (M <= kFewRows) {
+    const int64_t blocks = cdiv(N, bkc ? RowsTile<T, true>::COLS : RowsTile<T, false>::COLS);
+    return {16, 0, 1, rows_waves<T>(blocks, K, cus, M <= 16 ? 1 : 2, bkc)};
+  }
+  constexpr int64_t bk = 64 / (int64_t)sizeof(T);
+  const double k = (double)(cdiv(K, bk) * bk);
+  const int64_t t32 = cdiv(M, 32) * cdiv(N, 32);
+  GroupPlan best{32, 0, 1, direct_waves<T>(t32, K, cus)};
+  double least = direct_cycles<T>(t32, (double)K, K, best.nw, cus);
+  for (int bm = 64; bm <= 128; bm += 64) {
+    const int64_t n = cdiv(M, bm) * cdiv(N, bm);
+    const double c = tile_cycles(bm, (double)cdiv(n, cus) * k, (double)n, cus, sizeof(T));
+    if (c < least) {
+      least = c;
+      best = {bm, 0, 1, 0};
+    }
+  }
+  return best;
 }
-
-int64_t stats_parts(int dtype, int64_t M, int64_t N, int64_t K) { return 2 * cdiv(N, stats_tile(dtype, M, N, K)); }
 
 template <typename T>
-static int stats_launch(int dtype, int bkc, StatsArgs& a) {
+static int64_t parts_of(const GroupPlan& p, int bkc, int64_t N) {
+  if (p.tile == 16) return cdiv(N, bkc ? RowsTile<T, true>::COLS : RowsTile<T, false>::COLS);
+  // a wave's columns: MFMA tiles of 32, or half a block tile
+  return p.tile == 32 ? cdiv(N, 32) * (32 / MF<T>::MT) : 2 * cdiv(N, p.tile);
+}
+
+int64_t stats_parts(int dtype, int bkc, int64_t M, int64_t N, int64_t K) {
+  return dtype == DTMI_F32 ? parts_of<float>(plan_stats<float>(bkc, M, N, K), bkc, N)
+                           : parts_of<double>(plan_stats<double>(bkc, M, N, K), bkc, N);
+}
+
+template <typename T>
+static int stats_launch(int bkc, StatsArgs& a) {
   constexpr int V = MF<T>::VEC;
   DTMI_CHECK(a.lda <= kTileMaxLd<T> && a.ldb <= kTileMaxLd<T> && a.ldc <= kTileMaxLd<T>,
              "statistics product: rows of 2^24 bytes or more are not supported");
+  const GroupPlan p = plan_stats<T>(bkc, a.M, a.N, a.K);
   const bool vec = aligned(a.A, 16) && aligned(a.B, 16) && a.lda % V == 0 && a.ldb % V == 0 && a.K % V == 0 &&
                    (bkc || a.N % V == 0);
-  const int tile = stats_tile(dtype, a.M, a.N, a.K);
-  DTMI_CHECK(cdiv(a.M, tile) * cdiv(a.N, tile) < (1LL << 30), "statistics product: too large");
-  a.tiles_m = (int)cdiv(a.M, tile);
-  a.tiles_n = (int)cdiv(a.N, tile);
+  DTMI_CHECK(cdiv(a.M, p.tile) * cdiv(a.N, p.tile) < (1LL << 30), "statistics product: too large");
+  const int mr = a.M <= 16 ? 1 : 2;
+  a.tiles_m = p.tile == 16 ? 1 : (int)cdiv(a.M, p.tile);
+  a.tiles_n = (int)(p.tile == 16 ? parts_of<T>(p, bkc, a.N) : cdiv(a.N, p.tile));
   {
     TimedLaunch tl(DTMI_FAM_GEMM, 2.0 * (double)a.M * a.N * a.K);
-    if (tile == 64)
+    if (p.tile == 16)
+      launch_stats_rows<T>(a, bkc, mr, p.nw);
+    else if (p.tile == 32)
+      launch_stats_direct<T>(a, bkc, p.nw);
+    else if (p.tile == 64)
       launch_stats<T, 64>(a, bkc, vec);
     else
       launch_stats<T, 128>(a, bkc, vec);
   }
-  LAUNCH_CHECK("gemm_stats_kernel");
+  LAUNCH_CHECK("statistics kernels");
   return DTMI_OK;
 }
 
 int run_stats(int dtype, int bkc, StatsArgs a) {
-  return dtype == DTMI_F32 ? stats_launch<float>(dtype, bkc, a) : stats_launch<double>(dtype, bkc, a);
+  return dtype == DTMI_F32 ? stats_launch<float>(bkc, a) : stats_launch<double>(bkc, a);
 }
 
 }  // namespace dtmi

@@ -26,59 +26,64 @@ __device__ __forceinline__ T exp_e(T x) {
   return exp(x);
 }
 
-// A row's statistics from its parts: 32 rows a block, 32 lanes of a half-wave on
-// consecutive rows, the parts dealt to 32 groups that are joined through LDS. The
-// parts' order is fixed.
 template <typename T>
+struct RowStat {
+  T m = -INFINITY, s = T(0);
+  // NaN: dropped by the maximum, kept by the sum; parts of -inf alone have sum 0
+  __device__ __forceinline__ void add(T m2, T s2) {
+    const T top = fmax(m, m2), ref = top == -INFINITY ? T(0) : top;
+    s = s * exp_e<T>(m - ref) + s2 * exp_e<T>(m2 - ref);
+    m = top;
+  }
+};
+
+// A row's statistics from its parts, joined in a fixed order: ROWS rows a block, on
+// consecutive lanes, the parts dealt to 1024 / ROWS groups that are joined through LDS.
+// 32 rows read whole lines of the parts; with few rows one a block is quicker, as no lane
+// then walks more than a few parts (5 rows of 1572 parts: 9 us with 32 rows a block).
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(1024) lxent_join_kernel(const T* __restrict__ pmax, const T* __restrict__ psum,
                                                           int64_t parts, int64_t M, const T* __restrict__ zt,
                                                           T* __restrict__ rmax, T* __restrict__ rsum,
                                                           T* __restrict__ losses) {
-  __shared__ T sm[32][33], ss[32][33];
-  const int r = threadIdx.x & 31, grp = threadIdx.x >> 5;
-  const int64_t m = (int64_t)blockIdx.x * 32 + r;
-  T mx = -INFINITY, s = T(0);
+  constexpr int GROUPS = 1024 / ROWS, U = ROWS == 1 ? 2 : 8;
+  __shared__ T sm[GROUPS][ROWS + 1], ss[GROUPS][ROWS + 1];
+  const int r = threadIdx.x % ROWS, grp = threadIdx.x / ROWS;
+  const int64_t m = (int64_t)blockIdx.x * ROWS + r;
+  RowStat<T> x;
   if (m < M) {
-    for (int64_t p0 = grp; p0 < parts; p0 += 32 * 8) {
-      T a[8], b[8];
+    for (int64_t p0 = grp; p0 < parts; p0 += GROUPS * U) {
+      T a[U], b[U];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int64_t p = p0 + 32 * u;
+      for (int u = 0; u < U; ++u) {
+        const int64_t p = p0 + GROUPS * u;
         const int64_t at = (p < parts ? p : p0) * M + m;
         a[u] = pmax[at];
         b[u] = p < parts ? psum[at] : T(0);
       }
-      T top = mx;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) top = fmax(top, a[u]);
-      const T ref = top == -INFINITY ? T(0) : top;
-      s = s * exp_e<T>(mx - ref);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) s += b[u] * exp_e<T>(a[u] - ref);
-      mx = top;
+      for (int u = 0; u < U; ++u) x.add(a[u], b[u]);
     }
   }
-  sm[grp][r] = mx;
-  ss[grp][r] = s;
+  sm[grp][r] = x.m;
+  ss[grp][r] = x.s;
   __syncthreads();
-  for (int half = 16; half >= 1; half >>= 1) {
+#pragma unroll
+  for (int half = GROUPS / 2; half >= 1; half >>= 1) {
     if (grp < half) {
-      const T a = sm[grp][r], b = sm[grp + half][r];
-      const T top = fmax(a, b), ref = top == -INFINITY ? T(0) : top;
-      ss[grp][r] = ss[grp][r] * exp_e<T>(a - ref) + ss[grp + half][r] * exp_e<T>(b - ref);
-      sm[grp][r] = top;
+      x.add(sm[grp + half][r], ss[grp + half][r]);
+      sm[grp][r] = x.m;
+      ss[grp][r] = x.s;
     }
     __syncthreads();
   }
   if (grp == 0 && m < M) {
-    mx = sm[0][r];
-    s = ss[0][r];
     if (rmax) {
-      rmax[m] = mx;
-      rsum[m] = s;
+      rmax[m] = x.m;
+      rsum[m] = x.s;
     }
     // log(sum) + (max - z): the difference first, as both may be large
-    if (losses) losses[m] = log(s) + (mx - zt[m]);
+    if (losses) losses[m] = log(x.s) + (x.m - zt[m]);
   }
 }
 
@@ -151,7 +156,7 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
   const bool grads = q.dX || q.dW || q.db;
   for (int64_t lo = 0; lo < q.R; lo += piece) {
     const int64_t n = q.R - lo < piece ? q.R - lo : piece;
-    const int64_t parts = stats_parts(dtype, n, q.V, q.C);
+    const int64_t parts = stats_parts(dtype, q.tied, n, q.V, q.C);
     T* rmax = (T*)stats;
     T* rsum = rmax + n;
     T* zt = rsum + n;
@@ -174,11 +179,16 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
     a.lda = q.C;
     a.ldb = q.tied ? q.C : q.V;
     a.ldc = q.V;
+    a.nz = q.V;
     int rc = run_stats(dtype, q.tied, a);
     if (rc) return rc;
     {
       TimedLaunch tl(DTMI_FAM_XENT, 2.0 * (double)(parts * n) * es);
-      lxent_join_kernel<T><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum, losses);
+      if (n <= 512)
+        lxent_join_kernel<T, 1><<<(unsigned)n, 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum, losses);
+      else
+        lxent_join_kernel<T, 32><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum,
+                                                                               losses);
     }
     if (grads) {
       {
@@ -241,9 +251,9 @@ static int lxent_run(int dtype, LxentArgs& q) {
   }
   if (!rc) {
     const int64_t tail = q.R % piece;
-    int64_t parts = stats_parts(dtype, piece, q.V, q.C);
+    int64_t parts = stats_parts(dtype, q.tied, piece, q.V, q.C);
     if (tail) {
-      const int64_t p = stats_parts(dtype, tail, q.V, q.C);
+      const int64_t p = stats_parts(dtype, q.tied, tail, q.V, q.C);
       parts = p > parts ? p : parts;
     }
     rc = pool_alloc(&stats, (size_t)(3 + 2 * parts) * piece * es);

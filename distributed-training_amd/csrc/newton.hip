@@ -3,12 +3,13 @@
 //
 //   X = U / (|U|_F + eps);  `steps` times: G = X X^T, H = b G + c G G, X = a X + H X
 //
-// for a matrix of fewer rows than columns; of a taller one the same with X^T X on the
-// right. G and H are symmetric: their products run over the tiles on and below the
+// for a matrix of no more rows than columns; a taller one is worked on transposed, from
+// the pass that scales it to the last product, which writes it back the other way
+// round. G and H are symmetric: their products run over the tiles on and below the
 // diagonal and mirror the rest, so that a step of an m x n matrix (m <= n) costs m^2 n
 // + m^3 + 2 m^2 n operations, a third less than three plain products where m = n. All
-// matrices of a call share each launch (gemm_group.h), wide and tall ones apart for G.
-// Bound: MFMA; small matrices by the 3 steps launches one after the other.
+// matrices of a call share each launch (gemm_group.h).
+// Bound: MFMA; small matrices by 3 `steps` launches one after the other.
 #include <cmath>
 #include <utility>
 #include <vector>
@@ -18,92 +19,149 @@
 
 namespace dtmi {
 
-constexpr int kNormParts = 64;   // blocks that share a matrix's sum of squares
-constexpr int kNormTasks = 64;   // 40 bytes each: the arguments stay below 4 KB
+constexpr int kNormTasks = 56;  // 56 bytes each: the arguments stay below 4 KB
 
+// X is [rows, cols], or [cols, rows] of a matrix with more rows than columns, with both
+// rounded up to 16 bytes of elements and zeros there.
 struct NormTask {
   const void* g;
   void* m;  // momentum (NULL: u = g)
   void* x;  // u / (|u| + eps)
-  int64_t n;
-  double* part;  // [kNormParts]
+  double* part;  // [parts]
+  int rows, cols;
 };
 
 struct NormArgs {
-  int count, nesterov;
+  int nesterov, parts;
   double mu, eps, gscale;
   const double* gscale_dev;
   NormTask t[kNormTasks];
 };
 
-// The elements of block `part`: a range of whole vectors, the last block's to the end.
-__device__ __forceinline__ void norm_range(int64_t n, int part, int64_t& lo, int64_t& hi) {
-  const int64_t per = ((n + kNormParts - 1) / kNormParts + 3) / 4 * 4;
-  lo = part * per < n ? part * per : n;
-  hi = lo + per < n ? lo + per : n;
+// The step's u of V elements from element i on; m moved on where FIRST.
+template <typename T, int V, bool FIRST>
+__device__ __forceinline__ void norm_u(T (&u)[V], const NormArgs& a, const T* __restrict__ G, T* __restrict__ M,
+                                       int64_t i, T gs, T mu) {
+  vload<T, V>(u, G + i);
+#pragma unroll
+  for (int e = 0; e < V; ++e) u[e] = u[e] * gs;
+  if (!M) return;
+  T m[V];
+  vload<T, V>(m, M + i);
+  if constexpr (FIRST) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) m[e] = fma(mu, m[e], u[e]);
+    vstore<T, V>(M + i, m);
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) u[e] = a.nesterov ? fma(mu, m[e], u[e]) : m[e];
 }
 
-// PASS 0: m = mu m + g and the block's sum of squares of u = g + mu m (nesterov) or m;
-// PASS 1: x = u / (|u| + eps), u formed again from g and m (u itself would be written
-// and read once more). Sums in float64. V elements at a time.
-template <typename T, int PASS, int V>
-__device__ __forceinline__ void norm_body(const NormArgs& a, const NormTask& k, int64_t lo, int64_t hi, T gs, T mu,
-                                          double scale, double& sq) {
-  const T* __restrict__ G = (const T*)k.g;
-  T* __restrict__ M = (T*)k.m;
-  T* __restrict__ X = (T*)k.x;
-  for (int64_t i = lo + (int64_t)threadIdx.x * V; i + V <= hi; i += 256 * V) {
+// m = mu m + g, and the block's share of the sum of squares of u = g + mu m (nesterov)
+// or m, in float64.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_sum_kernel(NormArgs a) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const NormTask k = a.t[blockIdx.y];
+  const T* G = (const T*)k.g;
+  T* M = (T*)k.m;
+  const T gs = a.gscale_dev ? (T)*a.gscale_dev : (T)a.gscale, mu = (T)a.mu;
+  const int64_t n = (int64_t)k.rows * k.cols, stride = (int64_t)gridDim.x * 256;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t nv = aligned(G, 16) && aligned(M, 16) ? n / V : 0;
+  double sq = 0.0;
+  int64_t v = first;
+  for (; v + 3 * stride < nv; v += 4 * stride) {  // four vectors in flight
+    T u[4][V];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) norm_u<T, V, true>(u[q], a, G, M, (v + q * stride) * V, gs, mu);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sq += (double)u[q][e] * (double)u[q][e];
+  }
+  for (; v < nv; v += stride) {
     T u[V];
-    vload<T, V>(u, G + i);
+    norm_u<T, V, true>(u, a, G, M, v * V, gs, mu);
 #pragma unroll
-    for (int e = 0; e < V; ++e) u[e] = u[e] * gs;
-    if (M) {
-      T m[V];
-      vload<T, V>(m, M + i);
-      if constexpr (PASS == 0) {
+    for (int e = 0; e < V; ++e) sq += (double)u[e] * (double)u[e];
+  }
+  for (int64_t i = nv * V + first; i < n; i += stride) {
+    T u[1];
+    norm_u<T, 1, true>(u, a, G, M, i, gs, mu);
+    sq += (double)u[0] * (double)u[0];
+  }
+  __shared__ double sh[4];
 #pragma unroll
-        for (int e = 0; e < V; ++e) m[e] = fma(mu, m[e], u[e]);
-        vstore<T, V>(M + i, m);
+  for (int o = 32; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 64);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sq;
+  __syncthreads();
+  if (threadIdx.x == 0) k.part[blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+}
+
+// X = u / (|u| + eps), u formed again from g and m: written by the first pass it would be
+// read here just the same. The padding of X is set to 0.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_scale_kernel(NormArgs a) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const NormTask k = a.t[blockIdx.y];
+  const T* G = (const T*)k.g;
+  T* M = (T*)k.m;
+  T* X = (T*)k.x;
+  const T gs = a.gscale_dev ? (T)*a.gscale_dev : (T)a.gscale, mu = (T)a.mu;
+  double s = 0.0;  // every wave adds the parts in the same order
+  for (int i = threadIdx.x & 63; i < a.parts; i += 64) s += k.part[i];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  const double scale = 1.0 / (sqrt(s) + a.eps);
+  if (k.rows > k.cols) {  // block-uniform: 32 x 32 pieces turned through LDS
+    __shared__ T turned[32][33];
+    const uint32_t pr = (uint32_t)((k.rows + V - 1) / V * V), pc = (uint32_t)((k.cols + V - 1) / V * V);
+    const uint32_t across = (pc + 31) / 32, pieces = across * ((pr + 31) / 32);
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
+      const uint32_t r0 = p / across * 32, c0 = p % across * 32;
+#pragma unroll
+      for (int y = ty; y < 32; y += 8) {
+        const uint32_t r = r0 + y, c = c0 + tx;
+        T u[1] = {T(0)};
+        const bool in = r < (uint32_t)k.rows && c < (uint32_t)k.cols;
+        if (in) norm_u<T, 1, false>(u, a, G, M, (int64_t)r * k.cols + c, gs, mu);
+        turned[y][tx] = in ? (T)((double)u[0] * scale) : T(0);
       }
+      __syncthreads();
 #pragma unroll
-      for (int e = 0; e < V; ++e) u[e] = a.nesterov ? fma(mu, m[e], u[e]) : m[e];
+      for (int y = ty; y < 32; y += 8) {
+        const uint32_t c = c0 + y, r = r0 + tx;
+        if (c < pc && r < pr) X[(int64_t)c * pr + r] = turned[tx][y];
+      }
+      __syncthreads();
     }
-    if constexpr (PASS == 0) {
+    return;
+  }
+  const uint32_t per_row = (uint32_t)((k.cols + V - 1) / V);
+  const uint32_t rows = (uint32_t)((k.rows + V - 1) / V * V), total = rows * per_row;
+  const bool vec = aligned(G, 16) && aligned(M, 16) && k.cols % V == 0;
+  for (uint32_t v = blockIdx.x * 256 + threadIdx.x; v < total; v += gridDim.x * 256) {
+    const uint32_t r = v / per_row, c = (v - r * per_row) * V;
+    T x[V];
+    if (r >= (uint32_t)k.rows) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) sq += (double)u[e] * (double)u[e];
+      for (int e = 0; e < V; ++e) x[e] = T(0);
+    } else if (vec) {
+      norm_u<T, V, false>(x, a, G, M, (int64_t)r * k.cols + c, gs, mu);
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = (T)((double)x[e] * scale);
     } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) u[e] = (T)((double)u[e] * scale);
-      vstore<T, V>(X + i, u);
+      for (int e = 0; e < V; ++e) {
+        T u[1] = {T(0)};
+        if (c + e < (uint32_t)k.cols) norm_u<T, 1, false>(u, a, G, M, (int64_t)r * k.cols + c + e, gs, mu);
+        x[e] = (T)((double)u[0] * scale);
+        if (c + e >= (uint32_t)k.cols) x[e] = T(0);
+      }
     }
-  }
-}
-
-template <typename T, int PASS>
-__global__ void __launch_bounds__(256) norm_kernel(NormArgs a) {
-  const NormTask k = a.t[blockIdx.y];
-  const T gs = a.gscale_dev ? (T)*a.gscale_dev : (T)a.gscale;
-  __shared__ double sh[4];
-  double scale = 0.0, sq = 0.0;
-  if constexpr (PASS == 1) {
-    double s = k.part[threadIdx.x & 63];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    scale = 1.0 / (sqrt(s) + a.eps);
-  }
-  int64_t lo, hi;
-  norm_range(k.n, blockIdx.x, lo, hi);
-  constexpr int V = 16 / (int)sizeof(T);
-  const bool vec = aligned(k.g, 16) && aligned(k.m, 16) && aligned(k.x, 16);
-  const int64_t mid = vec ? lo + (hi - lo) / V * V : lo;
-  if (vec) norm_body<T, PASS, V>(a, k, lo, mid, gs, (T)a.mu, scale, sq);
-  norm_body<T, PASS, 1>(a, k, mid, hi, gs, (T)a.mu, scale, sq);
-  if constexpr (PASS == 0) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 64);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sq;
-    __syncthreads();
-    if (threadIdx.x == 0) k.part[blockIdx.x] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    vstore<T, V>(X + (int64_t)v * V, x);
   }
 }
 
@@ -121,16 +179,33 @@ struct NewtonArgs {
   const double* rate;
 };
 
+// Blocks per matrix of the norm kernels, by the largest one's elements: a vector a thread
+// up to `most` blocks.
+static int norm_blocks(int64_t elements, size_t es, int most) {
+  const int64_t p = cdiv(elements * (int64_t)es, 16 * 256);
+  return (int)(p < 1 ? 1 : p > most ? most : p);
+}
+
+static int64_t up(int64_t n, int64_t v) { return cdiv(n, v) * v; }
+static size_t bytes_of(int64_t r, int64_t c, size_t es) {
+  const int64_t v = 16 / (int64_t)es;
+  return ((size_t)up(r, v) * up(c, v) * es + 255) & ~(size_t)255;
+}
+
 template <typename T>
-static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& live, char* ws, size_t es) {
+static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& live, int64_t most, int np, char* ws) {
+  constexpr size_t es = sizeof(T);
+  // The workspace's matrices are padded to 16 bytes of elements both ways, with zeros, so
+  // that odd sizes run on 16-byte loads too: zero rows and columns stay zero through the
+  // steps. The last product writes the result as it lies.
+  constexpr int V = 16 / (int)sizeof(T);
   const int n = (int)live.size();
-  // the workspace: norm parts, then per matrix X twice and G and H
   std::vector<char*> x0(n), x1(n), G(n), H(n);
   double* parts = (double*)ws;
-  char* p = ws + (size_t)n * kNormParts * sizeof(double);
+  char* p = ws + (((size_t)n * np * sizeof(double) + 255) & ~(size_t)255);
   for (int i = 0; i < n; ++i) {
     const int64_t r = q.rows[live[i]], c = q.cols[live[i]], s = r < c ? r : c;
-    const size_t xb = ((size_t)r * c * es + 255) & ~(size_t)255, gb = ((size_t)s * s * es + 255) & ~(size_t)255;
+    const size_t xb = bytes_of(r, c, es), gb = bytes_of(s, s, es);
     x0[i] = p;
     x1[i] = p + xb;
     G[i] = p + 2 * xb;
@@ -139,44 +214,42 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
   }
   for (int lo = 0; lo < n; lo += kNormTasks) {
     NormArgs a{};
-    a.count = n - lo < kNormTasks ? n - lo : kNormTasks;
+    const int count = n - lo < kNormTasks ? n - lo : kNormTasks;
     a.nesterov = q.nesterov;
+    a.parts = np;
     a.mu = q.mu;
     a.eps = q.eps;
     a.gscale = q.gscale;
     a.gscale_dev = q.gscale_dev;
     double bytes = 0;
-    for (int i = 0; i < a.count; ++i) {
+    for (int i = 0; i < count; ++i) {
       const int j = live[lo + i];
-      a.t[i] = {q.g[j], q.m ? q.m[j] : nullptr, x0[lo + i], q.rows[j] * q.cols[j], parts + (size_t)(lo + i) * kNormParts};
-      bytes += (double)a.t[i].n * (double)es * (q.m ? 6 : 3);
+      a.t[i] = {q.g[j], q.m ? q.m[j] : nullptr, x0[lo + i], parts + (size_t)(lo + i) * np, (int)q.rows[j],
+                (int)q.cols[j]};
+      bytes += (double)q.rows[j] * (double)q.cols[j] * (double)es * (q.m ? 6 : 3);
     }
     TimedLaunch tl(DTMI_FAM_OTHER, bytes);
-    const dim3 grid(kNormParts, (unsigned)a.count);
-    norm_kernel<T, 0><<<grid, 256, 0, stream()>>>(a);
-    norm_kernel<T, 1><<<grid, 256, 0, stream()>>>(a);
-    LAUNCH_CHECK("norm_kernel");
+    norm_sum_kernel<T><<<dim3((unsigned)np, (unsigned)count), 256, 0, stream()>>>(a);
+    norm_scale_kernel<T><<<dim3((unsigned)norm_blocks(most, es, 4096 / count < 64 ? 64 : 4096 / count), (unsigned)count), 256,
+                           0, stream()>>>(a);
+    LAUNCH_CHECK("norm kernels");
   }
-  std::vector<GroupTask> wide, tall, sq(n), ap(n);
+  std::vector<GroupTask> gram(n), sq(n), ap(n);
   for (int s = 0; s < q.steps; ++s) {
     const bool last = s + 1 == q.steps;
-    wide.clear();
-    tall.clear();
     for (int i = 0; i < n; ++i) {
-      const int j = live[i], r = (int)q.rows[j], c = (int)q.cols[j], m = r < c ? r : c;
-      // G = X X^T, or X^T X of a tall matrix
-      (r <= c ? wide : tall).push_back({x0[i], x0[i], G[i], nullptr, m, m, r < c ? c : r, 0, 1.0});
-      // H = b G + c G G: G is symmetric, so either operand may be read either way
-      sq[i] = {G[i], G[i], H[i], G[i], m, m, m, 0, 1.0};
-      // X = a X + H X, or a X + X H; the last into the result
-      ap[i] = {r <= c ? H[i] : x0[i], r <= c ? x0[i] : H[i], last ? (char*)q.out[j] : x1[i], x0[i], r, c, m, 0,
+      const int j = live[i], tall = q.rows[j] > q.cols[j];
+      const int m = (int)(tall ? q.cols[j] : q.rows[j]), w = (int)(tall ? q.rows[j] : q.cols[j]);
+      gram[i] = {x0[i], x0[i], G[i], nullptr, m, m, w, 0, 1.0};  // G = X X^T
+      sq[i] = {G[i], G[i], H[i], G[i], m, m, m, 0, 1.0};         // H = b G + c G G (G = G^T)
+      // X = a X + H X, the last into the result
+      ap[i] = {H[i], x0[i], last ? (char*)q.out[j] : x1[i], x0[i], m, w, m, last && tall,
                last && q.rate ? q.rate[j] : 1.0};
     }
-    int rc = DTMI_OK;
-    if (!wide.empty()) rc = run_group(dtype, 1, 1, wide.data(), (int)wide.size(), kDNone, 1, 1.0, 0.0, 0.0);
-    if (!rc && !tall.empty()) rc = run_group(dtype, 0, 0, tall.data(), (int)tall.size(), kDNone, 1, 1.0, 0.0, 0.0);
-    if (!rc) rc = run_group(dtype, 1, 1, sq.data(), n, kDMatrix, 1, q.c, q.b, 0.0);
-    if (!rc) rc = run_group(dtype, 1, 0, ap.data(), n, kDMatrix, 0, 1.0, q.a, last && q.rate ? q.gamma : 0.0);
+    int rc = run_group(dtype, 1, 1, gram.data(), n, kDNone, 1, 1.0, 0.0, 0.0, V, V);
+    if (!rc) rc = run_group(dtype, 1, 1, sq.data(), n, kDMatrix, 1, q.c, q.b, 0.0, V, V);
+    if (!rc)
+      rc = run_group(dtype, 1, 0, ap.data(), n, kDMatrix, 0, 1.0, q.a, last && q.rate ? q.gamma : 0.0, V, last ? 1 : V);
     if (rc) return rc;
     std::swap(x0, x1);
   }
@@ -188,26 +261,28 @@ static int newton(const char* what, int dtype, const NewtonArgs& q) {
   DTMI_CHECK(q.n == 0 || (q.g && q.out && q.rows && q.cols), "%s: NULL array", what);
   const size_t es = dtype == DTMI_F32 ? 4 : 8;
   std::vector<int> live;
-  size_t bytes = 0;
+  size_t bytes = 256;
+  int64_t most = 0;
   for (int i = 0; i < q.n; ++i) {
-    const int64_t r = q.rows[i], c = q.cols[i];
+    const int64_t r = q.rows[i], c = q.cols[i], edge = (1 << 24) / (int64_t)es - 4;
     DTMI_CHECK(r >= 0 && c >= 0, "%s: negative size of matrix %d", what, i);
     if (r == 0 || c == 0) continue;
-    const int64_t most = (1 << 24) / (int64_t)es;
-    DTMI_CHECK(r < most && c < most, "%s: matrix %d, %lld x %lld, has rows or columns of 2^24 bytes or more", what, i,
+    DTMI_CHECK(r < edge && c < edge && up(r, 4) * up(c, 4) < (1LL << 32),
+               "%s: matrix %d, %lld x %lld, is too large (rows and columns below 2^24 bytes, 2^32 elements)", what, i,
                (long long)r, (long long)c);
     DTMI_CHECK(q.g[i] && q.out[i] && (!q.m || q.m[i]), "%s: NULL pointer of matrix %d", what, i);
     const int64_t s = r < c ? r : c;
-    bytes += (size_t)kNormParts * sizeof(double) + 2 * (((size_t)r * c * es + 255) & ~(size_t)255) +
-             2 * (((size_t)s * s * es + 255) & ~(size_t)255);
+    bytes += 2 * bytes_of(r, c, es) + 2 * bytes_of(s, s, es);
+    most = r * c > most ? r * c : most;
     live.push_back(i);
   }
   if (live.empty()) return DTMI_OK;
+  const int np = norm_blocks(most, es, 512);
   void* ws = nullptr;
-  int rc = pool_alloc(&ws, bytes);
+  int rc = pool_alloc(&ws, bytes + live.size() * (size_t)np * sizeof(double));
   if (rc) return rc;
-  rc = dtype == DTMI_F32 ? newton_run<float>(dtype, q, live, (char*)ws, es)
-                         : newton_run<double>(dtype, q, live, (char*)ws, es);
+  rc = dtype == DTMI_F32 ? newton_run<float>(dtype, q, live, most, np, (char*)ws)
+                         : newton_run<double>(dtype, q, live, most, np, (char*)ws);
   pool_free(ws);
   return rc;
 }

@@ -59,6 +59,10 @@ LOSS = [  # rows, C, V, bias, tied, ignored targets
     (200, 96, 1000, False, True, 0),
     (333, 51, 777, True, False, 100),
     (130, 132, 4100, True, False, 0),
+    (16, 300, 1000, True, True, 0),      # few rows
+    (32, 515, 777, True, False, 2),
+    (17, 1030, 514, False, True, 0),
+    (31, 90, 1029, False, False, 0),
 ]
 
 
@@ -325,6 +329,9 @@ EXPERTS = [  # R, K, N, sizes, bias
     (300, 100, 30, [0, 0], True),
     (515, 68, 257, [128, 129, 0, 255, 1], True),
     (600, 48, 20, [4] * 70 + [1, 100, 219], False),   # more experts than a launch holds
+    (20, 515, 201, [16, 0, 4], True),                 # few rows each
+    (41, 770, 131, [32, 7, 1], False),
+    (9, 36, 1000, [1, 8], True),
     (5000, 24, 40, [4000, 999], True),                # sums over rows long enough to be split
 ]
 
