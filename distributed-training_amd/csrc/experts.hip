@@ -5,6 +5,7 @@
 //
 // Bound: MFMA from about 30 rows an expert on (2 R K N operations over E K N
 // weights), below that reading the weights of the experts that have rows.
+#include <utility>
 #include <vector>
 
 #include "gemm_group.h"
@@ -34,9 +35,15 @@ static char* at(void* p, int64_t elements, int dtype) {
   return p ? (char*)p + elements * (dtype == DTMI_F32 ? 4 : 8) : nullptr;
 }
 
+static int run(int dtype, int akc, int bkc, std::vector<GroupTask> tasks, int dmode) {
+  std::vector<GroupLaunch> l;
+  int rc = plan_group(dtype, akc, bkc, std::move(tasks), dmode, 0, 1.0, 0.0, 0.0, 1, 1, l);
+  return rc ? rc : launch_group(dtype, l);
+}
+
 // rows of an [R, cols] result that no expert owns
 static int zero_tail(int dtype, void* p, int64_t used, int64_t R, int64_t cols) {
-  return dtmi_fill(dtype, at(p, used * cols, dtype), 0.0, (R - used) * cols);
+  return used < R ? dtmi_fill(dtype, at(p, used * cols, dtype), 0.0, (R - used) * cols) : DTMI_OK;
 }
 
 }  // namespace dtmi
@@ -59,7 +66,7 @@ DTMI_EXPORT int dtmi_expert_linear_fwd(int dtype, int64_t E, int64_t R, int64_t 
     t.push_back({at(x, off[e] * K, dtype), at(w, e * K * N, dtype), at(y, off[e] * N, dtype),
                  at(const_cast<void*>(b), e * N, dtype), (int)(off[e + 1] - off[e]), (int)N, (int)K, 0, 1.0});
   }
-  rc = run_group(dtype, 1, 0, t.data(), (int)t.size(), b ? kDRow : kDNone, 0, 1.0, 0.0, 0.0);
+  rc = run(dtype, 1, 0, std::move(t), b ? kDRow : kDNone);
   return rc ? rc : zero_tail(dtype, y, off[E], R, N);
   DTMI_BODY_END
 }
@@ -80,7 +87,7 @@ DTMI_EXPORT int dtmi_expert_linear_bwd_dx(int dtype, int64_t E, int64_t R, int64
     t.push_back({at(g, off[e] * N, dtype), at(w, e * K * N, dtype), at(dx, off[e] * K, dtype), nullptr,
                  (int)(off[e + 1] - off[e]), (int)K, (int)N, 0, 1.0});
   }
-  rc = run_group(dtype, 1, 1, t.data(), (int)t.size(), kDNone, 0, 1.0, 0.0, 0.0);
+  rc = run(dtype, 1, 1, std::move(t), kDNone);
   return rc ? rc : zero_tail(dtype, dx, off[E], R, K);
   DTMI_BODY_END
 }
@@ -107,6 +114,6 @@ DTMI_EXPORT int dtmi_expert_linear_bwd_dw(int dtype, int64_t E, int64_t R, int64
   for (int64_t e = 0; e < E; ++e)  // experts without rows: zeros
     t.push_back({at(x, off[e] * K, dtype), at(g, off[e] * N, dtype), at(dw, e * K * N, dtype), at(db, e * N, dtype),
                  (int)K, (int)N, (int)(off[e + 1] - off[e]), 0, 1.0});
-  return run_group(dtype, 0, 0, t.data(), (int)t.size(), db ? kDColsum : kDNone, 0, 1.0, 0.0, 0.0);
+  return run(dtype, 0, 0, std::move(t), db ? kDColsum : kDNone);
   DTMI_BODY_END
 }

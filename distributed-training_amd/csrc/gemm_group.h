@@ -9,6 +9,8 @@
 // captured graph.
 #pragma once
 
+#include <vector>
+
 #include "gemm_common.h"
 
 namespace dtmi {
@@ -61,7 +63,8 @@ struct GroupArgs {
 // Row statistics of Z = A B + bias over pieces of its columns, without Z (or with it,
 // where C is not NULL): part p of row m covers some columns (half a block tile's), pmax[p
 // M + m] is their maximum and psum[p M + m] the sum of exp(z - pmax) over them; zt[m] =
-// Z[m, targets[m]]. Columns N .. nz - 1 of C are set to -inf.
+// Z[m, targets[m]]. B has nz >= N columns (rows where k is contiguous): those past N are
+// read and not used, and set to -inf in C.
 struct StatsArgs {
   const void* A;
   const void* B;
@@ -91,10 +94,18 @@ void launch_group_rows(const GroupArgs& a, int bkc, int mr, int nw);
 template <typename T>
 void launch_stats_rows(const StatsArgs& a, int bkc, int mr, int nw);
 
-// Runs the tasks, longest k first, 64 to a launch. akc, bkc: which
-// operands are k-contiguous: (1, 0), (1, 1) or (0, 0).
-int run_group(int dtype, int akc, int bkc, GroupTask* tasks, int count, int dmode, int sym, double alpha, double beta,
-              double gamma, int pad = 1, int padc = 1);
+// One planned launch. tile: 128, 64, 32 (of nw waves) or 16 (few rows: mr tiles of 16).
+struct GroupLaunch {
+  GroupArgs a;
+  int akc, bkc, vec, tile, nw, mr;
+  size_t ws_bytes, cs_at;
+  double flops;
+};
+// Plans the tasks' launches, longest k first, 64 to a launch. akc, bkc: which operands
+// are k-contiguous: (1, 0), (1, 1) or (0, 0).
+int plan_group(int dtype, int akc, int bkc, std::vector<GroupTask> tasks, int dmode, int sym, double alpha, double beta,
+               double gamma, int pad, int padc, std::vector<GroupLaunch>& out);
+int launch_group(int dtype, const std::vector<GroupLaunch>& launches);
 // The parts a row's statistics come in.
 int64_t stats_parts(int dtype, int bkc, int64_t M, int64_t N, int64_t K);
 int run_stats(int dtype, int bkc, StatsArgs a);

@@ -65,7 +65,7 @@ static double split_cycles(int bm, int64_t cut, int splits, size_t es) {
 //   number of rounds;
 // - unequal k: the tiles of the longest tasks split.
 template <typename T>
-static GroupPlan plan_group(const GroupTask* t, int count, int sym, int pad, int64_t cus) {
+static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, int64_t cus) {
   constexpr size_t es = sizeof(T);
   constexpr int64_t bk = 64 / (int64_t)es;
   int64_t k[kGroupTasks];
@@ -139,13 +139,17 @@ static GroupPlan plan_group(const GroupTask* t, int count, int sym, int pad, int
 }
 
 template <typename T>
-static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmode, int sym, double alpha, double beta,
-                          double gamma, int pad, int padc) {
+static int plan_tasks(int akc, int bkc, std::vector<GroupTask>& tasks, int dmode, int sym, double alpha, double beta,
+                      double gamma, int pad, int padc, std::vector<GroupLaunch>& out) {
   constexpr int V = MF<T>::VEC;
   const int64_t cus = num_cus() > 0 ? num_cus() : 256;
-  std::stable_sort(tasks, tasks + count, [](const GroupTask& x, const GroupTask& y) { return x.K > y.K; });
+  const int count = (int)tasks.size();
+  std::stable_sort(tasks.begin(), tasks.end(), [](const GroupTask& x, const GroupTask& y) { return x.K > y.K; });
   for (int lo = 0; lo < count; lo += kGroupTasks) {
-    GroupArgs a{};
+    GroupLaunch l{};
+    GroupArgs& a = l.a;
+    l.akc = akc;
+    l.bkc = bkc;
     a.count = count - lo < kGroupTasks ? count - lo : kGroupTasks;
     a.dmode = dmode;
     a.sym = sym;
@@ -155,7 +159,7 @@ static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmo
     a.beta = beta;
     a.gamma = gamma;
     bool vec = true;
-    double flops = 0;
+    int rows = 0;
     for (int i = 0; i < a.count; ++i) {
       GroupTask& t = a.t[i];
       t = tasks[lo + i];
@@ -164,37 +168,29 @@ static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmo
                  "group of products: rows of 2^24 bytes or more are not supported");
       vec = vec && lda % V == 0 && ldb % V == 0 && aligned(t.A, 16) && aligned(t.B, 16) &&
             (!sym || (cdiv(t.N, padc) * padc % V == 0 && aligned(t.C, 16)));
-      flops += (sym ? 1.0 : 2.0) * (double)t.M * t.N * t.K;
+      rows = t.M > rows ? t.M : rows;
+      l.flops += (sym ? 1.0 : 2.0) * (double)t.M * t.N * t.K;
     }
-    int rows = 0;
-    for (int i = 0; i < a.count; ++i) rows = a.t[i].M > rows ? a.t[i].M : rows;
-    if (rows <= kFewRows && akc && !sym && pad == 1 && dmode != kDColsum) {
-      const int mr = rows <= 16 ? 1 : 2, cols = bkc ? RowsTile<T, true>::COLS : RowsTile<T, false>::COLS;
-      int64_t tiles = 0, kmax = 0;
-      for (int i = 0; i < a.count; ++i) {
-        a.first[i] = (int)tiles;
-        tiles += cdiv(a.t[i].M, 16 * mr) * cdiv(a.t[i].N, cols);
-        kmax = a.t[i].K > kmax ? a.t[i].K : kmax;
-      }
-      if (!tiles) continue;
-      a.tiles = (int)tiles;
-      TimedLaunch tl(DTMI_FAM_GEMM, flops);
-      launch_group_rows<T>(a, bkc, mr, rows_waves<T>(tiles, kmax, cus, mr, bkc));
-      LAUNCH_CHECK("group_rows_kernel");
-      continue;
-    }
-    const GroupPlan p = plan_group<T>(a.t, a.count, sym, pad, cus);
+    l.vec = vec;
+    const bool few = rows <= kFewRows && akc && !sym && pad == 1 && dmode != kDColsum;
+    const GroupPlan p = few ? GroupPlan{16, 0, 1, 0} : choose_plan<T>(a.t, a.count, sym, pad, cus);
+    l.tile = p.tile;
+    l.nw = p.nw;
+    l.mr = rows <= 16 ? 1 : 2;
+    const int tm_rows = few ? 16 * l.mr : p.tile;
+    const int tn_cols = few ? (bkc ? RowsTile<T, true>::COLS : RowsTile<T, false>::COLS) : p.tile;
     a.equal = 1;
-    for (int i = 1; i < a.count; ++i) a.equal = a.equal && a.t[i].K == a.t[0].K;
     int64_t tiles = 0;
     for (int i = 0; i < a.count; ++i) {
-      const int64_t tm = cdiv(a.t[i].M, p.tile), tn = cdiv(a.t[i].N, p.tile);
+      const int64_t tm = cdiv(a.t[i].M, tm_rows), tn = cdiv(a.t[i].N, tn_cols);
+      a.equal = a.equal && a.t[i].K == a.t[0].K;
       a.first[i] = (int)tiles;
       tiles += sym ? tm * (tm + 1) / 2 : tm * tn;
       DTMI_CHECK(tiles < (1LL << 26), "group of products: too large");
     }
     if (!tiles) continue;
     a.tiles = (int)tiles;
+    if (few) l.nw = rows_waves<T>(tiles, a.t[0].K, cus, l.mr, bkc);
     a.cut = p.cut < a.tiles ? p.cut : a.tiles;
     a.splits = p.splits;
     for (int i = 0; i < a.count && a.cut; ++i) {  // whole tiles that are longer than the pieces
@@ -210,35 +206,56 @@ static int group_launches(int akc, int bkc, GroupTask* tasks, int count, int dmo
         a.turned = (int)units;
       }
     }
-    void* ws = nullptr;
     if (a.cut) {
-      const size_t slots = (size_t)p.splits * a.cut, main_bytes = slots * p.tile * p.tile * sizeof(T);
-      int rc = pool_alloc(&ws, main_bytes + slots * p.tile * sizeof(T));
-      if (rc) return rc;
-      a.ws = ws;
-      a.csws = (char*)ws + main_bytes;
+      const size_t slots = (size_t)p.splits * a.cut;
+      l.cs_at = slots * p.tile * p.tile * sizeof(T);
+      l.ws_bytes = l.cs_at + (dmode == kDColsum ? slots * p.tile * sizeof(T) : 0);
     }
-    {
-      TimedLaunch tl(DTMI_FAM_GEMM, flops);
-      if (p.tile == 32)
-        launch_group_direct<T>(a, akc, bkc, p.nw);
-      else if (p.tile == 64)
-        launch_group<T, 64>(a, akc, bkc, vec);
-      else
-        launch_group<T, 128>(a, akc, bkc, vec);
-    }
-    const hipError_t e = hipGetLastError();
-    if (ws) pool_free(ws);
-    if (e != hipSuccess) return fail_hip(e, "group kernels", __FILE__, __LINE__);
+    out.push_back(l);
   }
   return DTMI_OK;
 }
 
-int run_group(int dtype, int akc, int bkc, GroupTask* tasks, int count, int dmode, int sym, double alpha, double beta,
-              double gamma, int pad, int padc) {
-  if (dtype == DTMI_F32)
-    return group_launches<float>(akc, bkc, tasks, count, dmode, sym, alpha, beta, gamma, pad, padc);
-  return group_launches<double>(akc, bkc, tasks, count, dmode, sym, alpha, beta, gamma, pad, padc);
+int plan_group(int dtype, int akc, int bkc, std::vector<GroupTask> tasks, int dmode, int sym, double alpha, double beta,
+               double gamma, int pad, int padc, std::vector<GroupLaunch>& out) {
+  out.clear();
+  if (dtype == DTMI_F32) return plan_tasks<float>(akc, bkc, tasks, dmode, sym, alpha, beta, gamma, pad, padc, out);
+  return plan_tasks<double>(akc, bkc, tasks, dmode, sym, alpha, beta, gamma, pad, padc, out);
+}
+
+template <typename T>
+static int launch_one(const GroupLaunch& l) {
+  void* ws = nullptr;
+  GroupArgs a = l.a;
+  if (l.ws_bytes) {
+    int rc = pool_alloc(&ws, l.ws_bytes);
+    if (rc) return rc;
+    a.ws = ws;
+    a.csws = (char*)ws + l.cs_at;
+  }
+  {
+    TimedLaunch tl(DTMI_FAM_GEMM, l.flops);
+    if (l.tile == 16)
+      launch_group_rows<T>(a, l.bkc, l.mr, l.nw);
+    else if (l.tile == 32)
+      launch_group_direct<T>(a, l.akc, l.bkc, l.nw);
+    else if (l.tile == 64)
+      launch_group<T, 64>(a, l.akc, l.bkc, l.vec);
+    else
+      launch_group<T, 128>(a, l.akc, l.bkc, l.vec);
+  }
+  const hipError_t e = hipGetLastError();
+  if (ws) pool_free(ws);
+  if (e != hipSuccess) return fail_hip(e, "group kernels", __FILE__, __LINE__);
+  return DTMI_OK;
+}
+
+int launch_group(int dtype, const std::vector<GroupLaunch>& launches) {
+  for (const GroupLaunch& l : launches) {
+    int rc = dtype == DTMI_F32 ? launch_one<float>(l) : launch_one<double>(l);
+    if (rc) return rc;
+  }
+  return DTMI_OK;
 }
 
 // Tile and waves of a statistics product (tile 16: few rows).
@@ -284,7 +301,7 @@ static int stats_launch(int bkc, StatsArgs& a) {
              "statistics product: rows of 2^24 bytes or more are not supported");
   const GroupPlan p = plan_stats<T>(bkc, a.M, a.N, a.K);
   const bool vec = aligned(a.A, 16) && aligned(a.B, 16) && a.lda % V == 0 && a.ldb % V == 0 && a.K % V == 0 &&
-                   (bkc || a.N % V == 0);
+                   (bkc || a.nz % V == 0);
   DTMI_CHECK(cdiv(a.M, p.tile) * cdiv(a.N, p.tile) < (1LL << 30), "statistics product: too large");
   const int mr = a.M <= 16 ? 1 : 2;
   a.tiles_m = p.tile == 16 ? 1 : (int)cdiv(a.M, p.tile);

@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(256, 2) gemm_stats_kernel(StatsArgs a) {
 #pragma unroll
     for (int j = 0; j < TW; ++j) acc[i][j] = typename MFT::acc_t(0);
   double csum = 0.0;
-  dma_product<T, BM, BM, true, BKC, VEC, VEC>(acc, lds, (const T*)a.A, a.lda, a.M, m0, (const T*)a.B, a.ldb, a.N, n0,
+  dma_product<T, BM, BM, true, BKC, VEC, VEC>(acc, lds, (const T*)a.A, a.lda, a.M, m0, (const T*)a.B, a.ldb, a.nz, n0,
                                               0, a.K, sizeof(T) == 4 ? 2 : 4, false, csum);
   const int64_t wm = m0 + (wave >> 1) * W, wn = n0 + (wave & 1) * W;
   T* C = (T*)a.C;

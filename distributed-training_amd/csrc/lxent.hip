@@ -12,13 +12,15 @@
 // piece.
 #include <cmath>
 
+#include "gemm_direct_tile.h"
 #include "gemm_group.h"
 
 namespace dtmi {
 
-// Rows of a piece. Fewer rows read and write dw more often, 8 C V bytes against 6 rows
-// C V operations; more take rows * V * 4 bytes of workspace.
-constexpr int64_t kPieceRows = 2048;
+// Logits of a piece, in bytes: pieces of fewer rows read and write dw more often, 8 C V
+// bytes against 6 rows C V operations: 8192 x 768 x 50304 takes 15.1 ms in pieces of 2048
+// rows, 14.5 in these (4096).
+constexpr int64_t kPieceBytes = 1LL << 30, kPieceRows = 1024;
 
 template <typename T>
 __device__ __forceinline__ T exp_e(T x) {
@@ -105,33 +107,37 @@ __global__ void __launch_bounds__(1024) lxent_mean_kernel(const T* __restrict__ 
   }
 }
 
-// dz in place of z: block (x, y) takes 4 vectors a thread of row y.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) lxent_dz_kernel(T* __restrict__ z, int64_t cols, const T* __restrict__ rmax,
-                                                       const T* __restrict__ rsum, const int64_t* __restrict__ targets,
-                                                       const T* __restrict__ g, int64_t g_stride, double coef) {
-  typedef T vt __attribute__((ext_vector_type(V == 1 ? 2 : V)));
-  const int64_t m = blockIdx.y;
-  T* row = z + m * cols;
-  const T mx = rmax[m], c = g ? (T)coef * g[m * g_stride] : (T)coef;
-  const T inv = T(1) / rsum[m];
-  const int64_t t = targets[m];
+// dz in place of z: block (x, y) takes 4 vectors a thread of rows y, y + gridDim.y, ...
+// Vectors need element alignment only, so a vocabulary that is no multiple of one runs the
+// same, with its last few elements one by one (1067 x 50257: 104 us element by element).
+template <typename T>
+__global__ void __launch_bounds__(256) lxent_dz_kernel(T* __restrict__ z, int64_t rows, int64_t cols,
+                                                       const T* __restrict__ rmax, const T* __restrict__ rsum,
+                                                       const int64_t* __restrict__ targets, const T* __restrict__ g,
+                                                       int64_t g_stride, double coef) {
+  constexpr int V = 16 / (int)sizeof(T);
+  typedef typename UVec<T>::type vt;
   const int64_t c0 = (int64_t)blockIdx.x * (256 * 4 * V);
+  for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
+    T* row = z + m * cols;
+    const T mx = rmax[m], c = g ? (T)coef * g[m * g_stride] : (T)coef;
+    const T inv = T(1) / rsum[m];
+    const int64_t t = targets[m];
+    auto dz = [&](T x, int64_t at) {
+      const T p = exp_e<T>(x - mx) * inv;
+      return c * (at == t ? p - T(1) : p);
+    };
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t at = c0 + (u * 256 + threadIdx.x) * V;
-    if (at >= cols) continue;
-    if constexpr (V == 1) {
-      const T p = exp_e<T>(row[at] - mx) * inv;
-      row[at] = c * (at == t ? p - T(1) : p);
-    } else {
-      vt v = *reinterpret_cast<const vt*>(row + at);
+    for (int u = 0; u < 4; ++u) {
+      const int64_t at = c0 + (u * 256 + threadIdx.x) * V;
+      if (at + V <= cols) {
+        typename MF<T>::vec_t v = *reinterpret_cast<const vt*>(row + at);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const T p = exp_e<T>(v[e] - mx) * inv;
-        v[e] = c * (at + e == t ? p - T(1) : p);
+        for (int e = 0; e < V; ++e) v[e] = dz(v[e], at + e);
+        *reinterpret_cast<vt*>(row + at) = v;
+      } else {
+        for (int64_t i = at; i < cols; ++i) row[i] = dz(row[i], i);
       }
-      *reinterpret_cast<vt*>(row + at) = v;
     }
   }
 }
@@ -148,6 +154,14 @@ struct LxentArgs {
   int64_t g_stride;
   double coef;
   char *dX, *dW, *db;
+};
+
+// Pool memory that goes back at the end of the call's enqueuing.
+struct Scratch {
+  void* p = nullptr;
+  ~Scratch() {
+    if (p) pool_free(p);
+  }
 };
 
 template <typename T>
@@ -195,12 +209,9 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
         TimedLaunch tl(DTMI_FAM_XENT, 2.0 * (double)n * (double)q.V * es);
         constexpr int V = 16 / (int)sizeof(T);
         const T* g = q.g ? (const T*)q.g + lo * q.g_stride : nullptr;
-        if (q.V % V == 0)
-          lxent_dz_kernel<T, V><<<dim3((unsigned)cdiv(q.V, 1024 * V), (unsigned)n), 256, 0, stream()>>>(
-              (T*)Z, q.V, rmax, rsum, a.targets, g, q.g_stride, q.coef);
-        else
-          lxent_dz_kernel<T, 1><<<dim3((unsigned)cdiv(q.V, 1024), (unsigned)n), 256, 0, stream()>>>(
-              (T*)Z, q.V, rmax, rsum, a.targets, g, q.g_stride, q.coef);
+        const unsigned ny = (unsigned)(n < 32768 ? n : 32768);
+        lxent_dz_kernel<T><<<dim3((unsigned)cdiv(q.V, 1024 * V), ny), 256, 0, stream()>>>(
+            (T*)Z, n, q.V, rmax, rsum, a.targets, g, q.g_stride, q.coef);
       }
       LAUNCH_CHECK("lxent_dz_kernel");
       const int add = lo > 0;
@@ -229,42 +240,57 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
   return DTMI_OK;
 }
 
-static int lxent_run(int dtype, LxentArgs& q) {
-  const size_t es = dtype == DTMI_F32 ? 4 : 8;
+template <typename T>
+static int lxent_run(int dtype, LxentArgs q) {
+  constexpr int64_t es = sizeof(T);
   const bool grads = q.dX || q.dW || q.db;
-  void *own = nullptr, *Z = nullptr, *stats = nullptr;
-  int64_t piece = q.R;
+  Scratch losses, Z, stats;
   int rc = DTMI_OK;
   if (!q.losses) {
-    rc = pool_alloc(&own, (size_t)q.R * es);
+    rc = pool_alloc(&losses.p, (size_t)(q.R * es));
     if (rc) return rc;
-    q.losses = (char*)own;
+    q.losses = (char*)losses.p;
   }
+  int64_t piece = q.R;
   if (grads) {
-    piece = cdiv(cdiv(q.R, cdiv(q.R, kPieceRows)), 128) * 128;
+    int64_t most = kPieceBytes / (q.V * es);
+    most = most < kPieceRows ? kPieceRows : most;
+    piece = cdiv(cdiv(q.R, cdiv(q.R, most)), 128) * 128;
     if (piece > q.R) piece = q.R;
-    rc = pool_alloc(&Z, (size_t)piece * q.V * es);
+    rc = pool_alloc(&Z.p, (size_t)(piece * q.V * es));
     while (rc == DTMI_ERR_OOM && piece > 128) {  // smaller pieces where memory is short
       piece = cdiv(piece / 2, 128) * 128;
-      rc = pool_alloc(&Z, (size_t)piece * q.V * es);
+      rc = pool_alloc(&Z.p, (size_t)(piece * q.V * es));
     }
+    if (rc) return rc;
   }
-  if (!rc) {
-    const int64_t tail = q.R % piece;
-    int64_t parts = stats_parts(dtype, q.tied, piece, q.V, q.C);
-    if (tail) {
-      const int64_t p = stats_parts(dtype, q.tied, tail, q.V, q.C);
-      parts = p > parts ? p : parts;
-    }
-    rc = pool_alloc(&stats, (size_t)(3 + 2 * parts) * piece * es);
+  const int64_t tail = q.R % piece;
+  int64_t parts = stats_parts(dtype, q.tied, piece, q.V, q.C);
+  if (tail) {
+    const int64_t p = stats_parts(dtype, q.tied, tail, q.V, q.C);
+    parts = p > parts ? p : parts;
   }
-  if (!rc)
-    rc = dtype == DTMI_F32 ? lxent_pieces<float>(dtype, q, piece, (char*)Z, (char*)stats)
-                           : lxent_pieces<double>(dtype, q, piece, (char*)Z, (char*)stats);
-  if (stats) pool_free(stats);
-  if (Z) pool_free(Z);
-  if (own) pool_free(own);
-  return rc;
+  rc = pool_alloc(&stats.p, (size_t)((3 + 2 * parts) * piece * es));
+  return rc ? rc : lxent_pieces<T>(dtype, q, piece, (char*)Z.p, (char*)stats.p);
+}
+
+struct ScaleArgs {
+  void* p[3];
+  int64_t n[3];
+};
+
+// blockIdx.y: the array. Leaves at once for a factor of 1.
+template <typename T>
+__global__ void __launch_bounds__(256) grad_scale_kernel(ScaleArgs a, const T* __restrict__ g) {
+  const T f = g[0];
+  if (f == T(1)) return;
+  constexpr int V = 16 / (int)sizeof(T);
+  typedef T vt __attribute__((ext_vector_type(V)));
+  T* p = (T*)a.p[blockIdx.y];
+  const int64_t n = a.n[blockIdx.y], nv = aligned(p, 16) ? n / V : 0, stride = (int64_t)gridDim.x * 256;
+  const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = i0; i < nv; i += stride) reinterpret_cast<vt*>(p)[i] *= f;
+  for (int64_t i = nv * V + i0; i < n; i += stride) p[i] *= f;
 }
 
 // out row rows[i] = in row i; one wave a row.
@@ -302,7 +328,34 @@ DTMI_EXPORT int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, con
   DTMI_CHECK(targets && (C == 0 || (X && W)), "%s: NULL pointer", __func__);
   LxentArgs q{R, C, V, (const char*)X, (const char*)W, tied ? 1 : 0, b, targets, (char*)losses, mean, (const char*)g,
               g_stride, coef, (char*)dX, (char*)dW, (char*)db};
-  return lxent_run(dtype, q);
+  return dtype == DTMI_F32 ? lxent_run<float>(dtype, q) : lxent_run<double>(dtype, q);
+  DTMI_BODY_END
+}
+
+DTMI_EXPORT int dtmi_grad_scale_multi(int dtype, int n, void* const* ptrs, const int64_t* counts, const void* g_dev) {
+  DTMI_BODY_BEGIN
+  DTMI_REQUIRE_INIT();
+  DTMI_DTYPE_OK(dtype);
+  DTMI_CHECK(n >= 1 && n <= 3 && ptrs && counts && g_dev, "%s: 1 to 3 arrays and a factor", __func__);
+  ScaleArgs a{};
+  int64_t most = 0, total = 0;
+  for (int i = 0; i < n; ++i) {
+    DTMI_CHECK(counts[i] >= 0 && (counts[i] == 0 || ptrs[i]), "%s: bad array %d", __func__, i);
+    a.p[i] = ptrs[i];
+    a.n[i] = counts[i];
+    most = counts[i] > most ? counts[i] : most;
+    total += counts[i];
+  }
+  if (!most) return DTMI_OK;
+  TimedLaunch tl(DTMI_FAM_OTHER, 2.0 * (double)total * (dtype == DTMI_F32 ? 4 : 8));
+  const int64_t blocks = cdiv(most, 4096);
+  const dim3 grid((unsigned)(blocks < 2048 ? blocks : 2048), (unsigned)n);
+  if (dtype == DTMI_F32)
+    grad_scale_kernel<float><<<grid, 256, 0, stream()>>>(a, (const float*)g_dev);
+  else
+    grad_scale_kernel<double><<<grid, 256, 0, stream()>>>(a, (const double*)g_dev);
+  LAUNCH_CHECK("grad_scale_kernel");
+  return DTMI_OK;
   DTMI_BODY_END
 }
 

@@ -234,26 +234,46 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
                            0, stream()>>>(a);
     LAUNCH_CHECK("norm kernels");
   }
-  std::vector<GroupTask> gram(n), sq(n), ap(n);
-  for (int s = 0; s < q.steps; ++s) {
-    const bool last = s + 1 == q.steps;
-    for (int i = 0; i < n; ++i) {
-      const int j = live[i], tall = q.rows[j] > q.cols[j];
-      const int m = (int)(tall ? q.cols[j] : q.rows[j]), w = (int)(tall ? q.rows[j] : q.cols[j]);
-      gram[i] = {x0[i], x0[i], G[i], nullptr, m, m, w, 0, 1.0};  // G = X X^T
-      sq[i] = {G[i], G[i], H[i], G[i], m, m, m, 0, 1.0};         // H = b G + c G G (G = G^T)
-      // X = a X + H X, the last into the result
-      ap[i] = {H[i], x0[i], last ? (char*)q.out[j] : x1[i], x0[i], m, w, m, last && tall,
-               last && q.rate ? q.rate[j] : 1.0};
+  // the launches of a step from x0 to x1 and of one from x1 to x0, and of the last
+  std::vector<GroupTask> t(n);
+  std::vector<GroupLaunch> gram[2], sq, apply[2], final;
+  auto of = [&](int i, int& m, int& w) {
+    const int64_t r = q.rows[live[i]], c = q.cols[live[i]];
+    m = (int)(r < c ? r : c);
+    w = (int)(r < c ? c : r);
+    return r > c;
+  };
+  int m, w, rc = DTMI_OK;
+  for (int i = 0; i < n; ++i) {  // H = b G + c G G (G = G^T)
+    of(i, m, w);
+    t[i] = {G[i], G[i], H[i], G[i], m, m, m, 0, 1.0};
+  }
+  rc = plan_group(dtype, 1, 1, t, kDMatrix, 1, q.c, q.b, 0.0, V, V, sq);
+  for (int odd = 0; odd < 2 && odd < q.steps && !rc; ++odd) {
+    for (int i = 0; i < n; ++i) {  // G = X X^T
+      of(i, m, w);
+      t[i] = {x0[i], x0[i], G[i], nullptr, m, m, w, 0, 1.0};
     }
-    int rc = run_group(dtype, 1, 1, gram.data(), n, kDNone, 1, 1.0, 0.0, 0.0, V, V);
-    if (!rc) rc = run_group(dtype, 1, 1, sq.data(), n, kDMatrix, 1, q.c, q.b, 0.0, V, V);
-    if (!rc)
-      rc = run_group(dtype, 1, 0, ap.data(), n, kDMatrix, 0, 1.0, q.a, last && q.rate ? q.gamma : 0.0, V, last ? 1 : V);
-    if (rc) return rc;
+    rc = plan_group(dtype, 1, 1, t, kDNone, 1, 1.0, 0.0, 0.0, V, V, gram[odd]);
+    const bool ends = (q.steps - 1) % 2 == odd;
+    for (int end = 0; end < 2 && !rc; ++end) {  // X = a X + H X, the last into the result
+      if (end ? !ends : q.steps < odd + 2) continue;
+      for (int i = 0; i < n; ++i) {
+        const bool tall = of(i, m, w);
+        t[i] = {H[i], x0[i], end ? (char*)q.out[live[i]] : x1[i], x0[i], m, w, m, end && tall,
+                end && q.rate ? q.rate[live[i]] : 1.0};
+      }
+      rc = plan_group(dtype, 1, 0, t, kDMatrix, 0, 1.0, q.a, end && q.rate ? q.gamma : 0.0, V, end ? 1 : V,
+                      end ? final : apply[odd]);
+    }
     std::swap(x0, x1);
   }
-  return DTMI_OK;
+  for (int s = 0; s < q.steps && !rc; ++s) {
+    rc = launch_group(dtype, gram[s % 2]);
+    if (!rc) rc = launch_group(dtype, sq);
+    if (!rc) rc = launch_group(dtype, s + 1 == q.steps ? final : apply[s % 2]);
+  }
+  return rc;
 }
 
 static int newton(const char* what, int dtype, const NewtonArgs& q) {

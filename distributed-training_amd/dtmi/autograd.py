@@ -323,7 +323,7 @@ class Indices:
     computed on first use and kept with it.
     """
 
-    __slots__ = ("host", "dev", "shape", "_segs", "_lo", "_hi")
+    __slots__ = ("host", "dev", "shape", "_segs", "_rows", "_lo", "_hi")
 
     def __init__(self, idx):
         self.host = np.asarray(idx)
@@ -333,7 +333,7 @@ class Indices:
         self._lo = int(self.host.min()) if self.host.size else 0
         self._hi = int(self.host.max()) if self.host.size else -1
         self.dev = dev.from_numpy(self.host.reshape(-1).astype(np.int64))
-        self._segs = None
+        self._segs = self._rows = None
 
     def check(self, n: int, what: str, allow_negative: bool):
         lo = -n if allow_negative else 0
@@ -352,6 +352,12 @@ class Indices:
         if self._segs is None:
             self._segs = K.embedding_segments(self.dev)
         return self._segs
+
+    def expert_rows(self):
+        """The host values as the rows of expert_linear's experts, checked once."""
+        if self._rows is None:
+            self._rows = K.ExpertRows(self.host)
+        return self._rows
 
 
 def as_indices(idx) -> Indices:
@@ -459,9 +465,8 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
     not read there. `reduction` "mean" gives the mean over the others (0 if there are
     none), "none" the loss of every row, which without gradients (`no_grad()`) is minus
     the log probability of its target: no logit is written then. The gradients of a mean
-    are computed by the forward pass, as cross_entropy's are, from the logits of up to
-    2048 rows at a time; those of single losses by backward, which forms the logits
-    again."""
+    are computed by the forward pass, as cross_entropy's are, from about 1 GiB of logits
+    at a time; those of single losses by backward, which forms the logits again."""
     if reduction not in ("mean", "none"):
         raise ValueError(f"linear_cross_entropy: reduction must be 'mean' or 'none', not {reduction!r}")
     X = _contig(x.data)
@@ -480,19 +485,23 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
         raise TypeError("indices must be integers")
     if host.shape != lead:
         raise ValueError(f"linear_cross_entropy: targets of shape {host.shape} for x {x.shape}")
-    host = host.reshape(-1)
     rows = host.size
+    lo, hi = (ix._lo, ix._hi) if ix is not None else (host.min(), host.max()) if rows else (0, -1)
     X2 = X.reshape(rows, C)
-    keep = None if ignore is None else host != ignore
     sel = None
-    if keep is not None and not keep.all():
-        # the rows that count, by themselves
-        sel = dev.from_numpy(np.flatnonzero(keep).astype(np.int64))
-        host = host[keep]
-        X2 = K.embedding_fwd(X2, sel, (host.size,))
-    if host.size and (host.min() < 0 or host.max() >= V):
+    if ignore is not None and lo <= ignore <= hi:
+        host = host.reshape(-1)
+        at = np.flatnonzero(host != ignore)
+        if at.size < rows:  # the rows that count, by themselves
+            host = host[at]
+            lo, hi = (host.min(), host.max()) if host.size else (0, -1)
+            ix = None
+    if lo < 0 or hi >= V:
         raise IndexError(f"target out of bounds for size {V}")
-    t = ix.dev if ix is not None and sel is None else dev.from_numpy(host.astype(np.int64))
+    if host.size < rows:
+        sel = dev.from_numpy(at.astype(np.int64))
+        X2 = K.embedding_fwd(X2, sel, (host.size,))
+    t = ix.dev if ix is not None else dev.from_numpy(host.reshape(-1).astype(np.int64))
     n = host.size
     mean = reduction == "mean"
     coef = 1.0 / n if mean and n else 1.0
@@ -505,20 +514,16 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
         return d if sel is None else K.scatter_rows(d.reshape(n, cols), sel, rows)
     pending = [made] if mean and any(need) else []
 
-    def scaled(d, g, dest):
-        if dest is None or d.shape != dest.shape:
-            return K.xent_grad_scale(d, g)
-        return K.scale(d, alpha_dev=g, out=dest)
-
     def bw(g):
         if mean:
             g1 = _contig(g).reshape(1)
-            dest = None if tied else grad_out(w), grad_out(b) if b is not None else None
             if pending:
-                dx, dw, db = pending.pop()
-                dx = K.xent_grad_scale(dx, g1) if dx is not None else None
-                dw = scaled(dw, g1, dest[0]) if dw is not None else None
-                db = scaled(db, g1, dest[1]) if db is not None else None
+                # into their destinations, or in place
+                made, dests = list(pending.pop()), (None, None if tied else grad_out(w),
+                                                    grad_out(b) if b is not None else None)
+                K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], g1)
+                dx, dw, db = [d if o is None or d is None else K.scale(d, alpha_dev=g1, out=o)
+                              for d, o in zip(made, dests)]
             else:
                 dx, dw, db = K.linear_xent(X2, W, bd, t, tied, coef, g=g1, **grads)[2:]
         else:
@@ -543,7 +548,10 @@ def expert_linear(x: Tensor, w: Tensor, sizes, b: Tensor | None = None) -> Tenso
     X, W = _contig(x.data), _contig(w.data)
     if X.ndim != 2:
         raise ValueError(f"expert_linear: x must be [rows, {w.shape[1] if len(w.shape) == 3 else 'K'}], not {x.shape}")
-    n = sizes.host if isinstance(sizes, Indices) else np.array(sizes)
+    if isinstance(sizes, Indices):
+        n = sizes.expert_rows()
+    else:
+        n = K.ExpertRows(sizes)
     y = K.expert_linear_fwd(X, W, n, _contig(b.data) if b is not None else None)
 
     def bw(g):

@@ -953,54 +953,64 @@ def scatter_rows(x2: DeviceArray, rows: DeviceArray, total: int) -> DeviceArray:
     return out
 
 
-def _expert_check(what, rows, w, sizes, K, N):
-    """E and the sizes as int64_t[]; sizes: host whole numbers, one per expert."""
+class ExpertRows:
+    """The rows each expert has, checked: host whole numbers, none negative."""
+
+    __slots__ = ("shape", "used", "c_sizes")
+
+    def __init__(self, sizes):
+        sizes = np.asarray(sizes)
+        if sizes.size and not np.issubdtype(sizes.dtype, np.integer):
+            raise TypeError("expert_linear: sizes must be integers")
+        self.shape = sizes.shape
+        n = [int(x) for x in sizes.reshape(-1).tolist()]
+        if n and min(n) < 0:
+            raise ValueError("expert_linear: negative size")
+        self.used = sum(n)
+        self.c_sizes = _lib.i64_array(n) if self.used < 2 ** 62 else None
+
+
+def _expert_check(rows: int, w: DeviceArray, sizes: ExpertRows, K, N):
     if w.ndim != 3 or (K is not None and w.shape[1] != K) or (N is not None and w.shape[2] != N):
-        raise ValueError(f"{what}: w must be [experts, {K}, {N}], not {w.shape}")
-    sizes = np.asarray(sizes)
-    if sizes.shape != (w.shape[0],):
-        raise ValueError(f"{what}: sizes must have one entry for each of the {w.shape[0]} experts, not shape {sizes.shape}")
-    if sizes.size and not np.issubdtype(sizes.dtype, np.integer):
-        raise TypeError(f"{what}: sizes must be integers")
-    sizes = sizes.astype(np.int64)
-    if sizes.size and sizes.min() < 0:
-        raise ValueError(f"{what}: negative size")
-    if sum(sizes.tolist()) > rows:
-        raise ValueError(f"{what}: sizes add up to {sum(sizes.tolist())}, more than the {rows} rows")
-    return _lib.i64_array(sizes)
+        raise ValueError(f"expert_linear: w must be [experts, {K}, {N}], not {w.shape}")
+    if sizes.shape != w.shape[:1]:
+        raise ValueError(f"expert_linear: sizes must have one entry for each of the {w.shape[0]} experts, not shape "
+                         f"{sizes.shape}")
+    if sizes.used > rows:
+        raise ValueError(f"expert_linear: sizes add up to {sizes.used}, more than the {rows} rows")
 
 
-def expert_linear_fwd(x: DeviceArray, w: DeviceArray, sizes, b: DeviceArray | None = None) -> DeviceArray:
-    """y [R, N] = x [R, K] @ w[e] (+ b[e]), the first sizes[0] rows with expert 0's, ..."""
+def expert_linear_fwd(x: DeviceArray, w: DeviceArray, sizes: ExpertRows, b: DeviceArray | None = None) -> DeviceArray:
+    """y [R, N] = x [R, K] @ w[e] (+ b[e]), the first rows with expert 0's, ..."""
     d = _dt(x, w)
     _contig(x, w)
     R, K_ = x.shape
-    s = _expert_check("expert_linear", R, w, sizes, K_, None)
+    _expert_check(R, w, sizes, K_, None)
     E, _, N = w.shape
     if b is not None:
         _same(b, (E, N), x.dtype, "expert_linear: b")
     y = empty((R, N), x.dtype)
-    _c("dtmi_expert_linear_fwd", d, E, R, K_, N, y.ptr, x.ptr, w.ptr, _opt_ptr(b), s)
+    _c("dtmi_expert_linear_fwd", d, E, R, K_, N, y.ptr, x.ptr, w.ptr, _opt_ptr(b), sizes.c_sizes)
     return y
 
 
-def expert_linear_bwd(x: DeviceArray, w: DeviceArray, g: DeviceArray, sizes, need_dx=True, need_dw=True,
+def expert_linear_bwd(x: DeviceArray, w: DeviceArray, g: DeviceArray, sizes: ExpertRows, need_dx=True, need_dw=True,
                       need_db=True, dw_out: DeviceArray | None = None, db_out: DeviceArray | None = None):
     """Returns (dx, dw, db), None where not asked for."""
+    d = _dt(x, w, g)
     _contig(x, w, g)
     R, K_ = x.shape
     E, _, N = w.shape
-    s = _expert_check("expert_linear", R, w, sizes, K_, N)
+    _expert_check(R, w, sizes, K_, N)
     _same(g, (R, N), x.dtype, "expert_linear: g")
-    d = _dt(x, w, g)
     dx = dw = db = None
     if need_dx:
         dx = empty(x.shape, x.dtype)
-        _c("dtmi_expert_linear_bwd_dx", d, E, R, K_, N, dx.ptr, g.ptr, w.ptr, s)
+        _c("dtmi_expert_linear_bwd_dx", d, E, R, K_, N, dx.ptr, g.ptr, w.ptr, sizes.c_sizes)
     if need_dw or need_db:
         dw = _out_or_new(dw_out, w.shape, x.dtype, "expert_linear")
         db = _out_or_new(db_out, (E, N), x.dtype, "expert_linear") if need_db else None
-        _c("dtmi_expert_linear_bwd_dw", d, E, R, K_, N, dw.ptr, _opt_ptr(db), x.ptr, g.ptr, s)
+        _c("dtmi_expert_linear_bwd_dw", d, E, R, K_, N, dw.ptr, _opt_ptr(db), x.ptr, g.ptr, sizes.c_sizes)
     return dx, dw if need_dw else None, db
 
 
@@ -1028,9 +1038,19 @@ class Matrices:
         """One pointer per matrix of arrays that are shaped as these."""
         ptrs = []
         for a, k in zip(arrays, self.per):
-            step = a.nbytes // k if k else 0
-            ptrs += [a.ptr + i * step for i in range(k)]
-        return _lib.ptr_array(ptrs)
+            p = a.ptr
+            if k == 1:
+                ptrs.append(p)
+            elif k:
+                step = a.nbytes // k
+                ptrs += [p + i * step for i in range(k)]
+        return (C.c_void_p * max(1, self.n))(*ptrs)
+
+    def check(self, arrays, what: str):
+        """ValueError unless the arrays have these ones' shapes and type, and no gaps."""
+        for p, a in zip(self.arrays, arrays):
+            if a.shape != p.shape or a.dtype != p.dtype or not a.is_contiguous:
+                _same(a, p.shape, p.dtype, what)
 
 
 def newton_schulz(ins: Matrices, outs, steps: int, coefficients, eps: float):
@@ -1039,14 +1059,23 @@ def newton_schulz(ins: Matrices, outs, steps: int, coefficients, eps: float):
        c, float(eps))
 
 
-def muon(ps: Matrices, gs, ms, rates, keep: float, momentum: float, nesterov: bool, steps: int, coefficients,
+def muon(ps: Matrices, gs, m_ptrs, rates, keep: float, momentum: float, nesterov: bool, steps: int, coefficients,
          eps: float, gscale: float = 1.0, gscale_dev: DeviceArray | None = None):
-    """p = keep p - rates[i] NS(u), see dtmi_muon; gs, ms: arrays shaped as ps's."""
-    for p, g, m in zip(ps.arrays, gs, ms):
-        _same(g, p.shape, p.dtype, "muon: gradient")
-        _same(m, p.shape, p.dtype, "muon: momentum")
-    a, b, c = (float(x) for x in coefficients)
-    rate = (C.c_double * max(1, ps.n))(*[float(r) for r in rates])
-    _c("dtmi_muon", ps.dtype, ps.n, ps.c_ptrs, ps.pointers(gs), ps.pointers(ms), ps.c_rows, ps.c_cols, rate, float(keep),
-       float(momentum), 1 if nesterov else 0, int(steps), a, b, c, float(eps), float(gscale),
-       gscale_dev.ptr if gscale_dev is not None else None)
+    """p = keep p - rates[i] NS(u), see dtmi_muon; gs: arrays shaped as ps's, m_ptrs: the
+    momenta's pointers (ps.pointers)."""
+    ps.check(gs, "muon: gradient")
+    a, b, c = coefficients
+    rate = (C.c_double * max(1, ps.n))(*rates)
+    _c("dtmi_muon", ps.dtype, ps.n, ps.c_ptrs, ps.pointers(gs), m_ptrs, ps.c_rows, ps.c_cols, rate, keep, momentum,
+       1 if nesterov else 0, steps, a, b, c, eps, gscale, gscale_dev.ptr if gscale_dev is not None else None)
+
+
+def grad_scale_multi(arrays, g: DeviceArray):
+    """Each array (up to 3, None left out) times g[0] in place unless g[0] == 1."""
+    arrays = [a for a in arrays if a is not None and a.size]
+    if not arrays:
+        return
+    _contig(*arrays)
+    _same(g, (1,), arrays[0].dtype, "grad_scale: g")
+    _c("dtmi_grad_scale_multi", _dt(*arrays), len(arrays), _lib.ptr_array([a.ptr for a in arrays]),
+       _lib.i64_array([a.size for a in arrays]), g.ptr)

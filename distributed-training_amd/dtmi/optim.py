@@ -119,7 +119,7 @@ class Muon:
                  coefficients=NEWTON_SCHULZ, eps=1e-7):
         self.params = list(params)
         self.lr, self.momentum, self.nesterov, self.wd = lr, momentum, nesterov, weight_decay
-        self.steps, self.coefficients, self.eps = steps, tuple(coefficients), eps
+        self.steps, self.coefficients, self.eps = steps, tuple(float(c) for c in coefficients), eps
         self._all = K.Matrices(self.params, "Muon")
         self._mflat = dev.zeros((max(sum(p.size for p in self.params), 1),),
                                 self.params[0].dtype if self.params else np.float32)
@@ -127,6 +127,7 @@ class Muon:
         for p in self.params:
             self.m.append(self._mflat[off:off + p.size].reshape(p.shape))
             off += p.size
+        self._m_ptrs = self._all.pointers(self.m)
 
     def step(self, grads, grad_scale=1.0):
         """grads: a DeviceArray or None (the parameter stays as it is) per parameter;
@@ -135,16 +136,16 @@ class Muon:
         if len(grads) != len(self.params):
             raise ValueError(f"Muon: {len(grads)} gradients for {len(self.params)} parameters")
         gs_dev = grad_scale if isinstance(grad_scale, DeviceArray) else None
-        ps, ms = self._all, self.m
+        ps, mp = self._all, self._m_ptrs
         if any(g is None for g in grads):
             live = [i for i, g in enumerate(grads) if g is not None]
             ps = K.Matrices([self.params[i] for i in live], "Muon")
-            ms, grads = [self.m[i] for i in live], [grads[i] for i in live]
+            mp, grads = ps.pointers([self.m[i] for i in live]), [grads[i] for i in live]
         if not ps.n:
             return
         rates = [self.lr * max(1.0, n / k) ** 0.5 for k, n in zip(ps.rows, ps.cols)]
-        K.muon(ps, grads, ms, rates, 1.0 - self.lr * self.wd, self.momentum, self.nesterov, self.steps,
-               self.coefficients, self.eps, 1.0 if gs_dev is not None else float(grad_scale), gs_dev)
+        K.muon(ps, grads, mp, rates, 1.0 - self.lr * self.wd, float(self.momentum), self.nesterov, int(self.steps),
+               self.coefficients, float(self.eps), 1.0 if gs_dev is not None else float(grad_scale), gs_dev)
 
     def state_bytes(self):
         return sum(a.nbytes for a in self.m)

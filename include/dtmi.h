@@ -506,11 +506,14 @@ int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int6
  *   dz[r, v] = coef * g[r g_stride] * (exp(z - m_r) / s_r - [v = t_r])  (g NULL: 1)
  *   dX = dz W^T, dW = X^T dz (tied: its transpose [V, C]), db = sum_r dz
  * losses, mean, dX, dW and db may be NULL. Without gradients no logit is written; with
- * any, those of up to 2048 rows at a time are, in a pooled workspace (fewer rows where
- * it cannot be allocated). R = 0: mean, dW and db are 0. C and V below 2^22. */
+ * any, about 1 GiB of them at a time are (1024 rows at least), in a pooled workspace (fewer
+ * where it cannot be allocated). R = 0: mean, dW and db are 0. C and V below 2^22. */
 int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, const void* X, const void* W, int tied,
                      const void* b, const int64_t* targets, void* losses, void* mean, const void* g,
                      int64_t g_stride, double coef, void* dX, void* dW, void* db);
+/* dtmi_xent_grad_scale for 1 to 3 arrays in one launch: each times *g_dev unless that is
+ * exactly 1. */
+int dtmi_grad_scale_multi(int dtype, int n, void* const* ptrs, const int64_t* counts, const void* g_dev);
 /* out [total, cols] = 0, then row rows[i] = in[i] for i < n (in [n, cols], rows int64 in
  * device memory, each once; those outside 0..total-1 are left out). */
 int dtmi_scatter_rows(int dtype, void* out, const void* in, const int64_t* rows, int64_t n, int64_t total,

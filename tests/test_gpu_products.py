@@ -133,17 +133,35 @@ def test_loss(dev, dt, reduction, case):
         assert not grads[0].numpy()[t < 0].any()
 
 
-def test_loss_over_pieces_of_rows(dev):
-    """More rows than a piece (2048) holds, their number no multiple of anything."""
-    case = (4999, 40, 129, True, False, 1300)
+@pytest.mark.parametrize("case", [
+    (3000, 12, 50001, True, False, 300),   # float64: three pieces of logits
+    (1100, 9, 130003, False, True, 0),     # a vocabulary of which a piece is the fewest rows
+], ids=["three", "fewest"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_loss_over_pieces_of_rows(dev, case, reduction):
+    """More logits than a piece holds (1 GiB, 1024 rows at least)."""
+    g = None if reduction == "mean" else np.random.default_rng(1).standard_normal(case[0])
+    (x, w, b, t), y, grads = loss_run(case, F64, reduction, g)
+    ry, rg = loss_ref(x, w, b, t, case[4], reduction, g)
+    by, bx, bw = loss_bars(case[1], case[0], case[2])
+    close(y, ry, F64, by, "loss")
+    for got, want, n, name in zip(grads, rg, (bx, bw, bw), ("dx", "dw", "db")):
+        close(got, want, F64, n, name)
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("C,V", [(37, 131), (36, 131), (37, 132)])
+def test_loss_of_odd_sizes_and_many_rows(dev, dt, tied, C, V):
+    case = (1030, C, V, True, tied, 13)
     for reduction in ("mean", "none"):
-        g = None if reduction == "mean" else np.random.default_rng(1).standard_normal(case[0])
-        (x, w, b, t), y, grads = loss_run(case, F64, reduction, g)
-        ry, rg = loss_ref(x, w, b, t, False, reduction, g)
-        by, bx, bw = loss_bars(case[1], case[0], case[2])
-        close(y, ry, F64, by, "loss")
+        g = None if reduction == "mean" else np.random.default_rng(1).standard_normal(case[0]).astype(dt)
+        (x, w, b, t), y, grads = loss_run(case, dt, reduction, g)
+        ry, rg = loss_ref(x, w, b, t, tied, reduction, g)
+        by, bx, bw = loss_bars(C, 1030, V)
+        close(y, ry, dt, by, "loss")
         for got, want, n, name in zip(grads, rg, (bx, bw, bw), ("dx", "dw", "db")):
-            close(got, want, F64, n, (reduction, name))
+            close(got, want, dt, n, (reduction, name))
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
