@@ -41,9 +41,9 @@ static int run(int dtype, int akc, int bkc, std::vector<GroupTask> tasks, int dm
   return rc ? rc : launch_group(dtype, l);
 }
 
-// rows of an [R, cols] result that no expert owns
-static int zero_tail(int dtype, void* p, int64_t used, int64_t R, int64_t cols) {
-  return used < R ? dtmi_fill(dtype, at(p, used * cols, dtype), 0.0, (R - used) * cols) : DTMI_OK;
+// Rows of an [R, cols] result that no expert owns: a product of no terms.
+static void add_tail(int dtype, void* p, int64_t used, int64_t R, int64_t cols, std::vector<GroupTask>& t) {
+  if (used < R) t.push_back({p, p, at(p, used * cols, dtype), nullptr, (int)(R - used), (int)cols, 0, 0, 1.0});
 }
 
 }  // namespace dtmi
@@ -66,8 +66,8 @@ DTMI_EXPORT int dtmi_expert_linear_fwd(int dtype, int64_t E, int64_t R, int64_t 
     t.push_back({at(x, off[e] * K, dtype), at(w, e * K * N, dtype), at(y, off[e] * N, dtype),
                  at(const_cast<void*>(b), e * N, dtype), (int)(off[e + 1] - off[e]), (int)N, (int)K, 0, 1.0});
   }
-  rc = run(dtype, 1, 0, std::move(t), b ? kDRow : kDNone);
-  return rc ? rc : zero_tail(dtype, y, off[E], R, N);
+  add_tail(dtype, y, off[E], R, N, t);
+  return run(dtype, 1, 0, std::move(t), b ? kDRow : kDNone);
   DTMI_BODY_END
 }
 
@@ -87,8 +87,8 @@ DTMI_EXPORT int dtmi_expert_linear_bwd_dx(int dtype, int64_t E, int64_t R, int64
     t.push_back({at(g, off[e] * N, dtype), at(w, e * K * N, dtype), at(dx, off[e] * K, dtype), nullptr,
                  (int)(off[e + 1] - off[e]), (int)K, (int)N, 0, 1.0});
   }
-  rc = run(dtype, 1, 1, std::move(t), kDNone);
-  return rc ? rc : zero_tail(dtype, dx, off[E], R, K);
+  add_tail(dtype, dx, off[E], R, K, t);
+  return run(dtype, 1, 1, std::move(t), kDNone);
   DTMI_BODY_END
 }
 

@@ -63,8 +63,6 @@ struct GroupArgs {
 // Row statistics of Z = A B + bias over pieces of its columns, without Z (or with it,
 // where C is not NULL): part p of row m covers some columns (half a block tile's), pmax[p
 // M + m] is their maximum and psum[p M + m] the sum of exp(z - pmax) over them; zt[m] =
-// Z[m, targets[m]]. B has nz >= N columns (rows where k is contiguous): those past N are
-// read and not used, and set to -inf in C.
 struct StatsArgs {
   const void* A;
   const void* B;
@@ -74,7 +72,7 @@ struct StatsArgs {
   void* psum;
   void* zt;
   const int64_t* targets;
-  int64_t M, N, K, lda, ldb, ldc, nz;
+  int64_t M, N, K, lda, ldb, ldc;
   int tiles_m, tiles_n;
 };
 

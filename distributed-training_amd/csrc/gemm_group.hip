@@ -29,11 +29,11 @@ static int rows_waves(int64_t blocks, int64_t K, int64_t cus, int mr, int bkc) {
   return (int)(w < batches ? w : batches);
 }
 
-// Waves of a small-product block: 16 per CU, each with at least a batch of k.
+// Waves of a small-product block: 8 per CU, each with at least a batch of k.
 template <typename T>
 static int direct_waves(int64_t tiles, int64_t K, int64_t cus) {
   int64_t w = 4;
-  while (w < kDirectMaxWaves<T> && tiles * w < 16 * cus) w *= 2;
+  while (w < kDirectMaxWaves<T> && tiles * w < 8 * cus) w *= 2;
   const int64_t batches = cdiv(K > 0 ? K : 1, kDirectBatch<T>);
   return (int)(w < batches ? w : batches);
 }
@@ -49,10 +49,12 @@ static double direct_cycles(int64_t tiles, double kavg, int64_t kmax, int nw, in
 
 // SIMD cycles of `units` blocks on BM-wide tiles, the busiest CU's k being `k`: as
 // tile_cost in gemm.hip (64-wide float32 tiles over several tasks reach less, 0.80 to
-// 0.89 of their MFMA rate).
+// 0.89 of their MFMA rate), with what a block costs before its first MFMA and after its
+// last, of which the others on its CU hide some: 64 experts' dw, 384 x 501 from 62 rows
+// each, took 42 us on 3072 64-wide tiles.
 static double tile_cycles(int bm, double k, double units, int64_t cus, size_t es) {
   const double eff = bm == 64 ? (units > cus ? (es == 4 ? 0.82 : 0.88) : 0.75) : units > 2.0 * cus ? 0.97 : units > cus ? 1.0 : 0.82;
-  return 8800.0 + k * (es == 4 ? 32.0 : 64.0) * (bm / 32) * (bm / 32) / 4.0 / eff;
+  return 8800.0 + 1500.0 * units / (double)cus + k * (es == 4 ? 32.0 : 64.0) * (bm / 32) * (bm / 32) / 4.0 / eff;
 }
 // and what a split adds: its partials' traffic and a launch
 static double split_cycles(int bm, int64_t cut, int splits, size_t es) {
@@ -93,6 +95,7 @@ static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, in
       if (n[i]) last = i;
     }
     if (!total) return best;
+    while (last > 0 && (k[last] == 0 || n[last] == 0)) --last;  // the shortest with anything to add up
     const bool equal = k[0] == k[last];
     // one chain of float32 sums: at most 4096 k on 128-wide tiles (64-wide ones fold theirs)
     const int64_t chain = bm == 128 && es == 4 ? 4096 : 1LL << 40;
@@ -168,7 +171,7 @@ static int plan_tasks(int akc, int bkc, std::vector<GroupTask>& tasks, int dmode
                  "group of products: rows of 2^24 bytes or more are not supported");
       vec = vec && lda % V == 0 && ldb % V == 0 && aligned(t.A, 16) && aligned(t.B, 16) &&
             (!sym || (cdiv(t.N, padc) * padc % V == 0 && aligned(t.C, 16)));
-      rows = t.M > rows ? t.M : rows;
+      if (t.K > 0 && t.M > rows) rows = t.M;  // (products of no terms only write)
       l.flops += (sym ? 1.0 : 2.0) * (double)t.M * t.N * t.K;
     }
     l.vec = vec;
@@ -183,7 +186,7 @@ static int plan_tasks(int akc, int bkc, std::vector<GroupTask>& tasks, int dmode
     int64_t tiles = 0;
     for (int i = 0; i < a.count; ++i) {
       const int64_t tm = cdiv(a.t[i].M, tm_rows), tn = cdiv(a.t[i].N, tn_cols);
-      a.equal = a.equal && a.t[i].K == a.t[0].K;
+      a.equal = a.equal && (a.t[i].K == a.t[0].K || a.t[i].K == 0);
       a.first[i] = (int)tiles;
       tiles += sym ? tm * (tm + 1) / 2 : tm * tn;
       DTMI_CHECK(tiles < (1LL << 26), "group of products: too large");
@@ -301,7 +304,7 @@ static int stats_launch(int bkc, StatsArgs& a) {
              "statistics product: rows of 2^24 bytes or more are not supported");
   const GroupPlan p = plan_stats<T>(bkc, a.M, a.N, a.K);
   const bool vec = aligned(a.A, 16) && aligned(a.B, 16) && a.lda % V == 0 && a.ldb % V == 0 && a.K % V == 0 &&
-                   (bkc || a.nz % V == 0);
+                   (bkc || a.N % V == 0);
   DTMI_CHECK(cdiv(a.M, p.tile) * cdiv(a.N, p.tile) < (1LL << 30), "statistics product: too large");
   const int mr = a.M <= 16 ? 1 : 2;
   a.tiles_m = p.tile == 16 ? 1 : (int)cdiv(a.M, p.tile);

@@ -80,7 +80,7 @@ struct GroupEpi {
 template <typename T>
 __device__ __forceinline__ GroupEpi<T> group_epi(const GroupArgs& a, const GroupTask& k, bool mirror) {
   const bool zeros = a.padc == a.pad;
-  return {(T)a.alpha, (T)a.beta, (T)a.gamma, (T)k.s, a.dmode, mirror, k.turned != 0, (const T*)k.D, (T*)k.C,
+  return {(T)a.alpha, (T)a.beta, (T)a.gamma, (T)k.s, k.D ? a.dmode : (int)kDNone, mirror, k.turned != 0, (const T*)k.D, (T*)k.C,
           (int64_t)pad_up(k.N, a.pad), (int64_t)pad_up(k.turned ? k.M : k.N, a.padc),
           zeros ? pad_up(k.M, a.pad) : k.M, zeros ? pad_up(k.N, a.pad) : k.N};
 }
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(256, 2) gemm_stats_kernel(StatsArgs a) {
 #pragma unroll
     for (int j = 0; j < TW; ++j) acc[i][j] = typename MFT::acc_t(0);
   double csum = 0.0;
-  dma_product<T, BM, BM, true, BKC, VEC, VEC>(acc, lds, (const T*)a.A, a.lda, a.M, m0, (const T*)a.B, a.ldb, a.nz, n0,
+  dma_product<T, BM, BM, true, BKC, VEC, VEC>(acc, lds, (const T*)a.A, a.lda, a.M, m0, (const T*)a.B, a.ldb, a.N, n0,
                                               0, a.K, sizeof(T) == 4 ? 2 : 4, false, csum);
   const int64_t wm = m0 + (wave >> 1) * W, wn = n0 + (wave & 1) * W;
   T* C = (T*)a.C;
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(256, 2) gemm_stats_kernel(StatsArgs a) {
         const int row = MFT::row(r, g);
         const T z = a.bias ? acc[i][j][r] + b : acc[i][j][r];
         R[row * LD + j * MT + c] = in ? z : -INFINITY;
-        if (C && n < a.nz && wm + i * MT + row < a.M) C[(wm + i * MT + row) * a.ldc + n] = in ? z : -INFINITY;
+        if (C && in && wm + i * MT + row < a.M) C[(wm + i * MT + row) * a.ldc + n] = z;
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(64 * kDirectMaxWaves<T>) stats_direct_kernel(S
 #pragma unroll
     for (int o = MT / 2; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
     if (m < a.M) {
-      if (C && n < a.nz) C[m * a.ldc + n] = z;
+      if (C && in) C[m * a.ldc + n] = z;
       if (a.targets && a.targets[m] == n) ((T*)a.zt)[m] = z;
       const int64_t p = (int64_t)tn * R + j;
       if (c == 0) {
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1
       z[t] = in ? v : -INFINITY;
       mx = fmax(mx, z[t]);
       if (m < a.M) {
-        if (a.C && n < a.nz) ((T*)a.C)[m * a.ldc + n] = z[t];
+        if (a.C && in) ((T*)a.C)[m * a.ldc + n] = z[t];
         if (tc == n) ((T*)a.zt)[m] = z[t];
       }
     }

@@ -193,7 +193,6 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
     a.lda = q.C;
     a.ldb = q.tied ? q.C : q.V;
     a.ldc = q.V;
-    a.nz = q.V;
     int rc = run_stats(dtype, q.tied, a);
     if (rc) return rc;
     {

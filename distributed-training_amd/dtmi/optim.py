@@ -1,4 +1,5 @@
-"""AdamW over device arrays with dtrain's API (dtrain/optim.py).
+"""AdamW over device arrays with dtrain's API (dtrain/optim.py); beside it `Muon`
+and `orthogonalize`, which dtrain does not have.
 
 `AdamW(params, lr, betas, eps, weight_decay)` keeps m and v in one flat device
 buffer (a view per parameter) and updates every (p, g, m, v) of a step in one
@@ -97,8 +98,8 @@ def orthogonalize(arrays, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float
     `steps` Newton-Schulz steps: X = G / (|G| + eps) with the Frobenius norm, then
     X = a X + (b A + c A A) X with A = X X^T (on the right, with X^T X, where G has more
     rows than columns). `arrays`: a contiguous DeviceArray [..., m, n], every matrix of a
-    stack by itself, or a list of such; all of them share the launches. Returns new
-    arrays of the same shapes."""
+    stack by itself, or a list of such; all of them share the launches. The norm is summed
+    in float64 (elements between 1e-150 and 1e150). Returns new arrays of the same shapes."""
     one = isinstance(arrays, DeviceArray)
     ins = K.Matrices([arrays] if one else arrays, "orthogonalize")
     outs = [dev.empty(a.shape, a.dtype) for a in ins.arrays]
@@ -121,6 +122,9 @@ class Muon:
         self.lr, self.momentum, self.nesterov, self.wd = lr, momentum, nesterov, weight_decay
         self.steps, self.coefficients, self.eps = steps, tuple(float(c) for c in coefficients), eps
         self._all = K.Matrices(self.params, "Muon")
+        spans = sorted((p.ptr, p.nbytes) for p in self.params if p.size)
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("Muon: parameters overlap")  # one step updates them all at once
         self._mflat = dev.zeros((max(sum(p.size for p in self.params), 1),),
                                 self.params[0].dtype if self.params else np.float32)
         self.m, off = [], 0
@@ -136,6 +140,8 @@ class Muon:
         if len(grads) != len(self.params):
             raise ValueError(f"Muon: {len(grads)} gradients for {len(self.params)} parameters")
         gs_dev = grad_scale if isinstance(grad_scale, DeviceArray) else None
+        if gs_dev is not None and (gs_dev.dtype != np.float64 or gs_dev.size != 1):
+            raise ValueError("Muon: a device grad_scale must be one float64")
         ps, mp = self._all, self._m_ptrs
         if any(g is None for g in grads):
             live = [i for i, g in enumerate(grads) if g is not None]

@@ -507,7 +507,8 @@ int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int6
  *   dX = dz W^T, dW = X^T dz (tied: its transpose [V, C]), db = sum_r dz
  * losses, mean, dX, dW and db may be NULL. Without gradients no logit is written; with
  * any, about 1 GiB of them at a time are (1024 rows at least), in a pooled workspace (fewer
- * where it cannot be allocated). R = 0: mean, dW and db are 0. C and V below 2^22. */
+ * where it cannot be allocated). R = 0: mean, dW and db are 0. Rows of X and W are shorter
+ * than 2^24 bytes. */
 int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, const void* X, const void* W, int tied,
                      const void* b, const int64_t* targets, void* losses, void* mean, const void* g,
                      int64_t g_stride, double coef, void* dX, void* dW, void* db);

@@ -297,6 +297,34 @@ def test_loss_gradients_are_scaled_shared_and_taken_twice(dev):
     assert X2.grad is None
 
 
+def test_loss_with_split_bf16_products(dev):
+    """Its gradient products follow the GEMM arithmetic that is set."""
+    from dtmi import _lib
+    case = (260, 64, 512, False, False, 0)
+    want = loss_ref(*loss_inputs(case, F32), False, "mean")
+    with _lib.use_gemm_math("bf16x6"):
+        _, y, grads = loss_run(case, F32, "mean", None)
+    by, bx, bw = loss_bars(64, 260, 512)
+    close(y, want[0], F32, by, "loss")
+    close(grads[0], want[1][0], F32, bx, "dx")
+    close(grads[1], want[1][1], F32, bw, "dw")
+
+
+def test_loss_of_one_position(dev):
+    """x without leading axes, a target without any."""
+    A, D = _mods()
+    x, w = np.linspace(-1, 1, 6), np.linspace(0, 2, 24).reshape(6, 4)
+    for reduction in ("mean", "none"):
+        X = A.Tensor(x, requires_grad=True)
+        y = A.linear_cross_entropy(X, A.Tensor(w), 2, reduction=reduction)
+        y.backward()
+        z = x @ w
+        p = np.exp(z - z.max()) / np.exp(z - z.max()).sum()
+        assert y.shape == () and X.grad.shape == (6,)
+        close(y, -np.log(p[2]), F64, 64, "loss")
+        close(X.grad, w @ (p - np.eye(4)[2]), F64, 64, "dx")
+
+
 def test_loss_matches_its_differences(dev):
     A, D = _mods()
     case = (20, 12, 33, True, False, 3)
@@ -626,6 +654,10 @@ def test_muon_keeps_to_its_matrices(dev):
     assert (f[4:4 + 221] != 5).all() and (f[4 + 442:-4] != 5).all()
     with pytest.raises(ValueError, match="gradients for"):
         opt.step([None])
+    g = D.from_numpy(rng.standard_normal((13, 17)).astype(F32))
+    for scale in (D.full((1,), 1.0, F32), D.full((2,), 1.0, F64)):
+        with pytest.raises(ValueError, match="float64"):
+            opt.step([g, None, None], grad_scale=scale)
 
 
 def test_a_training_step_of_a_model_with_experts(dev):

@@ -92,3 +92,8 @@ def test_updates_refuse():
     for bad in (arr(4, 8), arr(8, 4, dt=np.float64)):
         with pytest.raises(ValueError, match="gradient must be"):
             K.muon(ps, [bad], ps.pointers([arr(8, 4)]), [1.0], 1.0, 0.9, True, 5, (1.0, 1.0, 1.0), 0.0)
+    a = arr(8, 4)
+    with pytest.raises(ValueError, match="overlap"):
+        Muon([a, a])
+    with pytest.raises(ValueError, match="overlap"):
+        Muon([arr(2, 8, 4), DeviceArray(_Nowhere(), (4, 4), np.float32, 4 * 60)])
