@@ -33,7 +33,7 @@ static int rows_waves(int64_t blocks, int64_t K, int64_t cus, int mr, int bkc) {
 template <typename T>
 static int direct_waves(int64_t tiles, int64_t K, int64_t cus) {
   int64_t w = 4;
-  while (w < kDirectMaxWaves<T> && tiles * w < 8 * cus) w *= 2;
+  while (w < 8 && tiles * w < 8 * cus) w *= 2;
   const int64_t batches = cdiv(K > 0 ? K : 1, kDirectBatch<T>);
   return (int)(w < batches ? w : batches);
 }

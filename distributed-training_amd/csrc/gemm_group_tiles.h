@@ -292,10 +292,28 @@ __global__ void __launch_bounds__(256) group_sum_kernel(GroupArgs a) {
   }
 }
 
+// Waves of a small-product block. More (gemm_direct_kernel takes 16) leave a wave 128
+// registers, which the k-contiguous float32 loop spilled, and cost more in adding up their
+// tiles than their shares of k saved: 512 k of 128 x 128, 9.7 us with 16.
+constexpr int kGroupWaves = 8;
+
+// Register q of a wave's tiles in LDS, [wave][regs][lane], added over the waves in order;
+// all of them are read before the first is added.
+template <typename T>
+__device__ __forceinline__ T sum_waves(const T* __restrict__ part, int regs, int q, int lane, int nw) {
+  T v[kGroupWaves];
+#pragma unroll
+  for (int w = 0; w < kGroupWaves; ++w) v[w] = w < nw ? part[(w * regs + q) * 64 + lane] : T(0);
+  T s = v[0];
+#pragma unroll
+  for (int w = 1; w < kGroupWaves; ++w) s = s + v[w];
+  return s;
+}
+
 // Small products: a 32 x 32 tile a block, k over its waves, whose partial tiles are
 // added through LDS in wave order (gemm_direct_kernel for a group of tasks).
 template <typename T, bool AKC, bool BKC>
-__global__ void __launch_bounds__(64 * kDirectMaxWaves<T>) group_direct_kernel(GroupArgs a) {
+__global__ void __launch_bounds__(64 * kGroupWaves) group_direct_kernel(GroupArgs a) {
   using MFT = MF<T>;
   using Dt = DirectTile<T>;
   constexpr int MT = MFT::MT, NACC = MFT::NACC, VEC = MFT::VEC, R = Dt::R, KB = Dt::KB, NCH = KB / 8;
@@ -351,8 +369,7 @@ __global__ void __launch_bounds__(64 * kDirectMaxWaves<T>) group_direct_kernel(G
   __syncthreads();
   const GroupEpi<T> e = group_epi<T>(a, k, a.sym && tm != tn);
   for (int q = wave; q < Dt::REGS; q += nw) {
-    T v = part[q * 64 + lane];
-    for (int w = 1; w < nw; ++w) v = v + part[(w * Dt::REGS + q) * 64 + lane];
+    const T v = sum_waves(part, Dt::REGS, q, lane, nw);
     const int tt = q / NACC, r = q % NACC;
     const int64_t m = m0 + (tt / R) * MT + MFT::row(r, g), n = n0 + (tt % R) * MT + c;
     if (m < e.M && n < e.N) e.store(m, n, v);
@@ -465,7 +482,7 @@ __global__ void __launch_bounds__(256, 2) gemm_stats_kernel(StatsArgs a) {
 // A wave's lanes of one lane group hold MT columns of a row, so the statistics are
 // butterflies over them and a part is MT columns wide.
 template <typename T, bool BKC>
-__global__ void __launch_bounds__(64 * kDirectMaxWaves<T>) stats_direct_kernel(StatsArgs a) {
+__global__ void __launch_bounds__(64 * kGroupWaves) stats_direct_kernel(StatsArgs a) {
   using MFT = MF<T>;
   using Dt = DirectTile<T>;
   constexpr int MT = MFT::MT, NACC = MFT::NACC, R = Dt::R, KB = Dt::KB, NCH = KB / 8;
@@ -502,8 +519,7 @@ __global__ void __launch_bounds__(64 * kDirectMaxWaves<T>) stats_direct_kernel(S
     const int tt = q / NACC, r = q % NACC, j = tt % R;
     const int64_t m = m0 + (tt / R) * MT + MFT::row(r, g), n = n0 + j * MT + c;
     // rows past the last are computed from it and not stored
-    T z = part[q * 64 + lane];
-    for (int w = 1; w < nw; ++w) z = z + part[(w * Dt::REGS + q) * 64 + lane];
+    T z = sum_waves(part, Dt::REGS, q, lane, nw);
     const bool in = n < a.N;
     if (a.bias && in) z = z + ((const T*)a.bias)[n];
     if (!in) z = -INFINITY;

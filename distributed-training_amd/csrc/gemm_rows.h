@@ -170,9 +170,13 @@ struct RowsSum {
         for (int r = 0; r < 4; ++r) part[(wave * REGS + (i * NT + t) * 4 + r) * 64 + lane] = acc[i][t][r];
   }
   __device__ __forceinline__ T value(int q) const {
-    T v = part[q * 64 + lane];
-    for (int w = 1; w < nw; ++w) v = v + part[(w * REGS + q) * 64 + lane];
-    return v;
+    T v[kRowsMaxWaves];  // all read before the first is added
+#pragma unroll
+    for (int w = 0; w < kRowsMaxWaves; ++w) v[w] = w < nw ? part[(w * REGS + q) * 64 + lane] : T(0);
+    T s = v[0];
+#pragma unroll
+    for (int w = 1; w < kRowsMaxWaves; ++w) s = s + v[w];
+    return s;
   }
 };
 

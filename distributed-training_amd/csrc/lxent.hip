@@ -107,6 +107,38 @@ __global__ void __launch_bounds__(1024) lxent_mean_kernel(const T* __restrict__ 
   }
 }
 
+// The join and the mean together, for as few rows and parts as one block goes through at
+// once: a thread a row.
+constexpr int64_t kJoinMeanRows = 1024, kJoinMeanParts = 16;
+template <typename T>
+__global__ void __launch_bounds__(1024) lxent_join_mean_kernel(const T* __restrict__ pmax, const T* __restrict__ psum,
+                                                               int parts, int M, const T* __restrict__ zt,
+                                                               T* __restrict__ rmax, T* __restrict__ rsum,
+                                                               T* __restrict__ losses, double coef,
+                                                               T* __restrict__ mean) {
+  __shared__ double sh[16];
+  const int m = threadIdx.x;
+  double l = 0.0;
+  if (m < M) {
+    RowStat<T> x;
+    for (int p = 0; p < parts; ++p) x.add(pmax[(int64_t)p * M + m], psum[(int64_t)p * M + m]);
+    const T loss = log(x.s) + (x.m - zt[m]);
+    rmax[m] = x.m;
+    rsum[m] = x.s;
+    losses[m] = loss;
+    l = (double)loss;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, 64);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = l;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < 16; ++i) t += sh[i];
+    *mean = (T)(t * coef);
+  }
+}
+
 // dz in place of z: block (x, y) takes 4 vectors a thread of rows y, y + gridDim.y, ...
 // Vectors need element alignment only, so a vocabulary that is no multiple of one runs the
 // same, with its last few elements one by one (1067 x 50257: 104 us element by element).
@@ -168,6 +200,7 @@ template <typename T>
 static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, char* stats) {
   constexpr int64_t es = sizeof(T);
   const bool grads = q.dX || q.dW || q.db;
+  bool joint = false;
   for (int64_t lo = 0; lo < q.R; lo += piece) {
     const int64_t n = q.R - lo < piece ? q.R - lo : piece;
     const int64_t parts = stats_parts(dtype, q.tied, n, q.V, q.C);
@@ -195,9 +228,13 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
     a.ldc = q.V;
     int rc = run_stats(dtype, q.tied, a);
     if (rc) return rc;
+    joint = q.mean && n == q.R && n <= kJoinMeanRows && parts <= kJoinMeanParts;
     {
       TimedLaunch tl(DTMI_FAM_XENT, 2.0 * (double)(parts * n) * es);
-      if (n <= 512)
+      if (joint)
+        lxent_join_mean_kernel<T><<<1, 1024, 0, stream()>>>(pmax, psum, (int)parts, (int)n, zt, rmax, rsum, losses,
+                                                            q.coef, (T*)q.mean);
+      else if (n <= 512)
         lxent_join_kernel<T, 1><<<(unsigned)n, 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum, losses);
       else
         lxent_join_kernel<T, 32><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum,
@@ -232,7 +269,7 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
     }
     LAUNCH_CHECK("lxent kernels");
   }
-  if (q.mean) {
+  if (q.mean && !joint) {
     lxent_mean_kernel<T><<<1, 1024, 0, stream()>>>((const T*)q.losses, q.R, q.coef, (T*)q.mean);
     LAUNCH_CHECK("lxent_mean_kernel");
   }
