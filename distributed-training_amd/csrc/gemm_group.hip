@@ -113,8 +113,8 @@ static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, in
         take(tile_cycles(bm, busy, (double)(total * sp), cus, es) + split_cycles(bm, total, sp, es), {bm, kAll, sp, 0});
       }
       if (rest && k[0] <= chain) {
-        // the last whole tiles run beside fewer and fewer pieces
-        const double busy = ((double)(total / cus) * (double)k[0] + (double)cdiv(rest * sp, cus) * ks) / 0.9;
+        // a quarter tile more: the last whole tiles run beside fewer and fewer pieces
+        const double busy = ((double)(total / cus) + 0.25) * (double)k[0] + (double)cdiv(rest * sp, cus) * ks;
         take(tile_cycles(bm, busy, (double)(total + rest * (sp - 1)), cus, es) + split_cycles(bm, rest, sp, es),
              {bm, (int)rest, sp, 0});
       }
