@@ -9,7 +9,7 @@
 // about 30 rows reading w. A gradient needs a row's whole sum before its first element,
 // so pieces of the vocabulary would form every logit twice (8 R C V); pieces of the
 // rows form them once, and add up dw over them, which costs one read and write of it a
-// piece.
+// piece. Rows whose target is to be ignored are left out first: see lxent_rows_kernel.
 #include <cmath>
 
 #include "gemm_direct_tile.h"
@@ -21,6 +21,12 @@ namespace dtmi {
 // bytes against 6 rows C V operations: 8192 x 768 x 50304 takes 15.1 ms in pieces of 2048
 // rows, 14.5 in these (4096).
 constexpr int64_t kPieceBytes = 1LL << 30, kPieceRows = 1024;
+
+// Ignored rows are left out where a gradient is asked for (their x may hold anything, and
+// 0 x NaN would reach dw) or where their products are more operations than this, 16 us in
+// float32: leaving them out is three more launches (8 rows of 1039 words: 24 us a call in
+// place, 54 us when the host made the list).
+constexpr double kLeaveOut = 2e9;
 
 template <typename T>
 __device__ __forceinline__ T exp_e(T x) {
@@ -39,6 +45,77 @@ struct RowStat {
   }
 };
 
+// The rows whose target is not `ignore`, in order: sel their numbers, t their targets, and
+// for every row its place among them or -1. One block, four rows a thread at a time
+// (2683 rows: 3.4 us). n is the caller's count: no more are written, and what a count too
+// large leaves over names row 0.
+__global__ void __launch_bounds__(1024) lxent_rows_kernel(const int64_t* __restrict__ targets, int64_t R, int64_t ignore,
+                                                          int64_t n, int* __restrict__ sel, int64_t* __restrict__ t,
+                                                          int* __restrict__ place) {
+  constexpr int U = 4;
+  __shared__ int sh[2][U][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t base = 0;
+  for (int64_t r0 = 0, turn = 0; r0 < R; r0 += 1024 * U, turn ^= 1) {
+    int64_t v[U];
+    uint64_t in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * 1024 + threadIdx.x;
+      v[u] = r < R ? targets[r] : ignore;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      in[u] = __ballot(v[u] != ignore);
+      if (lane == 0) sh[turn][u][wave] = __popcll(in[u]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * 1024 + threadIdx.x;
+      int before = 0, total = 0;
+      for (int w = 0; w < 16; ++w) {
+        const int c = sh[turn][u][w];
+        before += w < wave ? c : 0;
+        total += c;
+      }
+      const int64_t at = base + before + __popcll(in[u] & ((1ULL << lane) - 1));
+      const bool kept = v[u] != ignore && at < n;
+      if (r < R) place[r] = kept ? (int)at : -1;
+      if (kept) {
+        sel[at] = (int)r;
+        t[at] = v[u];
+      }
+      base += total;
+    }
+  }
+  for (int64_t i = base + threadIdx.x; i < n; i += 1024) {
+    sel[i] = 0;
+    t[i] = 0;
+  }
+}
+
+// out row r = in row from[r], 0 where that is negative; lanes threads a row.
+template <typename T>
+__global__ void __launch_bounds__(256) lxent_pick_kernel(T* __restrict__ out, const T* __restrict__ in,
+                                                         const int* __restrict__ from, int64_t rows, int64_t cols,
+                                                         int lanes) {
+  const int64_t r = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  if (r >= rows) return;
+  const int64_t f = from[r];
+  for (int64_t c = threadIdx.x % lanes; c < cols; c += lanes) out[r * cols + c] = f >= 0 ? in[f * cols + c] : T(0);
+}
+
+template <typename T>
+static int pick_rows(T* out, const T* in, const int* from, int64_t rows, int64_t cols) {
+  if (!rows || !cols) return DTMI_OK;
+  const int lanes = cols >= 32 ? 64 : 1;
+  TimedLaunch tl(DTMI_FAM_OTHER, 2.0 * (double)(rows * cols) * (double)sizeof(T));
+  lxent_pick_kernel<T><<<(unsigned)cdiv(rows, 256 / lanes), 256, 0, stream()>>>(out, in, from, rows, cols, lanes);
+  LAUNCH_CHECK("lxent_pick_kernel");
+  return DTMI_OK;
+}
+
 // A row's statistics from its parts, joined in a fixed order: ROWS rows a block, on
 // consecutive lanes, the parts dealt to 1024 / ROWS groups that are joined through LDS.
 // 32 rows read whole lines of the parts; with few rows one a block is quicker, as no lane
@@ -46,6 +123,7 @@ struct RowStat {
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(1024) lxent_join_kernel(const T* __restrict__ pmax, const T* __restrict__ psum,
                                                           int64_t parts, int64_t M, const T* __restrict__ zt,
+                                                          const int64_t* __restrict__ targets, int64_t ignore,
                                                           T* __restrict__ rmax, T* __restrict__ rsum,
                                                           T* __restrict__ losses) {
   constexpr int GROUPS = 1024 / ROWS, U = ROWS == 1 ? 2 : 8;
@@ -80,12 +158,10 @@ __global__ void __launch_bounds__(1024) lxent_join_kernel(const T* __restrict__ 
     __syncthreads();
   }
   if (grp == 0 && m < M) {
-    if (rmax) {
-      rmax[m] = x.m;
-      rsum[m] = x.s;
-    }
+    rmax[m] = x.m;
+    rsum[m] = x.s;
     // log(sum) + (max - z): the difference first, as both may be large
-    if (losses) losses[m] = log(x.s) + (x.m - zt[m]);
+    losses[m] = targets[m] == ignore ? T(0) : log(x.s) + (x.m - zt[m]);
   }
 }
 
@@ -113,6 +189,7 @@ constexpr int64_t kJoinMeanRows = 1024, kJoinMeanParts = 16;
 template <typename T>
 __global__ void __launch_bounds__(1024) lxent_join_mean_kernel(const T* __restrict__ pmax, const T* __restrict__ psum,
                                                                int parts, int M, const T* __restrict__ zt,
+                                                               const int64_t* __restrict__ targets, int64_t ignore,
                                                                T* __restrict__ rmax, T* __restrict__ rsum,
                                                                T* __restrict__ losses, double coef,
                                                                T* __restrict__ mean) {
@@ -122,7 +199,7 @@ __global__ void __launch_bounds__(1024) lxent_join_mean_kernel(const T* __restri
   if (m < M) {
     RowStat<T> x;
     for (int p = 0; p < parts; ++p) x.add(pmax[(int64_t)p * M + m], psum[(int64_t)p * M + m]);
-    const T loss = log(x.s) + (x.m - zt[m]);
+    const T loss = targets[m] == ignore ? T(0) : log(x.s) + (x.m - zt[m]);
     rmax[m] = x.m;
     rsum[m] = x.s;
     losses[m] = loss;
@@ -142,17 +219,18 @@ __global__ void __launch_bounds__(1024) lxent_join_mean_kernel(const T* __restri
 // dz in place of z: block (x, y) takes 4 vectors a thread of rows y, y + gridDim.y, ...
 // Vectors need element alignment only, so a vocabulary that is no multiple of one runs the
 // same, with its last few elements one by one (1067 x 50257: 104 us element by element).
+// sel: the rows' own numbers, which g goes by, where some were left out.
 template <typename T>
 __global__ void __launch_bounds__(256) lxent_dz_kernel(T* __restrict__ z, int64_t rows, int64_t cols,
                                                        const T* __restrict__ rmax, const T* __restrict__ rsum,
-                                                       const int64_t* __restrict__ targets, const T* __restrict__ g,
-                                                       int64_t g_stride, double coef) {
+                                                       const int64_t* __restrict__ targets, const int* __restrict__ sel,
+                                                       const T* __restrict__ g, int64_t g_stride, double coef) {
   constexpr int V = 16 / (int)sizeof(T);
   typedef typename UVec<T>::type vt;
   const int64_t c0 = (int64_t)blockIdx.x * (256 * 4 * V);
   for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
     T* row = z + m * cols;
-    const T mx = rmax[m], c = g ? (T)coef * g[m * g_stride] : (T)coef;
+    const T mx = rmax[m], c = g ? (T)coef * g[(sel ? sel[m] : m) * g_stride] : (T)coef;
     const T inv = T(1) / rsum[m];
     const int64_t t = targets[m];
     auto dz = [&](T x, int64_t at) {
@@ -180,12 +258,14 @@ struct LxentArgs {
   int tied;
   const void* b;
   const int64_t* targets;
+  int64_t counted, ignore;
   char* losses;
   void* mean;
   const char* g;
   int64_t g_stride;
   double coef;
   char *dX, *dW, *db;
+  const int* sel = nullptr;  // the rows' numbers, where some are left out
 };
 
 // Pool memory that goes back at the end of the call's enqueuing.
@@ -232,31 +312,26 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
     {
       TimedLaunch tl(DTMI_FAM_XENT, 2.0 * (double)(parts * n) * es);
       if (joint)
-        lxent_join_mean_kernel<T><<<1, 1024, 0, stream()>>>(pmax, psum, (int)parts, (int)n, zt, rmax, rsum, losses,
-                                                            q.coef, (T*)q.mean);
+        lxent_join_mean_kernel<T><<<1, 1024, 0, stream()>>>(pmax, psum, (int)parts, (int)n, zt, a.targets, q.ignore, rmax,
+                                                            rsum, losses, q.coef, (T*)q.mean);
       else if (n <= 512)
-        lxent_join_kernel<T, 1><<<(unsigned)n, 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum, losses);
+        lxent_join_kernel<T, 1><<<(unsigned)n, 1024, 0, stream()>>>(pmax, psum, parts, n, zt, a.targets, q.ignore, rmax, rsum,
+                                                                    losses);
       else
-        lxent_join_kernel<T, 32><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, rmax, rsum,
-                                                                               losses);
+        lxent_join_kernel<T, 32><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, a.targets, q.ignore,
+                                                                               rmax, rsum, losses);
     }
     if (grads) {
       {
         TimedLaunch tl(DTMI_FAM_XENT, 2.0 * (double)n * (double)q.V * es);
         constexpr int V = 16 / (int)sizeof(T);
-        const T* g = q.g ? (const T*)q.g + lo * q.g_stride : nullptr;
+        const T* g = (const T*)q.g + (q.g && !q.sel ? lo * q.g_stride : 0);
         const unsigned ny = (unsigned)(n < 32768 ? n : 32768);
         lxent_dz_kernel<T><<<dim3((unsigned)cdiv(q.V, 1024 * V), ny), 256, 0, stream()>>>(
-            (T*)Z, n, q.V, rmax, rsum, a.targets, g, q.g_stride, q.coef);
+            (T*)Z, n, q.V, rmax, rsum, a.targets, q.sel ? q.sel + lo : nullptr, g, q.g_stride, q.coef);
       }
       LAUNCH_CHECK("lxent_dz_kernel");
       const int add = lo > 0;
-      if (q.dX) {
-        char* dX = q.dX + lo * q.C * es;
-        rc = q.tied ? dtmi_gemm(dtype, 1, 0, n, q.C, q.V, Z, q.V, 0, q.W, q.C, 0, dX, q.C, 0, 1, nullptr, 0, 0)
-                    : dtmi_linear_bwd_dx(dtype, dX, Z, q.W, n, q.C, q.V, 0);
-        if (rc) return rc;
-      }
       if (q.tied) {
         if (q.dW) rc = dtmi_gemm(dtype, 0, 0, q.V, q.C, n, Z, q.V, 0, X, q.C, 0, q.dW, q.C, 0, 1, nullptr, add, 0);
         if (!rc && q.db) rc = dtmi_colsum(dtype, q.db, Z, n, q.V, add);
@@ -264,6 +339,12 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
         rc = dtmi_linear_bwd_dw(dtype, q.dW, q.db, X, Z, n, q.C, q.V, add);
       } else if (q.db) {
         rc = dtmi_colsum(dtype, q.db, Z, n, q.V, add);
+      }
+      if (rc) return rc;
+      if (q.dX) {  // last: it may take the place of X
+        char* dX = q.dX + lo * q.C * es;
+        rc = q.tied ? dtmi_gemm(dtype, 1, 0, n, q.C, q.V, Z, q.V, 0, q.W, q.C, 0, dX, q.C, 0, 1, nullptr, 0, 0)
+                    : dtmi_linear_bwd_dx(dtype, dX, Z, q.W, n, q.C, q.V, 0);
       }
       if (rc) return rc;
     }
@@ -277,7 +358,7 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
 }
 
 template <typename T>
-static int lxent_run(int dtype, LxentArgs q) {
+static int lxent_counted(int dtype, LxentArgs q) {
   constexpr int64_t es = sizeof(T);
   const bool grads = q.dX || q.dW || q.db;
   Scratch losses, Z, stats;
@@ -310,6 +391,43 @@ static int lxent_run(int dtype, LxentArgs q) {
   return rc ? rc : lxent_pieces<T>(dtype, q, piece, (char*)Z.p, (char*)stats.p);
 }
 
+// The rows that count, by themselves: their x, or where a gradient of it is asked for the
+// gradient in its place, in a workspace.
+template <typename T>
+static int lxent_run(int dtype, const LxentArgs& q) {
+  constexpr int64_t es = sizeof(T);
+  const bool grads = q.dX || q.dW || q.db;
+  const int64_t n = q.counted;
+  if (n == q.R || (!grads && 2.0 * (double)(q.R - n) * (double)q.C * (double)q.V < kLeaveOut))
+    return lxent_counted<T>(dtype, q);
+  Scratch rows, x;
+  int rc = pool_alloc(&rows.p, (size_t)(n * 8 + (n + q.R) * 4 + n * es + 8));
+  if (!rc) rc = pool_alloc(&x.p, (size_t)(n * q.C * es + 8));
+  if (rc) return rc;
+  int64_t* t = (int64_t*)rows.p;
+  T* ls = (T*)(t + n);
+  int* sel = (int*)(ls + n);
+  int* place = sel + n;
+  {
+    TimedLaunch tl(DTMI_FAM_OTHER, (double)(q.R + n) * 12.0);
+    lxent_rows_kernel<<<1, 1024, 0, stream()>>>(q.targets, q.R, q.ignore, n, sel, t, place);
+  }
+  LAUNCH_CHECK("lxent_rows_kernel");
+  rc = pick_rows((T*)x.p, (const T*)q.X, sel, n, q.C);
+  if (rc) return rc;
+  LxentArgs c = q;
+  c.R = n;
+  c.X = (const char*)x.p;
+  c.targets = t;
+  c.losses = (char*)ls;
+  if (q.dX) c.dX = (char*)x.p;
+  c.sel = sel;
+  rc = lxent_counted<T>(dtype, c);
+  if (!rc && q.dX) rc = pick_rows((T*)q.dX, (const T*)x.p, place, q.R, q.C);
+  if (!rc && q.losses) rc = pick_rows((T*)q.losses, ls, place, q.R, 1);
+  return rc;
+}
+
 struct ScaleArgs {
   void* p[3];
   int64_t n[3];
@@ -329,25 +447,14 @@ __global__ void __launch_bounds__(256) grad_scale_kernel(ScaleArgs a, const T* _
   for (int64_t i = nv * V + i0; i < n; i += stride) p[i] *= f;
 }
 
-// out row rows[i] = in row i; one wave a row.
-template <typename T>
-__global__ void __launch_bounds__(256) scatter_rows_kernel(T* __restrict__ out, const T* __restrict__ in,
-                                                           const int64_t* __restrict__ rows, int64_t n, int64_t total,
-                                                           int64_t cols) {
-  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= n) return;
-  const int64_t r = rows[i];
-  if (r < 0 || r >= total) return;
-  for (int64_t c = threadIdx.x & 63; c < cols; c += 64) out[r * cols + c] = in[i * cols + c];
-}
-
 }  // namespace dtmi
 
 using namespace dtmi;
 
 DTMI_EXPORT int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, const void* X, const void* W, int tied,
-                                 const void* b, const int64_t* targets, void* losses, void* mean, const void* g,
-                                 int64_t g_stride, double coef, void* dX, void* dW, void* db) {
+                                 const void* b, const int64_t* targets, int64_t counted, int64_t ignore, void* losses,
+                                 void* mean, const void* g, int64_t g_stride, double coef, void* dX, void* dW,
+                                 void* db) {
   DTMI_BODY_BEGIN
   DTMI_REQUIRE_INIT();
   DTMI_DTYPE_OK(dtype);
@@ -355,15 +462,19 @@ DTMI_EXPORT int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, con
              (long long)V);
   DTMI_CHECK(R < (1LL << 31) && C < (1LL << 22) && V < (1LL << 22), "%s: too large", __func__);
   DTMI_CHECK(g_stride == 0 || g_stride == 1, "%s: g_stride must be 0 or 1", __func__);
-  if (R == 0) {
+  DTMI_CHECK(counted >= 0 && counted <= R, "%s: %lld of %lld rows that count", __func__, (long long)counted,
+             (long long)R);
+  if (counted == 0) {
     int rc = mean ? dtmi_fill(dtype, mean, 0.0, 1) : DTMI_OK;
     if (!rc && dW) rc = dtmi_fill(dtype, dW, 0.0, C * V);
     if (!rc && db) rc = dtmi_fill(dtype, db, 0.0, V);
+    if (!rc && dX) rc = dtmi_fill(dtype, dX, 0.0, R * C);
+    if (!rc && losses) rc = dtmi_fill(dtype, losses, 0.0, R);
     return rc;
   }
   DTMI_CHECK(targets && (C == 0 || (X && W)), "%s: NULL pointer", __func__);
-  LxentArgs q{R, C, V, (const char*)X, (const char*)W, tied ? 1 : 0, b, targets, (char*)losses, mean, (const char*)g,
-              g_stride, coef, (char*)dX, (char*)dW, (char*)db};
+  LxentArgs q{R, C, V, (const char*)X, (const char*)W, tied ? 1 : 0, b, targets, counted,
+              counted < R ? ignore : INT64_MIN, (char*)losses, mean, (const char*)g, g_stride, coef, (char*)dX, (char*)dW, (char*)db};
   return dtype == DTMI_F32 ? lxent_run<float>(dtype, q) : lxent_run<double>(dtype, q);
   DTMI_BODY_END
 }
@@ -391,28 +502,6 @@ DTMI_EXPORT int dtmi_grad_scale_multi(int dtype, int n, void* const* ptrs, const
   else
     grad_scale_kernel<double><<<grid, 256, 0, stream()>>>(a, (const double*)g_dev);
   LAUNCH_CHECK("grad_scale_kernel");
-  return DTMI_OK;
-  DTMI_BODY_END
-}
-
-DTMI_EXPORT int dtmi_scatter_rows(int dtype, void* out, const void* in, const int64_t* rows, int64_t n, int64_t total,
-                                  int64_t cols) {
-  DTMI_BODY_BEGIN
-  DTMI_REQUIRE_INIT();
-  DTMI_DTYPE_OK(dtype);
-  DTMI_CHECK(n >= 0 && total >= 0 && cols >= 0 && n < (1LL << 31), "%s: bad sizes", __func__);
-  if (total == 0 || cols == 0) return DTMI_OK;
-  DTMI_CHECK(out && (n == 0 || (in && rows)), "%s: NULL pointer", __func__);
-  int rc = dtmi_fill(dtype, out, 0.0, total * cols);
-  if (rc || n == 0) return rc;
-  TimedLaunch tl(DTMI_FAM_OTHER, 2.0 * (double)(n * cols) * (dtype == DTMI_F32 ? 4 : 8));
-  if (dtype == DTMI_F32)
-    scatter_rows_kernel<float><<<(unsigned)cdiv(n, 4), 256, 0, stream()>>>((float*)out, (const float*)in, rows, n, total,
-                                                                           cols);
-  else
-    scatter_rows_kernel<double><<<(unsigned)cdiv(n, 4), 256, 0, stream()>>>((double*)out, (const double*)in, rows, n,
-                                                                            total, cols);
-  LAUNCH_CHECK("scatter_rows_kernel");
   return DTMI_OK;
   DTMI_BODY_END
 }

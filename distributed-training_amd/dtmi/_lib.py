@@ -104,9 +104,8 @@ SIGNATURES: dict[str, list] = {
     "dtmi_xattn_fwd": [i32, i64, i64, i64, i64, i64, i64, f64, vp, pi64, vp, pi64, vp, pi64, vp, vp, pi64, vp, vp],
     "dtmi_xattn_bwd": [i32, i64, i64, i64, i64, i64, i64, f64, vp, pi64, vp, pi64, vp, pi64, vp, vp, pi64, vp, pi64,
                        vp, vp, vp, pi64, vp, pi64, vp, pi64],
-    "dtmi_linear_xent": [i32, i64, i64, i64, vp, vp, i32, vp, vp, vp, vp, vp, i64, f64, vp, vp, vp],
+    "dtmi_linear_xent": [i32, i64, i64, i64, vp, vp, i32, vp, vp, i64, i64, vp, vp, vp, i64, f64, vp, vp, vp],
     "dtmi_grad_scale_multi": [i32, i32, pvp, pi64, vp],
-    "dtmi_scatter_rows": [i32, vp, vp, vp, i64, i64, i64],
     "dtmi_expert_linear_fwd": [i32, i64, i64, i64, i64, vp, vp, vp, vp, pi64],
     "dtmi_expert_linear_bwd_dx": [i32, i64, i64, i64, i64, vp, vp, vp, pi64],
     "dtmi_expert_linear_bwd_dw": [i32, i64, i64, i64, i64, vp, vp, vp, vp, pi64],

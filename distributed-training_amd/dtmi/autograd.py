@@ -461,8 +461,8 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
     transposed embedding table [V, C] is read as it lies), b [V], `targets` a host
     integer array or an Indices of x's leading shape.
 
-    Rows whose target is `ignore` do not count: their loss and gradients are 0 and x is
-    not read there. `reduction` "mean" gives the mean over the others (0 if there are
+    Rows whose target is `ignore` do not count: their loss and gradients are 0, whatever
+    x holds there. `reduction` "mean" gives the mean over the others (0 if there are
     none), "none" the loss of every row, which without gradients (`no_grad()`) is minus
     the log probability of its target: no logit is written then. The gradients of a mean
     are computed by the forward pass, as cross_entropy's are, from about 1 GiB of logits
@@ -487,54 +487,38 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
         raise ValueError(f"linear_cross_entropy: targets of shape {host.shape} for x {x.shape}")
     rows = host.size
     lo, hi = (ix._lo, ix._hi) if ix is not None else (host.min(), host.max()) if rows else (0, -1)
-    X2 = X.reshape(rows, C)
-    sel = None
+    n = rows
     if ignore is not None and lo <= ignore <= hi:
-        host = host.reshape(-1)
-        at = np.flatnonzero(host != ignore)
-        if at.size < rows:  # the rows that count, by themselves
-            host = host[at]
-            lo, hi = (host.min(), host.max()) if host.size else (0, -1)
-            ix = None
+        keep = host != ignore
+        n = int(np.count_nonzero(keep))
+        if not 0 <= ignore < V and n < rows:
+            lo, hi = (host[keep].min(), host[keep].max()) if n else (0, -1)
     if lo < 0 or hi >= V:
         raise IndexError(f"target out of bounds for size {V}")
-    if host.size < rows:
-        sel = dev.from_numpy(at.astype(np.int64))
-        X2 = K.embedding_fwd(X2, sel, (host.size,))
+    X2 = X.reshape(rows, C)
     t = ix.dev if ix is not None else dev.from_numpy(host.reshape(-1).astype(np.int64))
-    n = host.size
     mean = reduction == "mean"
-    coef = 1.0 / n if mean and n else 1.0
     need = [_grad_enabled and p is not None and p.requires_grad for p in (x, w, b)]
     grads = dict(need_dx=need[0], need_dw=need[1], need_db=need[2])
-    ls, total, *made = K.linear_xent(X2, W, bd, t, tied, coef, losses=not mean, mean=mean,
-                                     **(grads if mean else {}))
-
-    def spread(d, cols):
-        return d if sel is None else K.scatter_rows(d.reshape(n, cols), sel, rows)
+    rest = dict(tied=tied, coef=1.0 / n if mean and n else 1.0, counted=n, ignore=int(ignore or 0))
+    ls, total, *made = K.linear_xent(X2, W, bd, t, losses=not mean, mean=mean, **rest, **(grads if mean else {}))
     pending = [made] if mean and any(need) else []
 
     def bw(g):
-        if mean:
+        if pending:
+            # into their destinations, or in place
+            made, dests = list(pending.pop()), (None, None if tied else grad_out(w),
+                                                grad_out(b) if b is not None else None)
             g1 = _contig(g).reshape(1)
-            if pending:
-                # into their destinations, or in place
-                made, dests = list(pending.pop()), (None, None if tied else grad_out(w),
-                                                    grad_out(b) if b is not None else None)
-                K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], g1)
-                dx, dw, db = [d if o is None or d is None else K.scale(d, alpha_dev=g1, out=o)
-                              for d, o in zip(made, dests)]
-            else:
-                dx, dw, db = K.linear_xent(X2, W, bd, t, tied, coef, g=g1, **grads)[2:]
+            K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], g1)
+            dx, dw, db = [d if o is None or d is None else K.scale(d, alpha_dev=g1, out=o)
+                          for d, o in zip(made, dests)]
         else:
-            g1 = _contig(g).reshape(rows)
-            if sel is not None:
-                g1 = K.embedding_fwd(g1.reshape(rows, 1), sel, (n,)).reshape(n)
-            dx, dw, db = K.linear_xent(X2, W, bd, t, tied, g=g1, **grads)[2:]
-        dx = spread(dx, C).reshape(x.shape) if dx is not None else None
+            dx, dw, db = K.linear_xent(X2, W, bd, t, g=_contig(g).reshape(-1), **rest, **grads)[2:]
+        dx = dx.reshape(x.shape) if dx is not None else None
         dw = dw.transpose(1, 0) if dw is not None and tied else dw
         return (dx, dw) if b is None else (dx, dw, db)
-    out = total if mean else spread(ls, 1).reshape(lead)
+    out = total if mean else ls.reshape(lead)
     return Tensor._make(out, (x, w) if b is None else (x, w, b), bw)
 
 

@@ -911,9 +911,11 @@ def xattn_bwd(q, k, v, o, dO, rowmax, rowsum, lengths=None, scale=None, dq=None,
 # --------------------------------------------- products of a training step
 def linear_xent(x2: DeviceArray, w: DeviceArray, b: DeviceArray | None, targets: DeviceArray, tied: bool = False,
                 coef: float = 1.0, losses: bool = False, mean: bool = False, g: DeviceArray | None = None,
-                need_dx: bool = False, need_dw: bool = False, need_db: bool = False):
+                need_dx: bool = False, need_dw: bool = False, need_db: bool = False, counted: int | None = None,
+                ignore: int = 0):
     """Cross entropy of x2 [R, C] @ w [C, V] (tied: w is [V, C]) + b against int64
-    targets [R], without the logits. Returns (losses [R], mean, dx, dw, db), None where
+    targets [R], without the logits; `counted` of them are not `ignore` (None: all), the
+    others have losses and gradients of 0. Returns (losses [R], mean, dx, dw, db), None where
     not asked for; the mean is coef times the sum of the losses, the gradients are coef
     times those of the sum, times g ([R], or one element for all) where given."""
     _contig(x2, w, targets)
@@ -937,20 +939,10 @@ def linear_xent(x2: DeviceArray, w: DeviceArray, b: DeviceArray | None, targets:
     dx = empty(x2.shape, x2.dtype) if need_dx else None
     dw = empty(w.shape, x2.dtype) if need_dw else None
     db = empty((V,), x2.dtype) if need_db else None
-    _c("dtmi_linear_xent", d, R, C_, V, x2.ptr, w.ptr, 1 if tied else 0, _opt_ptr(b), targets.ptr, _opt_ptr(ls),
-       _opt_ptr(mn), _opt_ptr(g), 1 if g is not None and g.size == R and R > 1 else 0, float(coef), _opt_ptr(dx),
+    _c("dtmi_linear_xent", d, R, C_, V, x2.ptr, w.ptr, 1 if tied else 0, _opt_ptr(b), targets.ptr,
+       R if counted is None else counted, ignore, _opt_ptr(ls), _opt_ptr(mn), _opt_ptr(g), 1 if g is not None and g.size == R and R > 1 else 0, float(coef), _opt_ptr(dx),
        _opt_ptr(dw), _opt_ptr(db))
     return ls, mn, dx, dw, db
-
-
-def scatter_rows(x2: DeviceArray, rows: DeviceArray, total: int) -> DeviceArray:
-    """[total, C] of zeros with row rows[i] = x2[i]; rows int64, each once."""
-    _contig(x2, rows)
-    if rows.dtype != np.int64 or rows.size != x2.shape[0]:
-        raise ValueError("scatter_rows: rows must be int64 with one entry per row")
-    out = empty((int(total), x2.shape[1]), x2.dtype)
-    _c("dtmi_scatter_rows", _dt(x2), out.ptr, x2.ptr, rows.ptr, x2.shape[0], int(total), x2.shape[1])
-    return out
 
 
 class ExpertRows:

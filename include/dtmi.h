@@ -501,24 +501,22 @@ int dtmi_xattn_bwd(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Tq, int6
  *
  * Softmax cross entropy of z = X W + b over a large vocabulary without the logits:
  * X [R, C], W [C, V] (tied != 0: [V, C], an embedding table), b [V] or NULL, targets
- * int64 [R] in 0..V-1. With m_r the largest z of a row and s_r = sum_v exp(z - m_r),
+ * int64 [R] in 0..V-1 or `ignore`, `counted` of them not (counted == R: ignore has no
+ * meaning). With m_r the largest z of a row and s_r = sum_v exp(z - m_r),
  *   losses[r] = log s_r + (m_r - z[r, t_r])    mean = coef * sum_r losses[r]
  *   dz[r, v] = coef * g[r g_stride] * (exp(z - m_r) / s_r - [v = t_r])  (g NULL: 1)
  *   dX = dz W^T, dW = X^T dz (tied: its transpose [V, C]), db = sum_r dz
+ * and 0 for rows whose target is `ignore`, whatever X holds there.
  * losses, mean, dX, dW and db may be NULL. Without gradients no logit is written; with
  * any, about 1 GiB of them at a time are (1024 rows at least), in a pooled workspace (fewer
- * where it cannot be allocated). R = 0: mean, dW and db are 0. Rows of X and W are shorter
- * than 2^24 bytes. */
+ * where it cannot be allocated). counted = 0: all results are 0. Rows of X and W are
+ * shorter than 2^24 bytes. */
 int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, const void* X, const void* W, int tied,
-                     const void* b, const int64_t* targets, void* losses, void* mean, const void* g,
-                     int64_t g_stride, double coef, void* dX, void* dW, void* db);
+                     const void* b, const int64_t* targets, int64_t counted, int64_t ignore, void* losses,
+                     void* mean, const void* g, int64_t g_stride, double coef, void* dX, void* dW, void* db);
 /* dtmi_xent_grad_scale for 1 to 3 arrays in one launch: each times *g_dev unless that is
  * exactly 1. */
 int dtmi_grad_scale_multi(int dtype, int n, void* const* ptrs, const int64_t* counts, const void* g_dev);
-/* out [total, cols] = 0, then row rows[i] = in[i] for i < n (in [n, cols], rows int64 in
- * device memory, each once; those outside 0..total-1 are left out). */
-int dtmi_scatter_rows(int dtype, void* out, const void* in, const int64_t* rows, int64_t n, int64_t total,
-                      int64_t cols);
 
 /* Products of E experts with ragged sizes: the first sizes[0] rows of x [R, K] belong to
  * expert 0, the next sizes[1] to expert 1, ... (sizes: host memory, their sum at most R);

@@ -188,6 +188,43 @@ def test_losses_without_gradients_are_the_same(dev):
     assert z._backward is None
 
 
+@pytest.mark.parametrize("case", [
+    (70, 64, 130, True, False, 41),       # ignored rows gone through with the others
+    (700, 256, 8000, False, True, 500),   # left out: 2 * 500 * 256 * 8000 operations
+], ids=["few", "many"])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("ignore", [-100, 2 ** 40, 3])
+def test_losses_alone_beside_ignored_rows(dev, case, reduction, ignore):
+    A, D = _mods()
+    x, w, b, t = loss_inputs(case, F32)
+    out = t < 0
+    t[~out & (t == ignore)] = 4
+    ry, _ = loss_ref(x, w, b, t, case[4], reduction, None if reduction == "mean" else np.ones(len(t)))
+    t[out], x[out] = ignore, np.nan
+    W = A.Tensor(w).transpose(1, 0) if case[4] else A.Tensor(w)
+    with A.no_grad():
+        y = A.linear_cross_entropy(A.Tensor(x), W, A.Indices(t), A.Tensor(b) if case[3] else None, ignore=ignore,
+                                   reduction=reduction)
+    close(y, ry, F32, loss_bars(case[1], case[0], case[2])[0], "loss")
+    if reduction == "none":
+        assert not y.numpy()[out].any()
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("ign", [1, 4000, 9999])
+def test_loss_leaves_rows_out_of_many(dev, dt, reduction, ign):
+    case = (10000, 5, 7, True, False, ign)
+    g = None if reduction == "mean" else np.random.default_rng(1).standard_normal(case[0]).astype(dt)
+    (x, w, b, t), y, grads = loss_run(case, dt, reduction, g)
+    ry, rg = loss_ref(x, w, b, t, False, reduction, g)
+    by, bx, bw = loss_bars(5, 10000, 7)
+    close(y, ry, dt, by, "loss")
+    for got, want, n, name in zip(grads, rg, (bx, bw, bw), ("dx", "dw", "db")):
+        close(got, want, dt, n, name)
+    assert not grads[0].numpy()[t < 0].any()
+
+
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_loss_with_every_target_ignored(dev, reduction):
     A, D = _mods()
