@@ -220,7 +220,7 @@ class Tensor:
         if grad is None:
             if self.data.size != 1:
                 raise ValueError("backward() without a gradient needs a scalar output")
-            grad = dev.full(self.data.shape, 1.0, self.data.dtype)
+            grad = dev.ones_later(self.data.shape, self.data.dtype)
         elif not isinstance(grad, DeviceArray):
             grad = dev.asarray(np.asarray(grad, dtype=self.dtype))
         order, seen, users = [], set(), {}
@@ -510,7 +510,8 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
             made, dests = list(pending.pop()), (None, None if tied else grad_out(w),
                                                 grad_out(b) if b is not None else None)
             g1 = _contig(g).reshape(1)
-            K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], g1)
+            if not dev.known_ones(g1):
+                K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], g1)
             dx, dw, db = [d if o is None or d is None else K.scale(d, alpha_dev=g1, out=o)
                           for d, o in zip(made, dests)]
         else:

@@ -42,6 +42,26 @@ class Block:
             self.ptr = None
 
 
+class OnesBlock(Block):
+    """Ones that are allocated and written when something first asks for their address, so
+    that who knows what they hold need not launch anything."""
+
+    __slots__ = ("count", "dtype", "made")
+
+    def __init__(self, count: int, dtype):
+        self.count, self.dtype, self.made = count, dtype, None
+        self.nbytes = count * _ITEMSIZE[dtype]
+
+    @property
+    def ptr(self):
+        if self.made is None:
+            self.made = full((self.count,), 1.0, self.dtype).block
+        return self.made.ptr
+
+    def __del__(self):
+        pass
+
+
 @lru_cache(maxsize=4096)
 def _contig_strides(shape: tuple):
     st, acc = [], 1
@@ -239,6 +259,16 @@ def zeros(shape, dtype=np.float32) -> DeviceArray:
 
 def full(shape, value, dtype=np.float32) -> DeviceArray:
     return empty(shape, dtype).fill_(value)
+
+
+def ones_later(shape, dtype=np.float32) -> DeviceArray:
+    dt = np.dtype(dtype)
+    return DeviceArray(OnesBlock(prod(shape), dt), shape, dt)
+
+
+def known_ones(a: DeviceArray) -> bool:
+    """Whether `a` is ones_later's (or a view of it) and nobody has had its address yet."""
+    return isinstance(a.block, OnesBlock) and a.block.made is None
 
 
 def from_numpy(a) -> DeviceArray:

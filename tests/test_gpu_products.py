@@ -225,6 +225,39 @@ def test_loss_leaves_rows_out_of_many(dev, dt, reduction, ign):
     assert not grads[0].numpy()[t < 0].any()
 
 
+def test_ones_are_written_when_they_are_asked_for(dev):
+    """backward()'s own gradient: what reads it finds ones, also in a view and twice over."""
+    A, D = _mods()
+    for dt in (F32, F64):
+        g = D.ones_later((2, 3), dt)
+        v = g.reshape(6)[1:]
+        assert D.known_ones(g) and D.known_ones(v)
+        assert (v.numpy() == 1).all() and not D.known_ones(g) and not D.known_ones(v)
+        v.assign(2.0)
+        assert g.numpy().tolist() == [[1, 2, 2], [2, 2, 2]]
+        x = A.Tensor(np.asarray(3.0, dt), requires_grad=True)
+        x.backward()
+        x.backward()
+        assert float(x.grad) == 2.0
+
+
+@pytest.mark.parametrize("dest", [False, True])
+def test_gradients_of_a_mean_by_itself_and_scaled(dev, dest):
+    """backward() leaves them as the forward pass made them, backward(g) scales them."""
+    A, D = _mods()
+    x, w, b, t = loss_inputs((40, 24, 130, True, False, 0), F32)
+    got = []
+    for g in (None, 1.0, 0.5):
+        X, W, B = (A.Tensor(D.from_numpy(v), requires_grad=True) for v in (x, w, b))
+        if dest:
+            W.grad_dest = D.zeros(w.shape, F32)
+        A.linear_cross_entropy(X, W, t, B).backward(g)
+        assert not dest or W.grad.ptr == W.grad_dest.ptr
+        got.append([p.grad.numpy() for p in (X, W, B)])
+    for one, same, half in zip(*got):
+        assert bits_equal(one, same) and bits_equal(0.5 * one, half)
+
+
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_loss_with_every_target_ignored(dev, reduction):
     A, D = _mods()
