@@ -41,7 +41,12 @@ enum GroupD { kDNone = 0, kDMatrix = 1, kDRow = 2, kDColsum = 3 };
 // their operands in its L2; where they differ that would give one XCD all of the longest
 // task (8 experts' dw 305 us), and tiles go round as they are numbered.
 struct GroupArgs {
-  int count, tiles, equal;
+  int count, tiles;
+  // The tiles with something to add up, which come first; dealt to the XCDs in ranges where
+  // all of those are equally long. The others, zeros alone, follow in their own order: in
+  // the ranges they left one XCD idle in eight (2854 rows of four experts and 713 of none,
+  // 619 x 1075: 58 us instead of 48).
+  int work, equal;
   // the first `cut` tiles are split in `splits` along k, their partials added by a second
   // kernel; `before` blocks of whole tiles run before them
   int cut, splits, before;

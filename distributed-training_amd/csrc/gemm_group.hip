@@ -51,9 +51,12 @@ static double direct_cycles(int64_t tiles, double kavg, int64_t kmax, int nw, in
 // tile_cost in gemm.hip (64-wide float32 tiles over several tasks reach less, 0.80 to
 // 0.89 of their MFMA rate), with what a block costs before its first MFMA and after its
 // last, of which the others on its CU hide some: 64 experts' dw, 384 x 501 from 62 rows
-// each, took 42 us on 3072 64-wide tiles.
-static double tile_cycles(int bm, double k, double units, int64_t cus, size_t es) {
-  const double eff = bm == 64 ? (units > cus ? (es == 4 ? 0.82 : 0.88) : 0.75) : units > 2.0 * cus ? 0.97 : units > cus ? 1.0 : 0.82;
+// each, took 42 us on 3072 64-wide tiles. A 128-wide float32 tile alone on its CU waits for
+// its loads, of single elements the more (vec false): four times 713 x 1075 with 619 terms,
+// 216 tiles: 55 us (816 64-wide ones: 48), 704 x 1088 with 640: 48 us.
+static double tile_cycles(int bm, double k, double units, int64_t cus, size_t es, bool vec) {
+  const double alone = es == 8 ? 0.82 : vec ? 0.78 : 0.66;
+  const double eff = bm == 64 ? (units > cus ? (es == 4 ? 0.82 : 0.88) : 0.75) : units > 2.0 * cus ? 0.97 : units > cus ? 1.0 : alone;
   return 8800.0 + 1500.0 * units / (double)cus + k * (es == 4 ? 32.0 : 64.0) * (bm / 32) * (bm / 32) / 4.0 / eff;
 }
 // and what a split adds: its partials' traffic and a launch
@@ -67,7 +70,7 @@ static double split_cycles(int bm, int64_t cut, int splits, size_t es) {
 //   number of rounds;
 // - unequal k: the tiles of the longest tasks split.
 template <typename T>
-static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, int64_t cus) {
+static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, int64_t cus, bool vec) {
   constexpr size_t es = sizeof(T);
   constexpr int64_t bk = 64 / (int64_t)es;
   int64_t k[kGroupTasks];
@@ -81,6 +84,7 @@ static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, in
     }
   };
   auto tiles_of = [&](int i, int bm) {
+    if (k[i] == 0) return (int64_t)0;  // these only write
     const int64_t tm = cdiv(t[i].M, bm), tn = cdiv(t[i].N, bm);
     return sym ? tm * (tm + 1) / 2 : tm * tn;
   };
@@ -103,19 +107,19 @@ static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, in
     if (k[0] <= chain) {
       const double busy = equal ? (double)cdiv(total, cus) * (double)k[0]
                                 : std::max((double)k[0], even + 0.5 * (double)k[last]);
-      take(tile_cycles(bm, busy, (double)total, cus, es), {bm, 0, 1, 0});
+      take(tile_cycles(bm, busy, (double)total, cus, es, vec), {bm, 0, 1, 0});
     }
     const int64_t rest = equal && total > cus ? total % cus : 0;
     for (int sp = 2; sp <= 16 && k[0] / sp >= 128; ++sp) {
       const double ks = (double)(cdiv(cdiv(k[0], sp), bk) * bk);
       if (ks <= (double)chain || sp == 16) {
         const double busy = equal ? (double)cdiv(total * sp, cus) * ks : std::max(ks, even + 0.5 * (double)k[last] / sp);
-        take(tile_cycles(bm, busy, (double)(total * sp), cus, es) + split_cycles(bm, total, sp, es), {bm, kAll, sp, 0});
+        take(tile_cycles(bm, busy, (double)(total * sp), cus, es, vec) + split_cycles(bm, total, sp, es), {bm, kAll, sp, 0});
       }
       if (rest && k[0] <= chain) {
         // a quarter tile more: the last whole tiles run beside fewer and fewer pieces
         const double busy = ((double)(total / cus) + 0.25) * (double)k[0] + (double)cdiv(rest * sp, cus) * ks;
-        take(tile_cycles(bm, busy, (double)(total + rest * (sp - 1)), cus, es) + split_cycles(bm, rest, sp, es),
+        take(tile_cycles(bm, busy, (double)(total + rest * (sp - 1)), cus, es, vec) + split_cycles(bm, rest, sp, es),
              {bm, (int)rest, sp, 0});
       }
       if (!equal && (sp <= 4 || sp % 4 == 0)) {
@@ -124,7 +128,7 @@ static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, in
           cut += n[i];
           if (k[i] == k[i + 1] || !cut || k[i + 1] > chain || ks > (double)chain) continue;
           const double busy = std::max(std::max(ks, (double)k[i + 1]), even + 0.5 * (double)k[last]);
-          take(tile_cycles(bm, busy, (double)(total + cut * (sp - 1)), cus, es) + split_cycles(bm, cut, sp, es),
+          take(tile_cycles(bm, busy, (double)(total + cut * (sp - 1)), cus, es, vec) + split_cycles(bm, cut, sp, es),
                {bm, (int)cut, sp, 0});
         }
       }
@@ -176,34 +180,34 @@ static int plan_tasks(int akc, int bkc, std::vector<GroupTask>& tasks, int dmode
     }
     l.vec = vec;
     const bool few = rows <= kFewRows && akc && !sym && pad == 1 && dmode != kDColsum;
-    const GroupPlan p = few ? GroupPlan{16, 0, 1, 0} : choose_plan<T>(a.t, a.count, sym, pad, cus);
+    const GroupPlan p = few ? GroupPlan{16, 0, 1, 0} : choose_plan<T>(a.t, a.count, sym, pad, cus, vec);
     l.tile = p.tile;
     l.nw = p.nw;
     l.mr = rows <= 16 ? 1 : 2;
     const int tm_rows = few ? 16 * l.mr : p.tile;
     const int tn_cols = few ? (bkc ? RowsTile<T, true>::COLS : RowsTile<T, false>::COLS) : p.tile;
     a.equal = 1;
-    int64_t tiles = 0;
+    int64_t tiles = 0, work = 0;
     for (int i = 0; i < a.count; ++i) {
       const int64_t tm = cdiv(a.t[i].M, tm_rows), tn = cdiv(a.t[i].N, tn_cols);
       a.equal = a.equal && (a.t[i].K == a.t[0].K || a.t[i].K == 0);
       a.first[i] = (int)tiles;
       tiles += sym ? tm * (tm + 1) / 2 : tm * tn;
+      if (a.t[i].K > 0) work = tiles;
       DTMI_CHECK(tiles < (1LL << 26), "group of products: too large");
     }
     if (!tiles) continue;
     a.tiles = (int)tiles;
+    a.work = (int)work;
     if (few) l.nw = rows_waves<T>(tiles, a.t[0].K, cus, l.mr, bkc);
-    a.cut = p.cut < a.tiles ? p.cut : a.tiles;
+    a.cut = p.cut < a.work ? p.cut : a.work;
     a.splits = p.splits;
     for (int i = 0; i < a.count && a.cut; ++i) {  // whole tiles that are longer than the pieces
       const int end = i + 1 < a.count ? a.first[i + 1] : a.tiles;
-      if (end > a.cut && a.t[i].K >= cdiv(a.t[0].K, p.splits)) a.before = end - a.cut;
+      if (end > a.cut && a.t[i].K > 0 && a.t[i].K >= cdiv(a.t[0].K, p.splits)) a.before = end - a.cut;
     }
     if (!a.equal && p.tile == 128) {  // the blocks that have something to do, longest first
-      int64_t units = a.tiles + (int64_t)a.cut * (p.splits - 1);
-      for (int i = a.count - 1; i >= 0 && a.t[i].K == 0; --i)
-        units -= (i + 1 < a.count ? a.first[i + 1] : a.tiles) - a.first[i];
+      const int64_t units = a.work + (int64_t)a.cut * (p.splits - 1);
       if (units > cus && units <= 2 * cus) {
         a.turn = (int)cus;
         a.turned = (int)units;
@@ -262,6 +266,16 @@ int launch_group(int dtype, const std::vector<GroupLaunch>& launches) {
 }
 
 // Tile and waves of a statistics product (tile 16: few rows).
+// What the statistics of a tile add to its product (exponentials, and the joins along its
+// rows): a block alone on its CU waits for all of it, the others hide two thirds. float32
+// 388 x 17704 with 66 terms: 42.8 us on 32-wide tiles, 24.2 on 64, 24.9 on 128; float64
+// 3224 x 161 with 339 terms: 19.8, 22.6 and 57.9.
+static double epilogue_cycles(int bm, int64_t units, int64_t cus, size_t es) {
+  const double one = es == 4 ? (bm == 128 ? 15000.0 : bm == 64 ? 5000.0 : 6000.0)
+                             : (bm == 128 ? 23000.0 : bm == 64 ? 15000.0 : 7000.0);
+  return one * (1.0 + 0.35 * (double)(cdiv(units, cus) - 1));
+}
+
 template <typename T>
 static GroupPlan plan_stats(int bkc, int64_t M, int64_t N, int64_t K) {
   const int64_t cus = num_cus() > 0 ? num_cus() : 256;
@@ -273,10 +287,11 @@ static GroupPlan plan_stats(int bkc, int64_t M, int64_t N, int64_t K) {
   const double k = (double)(cdiv(K, bk) * bk);
   const int64_t t32 = cdiv(M, 32) * cdiv(N, 32);
   GroupPlan best{32, 0, 1, direct_waves<T>(t32, K, cus)};
-  double least = direct_cycles<T>(t32, (double)K, K, best.nw, cus);
+  double least = direct_cycles<T>(t32, (double)K, K, best.nw, cus) + epilogue_cycles(32, t32, cus, sizeof(T));
   for (int bm = 64; bm <= 128; bm += 64) {
     const int64_t n = cdiv(M, bm) * cdiv(N, bm);
-    const double c = tile_cycles(bm, (double)cdiv(n, cus) * k, (double)n, cus, sizeof(T));
+    const double c = tile_cycles(bm, (double)cdiv(n, cus) * k, (double)n, cus, sizeof(T), true) +
+                     epilogue_cycles(bm, n, cus, sizeof(T));
     if (c < least) {
       least = c;
       best = {bm, 0, 1, 0};

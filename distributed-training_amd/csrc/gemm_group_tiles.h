@@ -16,6 +16,12 @@ __device__ __forceinline__ int xcd_tile(int b, int tiles) {
   return b < 8 * per ? (b & 7) * per + (b >> 3) : b;
 }
 
+// The tile of the launch's unit v of those past the split ones.
+__device__ __forceinline__ int whole_tile(const GroupArgs& a, int v) {
+  const int work = a.work - a.cut;
+  return a.cut + (a.equal && v < work ? xcd_tile(v, work) : v);
+}
+
 // Tile t of a task's own grid: groups of 8 rows of tiles, as tile_coords_of; or, of a
 // symmetric product, row by row the tiles on and below the diagonal.
 __device__ __forceinline__ void group_coords(int t, int tiles_m, int tiles_n, int sym, int& tm, int& tn) {
@@ -194,8 +200,7 @@ __global__ void __launch_bounds__(256, 2) gemm_group_kernel(GroupArgs a) {
     split = v / a.cut;
     v -= split * a.cut;
   } else {
-    v = b < a.before ? b : b - parts;
-    v = a.cut + (a.equal ? xcd_tile(v, a.tiles - a.cut) : v);
+    v = whole_tile(a, b < a.before ? b : b - parts);
   }
   int ti, tm, tn;
   group_tile(a, BM, v, ti, tm, tn);
@@ -321,7 +326,7 @@ __global__ void __launch_bounds__(64 * kGroupWaves) group_direct_kernel(GroupArg
   typedef typename MFT::vec_t VT;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
   int ti, tm, tn;
-  group_tile(a, 32, a.equal ? xcd_tile((int)blockIdx.x, a.tiles) : (int)blockIdx.x, ti, tm, tn);
+  group_tile(a, 32, whole_tile(a, (int)blockIdx.x), ti, tm, tn);
   const GroupTask k = a.t[ti];
   const int64_t m0 = (int64_t)tm * 32, n0 = (int64_t)tn * 32;
   const int lane = threadIdx.x & 63;
