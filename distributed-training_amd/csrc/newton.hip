@@ -9,12 +9,14 @@
 // diagonal and mirror the rest, so that a step of an m x n matrix (m <= n) costs m^2 n
 // + m^3 + 2 m^2 n operations, a third less than three plain products where m = n. All
 // matrices of a call share each launch (gemm_group.h).
-// Bound: MFMA; small matrices by 3 `steps` launches one after the other.
+// Bound: MFMA; small matrices by 3 `steps` launches one after the other, but for those of
+// newton_small.hip.
 #include <cmath>
 #include <utility>
 #include <vector>
 
 #include "gemm_group.h"
+#include "newton_small.h"
 #include "seqmath.h"
 
 namespace dtmi {
@@ -276,6 +278,51 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
   return rc;
 }
 
+// Whether every matrix fits a block of newton_small.hip, and those blocks are quicker than
+// the groups' launches, about 7 us each whatever their size. float32, five steps, one
+// block and the groups: 16 x 16 13 and 80 us, 15 of 35 x 264 51 and 115, 8 of 96 x 96 80
+// and 98, 8 of 96 x 192 119 and 99; float64, 6 of 64 x 96: 53 and 102.
+static bool all_small(int dtype, const NewtonArgs& q, const std::vector<int>& live) {
+  const double cus = num_cus() > 0 ? num_cus() : 256, rate = (dtype == DTMI_F32 ? 256.0 : 128.0) * cus;
+  double longest = 0, operations = 0;
+  for (int i : live) {
+    const int64_t r = q.rows[i], c = q.cols[i];
+    if (small_lds(dtype, r, c) > small_lds_limit()) return false;
+    const double cycles = small_cycles(dtype, r, c, q.steps), m = (double)(r < c ? r : c), w = (double)(r < c ? c : r);
+    longest = cycles > longest ? cycles : longest;
+    operations += q.steps * (3.0 * m * m * w + m * m * m);
+  }
+  return (double)cdiv((int64_t)live.size(), kSmallTasks) * longest < 3.0 * q.steps * 17000.0 + operations / rate;
+}
+
+static int run_small(int dtype, const NewtonArgs& q, const std::vector<int>& live) {
+  const double es = dtype == DTMI_F32 ? 4.0 : 8.0;
+  for (size_t lo = 0; lo < live.size(); lo += kSmallTasks) {
+    SmallArgs a{};
+    const size_t count = live.size() - lo < kSmallTasks ? live.size() - lo : kSmallTasks;
+    a.steps = q.steps;
+    a.nesterov = q.nesterov;
+    a.a = q.a;
+    a.b = q.b;
+    a.c = q.c;
+    a.eps = q.eps;
+    a.mu = q.mu;
+    a.gscale = q.gscale;
+    a.gscale_dev = q.gscale_dev;
+    a.gamma = q.rate ? q.gamma : 0.0;
+    double bytes = 0;
+    for (size_t i = 0; i < count; ++i) {
+      const int j = live[lo + i];
+      a.t[i] = {q.g[j], q.m ? q.m[j] : nullptr, q.out[j], q.rate ? q.rate[j] : 1.0, (int)q.rows[j], (int)q.cols[j]};
+      bytes += (double)q.rows[j] * (double)q.cols[j] * es * (q.m ? 5 : 2);
+    }
+    TimedLaunch tl(DTMI_FAM_OTHER, bytes);
+    const int rc = launch_small(dtype, a, (int)count);
+    if (rc) return rc;
+  }
+  return DTMI_OK;
+}
+
 static int newton(const char* what, int dtype, const NewtonArgs& q) {
   DTMI_CHECK(q.n >= 0 && q.steps >= 1 && q.steps <= 64, "%s: needs 1 to 64 steps, not %d", what, q.steps);
   DTMI_CHECK(q.n == 0 || (q.g && q.out && q.rows && q.cols), "%s: NULL array", what);
@@ -297,6 +344,7 @@ static int newton(const char* what, int dtype, const NewtonArgs& q) {
     live.push_back(i);
   }
   if (live.empty()) return DTMI_OK;
+  if (all_small(dtype, q, live)) return run_small(dtype, q, live);
   const int np = norm_blocks(most, es, 512);
   void* ws = nullptr;
   int rc = pool_alloc(&ws, bytes + live.size() * (size_t)np * sizeof(double));

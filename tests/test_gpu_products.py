@@ -610,6 +610,40 @@ def test_orthogonalize(dev, dt, shape):
     assert bits_equal(got.numpy(), orthogonalize(D.from_numpy(g)).numpy())
 
 
+# blocks of 16 rows, 2, 4 and 6 of them; columns that 8 or 16 waves share or go through in
+# turn; as much as a block holds (float32) and more; a square that only the groups take
+SMALL = [(15, 17), (16, 16), (17, 16), (5, 130), (31, 33), (32, 1000), (16, 2200), (48, 49), (50, 20), (33, 270),
+         (34, 608), (64, 65), (64, 400), (80, 96), (96, 96), (97, 97), (96, 130)]
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("shape", SMALL, ids=lambda s: f"{s[0]}x{s[1]}")
+def test_orthogonalize_small_ones_alone_and_beside_a_large_one(dev, dt, shape):
+    from dtmi import device as D
+    from dtmi.optim import orthogonalize
+    rng = np.random.default_rng(shape[0] + shape[1])
+    for s in {shape, shape[::-1]}:
+        g = rng.standard_normal(s).astype(dt)
+        alone = orthogonalize(D.from_numpy(g))
+        check_ns(alone, g, dt, what="alone")
+        assert bits_equal(alone.numpy(), orthogonalize([D.from_numpy(g), D.from_numpy(g)])[1].numpy())
+        big = rng.standard_normal((130, 140)).astype(dt)
+        outs = orthogonalize([D.from_numpy(big), D.from_numpy(g)])
+        check_ns(outs[0], big, dt, what="large")
+        check_ns(outs[1], g, dt, what="beside")
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+def test_orthogonalize_more_small_ones_than_a_launch_holds(dev, dt):
+    from dtmi import device as D
+    from dtmi.optim import orthogonalize
+    rng = np.random.default_rng(0)
+    gs = [rng.standard_normal(s).astype(dt) for s in [(40, 24), (3, 17, 5), (24, 40)] + [(12, 8)] * 70 + [(1, 1)]]
+    for o, g in zip(orthogonalize([D.from_numpy(g) for g in gs]), gs):
+        for at in np.ndindex(*g.shape[:-2]):
+            check_ns(o.numpy()[at], g[at], dt)
+
+
 @pytest.mark.parametrize("dt", [F32, F64])
 def test_orthogonalize_many_at_once(dev, dt):
     """Wide, tall, square and stacked matrices and more of them than a launch holds: each
@@ -671,13 +705,14 @@ def muon_ref(p, m, g, scale, lr, mu, nesterov, wd, dt):
 
 @pytest.mark.parametrize("dt", [F32, F64])
 @pytest.mark.parametrize("nesterov", [True, False])
-def test_muon(dev, dt, nesterov):
+@pytest.mark.parametrize("large", [False, True])
+def test_muon(dev, dt, nesterov, large):
     """Three steps, with a device-side gradient factor, a changed rate, a parameter
     without a gradient, a stack of matrices and a saved state."""
     from dtmi import device as D
     from dtmi.optim import Muon
     rng = np.random.default_rng(2)
-    shapes = [(16, 48), (48, 16), (33, 33), (3, 20, 12), (7, 9)]
+    shapes = [(16, 48), (48, 16), (33, 33), (3, 20, 12), (7, 9)] + [(150, 101)] * large
     P = [(0.1 * rng.standard_normal(s)).astype(dt) for s in shapes]
     ps = [D.from_numpy(p) for p in P]
     opt = Muon(ps, lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=0.1)
