@@ -165,6 +165,25 @@ def test_loss_of_odd_sizes_and_many_rows(dev, dt, tied, C, V):
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("tied", [False, True])
+def test_loss_whose_gradients_are_grouped_products(dev, dt, tied):
+    """Odd sizes of 1e9 operations and more: all gradients, and each by itself."""
+    A, D = _mods()
+    case = (1030, 259, 2001, True, tied, 7)
+    (x, w, b, t), y, grads = loss_run(case, dt, "mean", None)
+    ry, rg = loss_ref(x, w, b, t, tied, "mean")
+    by, bx, bw = loss_bars(*case[1:2], case[0], case[2])
+    close(y, ry, dt, by, "loss")
+    for got, want, n, name in zip(grads, rg, (bx, bw, bw), ("dx", "dw", "db")):
+        close(got, want, dt, n, name)
+    for i in range(3):
+        X, W, B = (A.Tensor(D.from_numpy(v), requires_grad=i == j) for j, v in enumerate((x, w, b)))
+        A.linear_cross_entropy(X, W.transpose(1, 0) if tied else W, t, B, ignore=-100).backward()
+        assert [p.grad is None for p in (X, W, B)] == [i != j for j in range(3)]
+        close((X, W, B)[i].grad, rg[i], dt, (bx, bw, bw)[i], i)
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
 def test_loss_on_wide_tiles(dev, dt):
     """Enough rows and columns for 128-wide tiles, with edges in both."""
     case = (2100, 72, 2500, False, False, 0)
