@@ -495,7 +495,7 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
             lo, hi = (host[keep].min(), host[keep].max()) if n else (0, -1)
     if lo < 0 or hi >= V:
         raise IndexError(f"target out of bounds for size {V}")
-    X2 = X.reshape(rows, C)
+    X2 = X if X.ndim == 2 else X.reshape(rows, C)
     t = ix.dev if ix is not None else dev.from_numpy(host.reshape(-1).astype(np.int64))
     mean = reduction == "mean"
     need = [_grad_enabled and p is not None and p.requires_grad for p in (x, w, b)]
@@ -509,14 +509,14 @@ def linear_cross_entropy(x: Tensor, w: Tensor, targets, b: Tensor | None = None,
             # into their destinations, or in place
             made, dests = list(pending.pop()), (None, None if tied else grad_out(w),
                                                 grad_out(b) if b is not None else None)
-            g1 = _contig(g).reshape(1)
-            if not dev.known_ones(g1):
-                K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], g1)
-            dx, dw, db = [d if o is None or d is None else K.scale(d, alpha_dev=g1, out=o)
+            if not dev.known_ones(g):
+                K.grad_scale_multi([d for d, o in zip(made, dests) if o is None], _contig(g).reshape(1))
+            dx, dw, db = [d if o is None or d is None else K.scale(d, alpha_dev=_contig(g).reshape(1), out=o)
                           for d, o in zip(made, dests)]
         else:
             dx, dw, db = K.linear_xent(X2, W, bd, t, g=_contig(g).reshape(-1), **rest, **grads)[2:]
-        dx = dx.reshape(x.shape) if dx is not None else None
+        if dx is not None and dx.shape != x.shape:
+            dx = dx.reshape(x.shape)
         dw = dw.transpose(1, 0) if dw is not None and tied else dw
         return (dx, dw) if b is None else (dx, dw, db)
     out = total if mean else ls.reshape(lead)
