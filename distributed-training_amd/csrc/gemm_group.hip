@@ -18,15 +18,32 @@ struct GroupPlan {
 // Few rows: gemm_rows.h, up to 32 (the tile is then 16 or 32 rows).
 constexpr int kFewRows = 32;
 
+// Bytes of a wave's tile of few rows.
+template <typename T>
+static int64_t rows_bytes(int mr, int bkc) {
+  return 4 * mr * (bkc ? RowsTile<T, true>::NT : RowsTile<T, false>::NT) * 64 * (int64_t)sizeof(T);
+}
+
 // Waves of a block of few rows: 16 per CU, each with at least a batch of k, and their
 // partial tiles within 64 KB.
 template <typename T>
 static int rows_waves(int64_t blocks, int64_t K, int64_t cus, int mr, int bkc) {
-  const int64_t bytes = 4 * mr * (bkc ? RowsTile<T, true>::NT : RowsTile<T, false>::NT) * 64 * (int64_t)sizeof(T);
+  const int64_t bytes = rows_bytes<T>(mr, bkc);
   int64_t w = 1;
   while (w < kRowsMaxWaves && blocks * w < 16 * cus && 2 * w * bytes <= 64 * 1024) w *= 2;
   const int64_t batches = cdiv(K > 0 ? K : 1, RowsTile<T, true>::BATCH);
   return (int)(w < batches ? w : batches);
+}
+
+// Blocks along k for few rows: a wave waits about 1.8 us for each batch of its share, and
+// joining the pieces is a launch of 6 us. Pieces of three batches from seven on, up to four
+// blocks a CU: one row of 3993 x 136 31 -> 12 us, two of 23011 x 1247 71 (the GEMM) -> 35.
+template <typename T>
+static int rows_splits(int64_t blocks, int64_t K, int64_t cus, int nw) {
+  const int64_t batches = cdiv(K, (int64_t)nw * RowsTile<T, true>::BATCH);
+  const int64_t want = cdiv(batches, 3), fit = 4 * cus / blocks;
+  const int64_t s = want < fit ? want : fit;
+  return batches > 6 && s > 1 ? (int)s : 1;
 }
 
 // Waves of a small-product block: 8 per CU, each with at least a batch of k.
@@ -200,8 +217,9 @@ static int plan_tasks(int akc, int bkc, std::vector<GroupTask>& tasks, int dmode
     a.tiles = (int)tiles;
     a.work = (int)work;
     if (few) l.nw = rows_waves<T>(tiles, a.t[0].K, cus, l.mr, bkc);
+    const int pieces = few ? rows_splits<T>(tiles, a.t[0].K, cus, l.nw) : p.splits;
     a.cut = p.cut < a.work ? p.cut : a.work;
-    a.splits = p.splits;
+    a.splits = pieces;
     for (int i = 0; i < a.count && a.cut; ++i) {  // whole tiles that are longer than the pieces
       const int end = i + 1 < a.count ? a.first[i + 1] : a.tiles;
       if (end > a.cut && a.t[i].K > 0 && a.t[i].K >= cdiv(a.t[0].K, p.splits)) a.before = end - a.cut;
@@ -213,6 +231,7 @@ static int plan_tasks(int akc, int bkc, std::vector<GroupTask>& tasks, int dmode
         a.turned = (int)units;
       }
     }
+    if (few && pieces > 1) l.ws_bytes = (size_t)pieces * tiles * rows_bytes<T>(l.mr, bkc);
     if (a.cut) {
       const size_t slots = (size_t)p.splits * a.cut;
       l.cs_at = slots * p.tile * p.tile * sizeof(T);

@@ -91,6 +91,13 @@ __device__ __forceinline__ GroupEpi<T> group_epi(const GroupArgs& a, const Group
           zeros ? pad_up(k.M, a.pad) : k.M, zeros ? pad_up(k.N, a.pad) : k.N};
 }
 
+// A column sum, added to the old one where C is.
+template <typename T>
+__device__ __forceinline__ void put_colsum(const GroupArgs& a, const GroupTask& k, int64_t n, T v) {
+  T* d = (T*)k.D + n;
+  *d = a.gamma != 0.0 ? fma((T)a.gamma, *d, v) : v;
+}
+
 // A wave tile's accumulators through the epilogue.
 template <typename T, int TW>
 __device__ __forceinline__ void group_write(const GroupEpi<T>& e, const typename MF<T>::acc_t (&acc)[TW][TW], int64_t wm,
@@ -236,7 +243,7 @@ __global__ void __launch_bounds__(256, 2) gemm_group_kernel(GroupArgs a) {
     if (take_colsum) ((T*)a.csws)[slot * BM + threadIdx.x] = (T)csum;
     return;
   }
-  if (take_colsum && k.D && n0 + threadIdx.x < k.N) ((T*)k.D)[n0 + threadIdx.x] = (T)csum;
+  if (take_colsum && k.D && n0 + threadIdx.x < k.N) put_colsum(a, k, n0 + threadIdx.x, (T)csum);
   group_write<T, TW>(group_epi<T>(a, k, a.sym && tm != tn), acc, m0 + wm, n0 + wn, g, c);
 }
 
@@ -293,7 +300,7 @@ __global__ void __launch_bounds__(256) group_sum_kernel(GroupArgs a) {
     const T* S = (const T*)a.csws + (int64_t)blockIdx.x * BM + threadIdx.x;
     T x = S[0];
     for (int q = 1; q < a.splits; ++q) x = x + S[(int64_t)q * a.cut * BM];
-    ((T*)k.D)[n] = x;
+    put_colsum(a, k, n, x);
   }
 }
 
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(64 * kGroupWaves) group_direct_kernel(GroupArg
     for (int n = threadIdx.x; n < 32 && n0 + n < k.N; n += blockDim.x) {
       double x = red[n];
       for (int w = 1; w < nw; ++w) x += red[w * 32 + n];
-      ((T*)k.D)[n0 + n] = (T)x;
+      put_colsum(a, k, n0 + n, (T)x);
     }
   }
 }
@@ -555,15 +562,17 @@ __global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1
   const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = (int)(blockDim.x >> 6);
   const int first = lane < a.count ? a.first[lane] : 0x7fffffff;
-  const int b = (int)blockIdx.x;
+  const int split = (int)blockIdx.x / a.tiles, b = (int)blockIdx.x - split * a.tiles;
   const int ti = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(__ballot(first <= b)));
   const GroupTask k = a.t[ti];
   const int tiles_m = (k.M + 16 * MR - 1) / (16 * MR);
   const int64_t m0 = (int64_t)((b - a.first[ti]) % tiles_m) * (16 * MR);
   const int64_t n0 = (int64_t)((b - a.first[ti]) / tiles_m) * RT::COLS;
-  const int per = ((k.K + nw - 1) / nw + RT::BATCH - 1) / RT::BATCH * RT::BATCH;
-  const int kbeg = wave * per < k.K ? wave * per : k.K;
-  const int kend = kbeg + per < k.K ? kbeg + per : k.K;
+  const int shares = nw * a.splits;  // of k
+  const int per = ((k.K + shares - 1) / shares + RT::BATCH - 1) / RT::BATCH * RT::BATCH;
+  const int64_t from = (int64_t)(split * nw + wave) * per;
+  const int kbeg = from < k.K ? (int)from : k.K;
+  const int kend = k.K - kbeg < per ? k.K : kbeg + per;
   RowsAcc<T> acc[MR][RT::NT];
 #pragma unroll
   for (int i = 0; i < MR; ++i)
@@ -573,12 +582,44 @@ __global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1
   const RS sum{reinterpret_cast<T*>(lds_raw), lane, nw};
   sum.put(acc, wave);
   __syncthreads();
+  if (a.splits > 1) {  // the raw partial
+    T* P = (T*)a.ws + (int64_t)blockIdx.x * (RS::REGS * 64) + lane;
+    for (int q = wave; q < RS::REGS; q += nw) P[q * 64] = sum.value(q);
+    return;
+  }
   const GroupEpi<T> e = group_epi<T>(a, k, false);
   for (int q = wave; q < RS::REGS; q += nw) {
     const int64_t m = m0 + 16 * (q / (4 * RT::NT)) + RowsMma<T>::row(q % 4, g), n = n0 + RT::col(c, q / 4 % RT::NT);
     const T v = sum.value(q);
     if (m < e.M && n < e.N) e.store(m, n, v);
   }
+}
+
+// The partials of a tile of few rows, added in split order, and the epilogue: block (v, y)
+// takes four registers of tile v, a wave each.
+template <typename T, int MR, bool BKC>
+__global__ void __launch_bounds__(256) rows_sum_kernel(GroupArgs a) {
+  using RT = RowsTile<T, BKC>;
+  using RS = RowsSum<T, MR, BKC>;
+  const int lane = threadIdx.x & 63, g = lane / 16, c = lane % 16, q = (int)blockIdx.y * 4 + (threadIdx.x >> 6);
+  const int first = lane < a.count ? a.first[lane] : 0x7fffffff, b = (int)blockIdx.x;
+  const int ti = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(__ballot(first <= b)));
+  const GroupTask k = a.t[ti];
+  const int tiles_m = (k.M + 16 * MR - 1) / (16 * MR);
+  const int64_t m = (int64_t)((b - a.first[ti]) % tiles_m) * (16 * MR) + 16 * (q / (4 * RT::NT)) + RowsMma<T>::row(q % 4, g);
+  const int64_t n = (int64_t)((b - a.first[ti]) / tiles_m) * RT::COLS + RT::col(c, q / 4 % RT::NT);
+  const T* P = (const T*)a.ws + (int64_t)b * (RS::REGS * 64) + q * 64 + lane;
+  const int64_t step = (int64_t)a.tiles * (RS::REGS * 64);
+  T v = T(0);
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    T x[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[s] = s0 + s < a.splits ? P[(s0 + s) * step] : T(0);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) v = v + x[s];
+  }
+  const GroupEpi<T> e = group_epi<T>(a, k, false);
+  if (m < e.M && n < e.N) e.store(m, n, v);
 }
 
 template <typename T, int MR, bool BKC>
@@ -669,23 +710,20 @@ void launch_group_direct(const GroupArgs& a, int akc, int bkc, int nw) {
     group_direct_kernel<T, false, false><<<grid, th, lds, stream()>>>(a);
 }
 
+template <typename T, int MR, bool BKC>
+static void launch_rows_tile(const GroupArgs& a, int nw) {
+  constexpr int REGS = RowsSum<T, MR, BKC>::REGS;
+  group_rows_kernel<T, MR, BKC>
+      <<<(unsigned)(a.tiles * a.splits), 64u * (unsigned)nw, (size_t)nw * REGS * 64 * sizeof(T), stream()>>>(a);
+  if (a.splits > 1) rows_sum_kernel<T, MR, BKC><<<dim3((unsigned)a.tiles, REGS / 4), 256, 0, stream()>>>(a);
+}
+
 template <typename T>
 void launch_group_rows(const GroupArgs& a, int bkc, int mr, int nw) {
-  const unsigned grid = (unsigned)a.tiles, th = 64u * (unsigned)nw;
-#define DTMI_ROWS(MR, BKK)                                                                      \
-  group_rows_kernel<T, MR, BKK><<<grid, th, (size_t)nw * RowsSum<T, MR, BKK>::REGS * 64 * sizeof(T), stream()>>>(a)
-  if (mr == 1) {
-    if (bkc)
-      DTMI_ROWS(1, true);
-    else
-      DTMI_ROWS(1, false);
-  } else {
-    if (bkc)
-      DTMI_ROWS(2, true);
-    else
-      DTMI_ROWS(2, false);
-  }
-#undef DTMI_ROWS
+  if (mr == 1)
+    bkc ? launch_rows_tile<T, 1, true>(a, nw) : launch_rows_tile<T, 1, false>(a, nw);
+  else
+    bkc ? launch_rows_tile<T, 2, true>(a, nw) : launch_rows_tile<T, 2, false>(a, nw);
 }
 
 template <typename T>

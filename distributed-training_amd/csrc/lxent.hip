@@ -277,26 +277,37 @@ struct Scratch {
   }
 };
 
+// Whether the products run in the type they are in: the split bf16 arithmetic is the GEMM's.
+template <typename T>
+static bool plain_products() {
+  int math = DTMI_GEMM_MATH_F32;
+  return sizeof(T) == 8 || (dtmi_get_gemm_math(&math) == DTMI_OK && math == DTMI_GEMM_MATH_F32);
+}
+
 // Whether a piece's gradients are products of gemm_group.h, whose ragged last rounds cost
 // less than the GEMM's: the largest (4096 x 768 x 50304, dw 2.13 ms and 2.32, dx 2.18 and
 // 2.18), and odd sizes (1067 x 515 x 50257 517 and 546 us, 531 and 565; float64 1000 x 385 x
 // 8001 123 and 145, 132 and 158). Others are quicker by the GEMM (4000 x 384 x 8000, dw 194
-// and 213 us), which also has the split bf16 arithmetic.
+// and 213 us).
 template <typename T>
 static bool grouped(int64_t R, int64_t C, int64_t V) {
-  int math = DTMI_GEMM_MATH_F32;
-  if (dtmi_get_gemm_math(&math) != DTMI_OK || (sizeof(T) == 4 && math != DTMI_GEMM_MATH_F32)) return false;
+  if (!plain_products<T>()) return false;
   const double operations = 2.0 * (double)R * (double)C * (double)V;
   return operations >= 1e11 || (operations >= 1e9 && (C % MF<T>::VEC || V % MF<T>::VEC));
 }
 
+// dx of few rows: their products split the vocabulary over more blocks than the GEMM's tiles
+// do (8 x 175 x 26217 15 us and 53, 32 x 515 x 50257 57 and 93, 4 x 605 x 1055 13 and 9).
+constexpr int64_t kFewRows = 32, kFewWords = 2000;
+
 // dw, db and dx of a piece of n rows with its dz in Z. dx last: it may take x's place.
 template <typename T>
 static int grad_products(int dtype, const LxentArgs& q, int64_t n, char* Z, const char* X, char* dX, int add) {
+  const int rows = (int)n, C = (int)q.C, V = (int)q.V;
+  const bool group = grouped<T>(n, q.C, q.V);
   int rc = DTMI_OK;
-  if (grouped<T>(n, q.C, q.V)) {
-    const int rows = (int)n, C = (int)q.C, V = (int)q.V;
-    const bool sums = q.db && q.dW && !q.tied && !add;  // db by the tiles of dw
+  if (group) {
+    const bool sums = q.db && q.dW && !q.tied;  // db by the tiles of dw
     std::vector<GroupLaunch> l;
     if (q.dW) {
       const GroupTask t = q.tied ? GroupTask{Z, X, q.dW, nullptr, V, C, rows, 0, 1.0}
@@ -305,14 +316,7 @@ static int grad_products(int dtype, const LxentArgs& q, int64_t n, char* Z, cons
       if (!rc) rc = launch_group(dtype, l);
     }
     if (!rc && q.db && !sums) rc = dtmi_colsum(dtype, q.db, Z, n, q.V, add);
-    if (!rc && dX) {
-      rc = plan_group(dtype, 1, q.tied ? 0 : 1, {GroupTask{Z, q.W, dX, nullptr, rows, C, V, 0, 1.0}}, kDNone, 0, 1.0,
-                      0.0, 0.0, 1, 1, l);
-      if (!rc) rc = launch_group(dtype, l);
-    }
-    return rc;
-  }
-  if (q.tied) {
+  } else if (q.tied) {
     if (q.dW) rc = dtmi_gemm(dtype, 0, 0, q.V, q.C, n, Z, q.V, 0, X, q.C, 0, q.dW, q.C, 0, 1, nullptr, add, 0);
     if (!rc && q.db) rc = dtmi_colsum(dtype, q.db, Z, n, q.V, add);
   } else if (q.dW) {
@@ -320,10 +324,15 @@ static int grad_products(int dtype, const LxentArgs& q, int64_t n, char* Z, cons
   } else if (q.db) {
     rc = dtmi_colsum(dtype, q.db, Z, n, q.V, add);
   }
-  if (!rc && dX)
-    rc = q.tied ? dtmi_gemm(dtype, 1, 0, n, q.C, q.V, Z, q.V, 0, q.W, q.C, 0, dX, q.C, 0, 1, nullptr, 0, 0)
+  if (rc || !dX || C == 0) return rc;
+  if (group || (n <= kFewRows && V >= kFewWords && plain_products<T>())) {
+    std::vector<GroupLaunch> l;
+    rc = plan_group(dtype, 1, q.tied ? 0 : 1, {GroupTask{Z, q.W, dX, nullptr, rows, C, V, 0, 1.0}}, kDNone, 0, 1.0, 0.0,
+                    0.0, 1, 1, l);
+    return rc ? rc : launch_group(dtype, l);
+  }
+  return q.tied ? dtmi_gemm(dtype, 1, 0, n, q.C, q.V, Z, q.V, 0, q.W, q.C, 0, dX, q.C, 0, 1, nullptr, 0, 0)
                 : dtmi_linear_bwd_dx(dtype, dX, Z, q.W, n, q.C, q.V, 0);
-  return rc;
 }
 
 template <typename T>

@@ -63,6 +63,9 @@ LOSS = [  # rows, C, V, bias, tied, ignored targets
     (32, 515, 777, True, False, 2),
     (17, 1030, 514, False, True, 0),
     (31, 90, 1029, False, False, 0),
+    (2, 129, 3001, True, False, 0),      # few rows and many words
+    (17, 40, 9001, False, True, 3),
+    (32, 70, 6000, True, False, 0),
 ]
 
 
@@ -467,6 +470,8 @@ EXPERTS = [  # R, K, N, sizes, bias
     (20, 515, 201, [16, 0, 4], True),                 # few rows each
     (41, 770, 131, [32, 7, 1], False),
     (9, 36, 1000, [1, 8], True),
+    (24, 5003, 70, [16, 0, 5], True),                 # and long rows, split over blocks
+    (33, 60, 4100, [1, 32], False),
     (5000, 24, 40, [4000, 999], True),                # sums over rows long enough to be split
 ]
 
