@@ -68,12 +68,15 @@ static double direct_cycles(int64_t tiles, double kavg, int64_t kmax, int nw, in
 // tile_cost in gemm.hip (64-wide float32 tiles over several tasks reach less, 0.80 to
 // 0.89 of their MFMA rate), with what a block costs before its first MFMA and after its
 // last, of which the others on its CU hide some: 64 experts' dw, 384 x 501 from 62 rows
-// each, took 42 us on 3072 64-wide tiles. A 128-wide float32 tile alone on its CU waits for
+// each, took 42 us on 48 64-wide tiles an expert. A 128-wide float32 tile alone on its CU waits for
 // its loads, of single elements the more (vec false): four times 713 x 1075 with 619 terms,
 // 216 tiles: 55 us (816 64-wide ones: 48), 704 x 1088 with 640: 48 us.
 static double tile_cycles(int bm, double k, double units, int64_t cus, size_t es, bool vec) {
   const double alone = es == 8 ? 0.82 : vec ? 0.78 : 0.66;
-  const double eff = bm == 64 ? (units > cus ? (es == 4 ? 0.82 : 0.88) : 0.75) : units > 2.0 * cus ? 0.97 : units > cus ? 1.0 : alone;
+  const double eff = bm == 64           ? (units > cus ? (es == 4 ? 0.82 : 0.88) : 0.75)
+                     : units > 2.0 * cus ? 0.97
+                     : units > cus       ? 1.0
+                                         : alone;
   return 8800.0 + 1500.0 * units / (double)cus + k * (es == 4 ? 32.0 : 64.0) * (bm / 32) * (bm / 32) / 4.0 / eff;
 }
 // and what a split adds: its partials' traffic and a launch
@@ -130,8 +133,10 @@ static GroupPlan choose_plan(const GroupTask* t, int count, int sym, int pad, in
     for (int sp = 2; sp <= 16 && k[0] / sp >= 128; ++sp) {
       const double ks = (double)(cdiv(cdiv(k[0], sp), bk) * bk);
       if (ks <= (double)chain || sp == 16) {
-        const double busy = equal ? (double)cdiv(total * sp, cus) * ks : std::max(ks, even + 0.5 * (double)k[last] / sp);
-        take(tile_cycles(bm, busy, (double)(total * sp), cus, es, vec) + split_cycles(bm, total, sp, es), {bm, kAll, sp, 0});
+        const double busy =
+            equal ? (double)cdiv(total * sp, cus) * ks : std::max(ks, even + 0.5 * (double)k[last] / sp);
+        take(tile_cycles(bm, busy, (double)(total * sp), cus, es, vec) + split_cycles(bm, total, sp, es),
+             {bm, kAll, sp, 0});
       }
       if (rest && k[0] <= chain) {
         // a quarter tile more: the last whole tiles run beside fewer and fewer pieces
@@ -284,7 +289,6 @@ int launch_group(int dtype, const std::vector<GroupLaunch>& launches) {
   return DTMI_OK;
 }
 
-// Tile and waves of a statistics product (tile 16: few rows).
 // What the statistics of a tile add to its product (exponentials, and the joins along its
 // rows): a block alone on its CU waits for all of it, the others hide two thirds. float32
 // 388 x 17704 with 66 terms: 42.8 us on 32-wide tiles, 24.2 on 64, 24.9 on 128; float64
@@ -295,6 +299,7 @@ static double epilogue_cycles(int bm, int64_t units, int64_t cus, size_t es) {
   return one * (1.0 + 0.35 * (double)(cdiv(units, cus) - 1));
 }
 
+// Tile and waves of a statistics product (tile 16: few rows).
 template <typename T>
 static GroupPlan plan_stats(int bkc, int64_t M, int64_t N, int64_t K) {
   const int64_t cus = num_cus() > 0 ? num_cus() : 256;

@@ -86,7 +86,8 @@ struct GroupEpi {
 template <typename T>
 __device__ __forceinline__ GroupEpi<T> group_epi(const GroupArgs& a, const GroupTask& k, bool mirror) {
   const bool zeros = a.padc == a.pad;
-  return {(T)a.alpha, (T)a.beta, (T)a.gamma, (T)k.s, k.D ? a.dmode : (int)kDNone, mirror, k.turned != 0, (const T*)k.D, (T*)k.C,
+  return {(T)a.alpha, (T)a.beta, (T)a.gamma, (T)k.s,
+          k.D ? a.dmode : (int)kDNone, mirror, k.turned != 0, (const T*)k.D, (T*)k.C,
           (int64_t)pad_up(k.N, a.pad), (int64_t)pad_up(k.turned ? k.M : k.N, a.padc),
           zeros ? pad_up(k.M, a.pad) : k.M, zeros ? pad_up(k.N, a.pad) : k.N};
 }
@@ -100,8 +101,8 @@ __device__ __forceinline__ void put_colsum(const GroupArgs& a, const GroupTask& 
 
 // A wave tile's accumulators through the epilogue.
 template <typename T, int TW>
-__device__ __forceinline__ void group_write(const GroupEpi<T>& e, const typename MF<T>::acc_t (&acc)[TW][TW], int64_t wm,
-                                            int64_t wn, int g, int c) {
+__device__ __forceinline__ void group_write(const GroupEpi<T>& e, const typename MF<T>::acc_t (&acc)[TW][TW],
+                                            int64_t wm, int64_t wn, int g, int c) {
   using MFT = MF<T>;
   constexpr int MT = MFT::MT, NACC = MFT::NACC, W = TW * MT;
   if constexpr (sizeof(T) == 4) {
@@ -555,7 +556,8 @@ __global__ void __launch_bounds__(64 * kGroupWaves) stats_direct_kernel(StatsArg
 
 // Few rows (gemm_rows.h): a tile of 16 MR rows a block.
 template <typename T, int MR, bool BKC>
-__global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1 ? 4 : 2)) group_rows_kernel(GroupArgs a) {
+__global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1 ? 4 : 2))
+    group_rows_kernel(GroupArgs a) {
   using RT = RowsTile<T, BKC>;
   using RS = RowsSum<T, MR, BKC>;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];
@@ -606,7 +608,8 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(GroupArgs a) {
   const int ti = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(__ballot(first <= b)));
   const GroupTask k = a.t[ti];
   const int tiles_m = (k.M + 16 * MR - 1) / (16 * MR);
-  const int64_t m = (int64_t)((b - a.first[ti]) % tiles_m) * (16 * MR) + 16 * (q / (4 * RT::NT)) + RowsMma<T>::row(q % 4, g);
+  const int64_t m =
+      (int64_t)((b - a.first[ti]) % tiles_m) * (16 * MR) + 16 * (q / (4 * RT::NT)) + RowsMma<T>::row(q % 4, g);
   const int64_t n = (int64_t)((b - a.first[ti]) / tiles_m) * RT::COLS + RT::col(c, q / 4 % RT::NT);
   const T* P = (const T*)a.ws + (int64_t)b * (RS::REGS * 64) + q * 64 + lane;
   const int64_t step = (int64_t)a.tiles * (RS::REGS * 64);
@@ -623,7 +626,8 @@ __global__ void __launch_bounds__(256) rows_sum_kernel(GroupArgs a) {
 }
 
 template <typename T, int MR, bool BKC>
-__global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1 ? 4 : 2)) stats_rows_kernel(StatsArgs a) {
+__global__ void __launch_bounds__(64 * kRowsMaxWaves, (sizeof(T) == 4 && MR == 1 ? 4 : 2))
+    stats_rows_kernel(StatsArgs a) {
   using RT = RowsTile<T, BKC>;
   using RS = RowsSum<T, MR, BKC>;
   extern __shared__ __attribute__((aligned(16))) char lds_raw[];

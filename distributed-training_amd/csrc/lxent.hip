@@ -50,9 +50,9 @@ struct RowStat {
 // for every row its place among them or -1. One block, four rows a thread at a time
 // (2683 rows: 3.4 us). n is the caller's count: no more are written, and what a count too
 // large leaves over names row 0.
-__global__ void __launch_bounds__(1024) lxent_rows_kernel(const int64_t* __restrict__ targets, int64_t R, int64_t ignore,
-                                                          int64_t n, int* __restrict__ sel, int64_t* __restrict__ t,
-                                                          int* __restrict__ place) {
+__global__ void __launch_bounds__(1024) lxent_rows_kernel(const int64_t* __restrict__ targets, int64_t R,
+                                                          int64_t ignore, int64_t n, int* __restrict__ sel,
+                                                          int64_t* __restrict__ t, int* __restrict__ place) {
   constexpr int U = 4;
   __shared__ int sh[2][U][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -371,14 +371,14 @@ static int lxent_pieces(int dtype, const LxentArgs& q, int64_t piece, char* Z, c
     {
       TimedLaunch tl(DTMI_FAM_XENT, 2.0 * (double)(parts * n) * es);
       if (joint)
-        lxent_join_mean_kernel<T><<<1, 1024, 0, stream()>>>(pmax, psum, (int)parts, (int)n, zt, a.targets, q.ignore, rmax,
-                                                            rsum, losses, q.coef, (T*)q.mean);
+        lxent_join_mean_kernel<T><<<1, 1024, 0, stream()>>>(pmax, psum, (int)parts, (int)n, zt, a.targets, q.ignore,
+                                                            rmax, rsum, losses, q.coef, (T*)q.mean);
       else if (n <= 512)
-        lxent_join_kernel<T, 1><<<(unsigned)n, 1024, 0, stream()>>>(pmax, psum, parts, n, zt, a.targets, q.ignore, rmax, rsum,
-                                                                    losses);
+        lxent_join_kernel<T, 1><<<(unsigned)n, 1024, 0, stream()>>>(pmax, psum, parts, n, zt, a.targets, q.ignore, rmax,
+                                                                    rsum, losses);
       else
-        lxent_join_kernel<T, 32><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, a.targets, q.ignore,
-                                                                               rmax, rsum, losses);
+        lxent_join_kernel<T, 32><<<(unsigned)cdiv(n, 32), 1024, 0, stream()>>>(pmax, psum, parts, n, zt, a.targets,
+                                                                               q.ignore, rmax, rsum, losses);
     }
     if (grads) {
       {
@@ -519,7 +519,8 @@ DTMI_EXPORT int dtmi_linear_xent(int dtype, int64_t R, int64_t C, int64_t V, con
   }
   DTMI_CHECK(targets && (C == 0 || (X && W)), "%s: NULL pointer", __func__);
   LxentArgs q{R, C, V, (const char*)X, (const char*)W, tied ? 1 : 0, b, targets, counted,
-              counted < R ? ignore : INT64_MIN, (char*)losses, mean, (const char*)g, g_stride, coef, (char*)dX, (char*)dW, (char*)db};
+              counted < R ? ignore : INT64_MIN, (char*)losses, mean, (const char*)g, g_stride, coef,
+              (char*)dX, (char*)dW, (char*)db};
   return dtype == DTMI_F32 ? lxent_run<float>(dtype, q) : lxent_run<double>(dtype, q);
   DTMI_BODY_END
 }

@@ -232,8 +232,8 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
     }
     TimedLaunch tl(DTMI_FAM_OTHER, bytes);
     norm_sum_kernel<T><<<dim3((unsigned)np, (unsigned)count), 256, 0, stream()>>>(a);
-    norm_scale_kernel<T><<<dim3((unsigned)norm_blocks(most, es, 4096 / count < 64 ? 64 : 4096 / count), (unsigned)count), 256,
-                           0, stream()>>>(a);
+    const int blocks = norm_blocks(most, es, 4096 / count < 64 ? 64 : 4096 / count);
+    norm_scale_kernel<T><<<dim3((unsigned)blocks, (unsigned)count), 256, 0, stream()>>>(a);
     LAUNCH_CHECK("norm kernels");
   }
   // the launches of a step from x0 to x1 and of one from x1 to x0, and of the last

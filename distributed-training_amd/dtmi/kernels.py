@@ -940,8 +940,8 @@ def linear_xent(x2: DeviceArray, w: DeviceArray, b: DeviceArray | None, targets:
     dw = empty(w.shape, x2.dtype) if need_dw else None
     db = empty((V,), x2.dtype) if need_db else None
     _c("dtmi_linear_xent", d, R, C_, V, x2.ptr, w.ptr, 1 if tied else 0, _opt_ptr(b), targets.ptr,
-       R if counted is None else counted, ignore, _opt_ptr(ls), _opt_ptr(mn), _opt_ptr(g), 1 if g is not None and g.size == R and R > 1 else 0, float(coef), _opt_ptr(dx),
-       _opt_ptr(dw), _opt_ptr(db))
+       R if counted is None else counted, ignore, _opt_ptr(ls), _opt_ptr(mn), _opt_ptr(g),
+       1 if g is not None and g.size == R and R > 1 else 0, float(coef), _opt_ptr(dx), _opt_ptr(dw), _opt_ptr(db))
     return ls, mn, dx, dw, db
 
 
