@@ -194,6 +194,36 @@ static size_t bytes_of(int64_t r, int64_t c, size_t es) {
   return ((size_t)up(r, v) * up(c, v) * es + 255) & ~(size_t)255;
 }
 
+// The sums of squares of all u, momenta moved on, and, with x, u / (|u| + eps) there.
+template <typename T>
+static int norms(const NewtonArgs& q, const std::vector<int>& live, int64_t most, int np, double* parts,
+                 const std::vector<char*>* x) {
+  const int n = (int)live.size();
+  for (int lo = 0; lo < n; lo += kNormTasks) {
+    NormArgs a{};
+    const int count = n - lo < kNormTasks ? n - lo : kNormTasks;
+    a.nesterov = q.nesterov;
+    a.parts = np;
+    a.mu = q.mu;
+    a.eps = q.eps;
+    a.gscale = q.gscale;
+    a.gscale_dev = q.gscale_dev;
+    double bytes = 0;
+    for (int i = 0; i < count; ++i) {
+      const int j = live[lo + i];
+      a.t[i] = {q.g[j], q.m ? q.m[j] : nullptr, x ? (*x)[lo + i] : nullptr, parts + (size_t)(lo + i) * np, (int)q.rows[j],
+                (int)q.cols[j]};
+      bytes += (double)q.rows[j] * (double)q.cols[j] * (double)sizeof(T) * (x ? (q.m ? 6 : 3) : (q.m ? 3 : 1));
+    }
+    TimedLaunch tl(DTMI_FAM_OTHER, bytes);
+    norm_sum_kernel<T><<<dim3((unsigned)np, (unsigned)count), 256, 0, stream()>>>(a);
+    const int blocks = norm_blocks(most, sizeof(T), 4096 / count < 64 ? 64 : 4096 / count);
+    if (x) norm_scale_kernel<T><<<dim3((unsigned)blocks, (unsigned)count), 256, 0, stream()>>>(a);
+    LAUNCH_CHECK("norm kernels");
+  }
+  return DTMI_OK;
+}
+
 template <typename T>
 static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& live, int64_t most, int np, char* ws) {
   constexpr size_t es = sizeof(T);
@@ -214,28 +244,8 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
     H[i] = G[i] + gb;
     p = H[i] + gb;
   }
-  for (int lo = 0; lo < n; lo += kNormTasks) {
-    NormArgs a{};
-    const int count = n - lo < kNormTasks ? n - lo : kNormTasks;
-    a.nesterov = q.nesterov;
-    a.parts = np;
-    a.mu = q.mu;
-    a.eps = q.eps;
-    a.gscale = q.gscale;
-    a.gscale_dev = q.gscale_dev;
-    double bytes = 0;
-    for (int i = 0; i < count; ++i) {
-      const int j = live[lo + i];
-      a.t[i] = {q.g[j], q.m ? q.m[j] : nullptr, x0[lo + i], parts + (size_t)(lo + i) * np, (int)q.rows[j],
-                (int)q.cols[j]};
-      bytes += (double)q.rows[j] * (double)q.cols[j] * (double)es * (q.m ? 6 : 3);
-    }
-    TimedLaunch tl(DTMI_FAM_OTHER, bytes);
-    norm_sum_kernel<T><<<dim3((unsigned)np, (unsigned)count), 256, 0, stream()>>>(a);
-    const int blocks = norm_blocks(most, es, 4096 / count < 64 ? 64 : 4096 / count);
-    norm_scale_kernel<T><<<dim3((unsigned)blocks, (unsigned)count), 256, 0, stream()>>>(a);
-    LAUNCH_CHECK("norm kernels");
-  }
+  int rc = norms<T>(q, live, most, np, parts, &x0);
+  if (rc) return rc;
   // the launches of a step from x0 to x1 and of one from x1 to x0, and of the last
   std::vector<GroupTask> t(n);
   std::vector<GroupLaunch> gram[2], sq, apply[2], final;
@@ -245,7 +255,7 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
     w = (int)(r < c ? c : r);
     return r > c;
   };
-  int m, w, rc = DTMI_OK;
+  int m, w;
   for (int i = 0; i < n; ++i) {  // H = b G + c G G (G = G^T)
     of(i, m, w);
     t[i] = {G[i], G[i], H[i], G[i], m, m, m, 0, 1.0};
@@ -323,6 +333,75 @@ static int run_small(int dtype, const NewtonArgs& q, const std::vector<int>& liv
   return DTMI_OK;
 }
 
+// Whether every matrix is thin, and the two launches a step of newton_small.hip are quicker
+// than the groups' three. Thin and groups, five steps: 21 x 1088 61 and 129 us, 2 of 1102 x
+// 41 76 and 144, 48 of 64 x 768 163 and 182, 16 of 64 x 8192 394 and 297; float64, 8 of
+// 30 x 1000: 70 and 172.
+static bool all_thin(int dtype, const NewtonArgs& q, const std::vector<int>& live, size_t& bytes) {
+  const int64_t cus = num_cus() > 0 ? num_cus() : 256;
+  const double rate = (dtype == DTMI_F32 ? 256.0 : 128.0) * (double)cus;
+  double longest = 0, operations = 0;
+  int64_t blocks = 0;
+  bytes = 256;
+  for (int i : live) {
+    if (thin_lds(dtype, q.rows[i], q.cols[i]) > small_lds_limit()) return false;
+    blocks += thin_blocks(q.rows[i], q.cols[i]);
+    bytes += thin_bytes(dtype, q.rows[i], q.cols[i]);
+  }
+  for (int i : live) {
+    const double cycles = thin_cycles(dtype, q.rows[i], q.cols[i], blocks, cus);
+    const double m = (double)(q.rows[i] < q.cols[i] ? q.rows[i] : q.cols[i]);
+    const double w = (double)(q.rows[i] < q.cols[i] ? q.cols[i] : q.rows[i]);
+    longest = cycles > longest ? cycles : longest;
+    operations += q.steps * (3.0 * m * m * w + m * m * m);
+  }
+  const double launches = (double)cdiv((int64_t)live.size(), kSmallTasks);
+  return blocks < (1 << 24) && launches * q.steps * longest < 3.0 * q.steps * 17000.0 + operations / rate;
+}
+
+template <typename T>
+static int run_thin(int dtype, const NewtonArgs& q, const std::vector<int>& live, int64_t most, int np, char* ws) {
+  double* parts = (double*)ws;
+  char* p = ws + ((live.size() * (size_t)np * sizeof(double) + 255) & ~(size_t)255);
+  int rc = norms<T>(q, live, most, np, parts, nullptr);
+  for (size_t lo = 0; lo < live.size() && !rc; lo += kSmallTasks) {
+    ThinArgs a{};
+    a.count = live.size() - lo < kSmallTasks ? (int)(live.size() - lo) : kSmallTasks;
+    a.nesterov = q.nesterov;
+    a.at = (int)lo;
+    a.part_count = np;
+    a.parts = parts;
+    a.a = q.a;
+    a.b = q.b;
+    a.c = q.c;
+    a.eps = q.eps;
+    a.mu = q.mu;
+    a.gscale = q.gscale;
+    a.gscale_dev = q.gscale_dev;
+    a.gamma = q.rate ? q.gamma : 0.0;
+    int64_t blocks = 0;
+    double operations = 0;
+    for (int i = 0; i < a.count; ++i) {
+      const int j = live[lo + i];
+      const int64_t r = q.rows[j], c = q.cols[j];
+      const double m = (double)(r < c ? r : c), w = (double)(r < c ? c : r);
+      a.t[i] = {q.g[j], q.m ? q.m[j] : nullptr, q.out[j], p, q.rate ? q.rate[j] : 1.0, (int)r, (int)c, (int)blocks};
+      p += thin_bytes(dtype, r, c);
+      blocks += thin_blocks(r, c);
+      operations += q.steps * (3.0 * m * m * w + m * m * m);
+    }
+    TimedLaunch tl(DTMI_FAM_GEMM, operations);
+    a.stage = kThinFirst;
+    rc = launch_thin(dtype, a, (int)blocks);
+    for (int s = 0; s < q.steps && !rc; ++s) {
+      rc = launch_thin(dtype, a, 0);
+      a.stage = s + 1 == q.steps ? kThinLast : kThinStep;
+      if (!rc) rc = launch_thin(dtype, a, (int)blocks);
+    }
+  }
+  return rc;
+}
+
 static int newton(const char* what, int dtype, const NewtonArgs& q) {
   DTMI_CHECK(q.n >= 0 && q.steps >= 1 && q.steps <= 64, "%s: needs 1 to 64 steps, not %d", what, q.steps);
   DTMI_CHECK(q.n == 0 || (q.g && q.out && q.rows && q.cols), "%s: NULL array", what);
@@ -345,12 +424,18 @@ static int newton(const char* what, int dtype, const NewtonArgs& q) {
   }
   if (live.empty()) return DTMI_OK;
   if (all_small(dtype, q, live)) return run_small(dtype, q, live);
+  size_t thin_ws = 0;
+  const bool thin = all_thin(dtype, q, live, thin_ws);
   const int np = norm_blocks(most, es, 512);
   void* ws = nullptr;
-  int rc = pool_alloc(&ws, bytes + live.size() * (size_t)np * sizeof(double));
+  int rc = pool_alloc(&ws, (thin ? thin_ws : bytes) + live.size() * (size_t)np * sizeof(double));
   if (rc) return rc;
-  rc = dtype == DTMI_F32 ? newton_run<float>(dtype, q, live, most, np, (char*)ws)
-                         : newton_run<double>(dtype, q, live, most, np, (char*)ws);
+  if (thin)
+    rc = dtype == DTMI_F32 ? run_thin<float>(dtype, q, live, most, np, (char*)ws)
+                           : run_thin<double>(dtype, q, live, most, np, (char*)ws);
+  else
+    rc = dtype == DTMI_F32 ? newton_run<float>(dtype, q, live, most, np, (char*)ws)
+                           : newton_run<double>(dtype, q, live, most, np, (char*)ws);
   pool_free(ws);
   return rc;
 }

@@ -637,7 +637,8 @@ def test_orthogonalize(dev, dt, shape):
 # blocks of 16 rows, 2, 4 and 6 of them; columns that 8 or 16 waves share or go through in
 # turn; as much as a block holds (float32) and more; a square that only the groups take
 SMALL = [(15, 17), (16, 16), (17, 16), (5, 130), (31, 33), (32, 1000), (16, 2200), (48, 49), (50, 20), (33, 270),
-         (34, 608), (64, 65), (64, 400), (80, 96), (96, 96), (97, 97), (96, 130)]
+         (34, 608), (64, 65), (64, 400), (80, 96), (96, 96), (97, 97), (96, 130),
+         (64, 1000), (21, 1089), (3, 5000), (32, 1025), (33, 2049), (65, 900)]  # thin, in pieces of 64 columns
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
@@ -650,7 +651,9 @@ def test_orthogonalize_small_ones_alone_and_beside_a_large_one(dev, dt, shape):
         g = rng.standard_normal(s).astype(dt)
         alone = orthogonalize(D.from_numpy(g))
         check_ns(alone, g, dt, what="alone")
-        assert bits_equal(alone.numpy(), orthogonalize([D.from_numpy(g), D.from_numpy(g)])[1].numpy())
+        assert bits_equal(alone.numpy(), orthogonalize(D.from_numpy(g)).numpy())
+        # (how a grouped product's sums are split goes by the whole call: no bits to compare)
+        check_ns(orthogonalize([D.from_numpy(g), D.from_numpy(g)])[1], g, dt, what="twice")
         big = rng.standard_normal((130, 140)).astype(dt)
         outs = orthogonalize([D.from_numpy(big), D.from_numpy(g)])
         check_ns(outs[0], big, dt, what="large")
@@ -666,6 +669,22 @@ def test_orthogonalize_more_small_ones_than_a_launch_holds(dev, dt):
     for o, g in zip(orthogonalize([D.from_numpy(g) for g in gs]), gs):
         for at in np.ndindex(*g.shape[:-2]):
             check_ns(o.numpy()[at], g[at], dt)
+
+
+@pytest.mark.parametrize("dt", [F32, F64])
+@pytest.mark.parametrize("steps", [1, 2, 5])
+def test_orthogonalize_thin_ones(dev, dt, steps):
+    """Wide and tall, stacked, more than a launch holds, by odd numbers of steps."""
+    from dtmi import device as D
+    from dtmi.optim import orthogonalize
+    rng = np.random.default_rng(0)
+    gs = [rng.standard_normal(s).astype(dt) for s in [(24, 2000), (1900, 17), (3, 30, 1300), (1, 3000)] + [(2, 70)] * 62]
+    outs = orthogonalize([D.from_numpy(g) for g in gs], steps)
+    for o, g in zip(outs, gs):
+        for at in np.ndindex(*g.shape[:-2]):
+            check_ns(o.numpy()[at], g[at], dt, steps)
+    again = orthogonalize([D.from_numpy(g) for g in gs], steps)
+    assert all(bits_equal(a.numpy(), b.numpy()) for a, b in zip(outs, again))
 
 
 @pytest.mark.parametrize("dt", [F32, F64])
@@ -729,14 +748,14 @@ def muon_ref(p, m, g, scale, lr, mu, nesterov, wd, dt):
 
 @pytest.mark.parametrize("dt", [F32, F64])
 @pytest.mark.parametrize("nesterov", [True, False])
-@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("large", [None, (150, 101), (1700, 30)], ids=["small", "groups", "thin"])
 def test_muon(dev, dt, nesterov, large):
     """Three steps, with a device-side gradient factor, a changed rate, a parameter
     without a gradient, a stack of matrices and a saved state."""
     from dtmi import device as D
     from dtmi.optim import Muon
     rng = np.random.default_rng(2)
-    shapes = [(16, 48), (48, 16), (33, 33), (3, 20, 12), (7, 9)] + [(150, 101)] * large
+    shapes = [(16, 48), (48, 16), (33, 33), (3, 20, 12), (7, 9)] + [large] * (large is not None)
     P = [(0.1 * rng.standard_normal(s)).astype(dt) for s in shapes]
     ps = [D.from_numpy(p) for p in P]
     opt = Muon(ps, lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=0.1)
