@@ -11,6 +11,7 @@
 // matrices of a call share each launch (gemm_group.h).
 // Bound: MFMA; small matrices by 3 `steps` launches one after the other, but for those of
 // newton_small.hip.
+#include <algorithm>
 #include <cmath>
 #include <utility>
 #include <vector>
@@ -288,21 +289,40 @@ static int newton_run(int dtype, const NewtonArgs& q, const std::vector<int>& li
   return rc;
 }
 
-// Whether every matrix fits a block of newton_small.hip, and those blocks are quicker than
-// the groups' launches, about 7 us each whatever their size. float32, five steps, one
-// block and the groups: 16 x 16 13 and 80 us, 15 of 35 x 264 51 and 115, 8 of 96 x 96 80
-// and 98, 8 of 96 x 192 119 and 99; float64, 6 of 64 x 96: 53 and 102.
-static bool all_small(int dtype, const NewtonArgs& q, const std::vector<int>& live) {
-  const double cus = num_cus() > 0 ? num_cus() : 256, rate = (dtype == DTMI_F32 ? 256.0 : 128.0) * cus;
-  double longest = 0, operations = 0;
+// How to run a call: by the least of what the three ways are estimated to take, in cycles.
+// Small and thin matrices (newton_small.hip) are so only all together: beside others they
+// cost the groups no launch. float32, five steps, microseconds:
+//                    small  thin  groups                     small  thin  groups
+//   16 x 16             13           80    2 of 1102 x 41             76   144
+//   15 of 35 x 264      51          115    48 of 64 x 768            163   182
+//   8 of 96 x 96        80           98    16 of 64 x 8192           394   297
+//   8 of 96 x 192      119           99    float64, 8 of 30 x 1000    70   172
+// A group's launch takes about 7 us whatever its size.
+enum NewtonWay { kSmall, kThin, kGroups };
+static NewtonWay newton_way(int dtype, const NewtonArgs& q, const std::vector<int>& live, size_t& thin_ws) {
+  const int64_t cus = num_cus() > 0 ? num_cus() : 256, limit = small_lds_limit();
+  const double never = 1e200, launches = (double)cdiv((int64_t)live.size(), kSmallTasks);
+  double small = 0, thin = 0, operations = 0;
+  int64_t blocks = 0;
+  thin_ws = 256;
   for (int i : live) {
     const int64_t r = q.rows[i], c = q.cols[i];
-    if (small_lds(dtype, r, c) > small_lds_limit()) return false;
-    const double cycles = small_cycles(dtype, r, c, q.steps), m = (double)(r < c ? r : c), w = (double)(r < c ? c : r);
-    longest = cycles > longest ? cycles : longest;
+    const double m = (double)(r < c ? r : c), w = (double)(r < c ? c : r);
     operations += q.steps * (3.0 * m * m * w + m * m * m);
+    small = small_lds(dtype, r, c) > limit ? never : std::max(small, small_cycles(dtype, r, c, q.steps));
+    if (thin_lds(dtype, r, c) > limit) thin = never;
+    if (thin == never) continue;
+    blocks += thin_blocks(r, c);
+    thin_ws += thin_bytes(dtype, r, c);
   }
-  return (double)cdiv((int64_t)live.size(), kSmallTasks) * longest < 3.0 * q.steps * 17000.0 + operations / rate;
+  if (blocks >= 1 << 24) thin = never;
+  for (int i : live)
+    if (thin != never) thin = std::max(thin, thin_cycles(dtype, q.rows[i], q.cols[i], blocks, cus));
+  const double rate = (dtype == DTMI_F32 ? 256.0 : 128.0) * (double)cus;
+  const double groups = 3.0 * q.steps * 17000.0 + operations / rate;
+  small *= launches;
+  thin = launches * (25000.0 + q.steps * thin);
+  return small <= thin && small < groups ? kSmall : thin < groups ? kThin : kGroups;
 }
 
 static int run_small(int dtype, const NewtonArgs& q, const std::vector<int>& live) {
@@ -331,32 +351,6 @@ static int run_small(int dtype, const NewtonArgs& q, const std::vector<int>& liv
     if (rc) return rc;
   }
   return DTMI_OK;
-}
-
-// Whether every matrix is thin, and the two launches a step of newton_small.hip are quicker
-// than the groups' three. Thin and groups, five steps: 21 x 1088 61 and 129 us, 2 of 1102 x
-// 41 76 and 144, 48 of 64 x 768 163 and 182, 16 of 64 x 8192 394 and 297; float64, 8 of
-// 30 x 1000: 70 and 172.
-static bool all_thin(int dtype, const NewtonArgs& q, const std::vector<int>& live, size_t& bytes) {
-  const int64_t cus = num_cus() > 0 ? num_cus() : 256;
-  const double rate = (dtype == DTMI_F32 ? 256.0 : 128.0) * (double)cus;
-  double longest = 0, operations = 0;
-  int64_t blocks = 0;
-  bytes = 256;
-  for (int i : live) {
-    if (thin_lds(dtype, q.rows[i], q.cols[i]) > small_lds_limit()) return false;
-    blocks += thin_blocks(q.rows[i], q.cols[i]);
-    bytes += thin_bytes(dtype, q.rows[i], q.cols[i]);
-  }
-  for (int i : live) {
-    const double cycles = thin_cycles(dtype, q.rows[i], q.cols[i], blocks, cus);
-    const double m = (double)(q.rows[i] < q.cols[i] ? q.rows[i] : q.cols[i]);
-    const double w = (double)(q.rows[i] < q.cols[i] ? q.cols[i] : q.rows[i]);
-    longest = cycles > longest ? cycles : longest;
-    operations += q.steps * (3.0 * m * m * w + m * m * m);
-  }
-  const double launches = (double)cdiv((int64_t)live.size(), kSmallTasks);
-  return blocks < (1 << 24) && launches * q.steps * longest < 3.0 * q.steps * 17000.0 + operations / rate;
 }
 
 template <typename T>
@@ -423,14 +417,14 @@ static int newton(const char* what, int dtype, const NewtonArgs& q) {
     live.push_back(i);
   }
   if (live.empty()) return DTMI_OK;
-  if (all_small(dtype, q, live)) return run_small(dtype, q, live);
   size_t thin_ws = 0;
-  const bool thin = all_thin(dtype, q, live, thin_ws);
+  const NewtonWay way = newton_way(dtype, q, live, thin_ws);
+  if (way == kSmall) return run_small(dtype, q, live);
   const int np = norm_blocks(most, es, 512);
   void* ws = nullptr;
-  int rc = pool_alloc(&ws, (thin ? thin_ws : bytes) + live.size() * (size_t)np * sizeof(double));
+  int rc = pool_alloc(&ws, (way == kThin ? thin_ws : bytes) + live.size() * (size_t)np * sizeof(double));
   if (rc) return rc;
-  if (thin)
+  if (way == kThin)
     rc = dtype == DTMI_F32 ? run_thin<float>(dtype, q, live, most, np, (char*)ws)
                            : run_thin<double>(dtype, q, live, most, np, (char*)ws);
   else
